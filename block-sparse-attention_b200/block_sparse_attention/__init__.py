@@ -22,6 +22,18 @@ _EXPORTS = {
     "pooled_scores": ".topk_index",
     "topk_q2k": ".topk_index",
     "pooled_topk_q2k": ".topk_index",
+    "window_attn_fwd": ".window_attn",
+    "window_attn_bwd": ".window_attn",
+    "window_attention": ".window_attn",
+    "WindowAttentionFunction": ".window_attn",
+    "cached_attn_fwd": ".cached_attn",
+    "tree_mask_from_parents": ".cached_attn",
+    "cache_append": ".cached_attn",
+    "cache_keep": ".cached_attn",
+    "rotary_frequencies": ".rotary",
+    "rotary_nd": ".rotary",
+    "rotary_embedding": ".rotary",
+    "RotaryFunction": ".rotary",
 }
 
 __all__ = sorted(_EXPORTS)

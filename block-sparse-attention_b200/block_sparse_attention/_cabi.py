@@ -113,9 +113,115 @@ class BwdArgs(ctypes.Structure):
     ]
 
 
+class WindowFwdArgs(ctypes.Structure):
+    """Mirror of ``struct bsa_window_fwd_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("partial_o", ctypes.c_void_p),
+        ("partial_lse", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("q_stride", _c_i64x3),
+        ("k_stride", _c_i64x3),
+        ("v_stride", _c_i64x3),
+        ("o_stride", _c_i64x3),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("Sq", ctypes.c_int32),
+        ("Sk", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("pack_gqa", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class WindowBwdArgs(ctypes.Structure):
+    """Mirror of ``struct bsa_window_bwd_args``."""
+
+    _fields_ = [
+        ("dout", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p),
+        ("dv", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("do_stride", _c_i64x3),
+        ("q_stride", _c_i64x3),
+        ("k_stride", _c_i64x3),
+        ("v_stride", _c_i64x3),
+        ("o_stride", _c_i64x3),
+        ("dq_stride", _c_i64x3),
+        ("dk_stride", _c_i64x3),
+        ("dv_stride", _c_i64x3),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("Sq", ctypes.c_int32),
+        ("Sk", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``struct bsa_rotary_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("q_stride", _c_i64x3),
+        ("k_stride", _c_i64x3),
+        ("qo_stride", _c_i64x3),
+        ("ko_stride", _c_i64x3),
+        ("pos_stride", ctypes.c_int64 * 2),
+        ("axis_pairs", ctypes.c_int32 * 4),
+        ("num_axes", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hk", ctypes.c_int32),
+        ("S", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/bsa_b200.h declares
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_pi64 = ctypes.POINTER(ctypes.c_int64)
 SIGNATURES = {
     "bsa_abi_version": (ctypes.c_int, []),
     "bsa_last_error": (ctypes.c_char_p, []),
@@ -137,6 +243,13 @@ SIGNATURES = {
     "bsa_topk_q2k": (ctypes.c_int, [_vp, ctypes.c_int64, _i32, _i32, _i32, _vp, _vp]),
     "bsa_bwd": (ctypes.c_int, [ctypes.POINTER(BwdArgs), _vp]),
     "bsa_bwd_workspace_bytes": (ctypes.c_int64, [_i32, _i32, _i32, _i32, _i32]),
+    "bsa_window_fwd": (ctypes.c_int, [ctypes.POINTER(WindowFwdArgs), _vp]),
+    "bsa_window_bwd": (ctypes.c_int, [ctypes.POINTER(WindowBwdArgs), _vp]),
+    "bsa_window_bwd_workspace_bytes": (ctypes.c_int64, [_i32] * 8),
+    "bsa_tree_mask": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp]),
+    "bsa_cache_append": (ctypes.c_int, [_vp] * 4 + [_pi64] * 4 + [_vp] * 2 + [_i32] * 7 + [_vp]),
+    "bsa_cache_keep": (ctypes.c_int, [_vp] * 2 + [_pi64] * 2 + [_vp] * 5 + [_i32] * 8 + [_vp]),
+    "bsa_rotary_nd": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), _vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,0 +1,237 @@
+// Writes of the paged key/value cache that bsa_window_fwd reads, and the ancestor masks of trees of drafts.
+//
+// The token at position j of sequence b lies in page page_table[b][j / page_size] at row j % page_size.  All of it is
+// bound by HBM (append) or by latency (keep, masks): 16 bytes per thread and access, K and V together.
+#include "bsa_b200.h"
+#include "bsa_common.cuh"
+#include "bsa_host.h"
+
+namespace bsa {
+namespace cache {
+
+struct Pages {
+  uint8_t* k;
+  uint8_t* v;
+  long long k_page, k_head, k_row, v_page, v_head, v_row;  // bytes
+  const int32_t* __restrict__ table;
+  int max_pages, page_size, num_pages;
+
+  // Byte offsets of (sequence, head, position) in K and V; false when the position has no page in the pool.
+  __device__ __forceinline__ bool at(int b, int h, int pos, long long& ko, long long& vo) const {
+    if (pos < 0) return false;
+    const int slot = pos / page_size;
+    if (slot >= max_pages) return false;
+    const int id = table[(long long)b * max_pages + slot];
+    if (id < 0 || id >= num_pages) return false;
+    const int row = pos - slot * page_size;
+    ko = id * k_page + h * k_head + row * k_row;
+    vo = id * v_page + h * v_head + row * v_row;
+    return true;
+  }
+};
+
+struct Source {
+  const uint8_t* k;
+  const uint8_t* v;
+  long long k_b, k_h, k_t, v_b, v_h, v_t;  // bytes
+};
+
+// One thread: one 16-byte chunk of K and of V of kRows consecutive tokens (all loads in flight before the stores).
+constexpr int kRows = 4;
+__global__ void __launch_bounds__(256)
+cache_append_kernel(const Source s, const Pages pg, const int32_t* __restrict__ lens, int B, int H, int T, int chunks,
+                    long long units) {
+  const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (unit >= units) return;
+  const int c = (int)(unit % chunks);
+  long long r = unit / chunks;
+  const int groups = (T + kRows - 1) / kRows;
+  const int t0 = (int)(r % groups) * kRows;
+  r /= groups;
+  const int h = (int)(r % H), b = (int)(r / H);
+  const int base = lens[b] - T;
+  uint4 kv[kRows], vv[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int t = min(t0 + i, T - 1);
+    kv[i] = *(reinterpret_cast<const uint4*>(s.k + b * s.k_b + h * s.k_h + t * s.k_t) + c);
+    vv[i] = *(reinterpret_cast<const uint4*>(s.v + b * s.v_b + h * s.v_h + t * s.v_t) + c);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    long long ko, vo;
+    if (t0 + i < T && pg.at(b, h, base + t0 + i, ko, vo)) {
+      *(reinterpret_cast<uint4*>(pg.k + ko) + c) = kv[i];
+      *(reinterpret_cast<uint4*>(pg.v + vo) + c) = vv[i];
+    }
+  }
+}
+
+// Accepted draft path[i] moves to place i.  A path is ascending, so path[i] >= i: with the moves of a sequence done in
+// order, none overwrites a source that a later one reads.  One thread carries one chunk of K and V through the whole
+// path, eight moves at a time (their loads before their stores, the order kept between the eights).
+__global__ void __launch_bounds__(128)
+cache_keep_kernel(const Pages pg, const int32_t* __restrict__ lens, const int32_t* __restrict__ path,
+                  const int32_t* __restrict__ path_lens, int32_t* __restrict__ new_lens, int B, int H, int T,
+                  int path_cap, int chunks, long long units) {
+  constexpr int kMoves = 8;
+  const long long unit = (long long)blockIdx.x * 128 + threadIdx.x;
+  if (unit >= units) return;
+  const int c = (int)(unit % chunks);
+  const long long r = unit / chunks;
+  const int h = (int)(r % H), b = (int)(r / H);
+  const int len = lens[b], base = len - T;
+  const int32_t* mine = path + (long long)b * path_cap;
+  int n = base < 0 ? 0 : max(0, min(path_lens[b], path_cap));
+  int last = -1, kept = 0;
+  for (int i0 = 0; i0 < n; i0 += kMoves) {
+    uint4 kv[kMoves], vv[kMoves];
+    bool have[kMoves];
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      have[i] = false;
+      if (i0 + i < n) {
+        const int u = mine[i0 + i];
+        if (u <= last || u >= T) {
+          n = i0 + i;  // the path ends here
+        } else {
+          last = u;
+          kept = i0 + i + 1;
+          long long ko, vo;
+          if (u != i0 + i && pg.at(b, h, base + u, ko, vo)) {
+            have[i] = true;
+            kv[i] = *(reinterpret_cast<const uint4*>(pg.k + ko) + c);
+            vv[i] = *(reinterpret_cast<const uint4*>(pg.v + vo) + c);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kMoves; ++i) {
+      long long ko, vo;
+      if (have[i] && pg.at(b, h, base + i0 + i, ko, vo)) {
+        *(reinterpret_cast<uint4*>(pg.k + ko) + c) = kv[i];
+        *(reinterpret_cast<uint4*>(pg.v + vo) + c) = vv[i];
+      }
+    }
+  }
+  if (h == 0 && c == 0) new_lens[b] = base < 0 ? len : base + kept;
+}
+
+// One thread per draft walks up its parents: at most T steps, as every parent is an earlier draft.
+__global__ void __launch_bounds__(64)
+tree_mask_kernel(const int32_t* __restrict__ parents, long long* __restrict__ mask, int T) {
+  __shared__ int up[64];
+  const int t = threadIdx.x;
+  const long long row = (long long)blockIdx.x * T;
+  if (t < T) up[t] = parents[row + t];
+  __syncthreads();
+  if (t >= T) return;
+  unsigned long long m = 0;
+  for (int u = t; u >= 0;) {
+    const int above = up[u];
+    if (above >= u || above < -1) {  // not a tree: an unused slot
+      m = 0;
+      break;
+    }
+    m |= 1ull << u;
+    u = above;
+  }
+  mask[row + t] = (long long)m;
+}
+
+static int check_pages(const char* what, const void* kc, const void* vc, const int64_t* ks, const int64_t* vs,
+                       const int32_t* table, const int32_t* lens, int B, int H, int T, int D, int max_pages,
+                       int page_size, int num_pages) {
+  if (!kc || !vc || !ks || !vs || !table || !lens) return set_error(BSA_ERR_INVALID, "%s: null pointer", what);
+  if (B < 1 || H < 1 || T < 1 || max_pages < 1 || page_size < 1 || num_pages < 1)
+    return set_error(BSA_ERR_INVALID, "%s: non-positive extent", what);
+  if (D < 8 || D % 8 != 0) return set_error(BSA_ERR_INVALID, "%s: D must be a multiple of 8", what);
+  if ((long long)max_pages * page_size > (1 << 29)) return set_error(BSA_ERR_UNSUPPORTED, "%s: more than 2^29 tokens per sequence", what);
+  if (((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & 15u) != 0)
+    return set_error(BSA_ERR_INVALID, "%s: the caches must be 16-byte aligned", what);
+  for (int i = 0; i < 3; ++i)
+    if ((ks[i] | vs[i]) % 8 != 0) return set_error(BSA_ERR_INVALID, "%s: cache strides must be multiples of 8 elements", what);
+  return BSA_OK;
+}
+
+static Pages make_pages(void* kc, void* vc, const int64_t* ks, const int64_t* vs, const int32_t* table, int max_pages,
+                        int page_size, int num_pages) {
+  Pages pg{};
+  pg.k = static_cast<uint8_t*>(kc);
+  pg.v = static_cast<uint8_t*>(vc);
+  pg.k_page = ks[0] * 2; pg.k_head = ks[1] * 2; pg.k_row = ks[2] * 2;
+  pg.v_page = vs[0] * 2; pg.v_head = vs[1] * 2; pg.v_row = vs[2] * 2;
+  pg.table = table;
+  pg.max_pages = max_pages;
+  pg.page_size = page_size;
+  pg.num_pages = num_pages;
+  return pg;
+}
+
+}  // namespace cache
+}  // namespace bsa
+
+using namespace bsa;
+
+extern "C" int bsa_tree_mask(const int32_t* parents, int32_t B, int32_t T, int64_t* mask, void* cuda_stream) {
+  if (!parents || !mask) return set_error(BSA_ERR_INVALID, "bsa_tree_mask: null pointer");
+  if (B < 1 || T < 1 || T > 64) return set_error(BSA_ERR_INVALID, "bsa_tree_mask: 1 to 64 drafts");
+  cache::tree_mask_kernel<<<(unsigned)B, 64, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
+      parents, reinterpret_cast<long long*>(mask), T);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "tree mask launch: %s", cudaGetErrorString(e));
+  return BSA_OK;
+}
+
+extern "C" int bsa_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int64_t k_stride[3],
+                                const int64_t v_stride[3], const int64_t kc_stride[3], const int64_t vc_stride[3],
+                                const int32_t* page_table, const int32_t* lens, int32_t B, int32_t H, int32_t T,
+                                int32_t D, int32_t max_pages, int32_t page_size, int32_t num_pages, void* cuda_stream) {
+  int rc = cache::check_pages("bsa_cache_append", k_cache, v_cache, kc_stride, vc_stride, page_table, lens, B, H, T, D,
+                              max_pages, page_size, num_pages);
+  if (rc) return rc;
+  if (!k || !v || !k_stride || !v_stride) return set_error(BSA_ERR_INVALID, "bsa_cache_append: null pointer");
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) != 0)
+    return set_error(BSA_ERR_INVALID, "bsa_cache_append: k and v must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if ((k_stride[i] | v_stride[i]) % 8 != 0)
+      return set_error(BSA_ERR_INVALID, "bsa_cache_append: strides must be multiples of 8 elements");
+  cache::Source s{};
+  s.k = static_cast<const uint8_t*>(k);
+  s.v = static_cast<const uint8_t*>(v);
+  s.k_b = k_stride[0] * 2; s.k_h = k_stride[1] * 2; s.k_t = k_stride[2] * 2;
+  s.v_b = v_stride[0] * 2; s.v_h = v_stride[1] * 2; s.v_t = v_stride[2] * 2;
+  const int chunks = D / 8;
+  const long long units = (long long)B * H * ((T + cache::kRows - 1) / cache::kRows) * chunks;
+  const long long blocks = (units + 255) / 256;
+  if (blocks > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_cache_append: too many tokens");
+  cache::cache_append_kernel<<<(unsigned)blocks, 256, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
+      s, cache::make_pages(k_cache, v_cache, kc_stride, vc_stride, page_table, max_pages, page_size, num_pages), lens,
+      B, H, T, chunks, units);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cache append launch: %s", cudaGetErrorString(e));
+  return BSA_OK;
+}
+
+extern "C" int bsa_cache_keep(void* k_cache, void* v_cache, const int64_t kc_stride[3], const int64_t vc_stride[3],
+                              const int32_t* page_table, const int32_t* lens, const int32_t* path,
+                              const int32_t* path_lens, int32_t* new_lens, int32_t B, int32_t H, int32_t T,
+                              int32_t path_cap, int32_t D, int32_t max_pages, int32_t page_size, int32_t num_pages,
+                              void* cuda_stream) {
+  int rc = cache::check_pages("bsa_cache_keep", k_cache, v_cache, kc_stride, vc_stride, page_table, lens, B, H, T, D,
+                              max_pages, page_size, num_pages);
+  if (rc) return rc;
+  if (!path || !path_lens || !new_lens) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: null pointer");
+  if (path_cap < 1) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: non-positive extent");
+  const int chunks = D / 8;
+  const long long units = (long long)B * H * chunks;
+  const long long blocks = (units + 127) / 128;
+  if (blocks > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_cache_keep: too many heads");
+  cache::cache_keep_kernel<<<(unsigned)blocks, 128, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
+      cache::make_pages(k_cache, v_cache, kc_stride, vc_stride, page_table, max_pages, page_size, num_pages), lens, path,
+      path_lens, new_lens, B, H, T, path_cap, chunks, units);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cache keep launch: %s", cudaGetErrorString(e));
+  return BSA_OK;
+}

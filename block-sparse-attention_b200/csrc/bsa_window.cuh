@@ -1,0 +1,59 @@
+// Geometry and masks of causal sliding-window attention with sink tokens, shared by the forward kernel (contiguous
+// and paged keys) and the two backward kernels.
+//
+// Keys sit at positions 0..len-1 of their sequence, query row i at position base + i (base = Sk - Sq, or the
+// sequence's length minus the number of new tokens over a cache).  Key j is visible to a row at position p iff
+//     0 <= p < len,   j <= p,   (j > p - window  or  j < sinks).
+// Rows of a tree of drafts hold a 64-bit mask: bit u = draft u (the key at base + u) is visible; the row's position
+// is base + popcount - 1 (its depth), and it sees the keys before base by the rule above.
+//
+// The kernels work on 128-token key tiles.  The tiles a query tile needs are those its rows' windows touch, walked
+// from the diagonal downwards (so the running maximum is set by visible scores from the first tile on), and then
+// tile 0 once more for the sinks if no window reaches it: sinks <= 128, so that is one tile.  A tile that every row
+// of the query tile sees entirely takes an unmasked path; in the others each thread builds one visibility bit per
+// column of its row.
+#pragma once
+
+#include "bsa_common.cuh"
+
+namespace bsa {
+
+constexpr int kMaxSinks = 128;
+constexpr int kWindowAll = 1 << 29;  // "no window": no length is larger, and its sums with positions stay inside 32 bits
+constexpr int kMaxTreeNodes = 64;
+
+// Bits [0, n) of a 32-bit word; n is clamped to [0, 32].
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : ((1u << n) - 1u));
+}
+// Word w (bits 32w .. 32w+31) of the bit range [lo, hi).
+__device__ __forceinline__ uint32_t range_word(int lo, int hi, int w) {
+  return low_bits(hi - 32 * w) & ~low_bits(lo - 32 * w);
+}
+
+// The key tiles of one query tile whose rows have positions in [p_lo, p_hi].
+struct TileList {
+  int n_win;  // window tiles t_hi, t_hi - 1, ..., t_hi - n_win + 1
+  int n;      // n_win, plus one when tile 0 follows for the sinks
+  int t_hi;
+  int k_lo;   // first key any window reaches
+  __device__ __forceinline__ int tile(int it) const { return it < n_win ? t_hi - it : 0; }
+};
+
+__device__ __forceinline__ TileList window_tiles(int p_lo, int p_hi, int len, int window, int sinks) {
+  TileList t;
+  p_lo = max(p_lo, 0);
+  p_hi = min(p_hi, len - 1);
+  t.n = t.n_win = 0;
+  t.t_hi = 0;
+  t.k_lo = 0;
+  if (p_lo > p_hi) return t;
+  t.k_lo = max(0, p_lo - window + 1);
+  t.t_hi = p_hi >> 7;
+  const int t_lo = t.k_lo >> 7;
+  t.n_win = t.t_hi - t_lo + 1;
+  t.n = t.n_win + ((sinks > 0 && t_lo > 0) ? 1 : 0);
+  return t;
+}
+
+}  // namespace bsa

@@ -1,0 +1,1092 @@
+// Causal sliding-window attention with sink tokens, backward, for sm_100a (contiguous keys, grouped heads).
+//
+//   delta_i = sum_d O_id dO_id,  P_ij = exp(scale q_i k_j - lse_i) on the visible pairs,  dS = P o (dO V^T - delta)
+//   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO     (dK, dV of a KV head sum over its G query heads)
+//
+// Four launches, no atomics, every sum in a fixed order:
+//   1. preprocess: -delta and -lse log2(e) per query row, padded to whole 128-row tiles
+//   2. dQ kernel: one item per query tile, over the key tiles its windows touch (and tile 0 for the sinks)
+//   3. dK/dV kernel: one item per key tile, over the (query head, query tile) pairs that see it.  Tile 0 holds the
+//      sinks, which every later query tile sees: those tiles beyond the windows' reach are dealt to further items of
+//      about the length of an ordinary one (G * n pairs of tiles against G * (W / 128 + 1): without the split, one CTA
+//      would work on tile 0 while the others have finished).  They and tile 0's own item leave fp32 sums of the sink
+//      rows in the workspace,
+//   4. which the reduce kernel adds up in order.
+// The structure of the two main kernels is the one that measured best for the block-sparse backward: warps 0-7 compute
+// (two groups of 128 threads, thread = tensor-memory lane, group g owns columns [64g, 64g + 64) of the score tiles),
+// warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
+// P and dS are rounded to 16 bits for the tensor cores (all sums are fp32); masked pairs are cleared in the packed
+// words, so that what padding holds - NaN included - reaches no sum; rows behind the end are zeroed in shared memory
+// where an MMA contracts over them.  With fp16, small gradients need the loss scaling that fp16 training uses anyway.
+#include "bsa_b200.h"
+#include "bsa_common.cuh"
+#include "bsa_host.h"
+#include "bsa_window.cuh"
+
+#include <cuda_fp16.h>
+
+namespace bsa {
+namespace winbwd {
+
+constexpr int kMmaWarp = 8;
+constexpr int kDqThreads = 384;
+constexpr int kDqLoadWarp = 11;
+constexpr int kDkvThreads = 352;
+constexpr int kDkvLoadWarp = 10;
+constexpr int kTile = 128 * 128 * 2;
+constexpr int kSlab = 128 * 128;
+constexpr int kBarBytes = 256 + 16;  // 32 mbarriers, tensor-memory base, abort flag
+
+struct Params {
+  const int32_t* __restrict__ kv_lens;
+  const float* __restrict__ lse_log2;  // [B, Hq, Nq * 128]  -lse * log2(e)
+  const float* __restrict__ delta;     // [B, Hq, Nq * 128]  -sum_d O dO
+  float* partial;                      // [B * Hkv, slots, 2 (dK, dV), sinks, D]
+  uint8_t* dq;
+  uint8_t* dk;
+  uint8_t* dv;
+  int* status;
+  long long dq_stride[3], dk_stride[3], dv_stride[3];  // elements
+  int B, Hq, Hkv, G, Sq, Sk, Nq, Nkv, D;
+  int window, sinks;
+  int sink_items;  // further items of tile 0 per (batch, KV head); the workspace holds sink_items + 1 slots
+  int sink_m0;     // first query tile beyond the reach of tile 0's windows
+  float scale_log2, softmax_scale;
+};
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack16(uint32_t u) {
+  float2 f;
+  if (F16) unpack_f16x2(u, f.x, f.y);
+  else {
+    f.x = __uint_as_float(u << 16);
+    f.y = __uint_as_float(u & 0xffff0000u);
+  }
+  return f;
+}
+// Mask of a packed pair of 16-bit values from visibility bits b0 (low) and b1 of `w`.
+__device__ __forceinline__ uint32_t pair_mask(uint32_t w, int bit) {
+  return (((w >> bit) & 1u) ? 0x0000ffffu : 0u) | (((w >> (bit + 1)) & 1u) ? 0xffff0000u : 0u);
+}
+
+__device__ __forceinline__ int seq_len(const Params& p, int b) {
+  return p.kv_lens ? max(0, min(p.kv_lens[b], p.Sk)) : p.Sk;
+}
+
+__device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Up to 64 fp32 accumulator columns of a row -> 16 bits, scaled -> global.
+template <bool F16>
+__device__ __forceinline__ void store_half(uint8_t* dst, const uint32_t* acc, float scale, int cols) {
+#pragma unroll
+  for (int ch = 0; ch < 8; ++ch) {
+    if (ch * 8 < cols) {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        u[e] = pack16<F16>(__uint_as_float(acc[ch * 8 + 2 * e]) * scale, __uint_as_float(acc[ch * 8 + 2 * e + 1]) * scale);
+      reinterpret_cast<uint4*>(dst)[ch] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+__device__ __forceinline__ void store_half_f32(float* dst, const uint32_t* acc, int cols) {
+#pragma unroll
+  for (int ch = 0; ch < 16; ++ch)
+    if (ch * 4 < cols) reinterpret_cast<uint4*>(dst)[ch] = make_uint4(acc[4 * ch], acc[4 * ch + 1], acc[4 * ch + 2], acc[4 * ch + 3]);
+}
+
+template <bool F16>
+struct Idesc {
+  static constexpr uint32_t kFmt = F16 ? 0u : 1u;
+  static constexpr uint32_t kKK = umma_idesc(kFmt, kFmt, 0, 0, 128, 128);
+  static __device__ __forceinline__ uint32_t kmn(int n) { return umma_idesc(kFmt, kFmt, 0, 1, 128, (uint32_t)n); }
+};
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t saddr) { return umma_desc_sw128(saddr, 0, 1024); }
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t saddr) { return umma_desc_sw128(saddr, kSlab, 1024); }
+constexpr uint64_t kTileStep = kTile >> 4;
+
+// D = A(smem, K-major) * B(smem, K-major)^T, contracting over the head dimension in `ksteps` = D / 16 steps.
+__device__ __forceinline__ void mma_ss_kk(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t led, int ksteps) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint64_t off = (uint64_t)((k >> 2) * (kSlab >> 4) + (k & 3) * 2);
+    umma_f16_ss_led(d, a_desc + off, b_desc + off, idesc, k > 0 ? 1u : 0u, (k < ksteps) ? led : 0u);
+  }
+}
+// D (+)= A(tmem, 16 bits, two 32-column halves) * B(smem, MN-major), contracting over 128 tokens.
+__device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint64_t b_desc, bool acc, uint32_t led, uint32_t idesc) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t a = (k < 4) ? (a_lo + (uint32_t)k * 8u) : (a_hi + (uint32_t)(k - 4) * 8u);
+    umma_f16_ts_led(d, a, b_desc + (uint64_t)(k * 128), idesc, (acc || k > 0) ? 1u : 0u, led);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// 1. preprocess: HBM-bound, reads O and dO once.  A warp handles eight consecutive padded rows: sixteen lanes per row
+//    with 16 bytes each, all loads of a thread in flight before the first use.
+// ------------------------------------------------------------------------------------------------
+template <bool F16>
+__global__ void __launch_bounds__(256)
+window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ d_o, const float* __restrict__ lse,
+                      float* __restrict__ lse_log2, float* __restrict__ delta, long long os_b, long long os_h,
+                      long long os_s, long long ds_b, long long ds_h, long long ds_s, int H, int Sq, int SqPad,
+                      long long rows_pad, int D) {
+  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8;
+  if (row0 >= rows_pad) return;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane >> 4, chunk = lane & 15;
+  const long long bh = row0 / SqPad;  // the eight rows lie in one (batch, head) plane: SqPad is a multiple of 128
+  const int s0 = (int)(row0 - bh * SqPad);
+  const int h = (int)(bh % H);
+  const long long b = bh / H;
+  const uint8_t* o_base = o + (b * os_b + h * os_h + chunk * 8) * 2;
+  const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
+  uint4 ov[4], dv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + 2 * i + sub;
+    ov[i] = make_uint4(0, 0, 0, 0);
+    dv[i] = make_uint4(0, 0, 0, 0);
+    if (s < Sq && chunk * 8 < D) {
+      ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * os_s * 2);
+      dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + 2 * i + sub;
+    const uint32_t ow[4] = {ov[i].x, ov[i].y, ov[i].z, ov[i].w}, dw[4] = {dv[i].x, dv[i].y, dv[i].z, dv[i].w};
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = unpack16<F16>(ow[e]), c = unpack16<F16>(dw[e]);
+      acc = fmaf(a.x, c.x, acc);
+      acc = fmaf(a.y, c.y, acc);
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (chunk == 0) {
+      float l = INFINITY;
+      if (s < Sq) {
+        const float lv = lse[bh * Sq + s];
+        l = (lv == -INFINITY) ? INFINITY : lv * kLog2e;
+      }
+      delta[bh * SqPad + s] = -acc;
+      lse_log2[bh * SqPad + s] = -l;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// 2. dQ kernel
+// ------------------------------------------------------------------------------------------------
+// smem: Q | dO | ring of 5 tiles (K_0, V_0, K_1, V_1, ...) | barriers.  Tensor memory: S @0, dP / dS buffers @128 and
+// @256 (dS overwrites the head of each group's half), dQ @384.  S_{j+1} is issued once every compute thread holds S_j
+// in registers and dP_{j+1} goes to the buffer that dQ_{j-1} has finished reading, so both run under the arithmetic of
+// iteration j.
+constexpr int kDqStages = 5;
+constexpr int kDqSmem = (2 + kDqStages) * kTile + kBarBytes;
+
+struct DqItem {
+  int b, h, m, len, base, p_lo, p_hi;
+  TileList tiles;
+};
+__device__ __forceinline__ DqItem dq_item(const Params& p, int w) {
+  DqItem t;
+  t.m = w % p.Nq;
+  t.h = (w / p.Nq) % p.Hq;
+  t.b = w / (p.Nq * p.Hq);
+  t.len = seq_len(p, t.b);
+  t.base = p.Sk - p.Sq;
+  t.p_lo = t.base + t.m * 128;
+  t.p_hi = t.base + min(p.Sq, t.m * 128 + 128) - 1;
+  t.tiles = window_tiles(t.p_lo, t.p_hi, t.len, p.window, p.sinks);
+  return t;
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(kDqThreads, 1)
+window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                 const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  constexpr int NS = kDqStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* sQ = smem_raw;
+  uint8_t* sdO = sQ + kTile;
+  uint8_t* sRing = sdO + kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRing + NS * kTile);
+  uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(bars + 32);
+  volatile int& s_abort = *reinterpret_cast<volatile int*>(bars + 33);
+  if ((smem_u32(smem_raw) & 1023u) != 0) {
+    if (threadIdx.x == 0 && atomicCAS(p.status, 0, (int)kStatusBadIndex) == 0) p.status[2] = 995;
+    return;
+  }
+  const uint32_t bar_base = smem_u32(bars);
+  auto BAR = [&](int i) { return bar_base + (uint32_t)i * 8u; };
+  constexpr int kRFull = 0, kREmpty = NS, kQFull = 2 * NS, kQEmpty = kQFull + 1, kDoFull = kQEmpty + 1,
+                kDoEmpty = kDoFull + 1, kSFull = kDoEmpty + 1, kSFree = kSFull + 1, kDpFull = kSFree + 1,
+                kDsFull = kDpFull + 2, kDsUsed = kDsFull + 2, kDqFinal = kDsUsed + 2, kDqFree = kDqFinal + 1,
+                kNumBars = kDqFree + 1;
+  static_assert(kNumBars <= 32, "barrier slots");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  WaitCtx wctx{&s_abort, p.status};
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(BAR(kRFull + i), 1);
+      mbar_init(BAR(kREmpty + i), 3);  // released once by each issuing warp
+    }
+    mbar_init(BAR(kQFull), 1);
+    mbar_init(BAR(kQEmpty), 1);
+    mbar_init(BAR(kDoFull), 1);
+    mbar_init(BAR(kDoEmpty), 1);
+    mbar_init(BAR(kSFull), 1);
+    mbar_init(BAR(kSFree), 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(BAR(kDpFull + i), 1);
+      mbar_init(BAR(kDsFull + i), 256);
+      mbar_init(BAR(kDsUsed + i), 1);
+    }
+    mbar_init(BAR(kDqFinal), 1);
+    mbar_init(BAR(kDqFree), 256);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&s_tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem_base;
+  const uint32_t tS = tmem, tdP = tmem + 128u, tdQ = tmem + 384u;
+  const int num_work = p.B * p.Hq * p.Nq;
+
+  if (warp == kDqLoadWarp) {
+    uint32_t r_cnt = 0, tile_cnt = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const DqItem t = dq_item(p, w);
+      const int n = t.tiles.n;
+      if (n == 0) continue;
+      for (int which = 0; which < 2 && ok; ++which) {  // Q, dO
+        const int full = which ? kDoFull : kQFull, empty = which ? kDoEmpty : kQEmpty;
+        ok = mbar_wait(BAR(empty), (tile_cnt & 1) ^ 1, wctx, 400);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(BAR(full), kTile);
+          const CUtensorMap* tm = which ? &tm_do : &tm_q;
+          for (int sl = 0; sl < 2; ++sl)
+            tma_load_4d(smem_u32((which ? sdO : sQ) + sl * kSlab), tm, BAR(full), sl * 64, t.m * 128, t.h, t.b);
+        }
+      }
+      ++tile_cnt;
+      for (int j = 0; j < n && ok; ++j) {
+        const int row = t.tiles.tile(j) * 128;
+        for (int which = 0; which < 2 && ok; ++which) {
+          const uint32_t stage = r_cnt % NS, ph = (r_cnt / NS) & 1;
+          ok = mbar_wait(BAR(kREmpty + stage), ph ^ 1, wctx, 401);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(BAR(kRFull + stage), kTile);
+            const CUtensorMap* tm = which ? &tm_v : &tm_k;
+            for (int sl = 0; sl < 2; ++sl)
+              tma_load_4d(smem_u32(sRing + stage * kTile + sl * kSlab), tm, BAR(kRFull + stage), sl * 64, row,
+                          t.h / p.G, t.b);
+          }
+          ++r_cnt;
+        }
+      }
+    }
+  } else if (warp >= kMmaWarp && warp < kMmaWarp + 3) {
+    // issuer 0: S_j = Q K_j^T;  issuer 1: dQ += dS_j K_j;  issuer 2: dP_j = dO V_j^T.  All three visit every ring
+    // position in order and release every stage once.
+    const int who = warp - kMmaWarp;
+    uint32_t r_cnt = 0, free_cnt = 0, s_issued = 0, dp_issued = 0, ds_seen = 0, tile_cnt = 0;
+    bool ok = true;
+    bool first_tile = true;
+    const uint32_t led = lane == 0;
+    const uint64_t ring_k = desc_k_major(smem_u32(sRing)), ring_mn = desc_mn_major(smem_u32(sRing));
+    const int ksteps = p.D / 16;
+    const uint32_t idesc_n = Idesc<F16>::kmn(p.D);
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const int n = dq_item(p, w).tiles.n;
+      if (n == 0) continue;
+      const uint32_t base = r_cnt;  // K_j at base + 2j, V_j at base + 2j + 1
+      auto stage_of = [&](uint32_t pos) { return pos % NS; };
+      auto wait_full = [&](uint32_t pos) { return mbar_wait(BAR(kRFull + stage_of(pos)), (pos / NS) & 1, wctx, 411); };
+      auto pass = [&](uint32_t pos) {  // a tile this issuer does not read
+        if (!wait_full(pos)) return false;
+        if (led) mbar_arrive(BAR(kREmpty + stage_of(pos)));
+        __syncwarp();
+        return true;
+      };
+      if (who == 0) {
+        ok = mbar_wait(BAR(kQFull), tile_cnt & 1, wctx, 410);
+        const uint64_t q_desc = desc_k_major(smem_u32(sQ));
+        for (int j = 0; j < n && ok; ++j) {
+          ok = wait_full(base + 2 * j);
+          if (!ok) break;
+          if (s_issued > 0) {  // the previous S is in the registers of every compute thread
+            ok = mbar_wait(BAR(kSFree), (s_issued - 1) & 1, wctx, 414);
+            if (!ok) break;
+          }
+          ++s_issued;
+          tc_fence_after();
+          const uint32_t sk = stage_of(base + 2 * j);
+          mma_ss_kk(tS, q_desc, ring_k + sk * kTileStep, Idesc<F16>::kKK, led, ksteps);
+          umma_commit_led(BAR(kSFull), led);
+          umma_commit_led(BAR(kREmpty + sk), led);
+          if (j == n - 1) umma_commit_led(BAR(kQEmpty), led);
+          __syncwarp();
+          ok = pass(base + 2 * j + 1);
+        }
+        if (!ok) break;
+      } else if (who == 2) {
+        ok = mbar_wait(BAR(kDoFull), tile_cnt & 1, wctx, 416);
+        const uint64_t do_desc = desc_k_major(smem_u32(sdO));
+        for (int j = 0; j < n && ok; ++j) {
+          ok = pass(base + 2 * j);
+          if (ok) ok = wait_full(base + 2 * j + 1);
+          if (!ok) break;
+          const uint32_t buf = dp_issued & 1;
+          if (dp_issued >= 2) {  // dS of two iterations back has been read from this buffer
+            ok = mbar_wait(BAR(kDsUsed + buf), ((dp_issued >> 1) - 1) & 1, wctx, 415);
+            if (!ok) break;
+          }
+          ++dp_issued;
+          tc_fence_after();
+          const uint32_t sv = stage_of(base + 2 * j + 1);
+          mma_ss_kk(tdP + buf * 128u, do_desc, ring_k + sv * kTileStep, Idesc<F16>::kKK, led, ksteps);
+          umma_commit_led(BAR(kDpFull + buf), led);
+          umma_commit_led(BAR(kREmpty + sv), led);
+          if (j == n - 1) umma_commit_led(BAR(kDoEmpty), led);
+          __syncwarp();
+        }
+        if (!ok) break;
+      } else {
+        for (int j = 0; j < n && ok; ++j) {
+          ok = wait_full(base + 2 * j);
+          if (ok) ok = pass(base + 2 * j + 1);
+          if (!ok) break;
+          const uint32_t buf = ds_seen & 1;
+          ok = mbar_wait(BAR(kDsFull + buf), (ds_seen >> 1) & 1, wctx, 412);
+          if (!ok) break;
+          ++ds_seen;
+          if (j == 0 && !first_tile) {  // the previous tile's epilogue has drained dQ
+            ok = mbar_wait(BAR(kDqFree), free_cnt & 1, wctx, 413);
+            if (!ok) break;
+            ++free_cnt;
+          }
+          tc_fence_after();
+          const uint32_t sk = stage_of(base + 2 * j);
+          const uint32_t t = tdP + buf * 128u;
+          mma_ts_kmn(tdQ, t, t + 64u, ring_mn + sk * kTileStep, j > 0, led, idesc_n);
+          umma_commit_led(BAR(kDsUsed + buf), led);
+          umma_commit_led(BAR(kREmpty + sk), led);
+          __syncwarp();
+        }
+        if (!ok) break;
+        umma_commit_led(BAR(kDqFinal), led);
+        __syncwarp();
+      }
+      r_cnt += 2 * n;
+      ++tile_cnt;
+      first_tile = false;
+    }
+  } else if (warp < 8) {
+    const int grp = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t s_cnt = 0, dp_cnt = 0, fin_cnt = 0, r_cnt = 0;
+    bool ok = true;
+    const int cols = p.D - grp * 64;  // output columns of this group (<= 0: none)
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const DqItem t = dq_item(p, w);
+      const int n = t.tiles.n;
+      const int seq = t.m * 128 + row, pos = t.base + seq;
+      const bool live = seq < p.Sq && pos >= 0 && pos < t.len;
+      uint8_t* dq_row = p.dq + (t.b * p.dq_stride[0] + t.h * p.dq_stride[1] + (long long)seq * p.dq_stride[2] + grp * 64) * 2;
+      uint32_t acc[64];
+      if (n > 0) {
+        const long long srow = ((long long)t.b * p.Hq + t.h) * ((long long)p.Nq * 128) + seq;
+        const float nlse = p.lse_log2[srow], ndlt = p.delta[srow];
+        const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2), nl2 = pack2(nlse, nlse), nd2 = pack2(ndlt, ndlt);
+        // every row of the tile sees all keys of [free_lo, free_hi)
+        const int free_lo = min(t.p_hi, t.len - 1) - p.window + 1, free_hi = t.p_lo + 1;
+        for (int j = 0; j < n && ok; ++j) {
+          const int j0 = t.tiles.tile(j) * 128;
+          ok = mbar_wait(BAR(kSFull), s_cnt & 1, wctx, 420);
+          if (!ok) break;
+          ++s_cnt;
+          tc_fence_after();
+          float pr[64];
+          {
+            uint32_t* u = reinterpret_cast<uint32_t*>(pr);
+            tmem_ld32(tS + lane_base + grp * 64, u);
+            tmem_ld32(tS + lane_base + grp * 64 + 32, u + 32);
+            tmem_wait_ld();
+          }
+          tc_fence_before();
+          mbar_arrive(BAR(kSFree));  // S_j is in registers: the next S may be computed
+          if (j0 + 128 > t.len) {    // K rows behind the end: dQ contracts over them (S_j has read the tile)
+            if (j0 + row >= t.len) {
+              uint4* k0 = reinterpret_cast<uint4*>(sRing + ((r_cnt + 2u * j) % NS) * kTile + grp * kSlab + row * 128);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) k0[c] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            float x0, x1;
+            unpack2(ffma2(pack2(pr[c], pr[c + 1]), sc2, nl2), x0, x1);
+            pr[c] = ex2_approx(x0);
+            pr[c + 1] = ex2_approx(x1);
+          }
+          const uint32_t buf = dp_cnt & 1;
+          ok = mbar_wait(BAR(kDpFull + buf), (dp_cnt >> 1) & 1, wctx, 421);
+          if (!ok) break;
+          ++dp_cnt;
+          tc_fence_after();
+          const uint32_t tbuf = tdP + buf * 128u + lane_base + grp * 64;
+          uint32_t dp[64];
+          tmem_ld32(tbuf, dp);
+          tmem_ld32(tbuf + 32, dp + 32);
+          tmem_wait_ld();
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float d0, d1;
+            unpack2(fmul2(pack2(pr[2 * e], pr[2 * e + 1]),
+                          fadd2(pack2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])), nd2)), d0, d1);
+            pk[e] = pack16<F16>(d0, d1);
+          }
+          if (!(j0 >= free_lo && j0 + 128 <= free_hi)) {
+            const int c0 = j0 + grp * 64;
+            uint32_t mw[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              mw[i] = live ? range_word(pos - p.window + 1 - c0, pos + 1 - c0, i) : 0u;
+              if (j0 == 0 && live) mw[i] |= range_word(0, min(p.sinks, pos + 1) - c0, i);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pk[e] &= pair_mask(mw[e >> 4], (2 * e) & 31);
+          }
+          tmem_st32(tbuf, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(BAR(kDsFull + buf));
+        }
+        if (!ok) break;
+        r_cnt += 2 * n;
+        ok = mbar_wait(BAR(kDqFinal), fin_cnt & 1, wctx, 422);
+        if (!ok) break;
+        ++fin_cnt;
+        tc_fence_after();
+        tmem_ld32(tdQ + lane_base + grp * 64, acc);
+        tmem_ld32(tdQ + lane_base + grp * 64 + 32, acc + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(BAR(kDqFree));
+      }
+      if (n == 0 || !live) {  // takes no part
+#pragma unroll
+        for (int c = 0; c < 64; ++c) acc[c] = 0u;
+      }
+      if (seq < p.Sq) store_half<F16>(dq_row, acc, p.softmax_scale, cols);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// 3. dK/dV kernel
+// ------------------------------------------------------------------------------------------------
+// smem: K | V | ring of 5 tiles (Q_i, dO_i alternating) | row statistics [2][2][128] f32 | barriers.  Tensor memory:
+// S @0 takes S^T_i; G @128 takes dP^T_i and then P^T_i (16 bits, first 32 of a thread's 64 columns) and dS^T_i (last
+// 32), the operands of dV @256 += P^T dO and dK @384 += dS^T Q.
+constexpr int kDkvStages = 5;
+constexpr int kStatSlots = 2;
+constexpr int kDkvSmem = 2 * kTile + kDkvStages * kTile + kStatSlots * 1024 + kBarBytes;
+
+struct DkvItem {
+  int b, hkv, nb;
+  int slot;    // workspace slot of the sink rows' sums; -1: every row is stored directly
+  bool extra;  // an item of the sinks only
+  int f0, m0, nm, T;  // pair i: f = f0 + i, query head f / nm of the group, query tile m0 + f % nm
+  int len, base;
+};
+__device__ __forceinline__ DkvItem dkv_item(const Params& p, int w) {
+  DkvItem t;
+  const int extras = p.B * p.Hkv * p.sink_items;
+  int bh, chunk = 0;
+  t.extra = w < extras;
+  if (t.extra) {
+    chunk = w % p.sink_items;
+    bh = w / p.sink_items;
+    t.nb = 0;
+    t.slot = 1 + chunk;
+  } else {
+    w -= extras;
+    t.nb = w % p.Nkv;
+    bh = w / p.Nkv;
+    t.slot = (t.nb == 0 && p.sink_items > 0) ? 0 : -1;
+  }
+  t.hkv = bh % p.Hkv;
+  t.b = bh / p.Hkv;
+  t.len = seq_len(p, t.b);
+  t.base = p.Sk - p.Sq;
+  t.f0 = t.m0 = t.T = 0;
+  t.nm = 1;
+  const int last = min(p.Sq, t.len - t.base) - 1;  // last query token that takes part
+  if (t.extra) {
+    const int nm = last < 0 ? 0 : (last >> 7) + 1 - p.sink_m0;
+    if (nm > 0) {
+      t.nm = nm;
+      t.m0 = p.sink_m0;
+      const int all = p.G * nm;
+      t.f0 = (int)((long long)all * chunk / p.sink_items);
+      t.T = (int)((long long)all * (chunk + 1) / p.sink_items) - t.f0;
+    }
+  } else {
+    const int first = max(0, t.nb * 128 - t.base);
+    const int reach = min(last, t.nb * 128 + 127 + p.window - 1 - t.base);
+    if (t.nb * 128 < t.len && first <= reach) {
+      t.m0 = first >> 7;
+      t.nm = (reach >> 7) - t.m0 + 1;
+      t.T = p.G * t.nm;
+    }
+  }
+  return t;
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(kDkvThreads, 1)
+window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  constexpr int NS = kDkvStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* sK = smem_raw;
+  uint8_t* sV = sK + kTile;
+  uint8_t* sRing = sV + kTile;
+  float* sStats = reinterpret_cast<float*>(sRing + NS * kTile);  // [slot][0: lse_log2, 1: delta][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStats) + kStatSlots * 1024);
+  uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(bars + 32);
+  volatile int& s_abort = *reinterpret_cast<volatile int*>(bars + 33);
+  if ((smem_u32(smem_raw) & 1023u) != 0) {
+    if (threadIdx.x == 0 && atomicCAS(p.status, 0, (int)kStatusBadIndex) == 0) p.status[2] = 994;
+    return;
+  }
+  const uint32_t bar_base = smem_u32(bars);
+  auto BAR = [&](int i) { return bar_base + (uint32_t)i * 8u; };
+  constexpr int kKvFull = 0, kKvEmpty = 1, kRFull = 2, kREmpty = 2 + NS, kSFull = 2 + 2 * NS, kSFree = kSFull + 1,
+                kDpFull = kSFree + 1, kPFull = kDpFull + 1, kDsFull = kPFull + 1, kGFree = kDsFull + 1,
+                kFinal = kGFree + 1, kFree = kFinal + 1, kNumBars = kFree + 1;
+  static_assert(kNumBars <= 32, "barrier slots");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  WaitCtx wctx{&s_abort, p.status};
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(BAR(kKvFull), 1);
+    mbar_init(BAR(kKvEmpty), 2);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(BAR(kRFull + i), 1);
+      mbar_init(BAR(kREmpty + i), 2);
+    }
+    mbar_init(BAR(kSFull), 1);
+    mbar_init(BAR(kDpFull), 1);
+    mbar_init(BAR(kSFree), 256);
+    mbar_init(BAR(kPFull), 256);
+    mbar_init(BAR(kDsFull), 256);
+    mbar_init(BAR(kGFree), 1);
+    mbar_init(BAR(kFinal), 2);
+    mbar_init(BAR(kFree), 256);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&s_tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem_base;
+  const uint32_t tS = tmem, tG = tmem + 128u, tdV = tmem + 256u, tdK = tmem + 384u;
+  const int num_work = p.B * p.Hkv * (p.Nkv + p.sink_items);
+
+  if (warp == kDkvLoadWarp) {
+    uint32_t r_cnt = 0, kv_cnt = 0, tile_cnt = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const DkvItem t = dkv_item(p, w);
+      if (t.T == 0) continue;
+      ok = mbar_wait(BAR(kKvEmpty), (kv_cnt & 1) ^ 1, wctx, 500);
+      if (!ok) break;
+      ++kv_cnt;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(BAR(kKvFull), 2 * kTile);
+        for (int sl = 0; sl < 2; ++sl) {
+          tma_load_4d(smem_u32(sK + sl * kSlab), &tm_k, BAR(kKvFull), sl * 64, t.nb * 128, t.hkv, t.b);
+          tma_load_4d(smem_u32(sV + sl * kSlab), &tm_v, BAR(kKvFull), sl * 64, t.nb * 128, t.hkv, t.b);
+        }
+      }
+      for (int i = 0; i < t.T && ok; ++i) {
+        const int f = t.f0 + i;
+        const int hq = t.hkv * p.G + f / t.nm, m = t.m0 + f % t.nm;
+        for (int which = 0; which < 2; ++which) {
+          const uint32_t stage = r_cnt % NS, ph = (r_cnt / NS) & 1;
+          ok = mbar_wait(BAR(kREmpty + stage), ph ^ 1, wctx, 501);
+          if (!ok) break;
+          if (lane == 0) {
+            const CUtensorMap* tm = which ? &tm_do : &tm_q;
+            mbar_arrive_expect_tx(BAR(kRFull + stage), kTile + (which ? 1024 : 0));
+            for (int sl = 0; sl < 2; ++sl)
+              tma_load_4d(smem_u32(sRing + stage * kTile + sl * kSlab), tm, BAR(kRFull + stage), sl * 64, m * 128, hq, t.b);
+            if (which) {
+              // the rows' statistics travel with their dO tile: its stage is re-used only after dK of the tile two
+              // back, when the statistics slot of that tile is long free (two slots)
+              float* st = sStats + (tile_cnt % kStatSlots) * 256;
+              const long long at = ((long long)t.b * p.Hq + hq) * ((long long)p.Nq * 128) + (long long)m * 128;
+              bulk_load_1d(smem_u32(st), p.lse_log2 + at, 512, BAR(kRFull + stage));
+              bulk_load_1d(smem_u32(st + 128), p.delta + at, 512, BAR(kRFull + stage));
+            }
+          }
+          ++r_cnt;
+        }
+        ++tile_cnt;
+      }
+    }
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // issuer 0: S^T_i = K Q_i^T one tile ahead of the compute threads, and dV += P^T_i dO_i;
+    // issuer 1: the chain through region G: dP^T_i = V dO_i^T, dK += dS^T_i Q_i, then (once dV_i has read G) dP^T_{i+1}
+    const int who = warp - kMmaWarp;
+    const uint32_t led = lane == 0;
+    uint32_t r_cnt = 0, kv_cnt = 0, in_cnt = 0, ds_cnt = 0, free_cnt = 0;
+    bool ok = true, first_item = true;
+    const uint64_t k_desc = desc_k_major(smem_u32(sK)), v_desc = desc_k_major(smem_u32(sV));
+    const uint64_t ring_k = desc_k_major(smem_u32(sRing)), ring_mn = desc_mn_major(smem_u32(sRing));
+    const int ksteps = p.D / 16;
+    const uint32_t idesc_n = Idesc<F16>::kmn(p.D);
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const int T = dkv_item(p, w).T;
+      if (T == 0) continue;
+      ok = mbar_wait(BAR(kKvFull), kv_cnt & 1, wctx, 510);
+      if (!ok) break;
+      ++kv_cnt;
+      const uint32_t base = r_cnt;  // Q_i at base + 2i, dO_i at base + 2i + 1
+      auto stage_of = [&](uint32_t pos) { return pos % NS; };
+      auto wait_full = [&](uint32_t pos) { return mbar_wait(BAR(kRFull + stage_of(pos)), (pos / NS) & 1, wctx, 511); };
+      auto wait_free = [&]() -> bool {  // the previous item's epilogue has drained the accumulators
+        if (first_item) return true;
+        const bool r = mbar_wait(BAR(kFree), free_cnt & 1, wctx, 515);
+        ++free_cnt;
+        return r;
+      };
+      if (who == 0) {
+        auto issue_st = [&](int i) -> bool {
+          if (!wait_full(base + 2 * i)) return false;
+          if (in_cnt > 0 && !mbar_wait(BAR(kSFree), (in_cnt - 1) & 1, wctx, 512)) return false;
+          ++in_cnt;
+          tc_fence_after();
+          const uint32_t sq = stage_of(base + 2 * i);
+          mma_ss_kk(tS, k_desc, ring_k + sq * kTileStep, Idesc<F16>::kKK, led, ksteps);
+          umma_commit_led(BAR(kSFull), led);
+          umma_commit_led(BAR(kREmpty + sq), led);
+          __syncwarp();
+          return true;
+        };
+        ok = issue_st(0);
+        for (int i = 0; i < T && ok; ++i) {
+          if (i + 1 < T) ok = issue_st(i + 1);
+          if (ok) ok = wait_full(base + 2 * i + 1);
+          if (!ok) break;
+          ok = mbar_wait(BAR(kPFull), ds_cnt & 1, wctx, 513);
+          ++ds_cnt;
+          if (ok && i == 0) ok = wait_free();
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sd = stage_of(base + 2 * i + 1);
+          mma_ts_kmn(tdV, tG, tG + 64u, ring_mn + sd * kTileStep, i > 0, led, idesc_n);
+          umma_commit_led(BAR(kREmpty + sd), led);
+          umma_commit_led(BAR(kGFree), led);
+          __syncwarp();
+        }
+      } else {
+        auto issue_dp = [&](int i) -> bool {
+          if (!wait_full(base + 2 * i)) return false;
+          if (!wait_full(base + 2 * i + 1)) return false;
+          const uint32_t sd = stage_of(base + 2 * i + 1);
+          mma_ss_kk(tG, v_desc, ring_k + sd * kTileStep, Idesc<F16>::kKK, led, ksteps);
+          umma_commit_led(BAR(kDpFull), led);
+          umma_commit_led(BAR(kREmpty + sd), led);
+          __syncwarp();
+          return true;
+        };
+        ok = issue_dp(0);
+        for (int i = 0; i < T && ok; ++i) {
+          ok = mbar_wait(BAR(kDsFull), ds_cnt & 1, wctx, 514);
+          ++ds_cnt;
+          if (ok && i == 0) ok = wait_free();
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sq = stage_of(base + 2 * i);
+          mma_ts_kmn(tdK, tG + 32u, tG + 96u, ring_mn + sq * kTileStep, i > 0, led, idesc_n);
+          umma_commit_led(BAR(kREmpty + sq), led);
+          __syncwarp();
+          ok = mbar_wait(BAR(kGFree), in_cnt & 1, wctx, 516);  // dV_i has read region G as well
+          ++in_cnt;
+          if (ok && i + 1 < T) ok = issue_dp(i + 1);
+        }
+      }
+      if (!ok) break;
+      umma_commit_led(BAR(kFinal), led);
+      umma_commit_led(BAR(kKvEmpty), led);
+      __syncwarp();
+      r_cnt += 2 * T;
+      first_item = false;
+    }
+  } else if (warp < 8) {
+    const int grp = warp >> 2;
+    const int row = threadIdx.x & 127;  // key inside the tile = tensor-memory lane
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t s_cnt = 0, dp_cnt = 0, fin_cnt = 0, tile_cnt = 0, r_cnt = 0;
+    const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2);
+    const int cols = p.D - grp * 64;
+    bool ok = true;
+    for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
+      const DkvItem t = dkv_item(p, w);
+      const uint32_t base = r_cnt;
+      r_cnt += 2 * t.T;
+      const int kv = t.nb * 128 + row;
+      // query positions [kv, see_hi) see this key
+      const int see_hi = kv < p.sinks ? t.len : min(t.len, kv + p.window);
+      int m = t.m0 + t.f0 % t.nm;
+      for (int i = 0; i < t.T && ok; ++i) {
+        const float4* st_l = reinterpret_cast<const float4*>(sStats + (tile_cnt % kStatSlots) * 256 + grp * 64);
+        const float4* st_d = reinterpret_cast<const float4*>(sStats + (tile_cnt % kStatSlots) * 256 + 128 + grp * 64);
+        ++tile_cnt;
+        const int p0 = t.base + m * 128;  // position of the query tile's first row
+        if (++m == t.m0 + t.nm) m = t.m0;
+        ok = mbar_wait(BAR(kSFull), s_cnt & 1, wctx, 520);
+        if (!ok) break;
+        ++s_cnt;
+        const uint32_t pos = base + 2 * (uint32_t)i + 1;  // dO_i, whose barrier also brings the statistics
+        ok = mbar_wait(BAR(kRFull + pos % NS), (pos / NS) & 1, wctx, 523);
+        if (!ok) break;
+        tc_fence_after();
+        float pr[64];
+        {
+          uint32_t* u = reinterpret_cast<uint32_t*>(pr);
+          tmem_ld32(tS + lane_base + grp * 64, u);
+          tmem_ld32(tS + lane_base + grp * 64 + 32, u + 32);
+          tmem_wait_ld();
+        }
+        tc_fence_before();
+        mbar_arrive(BAR(kSFree));
+#pragma unroll
+        for (int c4 = 0; c4 < 16; ++c4) {
+          const float4 l = st_l[c4];  // negated
+          float x0, x1, x2, x3;
+          unpack2(ffma2(pack2(pr[c4 * 4 + 0], pr[c4 * 4 + 1]), sc2, pack2(l.x, l.y)), x0, x1);
+          unpack2(ffma2(pack2(pr[c4 * 4 + 2], pr[c4 * 4 + 3]), sc2, pack2(l.z, l.w)), x2, x3);
+          pr[c4 * 4 + 0] = ex2_approx(x0);
+          pr[c4 * 4 + 1] = ex2_approx(x1);
+          pr[c4 * 4 + 2] = ex2_approx(x2);
+          pr[c4 * 4 + 3] = ex2_approx(x3);
+        }
+        const bool whole = p0 >= t.nb * 128 + 127 && p0 + 127 < t.len && p0 + 127 < t.nb * 128 + p.window;
+        uint32_t mw[2] = {0xffffffffu, 0xffffffffu};
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) mw[h] = range_word(kv - p0 - grp * 64, see_hi - p0 - grp * 64, h);
+        }
+        ok = mbar_wait(BAR(kDpFull), dp_cnt & 1, wctx, 521);
+        if (!ok) break;
+        ++dp_cnt;
+        tc_fence_after();
+        if (p0 < 0 || p0 + 127 >= t.len) {
+          // query rows that take no part: dV contracts over the dO rows and dK over the Q rows (both tiles have been
+          // read by S^T_i and dP^T_i; their stages are held until dV_i and dK_i)
+          const int at = p0 + row;
+          if (at < 0 || at >= t.len) {
+            uint4* z0 = reinterpret_cast<uint4*>(sRing + (pos % NS) * kTile + grp * kSlab + row * 128);
+            uint4* z1 = reinterpret_cast<uint4*>(sRing + ((pos - 1) % NS) * kTile + grp * kSlab + row * 128);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              z0[c] = make_uint4(0, 0, 0, 0);
+              z1[c] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        uint32_t dp[64];
+        tmem_ld32(tG + lane_base + grp * 64, dp);
+        tmem_ld32(tG + lane_base + grp * 64 + 32, dp + 32);
+        tmem_wait_ld();
+        // dP^T_i is in registers: this thread's 64 columns of region G take P^T_i (first 32) and dS^T_i (last 32)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pk[e] = pack16<F16>(pr[16 * h + 2 * e], pr[16 * h + 2 * e + 1]);
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pk[e] &= pair_mask(mw[h >> 1], (16 * h + 2 * e) & 31);
+          }
+          tmem_st8(tG + lane_base + grp * 64 + h * 8, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(BAR(kPFull));
+        {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c4 = 0; c4 < 16; ++c4) {
+            const float4 d = st_d[c4];  // negated
+            float d0, d1, d2, d3;
+            unpack2(fmul2(pack2(pr[c4 * 4 + 0], pr[c4 * 4 + 1]),
+                          fadd2(pack2(__uint_as_float(dp[c4 * 4 + 0]), __uint_as_float(dp[c4 * 4 + 1])), pack2(d.x, d.y))),
+                    d0, d1);
+            unpack2(fmul2(pack2(pr[c4 * 4 + 2], pr[c4 * 4 + 3]),
+                          fadd2(pack2(__uint_as_float(dp[c4 * 4 + 2]), __uint_as_float(dp[c4 * 4 + 3])), pack2(d.z, d.w))),
+                    d2, d3);
+            pk[c4 * 2] = pack16<F16>(d0, d1);
+            pk[c4 * 2 + 1] = pack16<F16>(d2, d3);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pk[e] &= pair_mask(mw[e >> 4], (2 * e) & 31);
+          }
+          tmem_st32(tG + lane_base + grp * 64 + 32, pk);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(BAR(kDsFull));
+      }
+      if (!ok) break;
+      // ---- epilogue
+      const bool to_slot = t.slot >= 0 && row < p.sinks;
+      const bool to_row = !t.extra && !to_slot && kv < p.Sk && cols > 0;
+      float* part = p.partial;
+      if (to_slot)
+        part += ((((long long)t.b * p.Hkv + t.hkv) * (p.sink_items + 1) + t.slot) * 2 * p.sinks + row) * p.D + grp * 64;
+      uint8_t* dk_row = p.dk + (t.b * p.dk_stride[0] + t.hkv * p.dk_stride[1] + (long long)kv * p.dk_stride[2] + grp * 64) * 2;
+      uint8_t* dv_row = p.dv + (t.b * p.dv_stride[0] + t.hkv * p.dv_stride[1] + (long long)kv * p.dv_stride[2] + grp * 64) * 2;
+      uint32_t acc[64];
+      if (t.T > 0) {
+        ok = mbar_wait(BAR(kFinal), fin_cnt & 1, wctx, 522);
+        if (!ok) break;
+        ++fin_cnt;
+        tc_fence_after();
+        tmem_ld32(tdV + lane_base + grp * 64, acc);
+        tmem_ld32(tdV + lane_base + grp * 64 + 32, acc + 32);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) acc[c] = 0u;
+      }
+      if (to_row) store_half<F16>(dv_row, acc, 1.0f, cols);
+      if (to_slot) store_half_f32(part + (long long)p.sinks * p.D, acc, cols);
+      if (t.T > 0) {
+        __syncwarp();
+        tmem_ld32(tdK + lane_base + grp * 64, acc);
+        tmem_ld32(tdK + lane_base + grp * 64 + 32, acc + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(BAR(kFree));
+      }
+      if (to_row) store_half<F16>(dk_row, acc, p.softmax_scale, cols);
+      if (to_slot) store_half_f32(part, acc, cols);
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// 4. dK and dV of the sinks: the slots' sums in order.  One thread per element.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+window_bwd_reduce_kernel(const Params p) {
+  const int per = 2 * p.sinks * p.D;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)p.B * p.Hkv * per) return;
+  const int e = (int)(i % per), bh = (int)(i / per);
+  const int d = e % p.D, row = (e / p.D) % p.sinks, which = e / (p.D * p.sinks);
+  if (row >= p.Sk) return;
+  const int slots = p.sink_items + 1;
+  const float* src = p.partial + (long long)bh * slots * per + e;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < slots; ++s) sum += src[(long long)s * per];
+  const int hkv = bh % p.Hkv, b = bh / p.Hkv;
+  const long long* st = which ? p.dv_stride : p.dk_stride;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(which ? p.dv : p.dk) + b * st[0] + hkv * st[1] + row * st[2] + d;
+  if (!which) sum *= p.softmax_scale;
+  *dst = (uint16_t)(pack16<F16>(sum, 0.f) & 0xffffu);
+}
+
+// Split of the sinks' query tiles: first tile beyond the reach of tile 0's windows, and the number of further items.
+static void sink_split(int Hq, int Hkv, int Sq, int Sk, int window, int sinks, int* m0, int* items) {
+  const int Nq = (Sq + 127) / 128, G = Hq / Hkv;
+  const long long reach = 127LL + window - 1 - ((long long)Sk - Sq);
+  *m0 = reach < 0 ? 0 : (int)((reach >> 7) + 1 < Nq ? (reach >> 7) + 1 : Nq);
+  *items = 0;
+  if (sinks <= 0 || *m0 >= Nq) return;
+  const long long pairs = (long long)G * (Nq - *m0);
+  long long per = (long long)G * ((long long)window / 128 + 2);  // pairs of an ordinary item
+  if (per < 16) per = 16;                                         // (below that the prologue and the slot's stores show)
+  long long n = (pairs + per - 1) / per;
+  *items = (int)(n > 128 ? 128 : n);
+}
+
+template <bool F16>
+static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq, const CUtensorMap& tdo,
+                  const CUtensorMap& tk, const CUtensorMap& tv, float* lse_log2, float* delta, int num_sms, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(window_dq_kernel<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(window_dkv_kernel<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDkvSmem);
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "bsa_window_bwd: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
+  window_bwd_pre_kernel<F16><<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
+      static_cast<const uint8_t*>(a.out), static_cast<const uint8_t*>(a.dout), a.lse, lse_log2, delta, a.o_stride[0],
+      a.o_stride[1], a.o_stride[2], a.do_stride[0], a.do_stride[1], a.do_stride[2], p.Hq, p.Sq, p.Nq * 128, rows_pad, p.D);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward preprocess launch: %s", cudaGetErrorString(e));
+  const int work_q = p.B * p.Hq * p.Nq, work_kv = p.B * p.Hkv * (p.Nkv + p.sink_items);
+  window_dq_kernel<F16><<<work_q < num_sms ? work_q : num_sms, kDqThreads, kDqSmem, st>>>(tq, tdo, tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window dQ launch: %s", cudaGetErrorString(e));
+  window_dkv_kernel<F16><<<work_kv < num_sms ? work_kv : num_sms, kDkvThreads, kDkvSmem, st>>>(tq, tdo, tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window dK/dV launch: %s", cudaGetErrorString(e));
+  if (p.sink_items > 0) {
+    const long long n = (long long)p.B * p.Hkv * 2 * p.sinks * p.D;
+    window_bwd_reduce_kernel<F16><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward reduce launch: %s", cudaGetErrorString(e));
+  }
+  return BSA_OK;
+}
+
+}  // namespace winbwd
+}  // namespace bsa
+
+using namespace bsa;
+
+extern "C" int64_t bsa_window_bwd_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t D,
+                                                  int32_t window, int32_t sinks) {
+  if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || Sq < 1 || Sk < 1 || D < 1 || window < 1 || sinks < 0) return 0;
+  int m0, items;
+  winbwd::sink_split(Hq, Hkv, Sq, Sk, window < kWindowAll ? window : kWindowAll, sinks, &m0, &items);
+  const int64_t rows = (int64_t)B * Hq * ((Sq + 127) / 128) * 128;
+  const int64_t part = items > 0 ? (int64_t)B * Hkv * (items + 1) * 2 * sinks * D : 0;
+  return (2 * rows + part) * (int64_t)sizeof(float);
+}
+
+extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
+  if (!a) return set_error(BSA_ERR_INVALID, "bsa_window_bwd: null args");
+  if (a->dtype != BSA_DTYPE_BF16 && a->dtype != BSA_DTYPE_F16)
+    return set_error(BSA_ERR_INVALID, "bsa_window_bwd: dtype must be bf16 or f16");
+  if (a->D != 64 && a->D != 96 && a->D != 128)
+    return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_bwd: head dimension %d not built (64, 96 or 128)", a->D);
+  if (a->B < 1 || a->Hq < 1 || a->Hkv < 1 || a->Sq < 1 || a->Sk < 1) return set_error(BSA_ERR_INVALID, "bsa_window_bwd: non-positive extent");
+  if (a->Hq % a->Hkv != 0) return set_error(BSA_ERR_INVALID, "bsa_window_bwd: Hq %% Hkv != 0");
+  if (a->Sq > (1 << 29) || a->Sk > (1 << 29)) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_bwd: length out of [1, 2^29]");
+  if (!a->dout || !a->q || !a->k || !a->v || !a->out || !a->lse || !a->dq || !a->dk || !a->dv || !a->workspace || !a->status)
+    return set_error(BSA_ERR_INVALID, "bsa_window_bwd: null pointer");
+  if (a->window < 1 || a->sinks < 0 || a->sinks > kMaxSinks)
+    return set_error(BSA_ERR_INVALID, "bsa_window_bwd: window must be >= 1 and sinks in [0, %d]", kMaxSinks);
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.0e38f)
+    return set_error(BSA_ERR_INVALID, "bsa_window_bwd: softmax_scale must be positive and finite");
+  const int64_t need = bsa_window_bwd_workspace_bytes(a->B, a->Hq, a->Hkv, a->Sq, a->Sk, a->D, a->window, a->sinks);
+  if (a->workspace_bytes < need) return set_error(BSA_ERR_WORKSPACE, "bsa_window_bwd: workspace of %lld bytes needed", (long long)need);
+  for (int i = 0; i < 3; ++i)
+    if ((a->dq_stride[i] | a->dk_stride[i] | a->dv_stride[i] | a->o_stride[i] | a->do_stride[i]) % 8 != 0)
+      return set_error(BSA_ERR_INVALID, "bsa_window_bwd: strides must be multiples of 8 elements");
+  {
+    const void* vec16[6] = {a->out, a->dout, a->dq, a->dk, a->dv, a->workspace};
+    const char* names[6] = {"out", "dout", "dq", "dk", "dv", "workspace"};
+    for (int i = 0; i < 6; ++i)
+      if ((reinterpret_cast<uintptr_t>(vec16[i]) & 15u) != 0)
+        return set_error(BSA_ERR_INVALID, "%s: base address must be 16-byte aligned", names[i]);
+  }
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int num_sms = bsa_num_sms(dev);
+  if (num_sms <= 0) return set_error(BSA_ERR_CUDA, "bsa_window_bwd: cannot query the SM count");
+
+  winbwd::Params p{};
+  p.kv_lens = a->kv_lens;
+  p.dq = static_cast<uint8_t*>(a->dq);
+  p.dk = static_cast<uint8_t*>(a->dk);
+  p.dv = static_cast<uint8_t*>(a->dv);
+  p.status = a->status;
+  for (int i = 0; i < 3; ++i) {
+    p.dq_stride[i] = a->dq_stride[i];
+    p.dk_stride[i] = a->dk_stride[i];
+    p.dv_stride[i] = a->dv_stride[i];
+  }
+  p.B = a->B;
+  p.Hq = a->Hq;
+  p.Hkv = a->Hkv;
+  p.G = a->Hq / a->Hkv;
+  p.Sq = a->Sq;
+  p.Sk = a->Sk;
+  p.Nq = (a->Sq + 127) / 128;
+  p.Nkv = (a->Sk + 127) / 128;
+  p.D = a->D;
+  p.window = a->window < kWindowAll ? a->window : kWindowAll;
+  p.sinks = a->sinks;
+  winbwd::sink_split(a->Hq, a->Hkv, a->Sq, a->Sk, p.window, a->sinks, &p.sink_m0, &p.sink_items);
+  p.softmax_scale = a->softmax_scale;
+  p.scale_log2 = a->softmax_scale * kLog2e;
+  const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
+  if (rows_pad / 64 >= 0x7fffffffLL || (long long)p.B * p.Hkv * (p.Nkv + p.sink_items) > 0x7fffffffLL ||
+      (long long)p.G * p.Nq > 0x3fffffffLL)
+    return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_bwd: too many tiles");
+  float* lse_log2 = static_cast<float*>(a->workspace);
+  float* delta = lse_log2 + rows_pad;
+  p.lse_log2 = lse_log2;
+  p.delta = delta;
+  p.partial = delta + rows_pad;
+
+  const CUtensorMapDataType dt = a->dtype == BSA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap tq, tdo, tk, tv;
+  {
+    uint64_t qd[4] = {(uint64_t)a->D, (uint64_t)a->Sq, (uint64_t)a->Hq, (uint64_t)a->B};
+    uint64_t kd[4] = {(uint64_t)a->D, (uint64_t)a->Sk, (uint64_t)a->Hkv, (uint64_t)a->B};
+    uint32_t box[4] = {64, 128, 1, 1};
+    auto map = [&](CUtensorMap* m, const void* base, const int64_t* s, const uint64_t* dims, const char* name) {
+      uint64_t sb[3] = {(uint64_t)s[2] * 2, (uint64_t)s[1] * 2, (uint64_t)s[0] * 2};
+      return make_tensor_map(m, dt, 4, base, dims, sb, box, name);
+    };
+    int rc;
+    if ((rc = map(&tq, a->q, a->q_stride, qd, "q"))) return rc;
+    if ((rc = map(&tdo, a->dout, a->do_stride, qd, "dout"))) return rc;
+    if ((rc = map(&tk, a->k, a->k_stride, kd, "k"))) return rc;
+    if ((rc = map(&tv, a->v, a->v_stride, kd, "v"))) return rc;
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  if (a->dtype == BSA_DTYPE_F16) return winbwd::launch<true>(*a, p, tq, tdo, tk, tv, lse_log2, delta, num_sms, st);
+  return winbwd::launch<false>(*a, p, tq, tdo, tk, tv, lse_log2, delta, num_sms, st);
+}

@@ -288,6 +288,155 @@ typedef struct bsa_bwd_args {
 int bsa_bwd(const bsa_bwd_args* args, void* cuda_stream);
 int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, int32_t D);
 
+/*
+ * Causal sliding-window attention with sink tokens.  The reference has no counterpart.
+ *
+ * Keys sit at positions 0..len-1 of their sequence, query row i at position p = base + i.  Key j is visible iff
+ *   0 <= p < len,  j <= p,  and (j > p - window  or  j < sinks).
+ * Rows that see nothing give out = 0, lse = -inf.  Layouts as in bsa_fwd (strides in elements, innermost contiguous).
+ *
+ * Contiguous keys (page_table == NULL): k, v [B, Hkv, Sk, D]; len = kv_lens[b] (NULL: Sk); base = Sk - Sq.
+ * Paged keys: k, v [num_pages, Hkv, page_size, D]; the token at position j of sequence b lies in page
+ *   page_table[b][j / page_size] at row j % page_size; len = kv_lens[b], at most max_pages * page_size; base =
+ *   len - Sq, i.e. the Sq query tokens are the newest tokens of the sequence and their keys are in the cache
+ *   already.  Tokens whose table entry is outside [0, num_pages) are not visible.
+ * tree_mask [B, Sq] (paged, Sq <= 64): bit u of word t = draft u (the key at base + u) is visible to draft t.  The
+ *   draft's position is then base + popcount - 1, that of a key u likewise; word 0 marks an unused slot (out = 0).
+ *
+ * pack_gqa != 0: the rows of a tile are floor(128 / G) tokens x the G heads of a KV head.
+ * splits > 1: the key tiles of a query tile are dealt to `splits` CTAs; partial_o [splits, B, Hq, Sq, D] and
+ * partial_lse [splits, B, Hq, Sq] f32 hold their results, which a second launch of the same call joins.
+ * D = 64, 96 or 128; window >= 1 (2^29 and more: everything before the row); 0 <= sinks <= 128;
+ * softmax_scale > 0; page_size 16, 32, 64 or a multiple of 128; lengths up to 2^29.
+ */
+typedef struct bsa_window_fwd_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse; /* [B, Hq, Sq] or NULL */
+  const int32_t* kv_lens;
+  const int32_t* page_table;
+  const int64_t* tree_mask;
+  float* partial_o;
+  float* partial_lse;
+  int32_t* status;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int32_t dtype; /* BSA_DTYPE_BF16 or BSA_DTYPE_F16 */
+  int32_t B, Hq, Hkv, Sq, Sk, D;
+  int32_t window;
+  int32_t sinks;
+  int32_t max_pages;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t pack_gqa;
+  int32_t splits;
+  float softmax_scale;
+} bsa_window_fwd_args;
+
+int bsa_window_fwd(const bsa_window_fwd_args* args, void* cuda_stream);
+
+/*
+ * Backward of the contiguous form of bsa_window_fwd: dQ, dK, dV from dO, Q, K, V, O, LSE; the gradients of a KV head
+ * sum over its G query heads.  No atomics: repeated calls are bit-identical.  Gradients of rows and keys that take no
+ * part are zero.  workspace: bsa_window_bwd_workspace_bytes(...) bytes of device memory, contents unspecified on entry.
+ */
+typedef struct bsa_window_bwd_args {
+  const void* dout;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* out;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  const int32_t* kv_lens;
+  void* workspace;
+  int32_t* status;
+  int64_t workspace_bytes;
+  int64_t do_stride[3];
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+  int32_t dtype;
+  int32_t B, Hq, Hkv, Sq, Sk, D;
+  int32_t window;
+  int32_t sinks;
+  float softmax_scale;
+  int32_t reserved;
+} bsa_window_bwd_args;
+
+int bsa_window_bwd(const bsa_window_bwd_args* args, void* cuda_stream);
+int64_t bsa_window_bwd_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t D,
+                                       int32_t window, int32_t sinks);
+
+/*
+ * Ancestor masks of trees of drafts: parents [B, T] int32 (T <= 64; -1 = child of the last committed token, otherwise
+ * an earlier draft) -> mask [B, T] int64, bit u of word t set iff u is t or an ancestor of t.  A draft whose parent is
+ * neither (parent < -1 or >= t), or whose ancestor is such a draft, gets mask 0: an unused slot.
+ */
+int bsa_tree_mask(const int32_t* parents, int32_t B, int32_t T, int64_t* mask, void* cuda_stream);
+
+/*
+ * Writes of a paged cache (pages as in bsa_window_fwd, 16-bit elements, D a multiple of 8, all rows 16-byte aligned).
+ *   bsa_cache_append: k, v [B, H, T, D] -> positions lens[b] - T .. lens[b] - 1 of every sequence.  Tokens at negative
+ *                     positions or whose page is not in the pool are dropped.
+ *   bsa_cache_keep:   the last T tokens of a sequence are drafts; the accepted ones, path[b][0..path_lens[b]) (draft
+ *                     numbers, ascending), move to positions lens[b] - T, lens[b] - T + 1, ...; new_lens[b] =
+ *                     lens[b] - T + the number kept.  A path ends at its first entry that is not ascending or not in
+ *                     [0, T).  A sequence with lens[b] < T keeps its length and is not touched.
+ * A page must not be written through two sequences' tables in one call.
+ */
+int bsa_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int64_t k_stride[3],
+                     const int64_t v_stride[3], const int64_t kc_stride[3], const int64_t vc_stride[3],
+                     const int32_t* page_table, const int32_t* lens, int32_t B, int32_t H, int32_t T, int32_t D,
+                     int32_t max_pages, int32_t page_size, int32_t num_pages, void* cuda_stream);
+int bsa_cache_keep(void* k_cache, void* v_cache, const int64_t kc_stride[3], const int64_t vc_stride[3],
+                   const int32_t* page_table, const int32_t* lens, const int32_t* path, const int32_t* path_lens,
+                   int32_t* new_lens, int32_t B, int32_t H, int32_t T, int32_t path_cap, int32_t D, int32_t max_pages,
+                   int32_t page_size, int32_t num_pages, void* cuda_stream);
+
+/*
+ * Rotary positions with several axes.  Pair p of a head (p < P = axis_pairs[0] + ... + axis_pairs[A-1]) turns by
+ *   angle = positions[b, s, axis of p] * inv_freq[p]   (sign changed when inverse != 0),
+ *   (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos),
+ * with (x0, x1) = (x[2p], x[2p+1]) when interleaved != 0, else (x[p], x[P+p]); channels from 2P on are copied.
+ * Angles are reduced in 64 bits, so far positions keep their fraction.  One launch serves q [B, Hq, S, D] and k
+ * [B, Hk, S, D] (Hk = 0: none); outputs may be the inputs themselves.
+ *   positions int32, element strides pos_stride (batch, token), axes contiguous; A <= 4; D even, at most 512.
+ */
+enum bsa_rotary_dtype { BSA_ROTARY_BF16 = 0, BSA_ROTARY_F16 = 2, BSA_ROTARY_F32 = 3 };
+typedef struct bsa_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const int32_t* positions;
+  const float* inv_freq; /* [P] */
+  int64_t q_stride[3];   /* batch, head, token */
+  int64_t k_stride[3];
+  int64_t qo_stride[3];
+  int64_t ko_stride[3];
+  int64_t pos_stride[2];
+  int32_t axis_pairs[4];
+  int32_t num_axes;
+  int32_t dtype; /* enum bsa_rotary_dtype */
+  int32_t B, Hq, Hk, S, D;
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t reserved;
+} bsa_rotary_args;
+
+int bsa_rotary_nd(const bsa_rotary_args* args, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,212 @@
+"""GPU parity of sliding-window attention with sinks (forward, backward) against a plain 64-bit implementation."""
+import math
+
+import pytest
+import torch
+
+from plain_ops import assert_close_norm, assert_within, attend, gradients, half_step, visible
+
+pytestmark = pytest.mark.gpu
+
+
+def make(B, Hq, Hkv, Sq, Sk, D, dtype, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q, do = ((torch.randn(B, Hq, Sq, D, generator=g) * spread).to(dtype) for _ in range(2))
+    k, v = ((torch.randn(B, Hkv, Sk, D, generator=g) * spread).to(dtype) for _ in range(2))
+    return q, k, v, do
+
+
+def masks(B, Sq, Sk, window, sinks, lens):
+    return torch.stack([visible(Sq, Sk, window, sinks, Sk if lens is None else lens[b]) for b in range(B)])
+
+
+def poison(t, lens, offset):
+    """Fills the tokens at positions >= lens[b] of [B, H, S, D] with NaN (token i is at i + offset)."""
+    t = t.clone()
+    for b, n in enumerate(lens):
+        t[b, :, max(0, n - offset):] = float("nan")
+    return t
+
+
+BF, HF = torch.bfloat16, torch.float16
+# B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens
+CASES = [
+    (1, 1, 1, 1, 1, 128, BF, 1, 0, None),
+    (1, 2, 1, 1, 200, 64, HF, 64, 3, None),
+    (2, 2, 2, 127, 127, 128, BF, 1, 0, None),          # every row sees itself only
+    (1, 2, 2, 128, 128, 96, BF, 128, 128, None),
+    (1, 4, 2, 129, 129, 128, HF, 100, 1, None),
+    (1, 2, 2, 640, 640, 128, BF, 256, 4, None),         # window of whole tiles
+    (1, 3, 1, 700, 700, 64, BF, 130, 100, None),        # three heads a KV head
+    (2, 4, 4, 513, 513, 96, HF, 77, 0, [513, 200]),     # padded batch
+    (3, 2, 1, 300, 300, 128, BF, 150, 5, [0, 1, 299]),  # sequences of no and of one token
+    (1, 6, 2, 50, 900, 128, BF, 300, 4, None),          # a chunk behind a long past, packed heads, split keys
+    (2, 5, 1, 33, 1000, 64, HF, 1 << 20, 0, [1000, 980]),   # five heads a KV head, window longer than all
+    (1, 1, 1, 200, 100, 128, BF, 40, 2, None),          # queries before the first key
+    (1, 2, 2, 1300, 1300, 128, BF, 1, 128, None),       # sinks only, and the row itself
+    (1, 4, 1, 1100, 1100, 64, HF, 200, 2, None),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+@pytest.mark.parametrize("layout", ["bhsd", "bshd"])
+def test_forward(case, layout):
+    from block_sparse_attention import window_attn_fwd
+    B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens = case
+    q, k, v, _ = make(B, Hq, Hkv, Sq, Sk, D, dtype)
+    ref, lse, tol, lse_tol, _, _ = attend(q.double(), k.double(), v.double(), masks(B, Sq, Sk, window, sinks, lens), D ** -0.5, dtype)
+    if lens is not None:
+        k, v, q = poison(k, lens, 0), poison(v, lens, 0), poison(q, lens, Sk - Sq)
+    qc, kc, vc = (t.cuda() if layout == "bhsd" else t.transpose(1, 2).contiguous().cuda() for t in (q, k, v))
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32).cuda()
+    out, got_lse = window_attn_fwd(qc, kc, vc, window, sinks, kv_lens=n, return_lse=True, layout=layout)
+    out = out if layout == "bhsd" else out.transpose(1, 2)
+    assert_within(out, ref, tol, "out")
+    assert_within(got_lse, lse, lse_tol, "lse")
+    out2, none = window_attn_fwd(qc, kc, vc, window, sinks, kv_lens=n, layout=layout)
+    assert none is None and torch.equal(out2 if layout == "bhsd" else out2.transpose(1, 2), out)
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+def test_backward(case):
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens = case
+    q, k, v, do = make(B, Hq, Hkv, Sq, Sk, D, dtype, seed=1)
+    mask = masks(B, Sq, Sk, window, sinks, lens)
+    refs, tols = gradients(q.double(), k.double(), v.double(), do.double(), mask, D ** -0.5, dtype)
+    if lens is not None:
+        k, v, q, do = poison(k, lens, 0), poison(v, lens, 0), poison(q, lens, Sk - Sq), poison(do, lens, Sk - Sq)
+    q, k, v, do = (t.cuda() for t in (q, k, v, do))
+    n = None if lens is None else torch.tensor(lens, dtype=torch.int32).cuda()
+    out, lse = window_attn_fwd(q, k, v, window, sinks, kv_lens=n, return_lse=True)
+    grads = window_attn_bwd(do, q, k, v, out, lse, window, sinks, kv_lens=n)
+    for name, g, ref, tol in zip(("dq", "dk", "dv"), grads, refs, tols):
+        assert_within(g, ref, tol, name)
+    if window > 1:  # (with one visible key dQ and dK are zero but for rounding)
+        for name, g, ref in zip(("dq", "dk", "dv"), grads, refs):
+            # P, out, dS and the result are rounded, each independently
+            assert_close_norm(g, ref, 4 * half_step(dtype), name)
+    again = window_attn_bwd(do, q, k, v, out, lse, window, sinks, kv_lens=n)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+def test_large_scores_and_long_rows():
+    """Scores far apart: the running maximum moves many times; the last tile walked (the sinks) may hold the largest."""
+    from block_sparse_attention import window_attn_fwd
+    q, k, v, _ = make(1, 2, 2, 900, 900, 128, BF, seed=3, spread=4.0)
+    k[:, :, :4] *= 4.0
+    ref, lse, tol, lse_tol, _, _ = attend(q.double(), k.double(), v.double(), masks(1, 900, 900, 400, 4, None), 0.3, BF)
+    out, got = window_attn_fwd(q.cuda(), k.cuda(), v.cuda(), 400, 4, softmax_scale=0.3, return_lse=True)
+    assert_within(out, ref, tol, "out")
+    assert_within(got, lse, lse_tol, "lse")
+
+
+def test_autograd_strided_and_broadcast_inputs():
+    """Views of one fused projection, a KV head broadcast over the batch, and a broadcast output gradient."""
+    from block_sparse_attention import window_attention
+    B, H, S, D = 2, 4, 260, 64
+    g = torch.Generator().manual_seed(5)
+    fused = torch.randn(B, S, 3, H, D, generator=g).bfloat16()
+    one = torch.randn(1, 2, S, D, generator=g).bfloat16()
+    f = fused.cuda().requires_grad_()
+    shared = one.cuda().requires_grad_()
+    q, k = f[:, :, 0], f[:, :, 1]
+    out = window_attention(q, k, f[:, :, 2], 100, 3, layout="bshd")
+    kb = shared.expand(B, 2, S, D)
+    out2 = window_attention(q.transpose(1, 2), kb, kb, 100, 3)
+    (out.float().sum() + 2 * out2.float().sum()).backward()
+    fd, od = fused.double(), one.double()
+    mask = masks(B, S, S, 100, 3, None)
+    tr = lambda t: t.transpose(1, 2)  # noqa: E731
+    ones = torch.ones(B, H, S, D, dtype=torch.float64)
+    r1, t1 = gradients(tr(fd[:, :, 0]), tr(fd[:, :, 1]), tr(fd[:, :, 2]), ones, mask, D ** -0.5, BF)
+    kd = od.expand(B, 2, S, D)
+    r2, t2 = gradients(tr(fd[:, :, 0]), kd, kd, 2 * ones, mask, D ** -0.5, BF)
+    u = half_step(BF)
+    # autograd adds the two uses in bf16: one more rounding of each sum
+    want = torch.stack([tr(r1[0] + r2[0]), tr(r1[1]), tr(r1[2])], 2)
+    tol = torch.stack([tr(t1[0] + t2[0]), tr(t1[1]), tr(t1[2])], 2) + u * want.abs() * 2
+    assert_within(f.grad, want, tol, "fused")
+    kv = (r2[1] + r2[2])
+    kv_tol = t2[1] + t2[2] + 2 * u * kv.abs()
+    assert_within(shared.grad, kv.sum(0, keepdim=True), kv_tol.sum(0, keepdim=True) + 2 * u * kv.abs().sum(0, keepdim=True), "shared")
+
+
+def test_out_lse_and_gradient_buffers():
+    """Buffers of the caller: strided, unaligned, longer than the call; what lies around them is left alone."""
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    q, k, v, do = (t.cuda() for t in make(1, 2, 2, 200, 200, 128, BF, seed=6))
+    ref, lse = window_attn_fwd(q, k, v, 60, 2, return_lse=True)
+    big = torch.full((1, 2, 300, 128), 7.0, dtype=BF, device="cuda")
+    lse_big = torch.full((1, 2, 300), 7.0, device="cuda")
+    out, got = window_attn_fwd(q, k, v, 60, 2, out=big[:, :, 50:250], lse=lse_big[:, :, 50:250])
+    assert torch.equal(out, ref) and torch.equal(got, lse)
+    assert (big[:, :, :50] == 7).all() and (big[:, :, 250:] == 7).all() and (lse_big[:, :, :50] == 7).all()
+    odd = torch.zeros(2 * 200 * 128 + 3, dtype=BF, device="cuda")[3:].view(1, 2, 200, 128)
+    assert torch.equal(window_attn_fwd(q, k, v, 60, 2, out=odd)[0], ref) and torch.equal(odd, ref)
+    shifted = torch.empty(2 * 200 * 128 + 3, dtype=BF, device="cuda")[3:].view(1, 2, 200, 128).copy_(k)
+    assert torch.equal(window_attn_fwd(q, shifted, v, 60, 2)[0], ref)
+    grads = window_attn_bwd(do, q, k, v, ref, lse, 60, 2)
+    hold = [torch.full((1, 2, 300, 128), 7.0, dtype=BF, device="cuda") for _ in range(3)]
+    window_attn_bwd(do, q, k, v, ref, lse, 60, 2, dq=hold[0][:, :, 9:209], dk=hold[1][:, :, 9:209], dv=hold[2][:, :, 9:209])
+    for h, g in zip(hold, grads):
+        assert torch.equal(h[:, :, 9:209], g) and (h[:, :, :9] == 7).all() and (h[:, :, 209:] == 7).all()
+
+
+def test_empty_extents():
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    z = lambda *s: torch.zeros(*s, dtype=BF, device="cuda")  # noqa: E731
+    out, lse = window_attn_fwd(z(2, 2, 0, 64), z(2, 2, 5, 64), z(2, 2, 5, 64), 4, return_lse=True)
+    assert out.shape == (2, 2, 0, 64) and lse.shape == (2, 2, 0)
+    q = torch.ones(1, 2, 3, 64, dtype=BF, device="cuda")
+    out, lse = window_attn_fwd(q, z(1, 2, 0, 64), z(1, 2, 0, 64), 4, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    dq, dk, dv = window_attn_bwd(q, q, z(1, 2, 0, 64), z(1, 2, 0, 64), out, lse, 4)
+    assert (dq == 0).all() and dk.shape == dv.shape == (1, 2, 0, 64)
+
+
+def test_streams_and_graphs():
+    """A side stream, and two captured graphs replayed in turn on new inputs, against direct calls."""
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    sets = [[t.cuda() for t in make(1, 4, 2, 300, 300, 128, BF, seed=s)] for s in range(2)]
+
+    def step(q, k, v, do):
+        out, lse = window_attn_fwd(q, k, v, 90, 3, return_lse=True)
+        return (out,) + window_attn_bwd(do, q, k, v, out, lse, 90, 3)
+
+    want = [step(*s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [step(*s) for s in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    graphs = []
+    for s in sets:
+        held = [t.clone() for t in s]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step(*held)
+        graphs.append((graph, held, res))
+    for turn in range(2):
+        for i, (graph, held, res) in enumerate(graphs):
+            for h, t in zip(held, sets[(i + turn) % 2]):
+                h.copy_(t)
+            graph.replay()
+        torch.cuda.synchronize()
+        for i, (_, _, res) in enumerate(graphs):
+            assert all(torch.equal(x, y) for x, y in zip(res, want[(i + turn) % 2]))
+
+
+def test_matches_dense_block_sparse_operator():
+    """A window over everything, queries at the end of the keys: the last row equals full attention by the
+    block-sparse operator over all blocks (both round P and the result: two half steps each)."""
+    from block_sparse_attention import bsa_attn_fwd, window_attn_fwd
+    q, k, v, _ = (t.cuda() for t in make(1, 2, 2, 1, 512, 128, BF, seed=8))
+    index = torch.arange(4, dtype=torch.int32, device="cuda").expand(1, 2, 1, 4).contiguous()
+    a, la = bsa_attn_fwd(q, k, v, index, 4, return_lse=True, sparse_block_size=128)
+    b, lb = window_attn_fwd(q, k, v, 512, 0, return_lse=True)
+    _, _, tol, lse_tol, _, _ = attend(q.double().cpu(), k.double().cpu(), v.double().cpu(), torch.ones(1, 1, 512, dtype=torch.bool), 128 ** -0.5, BF)
+    assert_within(a, b.double().cpu(), 2 * tol, "out")
+    assert_within(la, lb.double().cpu(), 2 * lse_tol, "lse")
