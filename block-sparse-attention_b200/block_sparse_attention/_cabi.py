@@ -302,6 +302,24 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The same handle without building a Stream object (2.2 -> 0.1 us a call); the object where torch has no such function.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(fn, what: str, device: torch.device, *args) -> None:
+    """Calls an entry point on the current stream of ``device`` and maps its return code; switches devices only when
+    another one is current (a device context costs as much as a small launch)."""
+    index = device.index
+    stream = stream_ptr(device) if _raw_stream is None else _raw_stream(index)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != 0:
+        check(rc, what)
+
+
 def strides3(t: torch.Tensor):
     """(batch, head, seq) element strides of a BHSD view."""
     return _c_i64x3(t.stride(0), t.stride(1), t.stride(2))

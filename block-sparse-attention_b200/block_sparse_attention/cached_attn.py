@@ -16,9 +16,10 @@ from typing import Optional, Tuple
 import torch
 
 from . import _cabi
-from .bsa_attn_interface import _ceil_div, maybe_contiguous
-from .window_attn import (_MAX_LEN, _check_lens, _check_qkv, _check_scale, _check_window, _launch_window_fwd,
-                          _out_buffers, _views)
+from .bsa_attn_interface import _ceil_div
+from .window_attn import _MAX_LEN, _check_lens, _check_qkv, _check_scale, _check_window, _launch_window_fwd, _out_buffers
+
+_c_i64x3 = _cabi._c_i64x3
 
 __all__ = ["cached_attn_fwd", "tree_mask_from_parents", "cache_append", "cache_keep"]
 
@@ -26,12 +27,13 @@ MAX_TREE_TOKENS = 64
 
 
 def _check_cache(k_cache, v_cache, page_table, cache_lens, B: int, device):
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        assert t.dim() == 4 and t.device == device, f"{name} must be [num_pages, Hkv, page_size, D] on the device of q"
+    for t in (k_cache, v_cache):
+        assert t.dim() == 4 and t.device == device, "the pools must be [num_pages, Hkv, page_size, D] on the device of q"
         # a pool is never copied: its rows have to be addressable as they lie
-        assert t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.shape[d] == 1 or (t.stride(d) > 0 and t.stride(d) % 8 == 0) for d in range(3)), (
-            f"{name} must have unit last stride, 16-byte aligned rows and no broadcast dimension")
+        st = t.stride()
+        assert (st[3] == 1 and t.data_ptr() % 16 == 0 and st[0] > 0 and st[1] > 0 and st[2] > 0
+                and (st[0] | st[1] | st[2]) % 8 == 0), (
+            "the pools must have unit last stride, 16-byte aligned rows and no broadcast dimension")
     assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype, "K and V pools must match"
     num_pages, Hkv, page_size, D = k_cache.shape
     assert num_pages >= 1 and Hkv >= 1 and page_size >= 1, "the pools hold no page"
@@ -76,9 +78,8 @@ def cached_attn_fwd(
     """
     window, sink_tokens = _check_window(_MAX_LEN if window is None else window, sink_tokens)
     _check_qkv(q, k_cache, v_cache, layout)
-    q = maybe_contiguous(q)
-    qb = _views(layout, q)[0]
-    B, Hq, T, D = qb.shape
+    shape = q.shape
+    B, Hq, T, D = shape if layout == "bhsd" else (shape[0], shape[2], shape[1], shape[3])
     page_table, cache_lens = _check_cache(k_cache, v_cache, page_table, cache_lens, B, q.device)
     Hkv, page_size = k_cache.shape[1], k_cache.shape[2]
     assert k_cache.shape[3] == D and Hq % Hkv == 0, "the pools must match q's head dimension, and Hkv divide Hq"
@@ -102,9 +103,9 @@ def cached_attn_fwd(
     capacity = page_table.shape[1] * page_size
     span = min(T, 128) + min(window, capacity)
     key_tiles = min(_ceil_div(capacity, 128), _ceil_div(span, 128) + 2)
-    _launch_window_fwd(q=qb, k=k_cache, v=v_cache, out=_views(layout, out)[0], lse=lse_buf, kv_lens=cache_lens,
-                       window=window, sinks=sink_tokens, scale=scale, page_table=page_table, tree_mask=tree_mask,
-                       pack_gqa=pack, page_size=page_size, key_tiles=key_tiles)
+    _launch_window_fwd(q, k_cache, v_cache, out, lse_buf, layout, (B, Hq, Hkv, T, 0, D), kv_lens=cache_lens,
+                       window=window, sinks=sink_tokens, scale=scale, pack_gqa=pack, key_tiles=key_tiles,
+                       page_table=page_table, tree_mask=tree_mask, page_size=page_size)
     return out, lse_buf
 
 
@@ -122,9 +123,7 @@ def tree_mask_from_parents(parents: torch.Tensor) -> torch.Tensor:
     mask = torch.empty((B, T), dtype=torch.int64, device=parents.device)
     if mask.numel() == 0:
         return mask
-    with torch.cuda.device(parents.device):
-        _cabi.check(_cabi.load().bsa_tree_mask(parents.data_ptr(), B, T, mask.data_ptr(), _cabi.stream_ptr(parents.device)),
-                    "bsa_tree_mask")
+    _cabi.launch(_cabi.load().bsa_tree_mask, "bsa_tree_mask", parents.device, parents.data_ptr(), B, T, mask.data_ptr())
     return mask
 
 
@@ -141,23 +140,25 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     assert k.dim() == 4 and k.shape == v.shape and k.is_cuda and v.device == k.device, "k and v must match, on CUDA"
     assert k.dtype == v.dtype == k_cache.dtype and k.dtype in (torch.float16, torch.bfloat16), (
         "k, v and the pools must all be float16 or all bfloat16")
-    kb, vb = _views(layout, k, v)
-    B, H, T, D = kb.shape
+    shape = k.shape
+    B, H, T, D = shape if layout == "bhsd" else (shape[0], shape[2], shape[1], shape[3])
     page_table, cache_lens = _check_cache(k_cache, v_cache, page_table, cache_lens, B, k.device)
-    assert k_cache.shape[1] == H and k_cache.shape[3] == D and D % 8 == 0, "the pools must match k's heads and head dimension"
-    if k.numel() == 0 or page_table.shape[1] == 0:
+    num_pages, pool_heads, page_size, pool_dim = k_cache.shape
+    assert pool_heads == H and pool_dim == D and D % 8 == 0, "the pools must match k's heads and head dimension"
+    if B == 0 or T == 0 or page_table.shape[1] == 0:
         return k_cache, v_cache
 
     def rows(t):
-        ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:3])
-        return t if ok else t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+        if st[3] != 1 or t.data_ptr() % 16 != 0 or (st[0] | st[1] | st[2]) % 8 != 0:
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = t.stride()
+        return t, _c_i64x3(st[0], st[1], st[2]) if layout == "bhsd" else _c_i64x3(st[0], st[2], st[1])
 
-    kb, vb = rows(kb), rows(vb)
-    with torch.cuda.device(k.device):
-        _cabi.check(_cabi.load().bsa_cache_append(
-            kb.data_ptr(), vb.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _cabi.strides3(kb), _cabi.strides3(vb),
-            _cabi.strides3(k_cache), _cabi.strides3(v_cache), page_table.data_ptr(), cache_lens.data_ptr(), B, H, T, D,
-            page_table.shape[1], k_cache.shape[2], k_cache.shape[0], _cabi.stream_ptr(k.device)), "bsa_cache_append")
+    (k_k, k_st), (v_k, v_st) = rows(k), rows(v)
+    _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, k_k.data_ptr(), v_k.data_ptr(),
+                 k_cache.data_ptr(), v_cache.data_ptr(), k_st, v_st, _cabi.strides3(k_cache), _cabi.strides3(v_cache),
+                 page_table.data_ptr(), cache_lens.data_ptr(), B, H, T, D, page_table.shape[1], page_size, num_pages)
     return k_cache, v_cache
 
 
@@ -188,10 +189,9 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     if page_table.shape[1] == 0:
         page_table = torch.full((B, 1), -1, dtype=torch.int32, device=device)
     new_lens = torch.empty_like(cache_lens)
-    with torch.cuda.device(device):
-        _cabi.check(_cabi.load().bsa_cache_keep(
-            k_cache.data_ptr(), v_cache.data_ptr(), _cabi.strides3(k_cache), _cabi.strides3(v_cache),
-            page_table.data_ptr(), cache_lens.data_ptr(), path.data_ptr(), path_lens.data_ptr(), new_lens.data_ptr(), B,
-            k_cache.shape[1], num_drafts, path.shape[1], k_cache.shape[3], page_table.shape[1], k_cache.shape[2],
-            k_cache.shape[0], _cabi.stream_ptr(device)), "bsa_cache_keep")
+    num_pages, H, page_size, D = k_cache.shape
+    _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", device, k_cache.data_ptr(), v_cache.data_ptr(),
+                 _cabi.strides3(k_cache), _cabi.strides3(v_cache), page_table.data_ptr(), cache_lens.data_ptr(),
+                 path.data_ptr(), path_lens.data_ptr(), new_lens.data_ptr(), B, H, num_drafts, path.shape[1], D,
+                 page_table.shape[1], page_size, num_pages)
     return new_lens

@@ -66,40 +66,72 @@ def rotary_nd(
     """
     assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
     assert q.dim() == 4 and q.is_cuda, "q must be a 4-D CUDA tensor"
-    assert q.dtype in _DTYPES, "q must be bfloat16, float16 or float32"
-    assert k is None or (k.dim() == 4 and k.dtype == q.dtype and k.device == q.device), "k must match q's type and device"
+    code = _DTYPES.get(q.dtype)
+    assert code is not None, "q must be bfloat16, float16 or float32"
     device = q.device
-    tr = (lambda t: t) if layout == "bhsd" else (lambda t: t.transpose(1, 2))
-    pairs = [int(n) for n in axis_pairs]
-    P = sum(pairs)
-    B, Hq, S, D = tr(q).shape
+    h, s = (1, 2) if layout == "bhsd" else (2, 1)  # dimensions of heads and tokens
+    shape = q.shape
+    B, Hq, S, D = shape[0], shape[h], shape[s], shape[3]
     assert D % 2 == 0 and 2 <= D <= 512, f"head dimension must be even and at most 512, got {D}"
-    assert 1 <= len(pairs) <= 4 and min(pairs) >= 0 and 1 <= P and 2 * P <= D, (
-        f"axis_pairs {tuple(pairs)} must be 1 to 4 axes with 1 to {D // 2} pairs in all")
+    pairs = tuple(axis_pairs)
+    P, A = sum(pairs), len(pairs)
+    assert 1 <= A <= 4 and min(pairs) >= 0 and 1 <= P and 2 * P <= D, (
+        f"axis_pairs {pairs} must be 1 to 4 axes with 1 to {D // 2} pairs in all")
+    Hk = 0
     if k is not None:
-        assert tr(k).shape[0] == B and tr(k).shape[2:] == (S, D), "k must match q's batch, tokens and head dimension"
+        assert k.dim() == 4 and k.dtype == q.dtype and k.device == device, "k must match q's type and device"
+        Hk = k.shape[h]
+        assert k.shape[0] == B and k.shape[s] == S and k.shape[3] == D, "k must match q's batch, tokens and head dimension"
     assert positions.dtype == torch.int32 and positions.device == device, "positions must be int32 on the device of q"
-    assert tuple(positions.shape) in ((S, len(pairs)), (B, S, len(pairs))), (
-        f"positions has shape {tuple(positions.shape)}, expected ({S}, {len(pairs)}) or ({B}, {S}, {len(pairs)})")
+    at = tuple(positions.shape)
+    assert at == (S, A) or at == (B, S, A), f"positions has shape {at}, expected ({S}, {A}) or ({B}, {S}, {A})"
     assert inv_freq.dtype == torch.float32 and inv_freq.device == device and tuple(inv_freq.shape) == (P,), (
         f"inv_freq must be float32 of shape ({P},) on the device of q")
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
     inv_freq = inv_freq.contiguous()
-
-    def prepare(x, out, name):
-        x = x if x.stride(-1) == 1 else x.contiguous()
-        if out is None:
-            return x, torch.empty(x.shape, dtype=x.dtype, device=device)
-        assert out.shape == x.shape and out.dtype == x.dtype and out.device == device, f"{name} must match its input"
-        assert out.stride(-1) == 1 and all(n == 1 or s > 0 for n, s in zip(out.shape, out.stride())), (
-            f"{name} must have unit last stride and no broadcast dimension")
-        return x, out
-
-    q, qo = prepare(q, q_out, "q_out")
-    k, ko = (None, None) if k is None else prepare(k, k_out, "k_out")
-    if q.numel() == 0 and (k is None or k.numel() == 0):
+    qo, ko = q_out, k_out
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    if q_out is None:
+        qo = torch.empty_like(q)
+    if k is None:
+        ko = None
+    elif k_out is None:
+        ko = torch.empty_like(k)
+    if q_out is not None or (k is not None and k_out is not None):  # fresh outputs overlap nothing
+        _check_outputs(q, qo, k, ko)
+    if B == 0 or S == 0 or (Hq == 0 and Hk == 0):
         return qo, ko
+    assert Hq >= 1, "q has no heads"
+    zero = (0, 0, 0)
+
+    def strides(t):
+        if t is None:
+            return zero
+        st = t.stride()
+        return st[0], st[h], st[s]
+
+    pos_st = positions.stride()
+    a = _cabi.RotaryArgs(
+        q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr(),
+        positions.data_ptr(), inv_freq.data_ptr(), strides(q), strides(k), strides(qo), strides(ko),
+        (pos_st[0] if len(at) == 3 else 0, pos_st[-2]), pairs, A, code, B, Hq, Hk, S, D, 1 if interleaved else 0,
+        1 if inverse else 0)
+    _cabi.launch(_cabi.load().bsa_rotary_nd, "bsa_rotary_nd", device, a)
+    return qo, ko
+
+
+def _check_outputs(q, qo, k, ko) -> None:
+    for name, x, out in (("q_out", q, qo), ("k_out", k, ko)):
+        if out is not None:
+            assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, f"{name} must match its input"
+            assert out.stride(-1) == 1 and all(n == 1 or st > 0 for n, st in zip(out.shape, out.stride())), (
+                f"{name} must have unit last stride and no broadcast dimension")
+    if any(t is not None and t.numel() == 0 for t in (q, k)):
+        return
     for out, own, other, other_out in ((qo, q, k, ko), (ko, k, q, qo)):
         if out is None:
             continue
@@ -109,27 +141,6 @@ def rotary_nd(
             apart = not _overlap(out, other) and not _overlap(out, other_out)
             assert apart or (_same_view(out, own) and _same_view(other_out, other) and out.data_ptr() != other.data_ptr()), (
                 "q and k and their outputs must not overlap, unless both are rotated in place")
-    a = _cabi.RotaryArgs()
-    qv, qov = tr(q), tr(qo)
-    a.q, a.q_out = qv.data_ptr(), qov.data_ptr()
-    a.q_stride, a.qo_stride = _cabi.strides3(qv), _cabi.strides3(qov)
-    if k is not None:
-        kv, kov = tr(k), tr(ko)
-        a.k, a.k_out = kv.data_ptr(), kov.data_ptr()
-        a.k_stride, a.ko_stride = _cabi.strides3(kv), _cabi.strides3(kov)
-        a.Hk = kv.shape[1]
-    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-    a.pos_stride[0] = positions.stride(0) if positions.dim() == 3 else 0
-    a.pos_stride[1] = positions.stride(-2)
-    for i, n in enumerate(pairs):
-        a.axis_pairs[i] = n
-    a.num_axes = len(pairs)
-    a.dtype = _DTYPES[q.dtype]
-    a.B, a.Hq, a.S, a.D = B, Hq, S, D
-    a.interleaved, a.inverse = int(bool(interleaved)), int(bool(inverse))
-    with torch.cuda.device(device):
-        _cabi.check(_cabi.load().bsa_rotary_nd(a, _cabi.stream_ptr(device)), "bsa_rotary_nd")
-    return qo, ko
 
 
 class RotaryFunction(torch.autograd.Function):

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _cabi
-from .bsa_attn_interface import _ceil_div, _tma_ready, maybe_contiguous
+from .bsa_attn_interface import _ceil_div, _tma_ready
 
 __all__ = ["window_attn_fwd", "window_attn_bwd", "window_attention", "WindowAttentionFunction"]
 
@@ -49,16 +49,22 @@ def _dtype_code(dtype) -> int:
     return _cabi.BSA_DTYPE_F16 if dtype == torch.float16 else _cabi.BSA_DTYPE_BF16
 
 
-def _addressable(t: torch.Tensor) -> torch.Tensor:
-    """``_tma_ready``, and a copy also of contiguous tensors that start between two 16-byte boundaries."""
-    r = _tma_ready(t, 2)
-    return r if r.data_ptr() % 16 == 0 else _tma_ready(t.clone(memory_format=torch.contiguous_format), 2)
+def _rows(t: torch.Tensor, layout: str):
+    """(tensor, BHSD strides) the tensor maps can address; copies only views that they cannot."""
+    st = t.stride()
+    st = (st[0], st[1], st[2], st[3]) if layout == "bhsd" else (st[0], st[2], st[1], st[3])
+    if st[3] == 1 and st[0] > 0 and st[1] > 0 and st[2] > 0 and (st[0] | st[1] | st[2]) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, st[:3]
+    view = _tma_ready(t if layout == "bhsd" else t.transpose(1, 2), 2)
+    if view.data_ptr() % 16 != 0:  # contiguous, but starting between two 16-byte boundaries
+        view = _tma_ready(view.clone(memory_format=torch.contiguous_format), 2)
+    return view, view.stride()[:3]
 
 
-def _can_hold(t: torch.Tensor) -> bool:
-    """Whether the kernels can write rows of this BHSD view with 16-byte stores."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(t.shape[d] == 1 or (t.stride(d) > 0 and t.stride(d) % 8 == 0) for d in range(3)))
+def _can_hold(t: torch.Tensor, st) -> bool:
+    """Whether the kernels can write the rows of a buffer with 16-byte stores."""
+    return (t.stride(3) == 1 and st[0] > 0 and st[1] > 0 and st[2] > 0 and (st[0] | st[1] | st[2]) % 8 == 0
+            and t.data_ptr() % 16 == 0)
 
 
 def _window_splits(items: int, key_tiles: int, num_sms: int) -> int:
@@ -71,47 +77,40 @@ def _window_splits(items: int, key_tiles: int, num_sms: int) -> int:
     return max(1, min(places // items, key_tiles, 256))
 
 
-def _launch_window_fwd(*, q, k, v, out, lse, kv_lens, window, sinks, scale, page_table=None, tree_mask=None,
-                       pack_gqa=False, page_size=0, key_tiles=1):
-    """q, out are BHSD views; k, v BHSD views or (with a page table) [pages, H, page_size, D] pools."""
+def _launch_window_fwd(q, k, v, out, lse, layout, shape, *, kv_lens, window, sinks, scale, pack_gqa, key_tiles,
+                       page_table=None, tree_mask=None, page_size=0):
+    """``shape`` is (B, Hq, Hkv, Sq, Sk, D); with a page table, k and v are [pages, Hkv, page_size, D] pools."""
     lib = _cabi.load()
     device = q.device
-    B, Hq, Sq, D = q.shape
-    Hkv = k.shape[1]
-    q_k, k_k, v_k = _addressable(q), _addressable(k), _addressable(v)
-    out_k = out if _can_hold(out) else torch.empty(out.shape, dtype=out.dtype, device=device)
-    out_view = _tma_ready(out_k, 2)
+    B, Hq, Hkv, Sq, Sk, D = shape
+    kv_layout = layout if page_table is None else "bhsd"
+    (q_k, q_st), (k_k, k_st), (v_k, v_st) = _rows(q, layout), _rows(k, kv_layout), _rows(v, kv_layout)
+    out_k, o_st = out, out.stride()
+    o_st = (o_st[0], o_st[1], o_st[2]) if layout == "bhsd" else (o_st[0], o_st[2], o_st[1])
+    if not _can_hold(out, o_st):
+        out_k = torch.empty((B, Hq, Sq, D), dtype=out.dtype, device=device)
+        o_st = out_k.stride()[:3]
     lse_k = lse
     if lse is not None and not lse.is_contiguous():
         lse_k = torch.empty(lse.shape, dtype=torch.float32, device=device)
 
-    G = Hq // Hkv
-    tiles = _ceil_div(Sq, 128 // G) * Hkv if pack_gqa else _ceil_div(Sq, 128) * Hq
-    splits = _window_splits(B * tiles, key_tiles, int(lib.bsa_num_sms(device.index or 0)))
-    args = _cabi.WindowFwdArgs()
-    args.q, args.k, args.v = q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr()
-    args.out, args.lse = out_view.data_ptr(), _cabi.ptr(lse_k)
-    args.kv_lens, args.page_table, args.tree_mask = _cabi.ptr(kv_lens), _cabi.ptr(page_table), _cabi.ptr(tree_mask)
+    items = B * (_ceil_div(Sq, 128 // (Hq // Hkv)) * Hkv if pack_gqa else _ceil_div(Sq, 128) * Hq)
+    splits = _window_splits(items, key_tiles, lib.bsa_num_sms(device.index))
     partial_o = partial_lse = None
     if splits > 1:
-        partial_o = torch.empty((splits, B, Hq, Sq, D), dtype=torch.float32, device=device)
-        partial_lse = torch.empty((splits, B, Hq, Sq), dtype=torch.float32, device=device)
-        args.partial_o, args.partial_lse = partial_o.data_ptr(), partial_lse.data_ptr()
-    args.status = _cabi.status_buffer(device).data_ptr()
-    args.q_stride, args.k_stride, args.v_stride = _cabi.strides3(q_k), _cabi.strides3(k_k), _cabi.strides3(v_k)
-    args.o_stride = _cabi.strides3(out_view)
-    args.dtype = _dtype_code(q.dtype)
-    args.B, args.Hq, args.Hkv, args.Sq, args.Sk, args.D = B, Hq, Hkv, Sq, (0 if page_size else k.shape[2]), D
-    args.window, args.sinks = window, sinks
-    if page_table is not None:
-        args.max_pages, args.page_size, args.num_pages = page_table.shape[1], page_size, k.shape[0]
-    args.pack_gqa = 1 if pack_gqa else 0
-    args.splits = splits
-    args.softmax_scale = scale
-    with torch.cuda.device(device):
-        _cabi.check(lib.bsa_window_fwd(args, _cabi.stream_ptr(device)), "bsa_window_fwd")
+        rows = splits * B * Hq * Sq
+        partial = q.new_empty(rows * (D + 1), dtype=torch.float32)
+        partial_o = partial.data_ptr()
+        partial_lse = partial_o + 4 * rows * D
+    paged = page_table is not None
+    args = _cabi.WindowFwdArgs(
+        q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr(), out_k.data_ptr(), _cabi.ptr(lse_k), _cabi.ptr(kv_lens),
+        _cabi.ptr(page_table), _cabi.ptr(tree_mask), partial_o, partial_lse, _cabi.status_buffer(device).data_ptr(), q_st,
+        k_st, v_st, o_st, _dtype_code(q.dtype), B, Hq, Hkv, Sq, Sk, D, window, sinks, page_table.shape[1] if paged else 0,
+        page_size, k.shape[0] if paged else 0, 1 if pack_gqa else 0, splits, scale)
+    _cabi.launch(lib.bsa_window_fwd, "bsa_window_fwd", device, args)
     if out_k is not out:
-        out.copy_(out_k)
+        (out if layout == "bhsd" else out.transpose(1, 2)).copy_(out_k)
     if lse is not None and lse_k is not lse:
         lse.copy_(lse_k)
 
@@ -119,7 +118,7 @@ def _launch_window_fwd(*, q, k, v, out, lse, kv_lens, window, sinks, scale, page
 def _out_buffers(q, out, lse, want_lse, B, H, S):
     device = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q)
     else:
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == device
         assert out.stride(-1) == 1
@@ -132,7 +131,7 @@ def _out_buffers(q, out, lse, want_lse, B, H, S):
 
 def _check_qkv(q, k, v, layout):
     assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
-    assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4
+    assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "inputs must be 4-D"
     assert q.is_cuda and k.is_cuda and v.is_cuda, "inputs must be on CUDA device"
     assert q.device == k.device == v.device, "Q/K/V must be on the same CUDA device"
     assert q.dtype == k.dtype == v.dtype, "inputs must have the same dtype"
@@ -140,14 +139,11 @@ def _check_qkv(q, k, v, layout):
     assert q.shape[-1] in (64, 96, 128), f"head dimension must be 64, 96 or 128, got {q.shape[-1]}"
 
 
-def _views(layout, *tensors):
-    return [t if layout == "bhsd" else t.transpose(1, 2) for t in tensors]
-
-
-def _check_shapes(qb, kb, vb):
-    B, Hq, Sq, D = qb.shape
-    Bk, Hkv, Sk, Dk = kb.shape
-    assert vb.shape == kb.shape and Bk == B and Dk == D, "K and V must match Q's batch and head dimension, and each other"
+def _check_shapes(q, k, v, layout):
+    h, n = (1, 2) if layout == "bhsd" else (2, 1)
+    qs, ks = q.shape, k.shape
+    B, Hq, Sq, D, Hkv, Sk = qs[0], qs[h], qs[n], qs[3], ks[h], ks[n]
+    assert v.shape == ks and ks[0] == B and ks[3] == D, "K and V must match Q's batch and head dimension, and each other"
     assert Hkv >= 1 and Hq % Hkv == 0, "the number of query heads must be a multiple of the number of KV heads"
     assert Sq <= _MAX_LEN and Sk <= _MAX_LEN
     return B, Hq, Hkv, Sq, Sk, D
@@ -182,9 +178,7 @@ def window_attn_fwd(
     window, sink_tokens = _check_window(window, sink_tokens)
     _check_qkv(q, k, v, layout)
     want_lse = return_lse or lse is not None or q.requires_grad or k.requires_grad or v.requires_grad
-    q, k, v = [maybe_contiguous(t) for t in (q, k, v)]
-    qb, kb, vb = _views(layout, q, k, v)
-    B, Hq, Hkv, Sq, Sk, D = _check_shapes(qb, kb, vb)
+    shape = B, Hq, Hkv, Sq, Sk, D = _check_shapes(q, k, v, layout)
     kv_lens = _check_lens(kv_lens, B, q.device, "kv_lens")
     scale = _check_scale(softmax_scale, D)
     out, lse_buf = _out_buffers(q, out, lse, want_lse, B, Hq, Sq)
@@ -197,8 +191,8 @@ def window_attn_fwd(
     pack = Hq > Hkv and Sq < 128 and Hq // Hkv <= 128
     span = min(Sq, 128) + min(window, Sk)
     key_tiles = min(_ceil_div(Sk, 128), _ceil_div(span, 128) + 2)
-    _launch_window_fwd(q=qb, k=kb, v=vb, out=_views(layout, out)[0], lse=lse_buf, kv_lens=kv_lens, window=window,
-                       sinks=sink_tokens, scale=scale, pack_gqa=pack, key_tiles=key_tiles)
+    _launch_window_fwd(q, k, v, out, lse_buf, layout, shape, kv_lens=kv_lens, window=window, sinks=sink_tokens,
+                       scale=scale, pack_gqa=pack, key_tiles=key_tiles)
     return out, lse_buf
 
 
@@ -227,54 +221,51 @@ def window_attn_bwd(
     """
     window, sink_tokens = _check_window(window, sink_tokens)
     _check_qkv(q, k, v, layout)
-    q, k, v, out, dout = [maybe_contiguous(t) for t in (q, k, v, out, dout)]
     assert out.dtype == dout.dtype == q.dtype and lse.dtype == torch.float32
-    assert all(t.device == q.device for t in (out, dout, lse)), "all tensors must be on the device of q"
-    assert out.shape == q.shape and dout.shape == q.shape
-    qb, kb, vb, ob, dob = _views(layout, q, k, v, out, dout)
-    B, Hq, Hkv, Sq, Sk, D = _check_shapes(qb, kb, vb)
-    assert lse.shape == (B, Hq, Sq)
     device = q.device
+    assert out.device == dout.device == lse.device == device, "all tensors must be on the device of q"
+    assert out.shape == q.shape and dout.shape == q.shape
+    B, Hq, Hkv, Sq, Sk, D = _check_shapes(q, k, v, layout)
+    assert lse.shape == (B, Hq, Sq)
     kv_lens = _check_lens(kv_lens, B, device, "kv_lens")
     scale = _check_scale(softmax_scale, D)
 
     def _grad(buf, like):
         if buf is None:
-            return torch.empty(like.shape, dtype=like.dtype, device=device)
+            return torch.empty_like(like)
         assert buf.shape == like.shape and buf.dtype == like.dtype and buf.device == device
         return buf
 
-    grads = [_grad(dq, q), _grad(dk, k), _grad(dv, v)]
+    grads = dq, dk, dv = _grad(dq, q), _grad(dk, k), _grad(dv, v)
     if q.numel() == 0 or k.numel() == 0:
         for g in grads:
             g.zero_()
-        return tuple(grads)
+        return grads
     lib = _cabi.load()
-    held = [g if _can_hold(g) else torch.empty(g.shape, dtype=g.dtype, device=device) for g in _views(layout, *grads)]
-    held = [_tma_ready(h, 2) for h in held]
-    views = [_addressable(t) for t in (dob, qb, kb, vb, ob)]
+    held, held_st = [], []
+    for g in grads:
+        st = g.stride()
+        st = (st[0], st[1], st[2]) if layout == "bhsd" else (st[0], st[2], st[1])
+        if not _can_hold(g, st):
+            g = torch.empty((B, g.shape[1], g.shape[2], D) if layout == "bhsd" else (B, g.shape[2], g.shape[1], D),
+                            dtype=g.dtype, device=device)
+            st = g.stride()[:3]
+        held.append(g)
+        held_st.append(st)
+    (do_k, do_st), (q_k, q_st), (k_k, k_st), (v_k, v_st), (o_k, o_st) = (_rows(t, layout) for t in (dout, q, k, v, out))
     lse_c = lse.contiguous()
-    ws_bytes = int(lib.bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sink_tokens))
-    workspace = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=device)
-    a = _cabi.WindowBwdArgs()
-    a.dout, a.q, a.k, a.v, a.out = (t.data_ptr() for t in views)
-    a.lse = lse_c.data_ptr()
-    a.dq, a.dk, a.dv = (t.data_ptr() for t in held)
-    a.kv_lens = _cabi.ptr(kv_lens)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    a.status = _cabi.status_buffer(device).data_ptr()
-    a.do_stride, a.q_stride, a.k_stride, a.v_stride, a.o_stride = (_cabi.strides3(t) for t in views)
-    a.dq_stride, a.dk_stride, a.dv_stride = (_cabi.strides3(t) for t in held)
-    a.dtype = _dtype_code(q.dtype)
-    a.B, a.Hq, a.Hkv, a.Sq, a.Sk, a.D = B, Hq, Hkv, Sq, Sk, D
-    a.window, a.sinks = window, sink_tokens
-    a.softmax_scale = scale
-    with torch.cuda.device(device):
-        _cabi.check(lib.bsa_window_bwd(a, _cabi.stream_ptr(device)), "bsa_window_bwd")
-    for g, h in zip(_views(layout, *grads), held):
-        if h.data_ptr() != g.data_ptr():
-            g.copy_(h)
-    return tuple(grads)
+    ws_bytes = max(16, lib.bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sink_tokens))
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
+    a = _cabi.WindowBwdArgs(
+        do_k.data_ptr(), q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr(), o_k.data_ptr(), lse_c.data_ptr(),
+        held[0].data_ptr(), held[1].data_ptr(), held[2].data_ptr(), _cabi.ptr(kv_lens), workspace.data_ptr(),
+        _cabi.status_buffer(device).data_ptr(), ws_bytes, do_st, q_st, k_st, v_st, o_st, held_st[0], held_st[1], held_st[2],
+        _dtype_code(q.dtype), B, Hq, Hkv, Sq, Sk, D, window, sink_tokens, scale)
+    _cabi.launch(lib.bsa_window_bwd, "bsa_window_bwd", device, a)
+    for g, t in zip(grads, held):
+        if t is not g:
+            (g if layout == "bhsd" else g.transpose(1, 2)).copy_(t)
+    return grads
 
 
 class WindowAttentionFunction(torch.autograd.Function):

@@ -6,7 +6,25 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace bsa {
+
+// Asks for a kernel's dynamic shared memory once per device (the call costs as much as a launch's other host work).
+// One static object per kernel; concurrent first calls set the same value.
+struct SmemAttribute {
+  std::atomic<bool> done[64] = {};
+  cudaError_t set(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool known = dev >= 0 && dev < 64;
+    if (known && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && known) done[dev].store(true, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 // Stores a printf-style message for bsa_last_error() and returns `code`.
 int set_error(int code, const char* fmt, ...);

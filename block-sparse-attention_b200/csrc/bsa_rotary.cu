@@ -1,9 +1,10 @@
 // Rotary positions with several axes (text, images, video): pair p of a head turns by
 //   angle(b, s, p) = positions[b, s, axis(p)] * inv_freq[p].
 //
-// Bound by HBM: q and k are read and written once, three multiply-adds per element.  A thread owns one 16-byte chunk
-// of a token (half-split pairing: the two chunks its pairs connect) and walks over the heads: the sines and cosines of
-// its pairs are computed once, in registers, and serve every head of q and of k.  Four heads are in flight at a time.
+// Bound by HBM: q and k are read and written once, three multiply-adds per element.  A block holds a few whole tokens:
+// its threads first compute the sines and cosines of the tokens' pairs, about one each, into shared memory; then a
+// thread owns one 16-byte chunk of a token (half-split pairing: the two chunks its pairs connect), takes its pairs'
+// values into registers and walks over every head_lanes-th head of q and k, four heads in flight at a time.
 //
 // The angle of position 10^5 at frequency 1 is 10^5 radians; in 32 bits its fraction of a turn would be off by 10^-3.
 // So position * (inv_freq / 2 pi) is formed and reduced to [-1/2, 1/2] turns in 64 bits, and only the reduced turn is
@@ -29,11 +30,14 @@ struct Params {
   long long q_b, q_h, q_s, k_b, k_h, k_s;      // bytes
   long long qo_b, qo_h, qo_s, ko_b, ko_h, ko_s;
   long long pos_b, pos_s;  // elements
-  long long units;         // B * S * units per token
+  long long units;         // element form: B * S * units per token
   int end0, end1, end2;    // first pair of axes 1, 2, 3
   int Hq, heads, S, D, P;
   int per_token;           // units per token
   int heads_per_cta;
+  long long tokens;        // B * S
+  int tokens_per_block;    // vector form: whole tokens of a block, at most kThreads units
+  int head_lanes;          // ... and the heads its threads work on side by side
   float sign;
 };
 
@@ -102,19 +106,30 @@ __device__ __forceinline__ void row_of(const Params& p, int h, long long b, int 
 
 // Vector form: 16-byte chunks.  Interleaved: unit c = chunk c (its pairs lie inside it; pairs from P on are copied).
 // Half-split: units 0 .. P/V-1 are pairs of chunks (c, P/V + c), the rest single chunks that are copied.
+constexpr int kTable = 2048;  // P <= V * units per token, V <= 8, and a block's tokens have at most kThreads units
 template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
 rotary_vec_kernel(const Params p) {
   constexpr int V = 16 / sizeof(T);
   constexpr int kPairs = INTERLEAVED ? V / 2 : V;
   constexpr int kFly = 4;  // heads in flight
-  const long long unit = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (unit >= p.units) return;
-  const long long token = unit / p.per_token;
-  const int c = (int)(unit - token * p.per_token);
-  const long long b = token / p.S;
-  const int tok = (int)(token - b * p.S);
-  const int32_t* pos = p.positions + b * p.pos_b + tok * p.pos_s;
+  __shared__ float2 table[kTable];
+  const long long token0 = (long long)blockIdx.x * p.tokens_per_block;
+  const int here = (int)min((long long)p.tokens_per_block, p.tokens - token0);
+  for (int i = threadIdx.x; i < here * p.P; i += kThreads) {
+    const int t = i / p.P, pair = i - t * p.P;
+    const long long token = token0 + t, b = token / p.S;
+    float c, s;
+    pair_sincos(p, p.positions + b * p.pos_b + (token - b * p.S) * p.pos_s, pair, c, s);
+    table[i] = make_float2(c, s);
+  }
+  __syncthreads();
+  const int units = p.tokens_per_block * p.per_token;
+  const int lane = threadIdx.x / units, unit = threadIdx.x - lane * units;  // head lane, unit inside the block
+  const int t = unit / p.per_token, c = unit - t * p.per_token;
+  if (lane >= p.head_lanes || t >= here) return;
+  const long long b = (token0 + t) / p.S;
+  const int tok = (int)(token0 + t - b * p.S);
   const int half_chunks = p.P / V;
   const bool turned = INTERLEAVED || c < half_chunks;  // half-split: the tail units only copy
   float cs[kPairs], sn[kPairs];
@@ -123,26 +138,30 @@ rotary_vec_kernel(const Params p) {
     const int pair = c * kPairs + i;
     cs[i] = 1.f;
     sn[i] = 0.f;
-    if (turned && pair < p.P) pair_sincos(p, pos, pair, cs[i], sn[i]);
+    if (turned && pair < p.P) {
+      const float2 v = table[t * p.P + pair];
+      cs[i] = v.x;
+      sn[i] = v.y;
+    }
   }
-  const int chunk_a = INTERLEAVED || c < half_chunks ? c : half_chunks + c;
+  const int chunk_a = turned ? c : half_chunks + c;
   const int chunk_b = half_chunks + c;  // half-split only
-  const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(p.heads, h0 + p.heads_per_cta);
-  for (int h = h0; h < h1; h += kFly) {
+  const int h1 = min(p.heads, ((int)blockIdx.y + 1) * p.heads_per_cta), step = p.head_lanes;
+  for (int h = blockIdx.y * p.heads_per_cta + lane; h < h1; h += kFly * step) {
     uint4 a[kFly], z[kFly];
     uint8_t* out[kFly];
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
       const uint8_t* src;
-      row_of(p, min(h + i, h1 - 1), b, tok, src, out[i]);
-      if (h + i < h1) {
+      row_of(p, min(h + i * step, h1 - 1), b, tok, src, out[i]);
+      if (h + i * step < h1) {
         a[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_a);
         if (!INTERLEAVED && turned) z[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_b);
       }
     }
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
-      if (h + i >= h1) break;
+      if (h + i * step >= h1) break;
       uint4* dst = reinterpret_cast<uint4*>(out[i]);
       if (INTERLEAVED) {
         float x[V];
@@ -153,8 +172,16 @@ rotary_vec_kernel(const Params p) {
           x[2 * e] = x0 * cs[e] - x1 * sn[e];
           x[2 * e + 1] = x0 * sn[e] + x1 * cs[e];
         }
-        // (a chunk behind the turned channels leaves with its bits unchanged: NaN payloads too)
-        dst[chunk_a] = (c * kPairs < p.P) ? Io<T>::pack(x) : a[i];
+        uint4 r = Io<T>::pack(x);
+        if ((c + 1) * kPairs > p.P) {
+          // the chunk reaches behind the turned channels: those leave with their bits unchanged
+          const int turned_words = max(0, p.P - c * kPairs) * (int)(2 * sizeof(T)) / 4;
+          if (turned_words <= 0) r.x = a[i].x;
+          if (turned_words <= 1) r.y = a[i].y;
+          if (turned_words <= 2) r.z = a[i].z;
+          if (turned_words <= 3) r.w = a[i].w;
+        }
+        dst[chunk_a] = r;
       } else if (turned) {
         float x[V], y[V];
         Io<T>::unpack(a[i], x);
@@ -209,15 +236,34 @@ rotary_elt_kernel(const Params p) {
 template <typename T>
 static int launch(Params& p, const bsa_rotary_args& a, bool vec, int num_sms, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  if (vec) p.per_token = a.interleaved ? a.D / V : p.P / V + (a.D - 2 * p.P) / V;
-  else p.per_token = p.P + (a.D - 2 * p.P);
-  p.units = (long long)a.B * a.S * p.per_token;
-  const long long blocks = (p.units + kThreads - 1) / kThreads;
+  p.tokens = (long long)a.B * a.S;
+  long long blocks, groups;
+  if (vec) {
+    p.per_token = a.interleaved ? a.D / V : p.P / V + (a.D - 2 * p.P) / V;
+    // Many tokens to a block (head-major rows of neighbouring tokens are neighbours in memory), one head at a time; while
+    // that leaves SMs with less than four blocks, fewer tokens and more heads side by side.
+    p.head_lanes = 1;
+    p.tokens_per_block = kThreads / p.per_token;
+    while (p.tokens_per_block > 1 && 2 * p.head_lanes <= p.heads && p.tokens < 4LL * num_sms * p.tokens_per_block) {
+      p.head_lanes *= 2;
+      p.tokens_per_block = kThreads / (p.per_token * p.head_lanes);
+      if (p.tokens_per_block < 1) p.tokens_per_block = 1;
+    }
+    p.head_lanes = kThreads / (p.tokens_per_block * p.per_token);
+    if (p.head_lanes > p.heads) p.head_lanes = p.heads;
+    blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+    groups = (2LL * num_sms + blocks - 1) / blocks;  // blocks that share tokens, on different heads
+    const long long rounds = (p.heads + p.head_lanes - 1) / p.head_lanes;
+    if (groups > rounds) groups = rounds;
+  } else {
+    p.per_token = p.P + (a.D - 2 * p.P);
+    p.units = p.tokens * p.per_token;
+    blocks = (p.units + kThreads - 1) / kThreads;
+    // one thread serves every head of its pair; heads are dealt to more threads while SMs are short of warps
+    groups = (8LL * num_sms + blocks - 1) / blocks;
+    if (groups > p.heads) groups = p.heads;
+  }
   if (blocks > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_rotary_nd: too many tokens");
-  // One thread can serve every head (the sines are computed once then); heads are dealt to more threads only while
-  // the grid leaves SMs short of warps.
-  long long groups = (8LL * num_sms + blocks - 1) / blocks;
-  if (groups > p.heads) groups = p.heads;
   if (groups > 65535) groups = 65535;
   p.heads_per_cta = (int)((p.heads + groups - 1) / groups);
   const dim3 grid((unsigned)blocks, (unsigned)((p.heads + p.heads_per_cta - 1) / p.heads_per_cta));

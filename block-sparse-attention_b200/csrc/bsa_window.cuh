@@ -9,9 +9,9 @@
 //
 // The kernels work on 128-token key tiles.  The tiles a query tile needs are those its rows' windows touch, walked
 // from the diagonal downwards (so the running maximum is set by visible scores from the first tile on), and then
-// tile 0 once more for the sinks if no window reaches it: sinks <= 128, so that is one tile.  A tile that every row
-// of the query tile sees entirely takes an unmasked path; in the others each thread builds one visibility bit per
-// column of its row.
+// tile 0 once more for the sinks if no window reaches it: sinks <= 128, so that is one tile.  A tile that every row of
+// the query tile sees entirely takes an unmasked path; in the others each thread builds one visibility bit per column
+// of its row, and warps pass over the 32-column groups that none of their rows sees.
 #pragma once
 
 #include "bsa_common.cuh"

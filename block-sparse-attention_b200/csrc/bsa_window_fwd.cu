@@ -22,6 +22,8 @@
 #include "bsa_host.h"
 #include "bsa_window.cuh"
 
+#include <type_traits>
+
 namespace bsa {
 
 struct WinFwdParams {
@@ -38,7 +40,7 @@ struct WinFwdParams {
   int Sq, Sk, NqT, seq_per_tile;
   int D;
   int window, sinks;
-  int max_pages, page_size, num_pages, seg;  // seg = rows of one key box: min(page_size, 128), 128 when contiguous
+  int max_pages, page_size, num_pages, seg, seg_log2;  // seg = rows of one key box: min(page_size, 128), 128 when contiguous
   int splits, num_work;
   float scale_log2;
 };
@@ -136,28 +138,12 @@ __device__ __forceinline__ Row make_row(const WinFwdParams& p, const Item& t, in
   return r;
 }
 
-// Visibility bits of the row in the 128-key tile that starts at key j0.
-__device__ __forceinline__ void row_words(const Row& r, int base, int sinks, int j0, uint32_t* w) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = range_word(r.lo - j0, r.hi - j0, i);
-    if (j0 == 0) w[i] |= range_word(0, min(sinks, r.hi), i);
-  }
-  if (r.tree) {
-    const int d = base - j0;  // draft 0 is column d
-    unsigned long long lo64 = 0, hi64 = 0;
-    if (d > -64 && d < 128) {
-      if (d < 0) lo64 = r.tree >> (-d);
-      else if (d < 64) {
-        lo64 = r.tree << d;
-        hi64 = d ? r.tree >> (64 - d) : 0ull;
-      } else hi64 = r.tree << (d - 64);
-    }
-    w[0] |= (uint32_t)lo64;
-    w[1] |= (uint32_t)(lo64 >> 32);
-    w[2] |= (uint32_t)hi64;
-    w[3] |= (uint32_t)(hi64 >> 32);
-  }
+// Visibility bits of the row among the 32 keys from c0 on.
+__device__ __forceinline__ uint32_t row_word(const Row& r, int base, int sinks, int c0) {
+  uint32_t w = range_word(r.lo - c0, r.hi - c0, 0) | low_bits(min(sinks, r.hi) - c0);
+  const int d = base - c0;  // draft 0 is column d
+  if (r.tree != 0 && d < 32 && d > -64) w |= d >= 0 ? (uint32_t)r.tree << d : (uint32_t)(r.tree >> (-d));
+  return w;
 }
 
 template <bool F16, bool SPLIT>
@@ -414,18 +400,37 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           mbar_arrive(BAR(kPFull));
           continue;
         }
-        float sv[128];
-        uint32_t* su = reinterpret_cast<uint32_t*>(sv);
         const uint32_t t_row = tS + lane_base;
-        float bm;
-        if (whole) {
-          // two 64-column halves; the second arrives while the maximum of the first is taken
+        uint64_t s0 = pack2(0.f, 0.f), s1 = s0;
+        // One body for whole tiles and one for masked tiles, both straight-line: tests inside one body slowed every
+        // tile, and loops over the 32-column groups that a warp sees doubled the time of a tile on the diagonal (4000
+        // clocks against 2000 for the warp that sees all groups; the others wait for it).
+        auto tile = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          float sv[128];
+          uint32_t* su = reinterpret_cast<uint32_t*>(sv);
           float m0, m1;
           tmem_ld32(t_row + 0, su + 0);
           tmem_ld32(t_row + 32, su + 32);
+          uint32_t mw[4];
+          if (kMasked) {
+#pragma unroll
+            for (int c4 = 0; c4 < 4; ++c4) {
+              mw[c4] = row_word(r, t.base, p.sinks, j0 + c4 * 32);
+              if (pages_ok != 0xffffffffu) {  // keys of pages that are not in the pool
+                if (!((pages_ok >> ((c4 * 32) >> p.seg_log2)) & 1u)) mw[c4] &= 0xffff0000u;
+                if (!((pages_ok >> ((c4 * 32 + 16) >> p.seg_log2)) & 1u)) mw[c4] &= 0x0000ffffu;
+              }
+            }
+          }
           tmem_wait_ld();
+          // two 64-column halves; the second arrives while the maximum of the first is taken
           tmem_ld32(t_row + 64, su + 64);
           tmem_ld32(t_row + 96, su + 96);
+          if (kMasked) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c) sv[c] = ((mw[c >> 5] >> (c & 31)) & 1u) ? sv[c] : -INFINITY;
+          }
           m0 = fmax3(sv[0], sv[1], sv[2]);
           m1 = fmax3(sv[3], sv[4], sv[5]);
 #pragma unroll
@@ -435,51 +440,25 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           m0 = fmax3(m0, sv[62], sv[63]);
           tmem_wait_ld();
+          if (kMasked) {
+#pragma unroll
+            for (int c = 64; c < 128; ++c) sv[c] = ((mw[c >> 5] >> (c & 31)) & 1u) ? sv[c] : -INFINITY;
+          }
 #pragma unroll
           for (int c = 64; c < 128; c += 4) {
             m0 = fmax3(m0, sv[c], sv[c + 1]);
             m1 = fmax3(m1, sv[c + 2], sv[c + 3]);
           }
-          bm = fmaxf(m0, m1) * p.scale_log2;
-        } else {
-          uint32_t mw[4];
-          row_words(r, t.base, p.sinks, j0, mw);
-          if (pages_ok != 0xffffffffu) {
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-              uint32_t live = 0;
-              for (int s = 0; s < segs; ++s)
-                if ((pages_ok >> s) & 1u) live |= range_word(s * p.seg, (s + 1) * p.seg, i4);
-              mw[i4] &= live;
-            }
-          }
-          tmem_ld32(t_row + 0, su + 0);
-          tmem_ld32(t_row + 32, su + 32);
-          tmem_ld32(t_row + 64, su + 64);
-          tmem_ld32(t_row + 96, su + 96);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 128; ++c) sv[c] = ((mw[c >> 5] >> (c & 31)) & 1u) ? sv[c] : -INFINITY;
-          float m0 = sv[0], m1 = sv[1];
-#pragma unroll
-          for (int c = 2; c < 128; c += 4) {
-            m0 = fmax3(m0, sv[c], sv[c + 1]);
-            m1 = fmax3(m1, sv[(c + 2) & 127], sv[(c + 3) & 127]);
-          }
-          bm = fmaxf(m0, m1) * p.scale_log2;
-        }
-        const float m_new = fmaxf(m_cur, bm);
-        if (i == 0) {
-          m_cur = m_new;
-        } else {
-          const bool need = (m_new - m_cur) > kRescaleThreshold;
-          if (__any_sync(0xffffffffu, need)) {
+          // the running maximum; O and the sum are rescaled only when it grew by more than the threshold in some row
+          const float m_new = fmaxf(m_cur, fmaxf(m0, m1) * p.scale_log2);
+          if (i == 0) {
+            m_cur = m_new;
+          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > kRescaleThreshold)) {
             const float sc = (m_new == -INFINITY) ? 1.f : ex2_approx(m_cur - m_new);
             m_cur = m_new;
             l_sum *= sc;
-            // rescale O in tensor memory (the previous PV has completed: the commit that signalled this S was
-            // issued after it)
-#pragma unroll
+            // (the previous PV has completed: the commit that signalled this S was issued after it)
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
               tmem_ld32(tO + lane_base + c * 32, o);
@@ -490,38 +469,39 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             tmem_wait_st();
           }
-        }
-        const float neg_m = (m_cur == -INFINITY) ? 0.f : -m_cur;
-        // ---- exponentials, row sum (fp32, before P is rounded to 16 bits for the tensor cores), P to tensor memory
-        const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2);
-        const uint64_t nm2 = pack2(neg_m, neg_m);
-        uint64_t s0 = pack2(0.f, 0.f), s1 = s0;
+          const float neg_m = (m_cur == -INFINITY) ? 0.f : -m_cur;
+          // exponentials, row sum (fp32, before P is rounded to 16 bits for the tensor cores), P to tensor memory
+          const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2);
+          const uint64_t nm2 = pack2(neg_m, neg_m);
 #pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) {
-          uint32_t pk[16];
+          for (int c4 = 0; c4 < 4; ++c4) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = c4 * 32 + e * 2;
-            float x0, x1;
-            unpack2(ffma2(pack2(sv[c], sv[c + 1]), sc2, nm2), x0, x1);
-            x0 = ex2_approx(x0);
-            x1 = ex2_approx(x1);
-            if (e & 1) s1 = fadd2(s1, pack2(x0, x1));
-            else s0 = fadd2(s0, pack2(x0, x1));
-            pk[e] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
+            for (int e = 0; e < 16; ++e) {
+              const int c = c4 * 32 + e * 2;
+              float x0, x1;
+              unpack2(ffma2(pack2(sv[c], sv[c + 1]), sc2, nm2), x0, x1);
+              x0 = ex2_approx(x0);
+              x1 = ex2_approx(x1);
+              if (e & 1) s1 = fadd2(s1, pack2(x0, x1));
+              else s0 = fadd2(s0, pack2(x0, x1));
+              pk[e] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
+            }
+            if (c4 == 2) {  // the first half of P is released on its own barrier, its stores long landed
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(BAR(kPHalf));
+            }
+            tmem_st16(t_row + c4 * 16, pk);
           }
-          if (c4 == 2) {  // the first half of P is released on its own barrier, its stores long landed
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(BAR(kPHalf));
-          }
-          tmem_st16(tS + lane_base + c4 * 16, pk);
-        }
+          tmem_wait_st();
+        };
+        if (whole) tile(std::false_type{});
+        else tile(std::true_type{});
         float y0, y1, y2, y3;
         unpack2(s0, y0, y1);
         unpack2(s1, y2, y3);
         l_sum += (y0 + y1) + (y2 + y3);
-        tmem_wait_st();
         tc_fence_before();
         mbar_arrive(BAR(kPFull));
       }
@@ -529,9 +509,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ring_cnt += 2u * (uint32_t)max(n_it, 0);
 
       // ------------------------------------ tile epilogue ------------------------------------
-      const bool some = r.live && l_sum > 0.f;
-      const float inv = some ? (1.f / l_sum) : 0.f;
-      const float lse = some ? (m_cur + lg2_approx(l_sum)) * kLn2 : -INFINITY;
+      const bool seen = r.live && l_sum > 0.f;
+      const float inv = seen ? (1.f / l_sum) : 0.f;
+      const float lse = seen ? (m_cur + lg2_approx(l_sum)) * kLn2 : -INFINITY;
       if (n_it > 0) {
         ok = mbar_wait(BAR(kOFinal), of_cnt & 1, wctx, 310);
         if (!ok) break;
@@ -550,7 +530,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       // an empty split writes its -inf LSE only: the combine does not read its rows
       if (warp_active && !(SPLIT && n_it <= 0)) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < p.D) {
             float acc[32];
@@ -559,7 +539,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               tmem_ld32(tO + lane_base + c * 32, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) acc[e] = some ? __uint_as_float(o[e]) * inv : 0.f;
+              for (int e = 0; e < 32; ++e) acc[e] = seen ? __uint_as_float(o[e]) * inv : 0.f;
             } else {
 #pragma unroll
               for (int e = 0; e < 32; ++e) acc[e] = 0.f;
@@ -658,7 +638,8 @@ template <bool F16, bool SPLIT>
 static int launch(const WinFwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                   int num_sms, cudaStream_t stream) {
   auto kern = window_fwd_kernel<F16, SPLIT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  static SmemAttribute attribute;
+  cudaError_t e = attribute.set(reinterpret_cast<const void*>(kern), kSmemBytes);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
   const int grid = p.num_work < kCtasPerSm * num_sms ? p.num_work : kCtasPerSm * num_sms;
   kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
@@ -752,6 +733,7 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   p.page_size = paged ? a->page_size : 1;
   p.num_pages = a->num_pages;
   p.seg = paged ? (a->page_size < 128 ? a->page_size : 128) : 128;
+  for (p.seg_log2 = 4; (1 << p.seg_log2) < p.seg;) ++p.seg_log2;
   p.splits = a->splits;
   const long long work = (long long)p.B * p.Hidx * p.NqT * p.splits;
   if (work > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 work items");
