@@ -127,6 +127,7 @@ class WindowFwdArgs(ctypes.Structure):
         ("tree_mask", ctypes.c_void_p),
         ("partial_o", ctypes.c_void_p),
         ("partial_lse", ctypes.c_void_p),
+        ("joins", ctypes.c_void_p),
         ("status", ctypes.c_void_p),
         ("q_stride", _c_i64x3),
         ("k_stride", _c_i64x3),
@@ -145,7 +146,8 @@ class WindowFwdArgs(ctypes.Structure):
         ("page_size", ctypes.c_int32),
         ("num_pages", ctypes.c_int32),
         ("pack_gqa", ctypes.c_int32),
-        ("splits", ctypes.c_int32),
+        ("stream_ctas", ctypes.c_int32),
+        ("stream_lists", ctypes.c_int32),
         ("softmax_scale", ctypes.c_float),
     ]
 

@@ -102,9 +102,11 @@ def cached_attn_fwd(
     pack = 1 < G <= 128
     capacity = page_table.shape[1] * page_size
     span = min(T, 128) + min(window, capacity)
-    key_tiles = min(_ceil_div(capacity, 128), _ceil_div(span, 128) + 2)
+    key_tiles, in_window = _ceil_div(capacity, 128), _ceil_div(span, 128) + 2
+    ragged = key_tiles <= in_window  # the lists are as long as the sequences, not as the window
+    key_tiles = min(key_tiles, in_window)
     _launch_window_fwd(q, k_cache, v_cache, out, lse_buf, layout, (B, Hq, Hkv, T, 0, D), kv_lens=cache_lens,
-                       window=window, sinks=sink_tokens, scale=scale, pack_gqa=pack, key_tiles=key_tiles,
+                       window=window, sinks=sink_tokens, scale=scale, pack_gqa=pack, key_tiles=key_tiles, ragged=ragged,
                        page_table=page_table, tree_mask=tree_mask, page_size=page_size)
     return out, lse_buf
 

@@ -67,17 +67,18 @@ def _can_hold(t: torch.Tensor, st) -> bool:
             and t.data_ptr() % 16 == 0)
 
 
-def _window_splits(items: int, key_tiles: int, num_sms: int) -> int:
-    """Number of parts the key tiles of a query tile are dealt to.  Two CTAs fit an SM; when the query tiles alone fill
-    less than half of those places, each is split as often as the places (and its key tiles) allow.  Splitting costs a
-    second launch and fp32 partial rows, so a grid that is half full already stays unsplit."""
+def _stream_ctas(items: int, key_tiles: int, ragged: bool, num_sms: int) -> int:
+    """How the work of a call is dealt: 0 = whole query tiles in turn, otherwise the number of CTAs that share the list of
+    all key tiles evenly.  Sharing costs a second launch and fp32 rows of the cut query tiles, so it is for query tiles
+    that do not fill the two places of every SM, and for lists of unequal lengths that only the device knows while the
+    places get less than eight query tiles each (they do not even out)."""
     places = 2 * num_sms
-    if items < 1 or 2 * items > places:
-        return 1
-    return max(1, min(places // items, key_tiles, 256))
+    if items >= (8 * places if ragged else places) or key_tiles <= 1 or items * (key_tiles + 1) >= 1 << 31:
+        return 0
+    return min(places, items * key_tiles)
 
 
-def _launch_window_fwd(q, k, v, out, lse, layout, shape, *, kv_lens, window, sinks, scale, pack_gqa, key_tiles,
+def _launch_window_fwd(q, k, v, out, lse, layout, shape, *, kv_lens, window, sinks, scale, pack_gqa, key_tiles, ragged,
                        page_table=None, tree_mask=None, page_size=0):
     """``shape`` is (B, Hq, Hkv, Sq, Sk, D); with a page table, k and v are [pages, Hkv, page_size, D] pools."""
     lib = _cabi.load()
@@ -94,20 +95,27 @@ def _launch_window_fwd(q, k, v, out, lse, layout, shape, *, kv_lens, window, sin
     if lse is not None and not lse.is_contiguous():
         lse_k = torch.empty(lse.shape, dtype=torch.float32, device=device)
 
-    items = B * (_ceil_div(Sq, 128 // (Hq // Hkv)) * Hkv if pack_gqa else _ceil_div(Sq, 128) * Hq)
-    splits = _window_splits(items, key_tiles, lib.bsa_num_sms(device.index))
-    partial_o = partial_lse = None
-    if splits > 1:
-        rows = splits * B * Hq * Sq
-        partial = q.new_empty(rows * (D + 1), dtype=torch.float32)
-        partial_o = partial.data_ptr()
+    per_tile = 128 // (Hq // Hkv) if pack_gqa else 128  # query tokens of a tile
+    items = B * _ceil_div(Sq, per_tile) * (Hkv if pack_gqa else Hq)
+    ctas = _stream_ctas(items, key_tiles, ragged, lib.bsa_num_sms(device.index))
+    joins = partial_o = partial_lse = None
+    lists = 1
+    if ctas:
+        tiles = _ceil_div(Sq, per_tile)
+        if page_table is not None and 1 < tiles <= ctas:  # new tokens over a long past: nearly the same keys
+            lists = tiles
+            ctas -= ctas % lists
+        rows = 2 * ctas * min(Sq, per_tile) * (Hq // Hkv if pack_gqa else 1)
+        workspace = q.new_empty(4 * ctas + rows * (D + 1), dtype=torch.float32)
+        joins = workspace.data_ptr()
+        partial_o = joins + 16 * ctas
         partial_lse = partial_o + 4 * rows * D
     paged = page_table is not None
     args = _cabi.WindowFwdArgs(
         q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr(), out_k.data_ptr(), _cabi.ptr(lse_k), _cabi.ptr(kv_lens),
-        _cabi.ptr(page_table), _cabi.ptr(tree_mask), partial_o, partial_lse, _cabi.status_buffer(device).data_ptr(), q_st,
+        _cabi.ptr(page_table), _cabi.ptr(tree_mask), partial_o, partial_lse, joins, _cabi.status_buffer(device).data_ptr(), q_st,
         k_st, v_st, o_st, _dtype_code(q.dtype), B, Hq, Hkv, Sq, Sk, D, window, sinks, page_table.shape[1] if paged else 0,
-        page_size, k.shape[0] if paged else 0, 1 if pack_gqa else 0, splits, scale)
+        page_size, k.shape[0] if paged else 0, 1 if pack_gqa else 0, ctas, lists, scale)
     _cabi.launch(lib.bsa_window_fwd, "bsa_window_fwd", device, args)
     if out_k is not out:
         (out if layout == "bhsd" else out.transpose(1, 2)).copy_(out_k)
@@ -192,7 +200,7 @@ def window_attn_fwd(
     span = min(Sq, 128) + min(window, Sk)
     key_tiles = min(_ceil_div(Sk, 128), _ceil_div(span, 128) + 2)
     _launch_window_fwd(q, k, v, out, lse_buf, layout, shape, kv_lens=kv_lens, window=window, sinks=sink_tokens,
-                       scale=scale, pack_gqa=pack, key_tiles=key_tiles)
+                       scale=scale, pack_gqa=pack, key_tiles=key_tiles, ragged=False)
     return out, lse_buf
 
 

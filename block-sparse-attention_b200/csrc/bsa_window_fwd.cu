@@ -12,8 +12,12 @@
 //
 // Rows of a query tile: 128 positions of one head, or, packed, seq_per_tile = floor(128 / G) positions x the G heads
 // that share a KV head, so that a key tile is read once for the group.  Packing pays when one head cannot fill a
-// tile; the host packs below 128 query tokens.  With few items the key tiles of an item are dealt to several splits,
-// whose fp32 partial rows window_combine_kernel joins.
+// tile; the host packs below 128 query tokens.
+//
+// Two ways of dealing the work: whole query tiles in turn, or - when those are few or of unequal lengths - equal runs of
+// the list of all key tiles of all query tiles ("stream").  A run may begin and end inside a query tile: such pieces
+// leave fp32 rows and their LSE in one of the CTA's two slots of the workspace, and window_join_kernel joins them.  The
+// lengths are on the device only, so every warp finds its CTA's run itself from the lengths' prefix sums.
 //
 // Keys behind the sequence's end may hold anything (padding, the unused end of a page): their scores are replaced,
 // not added to, and their V rows are set to zero in shared memory before PV reads them (0 * NaN is NaN).
@@ -33,15 +37,17 @@ struct WinFwdParams {
   uint8_t* out;
   long long o_stride_b, o_stride_h, o_stride_s;  // bytes
   float* lse;
-  float* partial_o;
-  float* partial_lse;
+  float* partial_o;    // stream: [2 * CTAs, slot_rows, D]
+  float* partial_lse;  // [2 * CTAs, slot_rows]
+  int4* joins;         // [CTAs]: the query tile whose first piece ends the CTA's run (b, hidx, m, pieces), pieces 0: none
   int* status;
   int B, Hq, Hkv, G, Hidx, packed;
-  int Sq, Sk, NqT, seq_per_tile;
+  int Sq, Sk, NqT, seq_per_tile, slot_rows;
   int D;
   int window, sinks;
   int max_pages, page_size, num_pages, seg, seg_log2;  // seg = rows of one key box: min(page_size, 128), 128 when contiguous
-  int splits, num_work;
+  int ctas, lists;  // stream
+  int num_work;     // query tiles
   float scale_log2;
 };
 
@@ -51,30 +57,25 @@ constexpr int kSoftmaxThreads = 128;
 constexpr int kMmaWarp = 4;
 constexpr int kLoadWarp = 5;
 constexpr int kCtasPerSm = 2;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 48;  // 128 threads each: together the 256 x 128 the CTA is launched with
+static_assert(kSoftmaxRegs + kOtherRegs == 2 * 128, "register split");
 constexpr int kTileBytes = 128 * 128 * 2;
 constexpr int kSlabBytes = 128 * 128;
 constexpr int kStages = 2;
-constexpr int kSmemBytes = kTileBytes + kStages * kTileBytes + 256 + 16;
+constexpr int kSmemBytes = kTileBytes + kStages * kTileBytes + 256 + 16 + 8 * 32;  // tiles, barriers, misc, places
 static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 196 * 1024, "two CTAs per SM");
 
 struct Item {
-  int b, m, split;
-  int hkv, g, hidx;
-  int len, base;  // tokens of the sequence, position of query row 0
-  int seq0, nseq; // query tokens of the tile
-  int p_lo, p_hi; // range of the positions of its rows
+  int b, m, hkv, g, hidx;
+  int len, base;   // tokens of the sequence, position of query row 0
+  int seq0, nseq;  // query tokens of the tile
+  int p_lo, p_hi;  // range of the positions of its rows
   TileList tiles;
-  int it_begin, it_end;
+  int it_begin, it_end;  // this piece of the list of key tiles
+  int slot;              // workspace slot of the piece, -1: the piece is the whole list
 };
 
-__device__ __forceinline__ Item decode_item(const WinFwdParams& p, int w) {
-  Item t;
-  t.split = w % p.splits;
-  int r = w / p.splits;
-  t.m = r % p.NqT;
-  r /= p.NqT;
-  t.hidx = r % p.Hidx;
-  t.b = r / p.Hidx;
+__device__ __forceinline__ void describe(const WinFwdParams& p, Item& t) {
   t.hkv = p.packed ? t.hidx : t.hidx / p.G;
   t.g = p.packed ? 0 : t.hidx % p.G;
   t.len = p.kv_lens ? max(0, min(p.kv_lens[t.b], p.Sk)) : p.Sk;
@@ -89,9 +90,134 @@ __device__ __forceinline__ Item decode_item(const WinFwdParams& p, int w) {
     t.p_hi = t.p_lo + t.nseq - 1;
   }
   t.tiles = window_tiles(t.p_lo, t.p_hi, t.len, p.window, p.sinks);
-  t.it_begin = (int)(((long long)t.tiles.n * t.split) / p.splits);
-  t.it_end = (int)(((long long)t.tiles.n * (t.split + 1)) / p.splits);
-  return t;
+}
+
+// A query tile without key tiles still has its zeros to write: it counts as one.
+__device__ __forceinline__ int item_cost(const WinFwdParams& p, int b, int m) {
+  Item t;
+  t.b = b;
+  t.m = m;
+  t.hidx = 0;
+  describe(p, t);
+  return max(t.tiles.n, 1);
+}
+// The list that a stream run is cut from: (sequence, head, query tile) in this order, all query tiles or only the CTA's
+// one (p.lists = NqT lists side by side, whose CTAs walk the same keys at the same time: one read from HBM serves them).
+__device__ __forceinline__ int list_first(const WinFwdParams& p) { return p.lists > 1 ? (int)blockIdx.x % p.lists : 0; }
+__device__ __forceinline__ int list_end(const WinFwdParams& p) { return p.lists > 1 ? (int)blockIdx.x % p.lists + 1 : p.NqT; }
+__device__ __forceinline__ int head_cost(const WinFwdParams& p, int b) {  // one head's query tiles
+  int c = 0;
+  for (int m = list_first(p); m < list_end(p); ++m) c += item_cost(p, b, m);
+  return c;
+}
+
+// Where the next piece of a CTA begins.  Kept in shared memory, one copy for each warp: in registers it cost the
+// softmax warps spills.
+struct Place {
+  int b, hidx, m, it;
+  int left;  // key tiles left of the CTA's run
+  int q, r;  // of Runs
+};
+
+// CTA c of the n that have work gets all / n key tiles, and one of the all % n that are left over.
+struct Runs {
+  int q, r;
+  __device__ __forceinline__ int begin(int c) const { return c * q + min(c, r); }
+  __device__ __forceinline__ int holder(int x) const { return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q; }
+};
+
+// Called by whole warps.  (All sums fit 32 bits: the host deals whole query tiles otherwise.)
+__device__ __forceinline__ void first_place(const WinFwdParams& p, Place* at) {
+  const int lane = threadIdx.x & 31;
+  Place s;
+  s.b = s.hidx = s.it = s.left = 0;
+  s.m = list_first(p);
+  int all = 0;
+  for (int b = lane; b < p.B; b += 32) all += head_cost(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  all *= p.Hidx;
+  const int cta = (int)blockIdx.x / p.lists, n = min(all, p.ctas / p.lists);
+  const Runs runs{all / n, all % n};
+  s.q = runs.q;
+  s.r = runs.r;
+  if (cta < n) {
+    int lo = runs.begin(cta);
+    s.left = runs.begin(cta + 1) - lo;
+    int per_head = 1;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {  // the sequence that holds tile `lo` of the list
+      const int mine = b0 + lane < p.B ? head_cost(p, b0 + lane) : 0;
+      int upto = mine * p.Hidx;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += below;
+      }
+      const uint32_t over = __ballot_sync(0xffffffffu, upto > lo);
+      if (over) {
+        const int holder = __ffs(over) - 1;
+        s.b = b0 + holder;
+        per_head = __shfl_sync(0xffffffffu, mine, holder);
+        lo -= __shfl_sync(0xffffffffu, upto, holder) - per_head * p.Hidx;
+        break;
+      }
+      lo -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    s.hidx = lo / per_head;
+    lo -= s.hidx * per_head;
+    for (int c; lo >= (c = item_cost(p, s.b, s.m)); ++s.m) lo -= c;
+    s.it = lo;
+  }
+  if (lane == 0) *at = s;
+  __syncwarp();
+}
+
+// The CTA's next piece.  `whole` counts the query tiles when whole ones are dealt.
+template <bool STREAM>
+__device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int& whole, Item& t) {
+  if (STREAM) {
+    Place s = *at;
+    __syncwarp();
+    if (s.left <= 0) return false;
+    t.b = s.b;
+    t.hidx = s.hidx;
+    t.m = s.m;
+    describe(p, t);
+    const int cost = max(t.tiles.n, 1);
+    const int end = min(cost, s.it + s.left);
+    t.it_begin = s.it;
+    t.it_end = min(end, t.tiles.n);
+    t.slot = (s.it == 0 && end == cost) ? -1 : 2 * (int)blockIdx.x + (s.it > 0 ? 0 : 1);
+    s.left -= end - s.it;
+    s.it = 0;
+    if (++s.m == list_end(p)) {
+      s.m = list_first(p);
+      if (++s.hidx == p.Hidx) {
+        s.hidx = 0;
+        ++s.b;
+      }
+    }
+    if ((threadIdx.x & 31) == 0) *at = s;
+    __syncwarp();
+    return true;
+  }
+  if (whole >= p.num_work) return false;
+  int r = whole;
+  t.m = r % p.NqT;
+  r /= p.NqT;
+  t.hidx = r % p.Hidx;
+  t.b = r / p.Hidx;
+  describe(p, t);
+  t.it_begin = 0;
+  t.it_end = t.tiles.n;
+  t.slot = -1;
+  whole += gridDim.x;
+  return true;
+}
+
+// The sinks' tile takes MMAs of 32 or 64 columns where that holds them all (a fifth of a whole tile's time).
+__device__ __forceinline__ bool narrow_end(const WinFwdParams& p, const Item& t) {
+  return p.sinks <= 64 && t.tiles.n > t.tiles.n_win && t.it_end == t.tiles.n && t.it_begin < t.it_end;
 }
 
 // What a query row sees: keys [lo, hi) and [0, sinks) below hi, and the drafts of `tree` (bit u = key base + u).
@@ -146,7 +272,7 @@ __device__ __forceinline__ uint32_t row_word(const Row& r, int base, int sinks, 
   return w;
 }
 
-template <bool F16, bool SPLIT>
+template <bool F16, bool STREAM>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const WinFwdParams p) {
@@ -169,6 +295,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   WaitCtx wctx{&s_abort, p.status};
+  Place* place = reinterpret_cast<Place*>(reinterpret_cast<uint8_t*>(bars) + 272 + warp * 32);
+  static_assert(sizeof(Place) <= 32, "place");
 
   if (threadIdx.x == 0) {
     s_abort = 0;
@@ -190,6 +318,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tmem_alloc(smem_u32(&s_tmem_base), 256);
     tmem_relinquish();
   }
+  if (STREAM && warp <= kLoadWarp) first_place(p, place);  // every warp for itself
+  int whole_next = blockIdx.x;
   if (warp == kLoadWarp && lane == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
@@ -203,15 +333,22 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (warp == kLoadWarp) {
     // ======================================= TMA producer =======================================
-    setmaxnreg_dec<40>();
+    setmaxnreg_dec<kOtherRegs>();
     uint32_t ring_cnt = 0, q_cnt = 0;
     bool ok = true;
     const uint32_t q_bytes = 2u * 128u * (uint32_t)(p.packed ? p.G * p.seq_per_tile : 128);
     const int segs = 128 / p.seg;  // key boxes of a tile
-    for (int w = blockIdx.x; w < p.num_work && ok; w += gridDim.x) {
-      const Item t = decode_item(p, w);
+    int4 join = make_int4(0, 0, 0, 0);
+    Item t;
+    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       if (n_it <= 0) continue;
+      if (STREAM && t.slot >= 0 && (t.slot & 1)) {  // the rest of this query tile begins the runs of the CTAs behind
+        const Runs runs{place->q, place->r};
+        const int cta = (int)blockIdx.x / p.lists;
+        const int last = runs.holder(runs.begin(cta + 1) + t.tiles.n - t.it_end - 1);
+        join = make_int4(t.b, t.hidx, t.m, last - cta + 1);
+      }
       ok = mbar_wait(BAR(kQEmpty), (q_cnt & 1) ^ 1, wctx, 100);
       if (!ok) break;
       if (lane == 0) {
@@ -266,9 +403,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
       }
     }
+    if (STREAM && lane == 0) p.joins[blockIdx.x] = join;
   } else if (warp == kMmaWarp) {
     // ========================================= MMA issue ========================================
-    setmaxnreg_dec<40>();
+    setmaxnreg_dec<kOtherRegs>();
     constexpr uint32_t kFmt = F16 ? 0u : 1u;
     const uint32_t idesc_qk = umma_idesc(kFmt, kFmt, 0, 0, 128, 128);
     const uint32_t idesc_pv = umma_idesc(kFmt, kFmt, 0, 1, 128, (uint32_t)p.D);
@@ -279,23 +417,28 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint64_t k_desc0 = umma_desc_sw128(smem_u32(sKV), 0, 1024);                     // K-major view
     const uint64_t v_desc0 = umma_desc_sw128(smem_u32(sKV), (uint32_t)kSlabBytes, 1024);  // MN-major view
     bool ok = true;
-    for (int w = blockIdx.x; w < p.num_work && ok; w += gridDim.x) {
-      const Item t = decode_item(p, w);
+    Item t;
+    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       if (n_it <= 0) continue;
       ok = mbar_wait(BAR(kQFull), q_cnt & 1, wctx, 200);
       if (!ok) break;
       ++q_cnt;
-      auto issue_qk = [&](bool last) -> bool {
+      const bool narrow = narrow_end(p, t);
+      const int n_main = n_it - (narrow ? 1 : 0);
+      const int groups = (p.sinks + 31) / 32;  // of the narrow tile
+      auto issue_qk = [&](auto is_narrow, bool last) -> bool {
         const uint32_t stage = ring_pos % NS;
         if (!mbar_wait(BAR(kKvFull + stage), (ring_pos / NS) & 1, wctx, 201)) return false;
         ++ring_pos;
         tc_fence_after();
         const uint64_t kd = k_desc0 + (uint64_t)stage * (kTileBytes >> 4);
+        // (the columns of whole tiles are a constant: with a computed number every tile's MMAs were issued more slowly)
+        const uint32_t idesc = decltype(is_narrow)::value ? umma_idesc(kFmt, kFmt, 0, 0, 128, 32u * groups) : idesc_qk;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint64_t off = (uint64_t)((k >> 2) * (kSlabBytes >> 4) + (k & 3) * 2);
-          umma_f16_ss_led(tS, q_desc + off, kd + off, idesc_qk, k > 0, (k < qk_steps) ? led : 0u);
+          umma_f16_ss_led(tS, q_desc + off, kd + off, idesc, k > 0, (k < qk_steps) ? led : 0u);
         }
         umma_commit_led(BAR(kSFull), led);
         umma_commit_led(BAR(kKvEmpty + stage), led);
@@ -303,7 +446,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         __syncwarp();
         return true;
       };
-      auto issue_pv = [&](int i, bool last) -> bool {
+      auto issue_pv = [&](auto is_narrow, int i, bool last) -> bool {
         const uint32_t stage = ring_pos % NS;
         if (!mbar_wait(BAR(kKvFull + stage), (ring_pos / NS) & 1, wctx, 202)) return false;
         ++ring_pos;
@@ -315,25 +458,34 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           for (int k = k0; k < k1; ++k)
             umma_f16_ts_led(tO, tS + (uint32_t)k * 8u, vd + (uint64_t)(k * 128), idesc_pv, (i > 0) || (k > 0), led);
         };
-        pv_steps(0, 4);
+        if (decltype(is_narrow)::value) {
+          pv_steps(0, 2);
+          if (groups > 1) pv_steps(2, 4);
+        } else {
+          pv_steps(0, 4);
+        }
         if (!mbar_wait(BAR(kPFull), p_cnt & 1, wctx, 204)) return false;
         ++p_cnt;
         tc_fence_after();
-        pv_steps(4, 8);
+        if (!decltype(is_narrow)::value) pv_steps(4, 8);
         umma_commit_led(BAR(kKvEmpty + stage), led);
         if (last) umma_commit_led(BAR(kOFinal), led);
         __syncwarp();
         return true;
       };
-      ok = issue_qk(n_it == 1);
-      for (int i = 0; i < n_it && ok; ++i) {
-        ok = issue_pv(i, i == n_it - 1);
-        if (ok && i + 1 < n_it) ok = issue_qk(i + 2 == n_it);
+      ok = n_main > 0 ? issue_qk(std::false_type{}, n_it == 1) : true;
+      for (int i = 0; i < n_main && ok; ++i) {
+        ok = issue_pv(std::false_type{}, i, i == n_it - 1);
+        if (ok && i + 1 < n_main) ok = issue_qk(std::false_type{}, i + 2 == n_it);
+      }
+      if (narrow && ok) {
+        ok = issue_qk(std::true_type{}, true);
+        if (ok) ok = issue_pv(std::true_type{}, n_main, true);
       }
     }
   } else if (warp < 4) {
     // ===================================== softmax + epilogue ===================================
-    setmaxnreg_inc<216>();
+    setmaxnreg_inc<kSoftmaxRegs>();
     const int row = threadIdx.x;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     uint32_t s_cnt = 0, of_cnt = 0, ring_cnt = 0;
@@ -342,8 +494,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int heads = p.packed ? p.G : 1;  // heads of a tile's rows
     const int segs = 128 / p.seg;
 
-    for (int w = blockIdx.x; w < p.num_work && ok; w += gridDim.x) {
-      const Item t = decode_item(p, w);
+    Item t;
+    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       float m_cur = -INFINITY;  // running max, log2 domain (scale applied)
       float l_sum = 0.f;        // running sum relative to m_cur
@@ -355,6 +507,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // every row of the tile sees all keys of [free_lo, free_hi) that exist
       const int free_lo = min(t.p_hi, t.len - 1) - p.window + 1;
       const int free_hi = p.tree_mask ? t.base : t.p_lo + 1;
+      const bool narrow = narrow_end(p, t);
 
       for (int i = 0; i < n_it && ok; ++i) {
         const int it = t.it_begin + i;
@@ -402,6 +555,43 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         const uint32_t t_row = tS + lane_base;
         uint64_t s0 = pack2(0.f, 0.f), s1 = s0;
+        // The running maximum takes in a tile's largest score; O and the sum are rescaled only when it grew by more than
+        // the threshold in some row of the warp.  Returns the addend of the exponents.
+        auto grow = [&](float top) -> float {
+          const float m_new = fmaxf(m_cur, top * p.scale_log2);
+          if (i == 0) {
+            m_cur = m_new;
+          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > kRescaleThreshold)) {
+            const float sc = (m_new == -INFINITY) ? 1.f : ex2_approx(m_cur - m_new);
+            m_cur = m_new;
+            l_sum *= sc;
+            // (the previous PV has completed: the commit that signalled this S was issued after it)
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + lane_base + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * sc);
+              tmem_st32(tO + lane_base + c * 32, o);
+            }
+            tmem_wait_st();
+          }
+          return (m_cur == -INFINITY) ? 0.f : -m_cur;
+        };
+        // P of 32 columns, rounded to 16 bits for the tensor cores, and their sum, in fp32 before the rounding
+        auto exponentials = [&](const float* sv, uint64_t sc2, uint64_t nm2, uint32_t* pk) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            unpack2(ffma2(pack2(sv[2 * e], sv[2 * e + 1]), sc2, nm2), x0, x1);
+            x0 = ex2_approx(x0);
+            x1 = ex2_approx(x1);
+            if (e & 1) s1 = fadd2(s1, pack2(x0, x1));
+            else s0 = fadd2(s0, pack2(x0, x1));
+            pk[e] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
+          }
+        };
         // One body for whole tiles and one for masked tiles, both straight-line: tests inside one body slowed every
         // tile, and loops over the 32-column groups that a warp sees doubled the time of a tile on the diagonal (4000
         // clocks against 2000 for the warp that sees all groups; the others wait for it).
@@ -449,44 +639,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             m0 = fmax3(m0, sv[c], sv[c + 1]);
             m1 = fmax3(m1, sv[c + 2], sv[c + 3]);
           }
-          // the running maximum; O and the sum are rescaled only when it grew by more than the threshold in some row
-          const float m_new = fmaxf(m_cur, fmaxf(m0, m1) * p.scale_log2);
-          if (i == 0) {
-            m_cur = m_new;
-          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > kRescaleThreshold)) {
-            const float sc = (m_new == -INFINITY) ? 1.f : ex2_approx(m_cur - m_new);
-            m_cur = m_new;
-            l_sum *= sc;
-            // (the previous PV has completed: the commit that signalled this S was issued after it)
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + lane_base + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * sc);
-              tmem_st32(tO + lane_base + c * 32, o);
-            }
-            tmem_wait_st();
-          }
-          const float neg_m = (m_cur == -INFINITY) ? 0.f : -m_cur;
-          // exponentials, row sum (fp32, before P is rounded to 16 bits for the tensor cores), P to tensor memory
-          const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2);
-          const uint64_t nm2 = pack2(neg_m, neg_m);
+          const float neg_m = grow(fmaxf(m0, m1));
+          const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2), nm2 = pack2(neg_m, neg_m);
 #pragma unroll
           for (int c4 = 0; c4 < 4; ++c4) {
             uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int c = c4 * 32 + e * 2;
-              float x0, x1;
-              unpack2(ffma2(pack2(sv[c], sv[c + 1]), sc2, nm2), x0, x1);
-              x0 = ex2_approx(x0);
-              x1 = ex2_approx(x1);
-              if (e & 1) s1 = fadd2(s1, pack2(x0, x1));
-              else s0 = fadd2(s0, pack2(x0, x1));
-              pk[e] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
-            }
+            exponentials(sv + c4 * 32, sc2, nm2, pk);
             if (c4 == 2) {  // the first half of P is released on its own barrier, its stores long landed
               tmem_wait_st();
               tc_fence_before();
@@ -496,7 +654,42 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           tmem_wait_st();
         };
+        // the sinks' tile, 32 columns at a time
+        auto narrow_tile = [&]() {
+          float bm = -INFINITY;
+          const int groups = (p.sinks + 31) / 32;
+          auto load_group = [&](int g, float* sv) {
+            uint32_t w = low_bits(p.sinks - 32 * g);
+            if (!((pages_ok >> ((g * 32) >> p.seg_log2)) & 1u)) w &= 0xffff0000u;
+            if (!((pages_ok >> ((g * 32 + 16) >> p.seg_log2)) & 1u)) w &= 0x0000ffffu;
+            tmem_ld32(t_row + g * 32, reinterpret_cast<uint32_t*>(sv));
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sv[e] = ((w >> e) & 1u) ? sv[e] : -INFINITY;
+          };
+#pragma unroll 1
+          for (int g = 0; g < groups; ++g) {
+            float sv[32];
+            load_group(g, sv);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) bm = fmax3(bm, sv[e], sv[e + 1]);
+          }
+          const float neg_m = grow(bm);
+          const uint64_t sc2 = pack2(p.scale_log2, p.scale_log2), nm2 = pack2(neg_m, neg_m);
+#pragma unroll 1
+          for (int g = 0; g < groups; ++g) {  // (P of group 1 overwrites scores of group 0)
+            float sv[32];
+            uint32_t pk[16];
+            load_group(g, sv);
+            exponentials(sv, sc2, nm2, pk);
+            tmem_st16(t_row + g * 16, pk);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(BAR(kPHalf));
+        };
         if (whole) tile(std::false_type{});
+        else if (narrow && i == n_it - 1) narrow_tile();
         else tile(std::true_type{});
         float y0, y1, y2, y3;
         unpack2(s0, y0, y1);
@@ -521,15 +714,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       long long prow = 0;
       float4* dst_f = nullptr;
       uint4* dst_h = nullptr;
-      if (SPLIT) {
-        prow = (((long long)t.split * p.B + t.b) * p.Hq + hq) * p.Sq + seq;
+      const bool piece = STREAM && t.slot >= 0;  // uniform
+      if (piece) {
+        prow = (long long)t.slot * p.slot_rows + row;
         dst_f = reinterpret_cast<float4*>(p.partial_o + prow * p.D);
       } else {
         dst_h = reinterpret_cast<uint4*>(p.out + (long long)t.b * p.o_stride_b + (long long)hq * p.o_stride_h +
                                          (long long)seq * p.o_stride_s);
       }
-      // an empty split writes its -inf LSE only: the combine does not read its rows
-      if (warp_active && !(SPLIT && n_it <= 0)) {
+      if (warp_active) {
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < p.D) {
@@ -545,7 +738,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               for (int e = 0; e < 32; ++e) acc[e] = 0.f;
             }
             if (row_valid) {
-              if (SPLIT) {
+              if (piece) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   dst_f[c * 8 + e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
@@ -568,12 +761,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       tc_fence_before();
       if (row_valid) {
-        if (SPLIT) p.partial_lse[prow] = lse;
+        if (piece) p.partial_lse[prow] = lse;
         else if (p.lse != nullptr) p.lse[((long long)t.b * p.Hq + hq) * p.Sq + seq] = lse;
       }
     }
   } else {
-    setmaxnreg_dec<40>();
+    setmaxnreg_dec<kOtherRegs>();
   }
 
   tc_fence_before();
@@ -584,39 +777,45 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   }
 }
 
-// Joins the splits of a row: lse = log sum_s exp(lse_s), out = sum_s exp(lse_s - lse) O_s.  One warp per row, four
-// channels per lane; splits without a visible key carry -inf and are not read.
+// Joins the pieces of cut query tiles: lse = log sum_s exp(lse_s), out = sum_s exp(lse_s - lse) O_s.  Block (c, y) takes
+// eight rows of the query tile whose first piece ended CTA c's run, if there is one: one warp per row, four channels
+// per lane.  Pieces in which the row sees nothing carry -inf and are not read.
 template <bool F16>
 __global__ void __launch_bounds__(256)
-window_combine_kernel(const float* __restrict__ po, const float* __restrict__ plse, uint8_t* __restrict__ out,
-                      float* __restrict__ lse, int splits, long long rows, int H, int Sq, int D, long long os_b,
-                      long long os_h, long long os_s) {
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
+window_join_kernel(const WinFwdParams p) {
+  const int4 j = p.joins[blockIdx.x];
+  const int pieces = j.w;
+  if (pieces == 0) return;
+  const int heads = p.packed ? p.G : 1, lane = threadIdx.x & 31;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int seq = j.z * p.seq_per_tile + row / heads;
+  if (row >= p.slot_rows || seq >= p.Sq) return;
+  const int hq = p.packed ? j.y * p.G + row % heads : j.y;
+  // the first piece is the last of its CTA's run, each of the others the first of its CTA's
+  auto slot_row = [&](int s) { return (long long)(2 * ((int)blockIdx.x + s * p.lists) + (s == 0 ? 1 : 0)) * p.slot_rows + row; };
   float m = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, plse[(long long)s * rows + row]);
+  for (int s = lane; s < pieces; s += 32) m = fmaxf(m, p.partial_lse[slot_row(s)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float sum = 0.f;
   if (m != -INFINITY)
-    for (int s = lane; s < splits; s += 32) sum += __expf(plse[(long long)s * rows + row] - m);
+    for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot_row(s)] - m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  if (lane == 0 && lse != nullptr) lse[row] = sum > 0.f ? m + __logf(sum) : -INFINITY;
-  if (lane * 4 >= D) return;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[((long long)j.x * p.Hq + hq) * p.Sq + seq] = sum > 0.f ? m + __logf(sum) : -INFINITY;
+  if (lane * 4 >= p.D) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < splits; s0 += 8) {  // eight partial rows in flight
+  for (int s0 = 0; s0 < pieces; s0 += 8) {  // eight partial rows in flight
     float w[8];
     float4 v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int s = s0 + u;
-      const float l = s < splits ? plse[(long long)s * rows + row] : -INFINITY;
+      const float l = s0 + u < pieces ? p.partial_lse[slot_row(s0 + u)] : -INFINITY;
       w[u] = l == -INFINITY ? 0.f : __expf(l - m) * inv;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l != -INFINITY) v[u] = *reinterpret_cast<const float4*>(po + ((long long)s * rows + row) * D + lane * 4);
+      if (l != -INFINITY) v[u] = *reinterpret_cast<const float4*>(p.partial_o + slot_row(s0 + u) * p.D + lane * 4);
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -626,32 +825,28 @@ window_combine_kernel(const float* __restrict__ po, const float* __restrict__ pl
       acc.w = fmaf(w[u], v[u].w, acc.w);
     }
   }
-  const int sq = (int)(row % Sq);
-  const long long bh = row / Sq;
   uint2 packed;
   packed.x = F16 ? pack_f16x2(acc.x, acc.y) : pack_bf16x2(acc.x, acc.y);
   packed.y = F16 ? pack_f16x2(acc.z, acc.w) : pack_bf16x2(acc.z, acc.w);
-  *reinterpret_cast<uint2*>(out + (bh / H) * os_b + (bh % H) * os_h + (long long)sq * os_s + lane * 8) = packed;
+  *reinterpret_cast<uint2*>(p.out + (long long)j.x * p.o_stride_b + (long long)hq * p.o_stride_h +
+                            (long long)seq * p.o_stride_s + lane * 8) = packed;
 }
 
-template <bool F16, bool SPLIT>
+template <bool F16, bool STREAM>
 static int launch(const WinFwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                   int num_sms, cudaStream_t stream) {
-  auto kern = window_fwd_kernel<F16, SPLIT>;
+  auto kern = window_fwd_kernel<F16, STREAM>;
   static SmemAttribute attribute;
   cudaError_t e = attribute.set(reinterpret_cast<const void*>(kern), kSmemBytes);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
-  const int grid = p.num_work < kCtasPerSm * num_sms ? p.num_work : kCtasPerSm * num_sms;
+  const int grid = STREAM ? p.ctas : (p.num_work < kCtasPerSm * num_sms ? p.num_work : kCtasPerSm * num_sms);
   kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window forward launch: %s", cudaGetErrorString(e));
-  if (SPLIT) {
-    const long long rows = (long long)p.B * p.Hq * p.Sq;
-    window_combine_kernel<F16><<<(unsigned)((rows + 7) / 8), 256, 0, stream>>>(
-        p.partial_o, p.partial_lse, p.out, p.lse, p.splits, rows, p.Hq, p.Sq, p.D, p.o_stride_b, p.o_stride_h,
-        p.o_stride_s);
+  if (STREAM) {
+    window_join_kernel<F16><<<dim3((unsigned)p.ctas, (unsigned)((p.slot_rows + 7) / 8)), 256, 0, stream>>>(p);
     e = cudaGetLastError();
-    if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window combine launch: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window join launch: %s", cudaGetErrorString(e));
   }
   return BSA_OK;
 }
@@ -688,11 +883,13 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: a tree has at most %d drafts, over a paged cache", kMaxTreeNodes);
   if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.0e38f)  // the running maximum is taken before scaling
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: softmax_scale must be positive and finite");
-  if (a->splits < 1 || a->splits > 256) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: splits out of [1, 256]");
-  if (a->splits > 1 && (!a->partial_o || !a->partial_lse))
-    return set_error(BSA_ERR_INVALID, "bsa_window_fwd: a split run needs partial buffers");
-  if ((reinterpret_cast<uintptr_t>(a->out) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->partial_o) & 15u) != 0)
-    return set_error(BSA_ERR_INVALID, "out: base address must be 16-byte aligned");
+  if (a->stream_ctas < 0 || a->stream_ctas > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_ctas out of [0, 65535]");
+  if (a->stream_lists > 1 && a->stream_ctas % a->stream_lists != 0)
+    return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_ctas must be a multiple of stream_lists");
+  if (a->stream_ctas > 0 && (!a->partial_o || !a->partial_lse || !a->joins))
+    return set_error(BSA_ERR_INVALID, "bsa_window_fwd: a stream run needs its workspace");
+  if ((reinterpret_cast<uintptr_t>(a->out) & 15u) != 0 || ((reinterpret_cast<uintptr_t>(a->partial_o) | reinterpret_cast<uintptr_t>(a->joins)) & 15u) != 0)
+    return set_error(BSA_ERR_INVALID, "out, partial_o, joins: base address must be 16-byte aligned");
   if ((a->o_stride[0] | a->o_stride[1] | a->o_stride[2]) % 8 != 0)
     return set_error(BSA_ERR_INVALID, "out: strides must be multiples of 8 elements");
   const int G = a->Hq / a->Hkv;
@@ -715,6 +912,7 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   p.lse = a->lse;
   p.partial_o = a->partial_o;
   p.partial_lse = a->partial_lse;
+  p.joins = reinterpret_cast<int4*>(a->joins);
   p.status = a->status;
   p.B = a->B;
   p.Hq = a->Hq;
@@ -734,11 +932,16 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   p.num_pages = a->num_pages;
   p.seg = paged ? (a->page_size < 128 ? a->page_size : 128) : 128;
   for (p.seg_log2 = 4; (1 << p.seg_log2) < p.seg;) ++p.seg_log2;
-  p.splits = a->splits;
-  const long long work = (long long)p.B * p.Hidx * p.NqT * p.splits;
+  p.ctas = a->stream_ctas;
+  p.lists = a->stream_lists > 1 ? a->stream_lists : 1;
+  p.slot_rows = (packed ? G : 1) * (a->Sq < p.seq_per_tile ? a->Sq : p.seq_per_tile);
+  const long long work = (long long)p.B * p.Hidx * p.NqT;
   if (work > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 work items");
-  if ((long long)p.B * p.Hq * p.Sq / 8 >= 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: too many rows");
   p.num_work = (int)work;
+  if (p.ctas > 0 && p.lists > 1 && p.lists != p.NqT)
+    return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_lists must be 1 or the number of query tiles per head (%d)", p.NqT);
+  if (p.ctas > 0 && work * ((Sk + 127) / 128 + 1) > 0x7fffffffLL)
+    return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 key tiles in a stream run");
   p.scale_log2 = a->softmax_scale * kLog2e;
 
   const CUtensorMapDataType dt = a->dtype == BSA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -765,8 +968,8 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   if (a->dtype == BSA_DTYPE_F16)
-    return p.splits > 1 ? winfwd::launch<true, true>(p, tq, tk, tv, num_sms, st)
-                        : winfwd::launch<true, false>(p, tq, tk, tv, num_sms, st);
-  return p.splits > 1 ? winfwd::launch<false, true>(p, tq, tk, tv, num_sms, st)
-                      : winfwd::launch<false, false>(p, tq, tk, tv, num_sms, st);
+    return p.ctas > 0 ? winfwd::launch<true, true>(p, tq, tk, tv, num_sms, st)
+                      : winfwd::launch<true, false>(p, tq, tk, tv, num_sms, st);
+  return p.ctas > 0 ? winfwd::launch<false, true>(p, tq, tk, tv, num_sms, st)
+                    : winfwd::launch<false, false>(p, tq, tk, tv, num_sms, st);
 }

@@ -304,8 +304,13 @@ int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, in
  *   draft's position is then base + popcount - 1, that of a key u likewise; word 0 marks an unused slot (out = 0).
  *
  * pack_gqa != 0: the rows of a tile are floor(128 / G) tokens x the G heads of a KV head.
- * splits > 1: the key tiles of a query tile are dealt to `splits` CTAs; partial_o [splits, B, Hq, Sq, D] and
- * partial_lse [splits, B, Hq, Sq] f32 hold their results, which a second launch of the same call joins.
+ * stream_ctas = 0: whole query tiles are dealt to the CTAs in turn.  stream_ctas > 0: the list of all key tiles of all
+ * query tiles is cut into that many equal runs, for few query tiles or unequal lengths (stream_lists = the number of
+ * query tiles per head: one list for each of them instead, stream_ctas / stream_lists runs each, worked on side by side
+ * so that they share their reads of the keys); partial_o [2 * stream_ctas, R,
+ * D] and partial_lse [2 * stream_ctas, R] f32 (R = rows of a query tile: min(Sq, 128), packed G * min(Sq,
+ * floor(128 / G))) hold the pieces of cut query tiles, joins [4 * stream_ctas] int32 their list; a second launch of the
+ * same call joins them.
  * D = 64, 96 or 128; window >= 1 (2^29 and more: everything before the row); 0 <= sinks <= 128;
  * softmax_scale > 0; page_size 16, 32, 64 or a multiple of 128; lengths up to 2^29.
  */
@@ -320,6 +325,7 @@ typedef struct bsa_window_fwd_args {
   const int64_t* tree_mask;
   float* partial_o;
   float* partial_lse;
+  int32_t* joins;
   int32_t* status;
   int64_t q_stride[3];
   int64_t k_stride[3];
@@ -333,7 +339,8 @@ typedef struct bsa_window_fwd_args {
   int32_t page_size;
   int32_t num_pages;
   int32_t pack_gqa;
-  int32_t splits;
+  int32_t stream_ctas;
+  int32_t stream_lists;
   float softmax_scale;
 } bsa_window_fwd_args;
 

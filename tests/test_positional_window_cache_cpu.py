@@ -124,7 +124,7 @@ def test_c_entry_points_refuse_bad_arguments():
         for n in ("q", "k", "v", "out", "status"):
             setattr(a, n, 1 << 20)
         a.B, a.Hq, a.Hkv, a.Sq, a.Sk, a.D = 1, 2, 2, 8, 8, 64
-        a.window, a.splits, a.softmax_scale = 4, 1, 1.0
+        a.window, a.softmax_scale = 4, 1.0
         for s in ("q_stride", "k_stride", "v_stride", "o_stride"):
             setattr(a, s, (ctypes.c_int64 * 3)(1024, 512, 64))
         for n, v in kw.items():
@@ -132,7 +132,7 @@ def test_c_entry_points_refuse_bad_arguments():
         return lib.bsa_window_fwd(a, None)
 
     for kw in (dict(dtype=1), dict(D=80), dict(B=0), dict(Hq=3), dict(q=None), dict(window=0), dict(sinks=129), dict(sinks=-1),
-               dict(splits=0), dict(splits=2), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(Sk=0),
+               dict(stream_ctas=-1), dict(stream_ctas=2), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(Sk=0),
                dict(Sk=(1 << 29) + 1), dict(out=(1 << 20) + 2), dict(o_stride=(ctypes.c_int64 * 3)(1024, 512, 60)),
                dict(tree_mask=1 << 20), dict(page_table=1 << 20), dict(page_table=1 << 20, page_size=24, max_pages=1, num_pages=1),
                dict(page_table=1 << 20, page_size=16, max_pages=1, num_pages=1),  # no lengths
@@ -157,13 +157,14 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.bsa_cache_keep(1 << 20, 1 << 20, st, st, 1 << 20, 1 << 20, None, 1 << 20, 1 << 20, 1, 1, 1, 1, 64, 1, 16, 1, None) < 0
 
 
-def test_split_rule():
-    from block_sparse_attention.window_attn import _window_splits
-    assert _window_splits(0, 9, 148) == 1
-    assert _window_splits(148, 100, 148) == 2   # half of the places: each tile in two
-    assert _window_splits(149, 100, 148) == 1
-    assert _window_splits(8, 9, 148) == 9       # no more parts than key tiles
-    assert _window_splits(1, 10 ** 6, 148) == 256
+def test_rule_of_dealing_the_work():
+    from block_sparse_attention.window_attn import _stream_ctas
+    assert _stream_ctas(296, 100, False, 148) == 0      # query tiles for both places of every SM
+    assert _stream_ctas(295, 100, False, 148) == 296
+    assert _stream_ctas(295, 1, False, 148) == 0        # nothing to cut
+    assert _stream_ctas(8, 9, False, 148) == 72         # no more CTAs than key tiles
+    assert _stream_ctas(2367, 100, True, 148) == 296    # lengths that only the device knows
+    assert _stream_ctas(2368, 100, True, 148) == 0
 
 
 def test_gradient_formula_against_differences():
