@@ -11,13 +11,15 @@ pages of each sequence in order; entries outside the pool (-1, say) are pages th
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import functools
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _cabi
 from .bsa_attn_interface import _ceil_div
-from .window_attn import _MAX_LEN, _check_lens, _check_qkv, _check_scale, _check_window, _launch_window_fwd, _out_buffers
+from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_lens, _check_qkv, _check_scale, _check_window, _copied, _dense, _fits,
+                          _make_plan, _meta, _run_plan)
 
 _c_i64x3 = _cabi._c_i64x3
 
@@ -26,23 +28,48 @@ __all__ = ["cached_attn_fwd", "tree_mask_from_parents", "cache_append", "cache_k
 MAX_TREE_TOKENS = 64
 
 
-def _check_cache(k_cache, v_cache, page_table, cache_lens, B: int, device):
+def _check_cache(k_cache, v_cache, page_table, cache_lens, B: int, device) -> None:
+    """Everything is a ``_meta``."""
     for t in (k_cache, v_cache):
-        assert t.dim() == 4 and t.device == device, "the pools must be [num_pages, Hkv, page_size, D] on the device of q"
+        assert len(t[0]) == 4 and t[3] == device, "the pools must be [num_pages, Hkv, page_size, D] on the device of q"
         # a pool is never copied: its rows have to be addressable as they lie
-        st = t.stride()
-        assert (st[3] == 1 and t.data_ptr() % 16 == 0 and st[0] > 0 and st[1] > 0 and st[2] > 0
-                and (st[0] | st[1] | st[2]) % 8 == 0), (
-            "the pools must have unit last stride, 16-byte aligned rows and no broadcast dimension")
-    assert k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype, "K and V pools must match"
-    num_pages, Hkv, page_size, D = k_cache.shape
+        assert _fits(t[1]), "the pools must have unit last stride, 16-byte aligned rows and no broadcast dimension"
+    assert k_cache[0] == v_cache[0] and k_cache[2] == v_cache[2], "K and V pools must match"
+    num_pages, Hkv, page_size, _ = k_cache[0]
     assert num_pages >= 1 and Hkv >= 1 and page_size >= 1, "the pools hold no page"
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B, (
+    assert page_table[2] == torch.int32 and len(page_table[0]) == 2 and page_table[0][0] == B, (
         f"page_table must be int32 of shape ({B}, max_pages)")
-    assert page_table.device == device and page_table.shape[1] * page_size <= _MAX_LEN
-    cache_lens = _check_lens(cache_lens, B, device, "cache_lens")
+    assert page_table[3] == device and page_table[0][1] * page_size <= _MAX_LEN
     assert cache_lens is not None, "cache_lens must be given"
-    return page_table.contiguous(), cache_lens
+    _check_lens(cache_lens, B, device, "cache_lens")
+
+
+def _check_pool_address(k_cache, v_cache) -> None:
+    assert (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the pools must be 16-byte aligned"
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _cached_plan(q, k_cache, v_cache, table, lens, tree, out, lse, window, sinks, softmax_scale, layout, want_lse) -> _Plan:
+    window, sinks = _check_window(_MAX_LEN if window is None else window, sinks)
+    _check_qkv(q, k_cache, v_cache, layout)
+    B, Hq, T, D = q[0] if layout == "bhsd" else (q[0][0], q[0][2], q[0][1], q[0][3])
+    _check_cache(k_cache, v_cache, table, lens, B, q[3])
+    _, Hkv, page_size, pool_dim = k_cache[0]
+    assert pool_dim == D and Hq % Hkv == 0, "the pools must match q's head dimension, and Hkv divide Hq"
+    assert page_size in (16, 32, 64) or page_size % 128 == 0, (
+        f"page_size must be 16, 32, 64 or a multiple of 128, got {page_size}")
+    if tree is not None:
+        assert T <= MAX_TREE_TOKENS, f"a tree has at most {MAX_TREE_TOKENS} drafts, got {T}"
+        assert tree[2] == torch.int64 and tree[0] == (B, T) and tree[3] == q[3], (
+            f"tree_mask must be int64 of shape ({B}, {T}) on the device of q")
+    assert T <= _MAX_LEN
+    capacity = table[0][1] * page_size
+    span = min(T, 128) + min(window, capacity)
+    key_tiles, in_window = _ceil_div(capacity, 128), _ceil_div(span, 128) + 2
+    # (within a window the lists of key tiles are about equal, otherwise as long as the sequences)
+    return _make_plan(q, k_cache, v_cache, out, lse, lens, layout, (B, Hq, Hkv, T, 0, D), window=window, sinks=sinks,
+                      scale=_check_scale(softmax_scale, D), pack_gqa=1 < Hq // Hkv <= 128, key_tiles=min(key_tiles, in_window),
+                      ragged=key_tiles <= in_window, empty=table[0][1] == 0, want_lse=want_lse, table=table, tree=tree)
 
 
 def cached_attn_fwd(
@@ -76,39 +103,20 @@ def cached_attn_fwd(
     (``cache_lens[b] < T``), sequences without pages.  Tokens whose page is not in the pool are not visible.  What the
     pages hold behind ``cache_lens[b]`` is never used.  The call is inference only: it has no gradient.
     """
-    window, sink_tokens = _check_window(_MAX_LEN if window is None else window, sink_tokens)
-    _check_qkv(q, k_cache, v_cache, layout)
-    shape = q.shape
-    B, Hq, T, D = shape if layout == "bhsd" else (shape[0], shape[2], shape[1], shape[3])
-    page_table, cache_lens = _check_cache(k_cache, v_cache, page_table, cache_lens, B, q.device)
-    Hkv, page_size = k_cache.shape[1], k_cache.shape[2]
-    assert k_cache.shape[3] == D and Hq % Hkv == 0, "the pools must match q's head dimension, and Hkv divide Hq"
-    assert page_size in (16, 32, 64) or page_size % 128 == 0, (
-        f"page_size must be 16, 32, 64 or a multiple of 128, got {page_size}")
-    scale = _check_scale(softmax_scale, D)
-    if tree_mask is not None:
-        assert T <= MAX_TREE_TOKENS, f"a tree has at most {MAX_TREE_TOKENS} drafts, got {T}"
-        assert tree_mask.dtype == torch.int64 and tree_mask.shape == (B, T) and tree_mask.device == q.device, (
-            f"tree_mask must be int64 of shape ({B}, {T}) on the device of q")
-        tree_mask = tree_mask.contiguous()
-    assert T <= _MAX_LEN
-    out, lse_buf = _out_buffers(q, out, lse, return_lse or lse is not None, B, Hq, T)
-    if out.numel() == 0 or page_table.shape[1] == 0:
-        out.zero_()
-        if lse_buf is not None:
-            lse_buf.fill_(float("-inf"))
-        return out, lse_buf
-    G = Hq // Hkv
-    pack = 1 < G <= 128
-    capacity = page_table.shape[1] * page_size
-    span = min(T, 128) + min(window, capacity)
-    key_tiles, in_window = _ceil_div(capacity, 128), _ceil_div(span, 128) + 2
-    ragged = key_tiles <= in_window  # the lists are as long as the sequences, not as the window
-    key_tiles = min(key_tiles, in_window)
-    _launch_window_fwd(q, k_cache, v_cache, out, lse_buf, layout, (B, Hq, Hkv, T, 0, D), kv_lens=cache_lens,
-                       window=window, sinks=sink_tokens, scale=scale, pack_gqa=pack, key_tiles=key_tiles, ragged=ragged,
-                       page_table=page_table, tree_mask=tree_mask, page_size=page_size)
-    return out, lse_buf
+    want_lse = return_lse or lse is not None
+    plan = _cached_plan(_meta(q), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(tree_mask),
+                        _meta(out), _meta(lse), window, sink_tokens, None if softmax_scale is None else float(softmax_scale),
+                        layout, want_lse)
+    _check_pool_address(k_cache, v_cache)
+    res = _run_plan(plan, q, k_cache, v_cache, out, lse, cache_lens, page_table, tree_mask) if plan.direct else None
+    if res is not None:
+        return res
+    page_table, cache_lens = page_table.contiguous(), cache_lens.contiguous()
+    tree_mask = None if tree_mask is None else tree_mask.contiguous()
+    return _copied(lambda q, k, v: cached_attn_fwd(q, k, v, page_table, cache_lens, tree_mask=tree_mask, window=window,
+                                                   sink_tokens=sink_tokens, softmax_scale=softmax_scale, return_lse=want_lse,
+                                                   layout=layout),
+                   q, k_cache, v_cache, out, lse, layout)
 
 
 def tree_mask_from_parents(parents: torch.Tensor) -> torch.Tensor:
@@ -129,6 +137,54 @@ def tree_mask_from_parents(parents: torch.Tensor) -> torch.Tensor:
     return mask
 
 
+class _WritePlan(NamedTuple):
+    """A checked write of the cache: everything but the addresses, kept as in ``window_attn._Plan``."""
+
+    direct: bool
+    empty: bool
+    strides: tuple = ()
+    sizes: tuple = ()
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _append_plan(k, v, k_cache, v_cache, table, lens, layout) -> _WritePlan:
+    assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
+    assert len(k[0]) == 4 and k[0] == v[0] and k[4] and v[3] == k[3], "k and v must match, on CUDA"
+    assert k[2] == v[2] == k_cache[2] and k[2] in (torch.float16, torch.bfloat16), (
+        "k, v and the pools must all be float16 or all bfloat16")
+    B, H, T, D = k[0] if layout == "bhsd" else (k[0][0], k[0][2], k[0][1], k[0][3])
+    _check_cache(k_cache, v_cache, table, lens, B, k[3])
+    num_pages, pool_heads, page_size, pool_dim = k_cache[0]
+    assert pool_heads == H and pool_dim == D and D % 8 == 0, "the pools must match k's heads and head dimension"
+    if B == 0 or T == 0 or table[0][1] == 0:
+        return _WritePlan(True, True)
+    rows_ok = all(t[1][3] == 1 and (t[1][0] | t[1][1] | t[1][2]) % 8 == 0 for t in (k, v))
+    if not (rows_ok and _dense(table) and _dense(lens)):
+        return _WritePlan(False, False)
+    return _WritePlan(True, False, (_c_i64x3(*_bhsd(k[1], layout)), _c_i64x3(*_bhsd(v[1], layout)), _c_i64x3(*k_cache[1][:3]),
+                                    _c_i64x3(*v_cache[1][:3])), (B, H, T, D, table[0][1], page_size, num_pages))
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _keep_plan(k_cache, v_cache, table, lens, path, path_lens, num_drafts) -> _WritePlan:
+    assert k_cache[4] and k_cache[2] in (torch.float16, torch.bfloat16), "the pools must be float16 or bfloat16 on CUDA"
+    assert isinstance(num_drafts, int) and not isinstance(num_drafts, bool) and num_drafts >= 1, "num_drafts must be an int >= 1"
+    B, device = table[0][0], k_cache[3]
+    _check_cache(k_cache, v_cache, table, lens, B, device)
+    num_pages, H, page_size, D = k_cache[0]
+    assert D % 8 == 0, "the head dimension must be a multiple of 8"
+    assert path[2] == torch.int32 and len(path[0]) == 2 and path[0][0] == B and path[3] == device, (
+        f"path must be int32 of shape ({B}, n) on the device of the pools")
+    assert path_lens is not None, "path_lens must be given"
+    _check_lens(path_lens, B, device, "path_lens")
+    if B == 0:
+        return _WritePlan(True, True)
+    if path[0][1] == 0 or table[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
+        return _WritePlan(False, False)
+    return _WritePlan(True, False, (_c_i64x3(*k_cache[1][:3]), _c_i64x3(*v_cache[1][:3])),
+                      (B, H, num_drafts, path[0][1], D, table[0][1], page_size, num_pages))
+
+
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                  page_table: torch.Tensor, cache_lens: torch.Tensor, *, layout: str = "bhsd"
                  ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -138,29 +194,16 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     Tokens at negative positions and tokens whose page is not in the pool are dropped; nothing else is touched.  A page
     must not be reached through two sequences' tables for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
     """
-    assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
-    assert k.dim() == 4 and k.shape == v.shape and k.is_cuda and v.device == k.device, "k and v must match, on CUDA"
-    assert k.dtype == v.dtype == k_cache.dtype and k.dtype in (torch.float16, torch.bfloat16), (
-        "k, v and the pools must all be float16 or all bfloat16")
-    shape = k.shape
-    B, H, T, D = shape if layout == "bhsd" else (shape[0], shape[2], shape[1], shape[3])
-    page_table, cache_lens = _check_cache(k_cache, v_cache, page_table, cache_lens, B, k.device)
-    num_pages, pool_heads, page_size, pool_dim = k_cache.shape
-    assert pool_heads == H and pool_dim == D and D % 8 == 0, "the pools must match k's heads and head dimension"
-    if B == 0 or T == 0 or page_table.shape[1] == 0:
+    plan = _append_plan(_meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), layout)
+    _check_pool_address(k_cache, v_cache)
+    if plan.empty:
         return k_cache, v_cache
-
-    def rows(t):
-        st = t.stride()
-        if st[3] != 1 or t.data_ptr() % 16 != 0 or (st[0] | st[1] | st[2]) % 8 != 0:
-            t = t.clone(memory_format=torch.contiguous_format)
-            st = t.stride()
-        return t, _c_i64x3(st[0], st[1], st[2]) if layout == "bhsd" else _c_i64x3(st[0], st[2], st[1])
-
-    (k_k, k_st), (v_k, v_st) = rows(k), rows(v)
-    _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, k_k.data_ptr(), v_k.data_ptr(),
-                 k_cache.data_ptr(), v_cache.data_ptr(), k_st, v_st, _cabi.strides3(k_cache), _cabi.strides3(v_cache),
-                 page_table.data_ptr(), cache_lens.data_ptr(), B, H, T, D, page_table.shape[1], page_size, num_pages)
+    at = k.data_ptr(), v.data_ptr()
+    if not plan.direct or (at[0] | at[1]) % 16 != 0:
+        k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+        return cache_append(k, v, k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), layout=layout)
+    _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, *at, k_cache.data_ptr(), v_cache.data_ptr(),
+                 *plan.strides, page_table.data_ptr(), cache_lens.data_ptr(), *plan.sizes)
     return k_cache, v_cache
 
 
@@ -174,26 +217,19 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     number kept.  A path ends early at an entry that is not ascending or not a draft.  A sequence with fewer than
     ``num_drafts`` tokens is left as it is.  A move from or to a page that is not in the pool is dropped.
     """
-    assert k_cache.is_cuda and k_cache.dtype in (torch.float16, torch.bfloat16), "the pools must be float16 or bfloat16 on CUDA"
-    assert isinstance(num_drafts, int) and not isinstance(num_drafts, bool) and num_drafts >= 1, "num_drafts must be an int >= 1"
-    B = cache_lens.shape[0]
-    device = k_cache.device
-    page_table, cache_lens = _check_cache(k_cache, v_cache, page_table, cache_lens, B, device)
-    assert k_cache.shape[3] % 8 == 0, "the head dimension must be a multiple of 8"
-    assert path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == B and path.device == device, (
-        f"path must be int32 of shape ({B}, n) on the device of the pools")
-    path, path_lens = path.contiguous(), _check_lens(path_lens, B, device, "path_lens")
-    assert path_lens is not None, "path_lens must be given"
-    if B == 0:
+    plan = _keep_plan(_meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(path), _meta(path_lens), num_drafts)
+    _check_pool_address(k_cache, v_cache)
+    if plan.empty:
         return cache_lens.clone()
-    if path.shape[1] == 0 or page_table.shape[1] == 0:
-        path = torch.full((B, 1), -1, dtype=torch.int32, device=device)
-    if page_table.shape[1] == 0:
-        page_table = torch.full((B, 1), -1, dtype=torch.int32, device=device)
+    if not plan.direct:
+        if path.shape[1] == 0:
+            path = path.new_full((path.shape[0], 1), -1)
+        if page_table.shape[1] == 0:
+            page_table = page_table.new_full((page_table.shape[0], 1), -1)
+        return cache_keep(k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), path.contiguous(),
+                          path_lens.contiguous(), num_drafts)
     new_lens = torch.empty_like(cache_lens)
-    num_pages, H, page_size, D = k_cache.shape
-    _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", device, k_cache.data_ptr(), v_cache.data_ptr(),
-                 _cabi.strides3(k_cache), _cabi.strides3(v_cache), page_table.data_ptr(), cache_lens.data_ptr(),
-                 path.data_ptr(), path_lens.data_ptr(), new_lens.data_ptr(), B, H, num_drafts, path.shape[1], D,
-                 page_table.shape[1], page_size, num_pages)
+    _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", k_cache.device, k_cache.data_ptr(), v_cache.data_ptr(),
+                 *plan.strides, page_table.data_ptr(), cache_lens.data_ptr(), path.data_ptr(), path_lens.data_ptr(),
+                 new_lens.data_ptr(), *plan.sizes)
     return new_lens

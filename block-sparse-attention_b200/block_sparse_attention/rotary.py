@@ -5,11 +5,13 @@ backward pass is the rotation by the opposite angles, so ``rotary_nd(..., invers
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+import functools
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
 from . import _cabi
+from .window_attn import _meta
 
 __all__ = ["rotary_frequencies", "rotary_nd", "rotary_embedding", "RotaryFunction"]
 
@@ -64,72 +66,102 @@ def rotary_nd(
     positions of any size keep their accuracy.  ``q_out`` / ``k_out`` may be q and k themselves (in place); other overlaps
     are refused.
     """
+    pairs = tuple(map(int, axis_pairs))
+    plan = _rotary_plan(_meta(q), _meta(k), _meta(positions), _meta(inv_freq), pairs, bool(interleaved), bool(inverse),
+                        _meta(q_out), _meta(k_out), layout)
+    if not plan.direct:
+        return rotary_nd(q if q.stride(3) == 1 else q.contiguous(), k if k is None or k.stride(3) == 1 else k.contiguous(),
+                         positions.contiguous(), inv_freq.contiguous(), pairs, interleaved=interleaved, inverse=inverse,
+                         q_out=q_out, k_out=k_out, layout=layout)
+    fresh = q_out is None and (k is None or k_out is None)
+    if q_out is None:
+        q_out = torch.empty_like(q) if plan.q_dense else q.new_empty(plan.q_shape)
+    if k is None:
+        k_out = None
+    elif k_out is None:
+        k_out = torch.empty_like(k) if plan.k_dense else q.new_empty(plan.k_shape)
+    if not fresh:  # fresh outputs overlap nothing
+        _check_overlap(q, q_out, k, k_out)
+    if plan.empty:
+        return q_out, k_out
+    a = _cabi.RotaryArgs.from_buffer_copy(plan.args)
+    a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
+    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    _cabi.launch(_cabi.load().bsa_rotary_nd, "bsa_rotary_nd", q.device, a)
+    return q_out, k_out
+
+
+def _contiguous(t) -> bool:
+    n = t[0]
+    return t[1] == (n[1] * n[2] * n[3], n[2] * n[3], n[3], 1)
+
+
+class _RotaryPlan(NamedTuple):
+    """A checked call: everything but the addresses, kept as in ``window_attn._Plan``."""
+
+    direct: bool  # unit last strides
+    empty: bool
+    q_shape: tuple
+    k_shape: Optional[tuple]
+    args: bytes
+    q_dense: bool = False  # contiguous: empty_like, the cheaper call, gives the same
+    k_dense: bool = False
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _rotary_plan(q, k, positions, inv_freq, pairs, interleaved, inverse, q_out, k_out, layout) -> _RotaryPlan:
     assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
-    assert q.dim() == 4 and q.is_cuda, "q must be a 4-D CUDA tensor"
-    code = _DTYPES.get(q.dtype)
+    assert len(q[0]) == 4 and q[4], "q must be a 4-D CUDA tensor"
+    code, device = _DTYPES.get(q[2]), q[3]
     assert code is not None, "q must be bfloat16, float16 or float32"
-    device = q.device
     h, s = (1, 2) if layout == "bhsd" else (2, 1)  # dimensions of heads and tokens
-    shape = q.shape
-    B, Hq, S, D = shape[0], shape[h], shape[s], shape[3]
+    B, Hq, S, D = q[0][0], q[0][h], q[0][s], q[0][3]
     assert D % 2 == 0 and 2 <= D <= 512, f"head dimension must be even and at most 512, got {D}"
-    pairs = tuple(axis_pairs)
     P, A = sum(pairs), len(pairs)
     assert 1 <= A <= 4 and min(pairs) >= 0 and 1 <= P and 2 * P <= D, (
         f"axis_pairs {pairs} must be 1 to 4 axes with 1 to {D // 2} pairs in all")
     Hk = 0
     if k is not None:
-        assert k.dim() == 4 and k.dtype == q.dtype and k.device == device, "k must match q's type and device"
-        Hk = k.shape[h]
-        assert k.shape[0] == B and k.shape[s] == S and k.shape[3] == D, "k must match q's batch, tokens and head dimension"
-    assert positions.dtype == torch.int32 and positions.device == device, "positions must be int32 on the device of q"
-    at = tuple(positions.shape)
+        assert len(k[0]) == 4 and k[2] == q[2] and k[3] == device, "k must match q's type and device"
+        Hk = k[0][h]
+        assert k[0][0] == B and k[0][s] == S and k[0][3] == D, "k must match q's batch, tokens and head dimension"
+    assert positions[2] == torch.int32 and positions[3] == device, "positions must be int32 on the device of q"
+    at = tuple(positions[0])
     assert at == (S, A) or at == (B, S, A), f"positions has shape {at}, expected ({S}, {A}) or ({B}, {S}, {A})"
-    assert inv_freq.dtype == torch.float32 and inv_freq.device == device and tuple(inv_freq.shape) == (P,), (
+    assert inv_freq[2] == torch.float32 and inv_freq[3] == device and inv_freq[0] == (P,), (
         f"inv_freq must be float32 of shape ({P},) on the device of q")
-    if positions.stride(-1) != 1:
-        positions = positions.contiguous()
-    inv_freq = inv_freq.contiguous()
-    qo, ko = q_out, k_out
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
-    if q_out is None:
-        qo = torch.empty_like(q)
-    if k is None:
-        ko = None
-    elif k_out is None:
-        ko = torch.empty_like(k)
-    if q_out is not None or (k is not None and k_out is not None):  # fresh outputs overlap nothing
-        _check_outputs(q, qo, k, ko)
+    for name, x, out in (("q_out", q, q_out), ("k_out", k, k_out)):
+        if out is not None:
+            assert x is not None and out[0] == x[0] and out[2] == x[2] and out[3] == device, f"{name} must match its input"
+            assert out[1][3] == 1 and all(n == 1 or st > 0 for n, st in zip(out[0], out[1])), (
+                f"{name} must have unit last stride and no broadcast dimension")
+    q_shape, k_shape = tuple(q[0]), None if k is None else tuple(k[0])
     if B == 0 or S == 0 or (Hq == 0 and Hk == 0):
-        return qo, ko
+        return _RotaryPlan(True, True, q_shape, k_shape, b"")
     assert Hq >= 1, "q has no heads"
-    zero = (0, 0, 0)
+    if q[1][3] != 1 or (k is not None and k[1][3] != 1) or (A > 1 and positions[1][-1] != 1) or (P > 1 and inv_freq[1] != (1,)):
+        return _RotaryPlan(False, False, q_shape, k_shape, b"")
 
-    def strides(t):
+    def strides(t, out=None):
         if t is None:
-            return zero
-        st = t.stride()
+            return 0, 0, 0
+        if out is None:  # a fresh contiguous tensor of t's shape
+            n = t[0]
+            st = (n[1] * n[2] * n[3], n[2] * n[3], n[3])
+        else:
+            st = out[1]
         return st[0], st[h], st[s]
 
-    pos_st = positions.stride()
-    a = _cabi.RotaryArgs(
-        q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr(),
-        positions.data_ptr(), inv_freq.data_ptr(), strides(q), strides(k), strides(qo), strides(ko),
-        (pos_st[0] if len(at) == 3 else 0, pos_st[-2]), pairs, A, code, B, Hq, Hk, S, D, 1 if interleaved else 0,
-        1 if inverse else 0)
-    _cabi.launch(_cabi.load().bsa_rotary_nd, "bsa_rotary_nd", device, a)
-    return qo, ko
+    pos_st = positions[1]
+    args = _cabi.RotaryArgs(None, None, None, None, None, None, strides(q, q), strides(k, k), strides(q, q_out), strides(k, k_out),
+                            (pos_st[0] if len(at) == 3 else 0, pos_st[-2]), pairs, A, code, B, Hq, Hk, S, D, int(interleaved),
+                            int(inverse))
+    return _RotaryPlan(True, False, q_shape, k_shape, bytes(args), _contiguous(q), k is not None and _contiguous(k))
 
 
-def _check_outputs(q, qo, k, ko) -> None:
-    for name, x, out in (("q_out", q, qo), ("k_out", k, ko)):
-        if out is not None:
-            assert out.shape == x.shape and out.dtype == x.dtype and out.device == x.device, f"{name} must match its input"
-            assert out.stride(-1) == 1 and all(n == 1 or st > 0 for n, st in zip(out.shape, out.stride())), (
-                f"{name} must have unit last stride and no broadcast dimension")
+def _check_overlap(q, qo, k, ko) -> None:
     if any(t is not None and t.numel() == 0 for t in (q, k)):
         return
     for out, own, other, other_out in ((qo, q, k, ko), (ko, k, q, qo)):

@@ -10,8 +10,9 @@ Query token ``i`` sits at position ``p = i + Sk - Sq``; key ``j`` is visible to 
 """
 from __future__ import annotations
 
+import functools
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -37,34 +38,48 @@ def _check_scale(softmax_scale, D: int) -> float:
     return scale
 
 
-def _check_lens(lens, B: int, device, name: str) -> Optional[torch.Tensor]:
-    if lens is None:
-        return None
-    assert lens.dtype == torch.int32 and lens.shape == (B,), f"{name} must be int32 of shape ({B},)"
-    assert lens.device == device, f"{name} must be on the device of q"
-    return lens.contiguous()
+def _meta(t: Optional[torch.Tensor]):
+    """What the checks of a call look at (everything but the address): the key of its plan."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.is_cuda)
+
+
+def _check_lens(lens, B: int, device, name: str) -> None:
+    """``lens`` is a ``_meta``."""
+    assert lens[2] == torch.int32 and lens[0] == (B,), f"{name} must be int32 of shape ({B},)"
+    assert lens[3] == device, f"{name} must be on the device of q"
 
 
 def _dtype_code(dtype) -> int:
     return _cabi.BSA_DTYPE_F16 if dtype == torch.float16 else _cabi.BSA_DTYPE_BF16
 
 
-def _rows(t: torch.Tensor, layout: str):
-    """(tensor, BHSD strides) the tensor maps can address; copies only views that they cannot."""
-    st = t.stride()
-    st = (st[0], st[1], st[2], st[3]) if layout == "bhsd" else (st[0], st[2], st[1], st[3])
-    if st[3] == 1 and st[0] > 0 and st[1] > 0 and st[2] > 0 and (st[0] | st[1] | st[2]) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, st[:3]
-    view = _tma_ready(t if layout == "bhsd" else t.transpose(1, 2), 2)
-    if view.data_ptr() % 16 != 0:  # contiguous, but starting between two 16-byte boundaries
-        view = _tma_ready(view.clone(memory_format=torch.contiguous_format), 2)
-    return view, view.stride()[:3]
+def _dense(t) -> bool:
+    """Whether a tensor (its ``_meta``) is contiguous; a dimension of size 1 may have any stride."""
+    n = 1
+    for size, st in zip(reversed(t[0]), reversed(t[1])):
+        if size != 1 and st != n:
+            return False
+        n *= size
+    return True
 
 
-def _can_hold(t: torch.Tensor, st) -> bool:
-    """Whether the kernels can write the rows of a buffer with 16-byte stores."""
-    return (t.stride(3) == 1 and st[0] > 0 and st[1] > 0 and st[2] > 0 and (st[0] | st[1] | st[2]) % 8 == 0
-            and t.data_ptr() % 16 == 0)
+def _bhsd(st, layout: str):
+    return (st[0], st[1], st[2]) if layout == "bhsd" else (st[0], st[2], st[1])
+
+
+def _fits(st) -> bool:
+    """Whether 16-byte accesses and tensor maps can address rows with these element strides (from an aligned address)."""
+    return st[3] == 1 and st[0] > 0 and st[1] > 0 and st[2] > 0 and (st[0] | st[1] | st[2]) % 8 == 0
+
+
+def _aligned(t: torch.Tensor, layout: str) -> torch.Tensor:
+    """The tensor itself if the kernels can address it, otherwise a copy that they can."""
+    if _fits(t.stride()) and t.data_ptr() % 16 == 0:
+        return t
+    bhsd = _tma_ready(t if layout == "bhsd" else t.transpose(1, 2), 2)
+    if bhsd.data_ptr() % 16 != 0:  # contiguous, but starting between two 16-byte boundaries
+        bhsd = _tma_ready(bhsd.clone(memory_format=torch.contiguous_format), 2)
+    return bhsd if layout == "bhsd" else bhsd.transpose(1, 2)
 
 
 def _stream_ctas(items: int, key_tiles: int, ragged: bool, num_sms: int) -> int:
@@ -78,83 +93,136 @@ def _stream_ctas(items: int, key_tiles: int, ragged: bool, num_sms: int) -> int:
     return min(places, items * key_tiles)
 
 
-def _launch_window_fwd(q, k, v, out, lse, layout, shape, *, kv_lens, window, sinks, scale, pack_gqa, key_tiles, ragged,
-                       page_table=None, tree_mask=None, page_size=0):
-    """``shape`` is (B, Hq, Hkv, Sq, Sk, D); with a page table, k and v are [pages, Hkv, page_size, D] pools."""
-    lib = _cabi.load()
-    device = q.device
-    B, Hq, Hkv, Sq, Sk, D = shape
-    kv_layout = layout if page_table is None else "bhsd"
-    (q_k, q_st), (k_k, k_st), (v_k, v_st) = _rows(q, layout), _rows(k, kv_layout), _rows(v, kv_layout)
-    out_k, o_st = out, out.stride()
-    o_st = (o_st[0], o_st[1], o_st[2]) if layout == "bhsd" else (o_st[0], o_st[2], o_st[1])
-    if not _can_hold(out, o_st):
-        out_k = torch.empty((B, Hq, Sq, D), dtype=out.dtype, device=device)
-        o_st = out_k.stride()[:3]
-    lse_k = lse
-    if lse is not None and not lse.is_contiguous():
-        lse_k = torch.empty(lse.shape, dtype=torch.float32, device=device)
+class _Plan(NamedTuple):
+    """A checked call: everything but the addresses.  Kept by the shapes, strides, types and options of the call (a
+    decoding loop makes the same call every step; the checks cost more than its launch)."""
 
-    per_tile = 128 // (Hq // Hkv) if pack_gqa else 128  # query tokens of a tile
-    items = B * _ceil_div(Sq, per_tile) * (Hkv if pack_gqa else Hq)
-    ctas = _stream_ctas(items, key_tiles, ragged, lib.bsa_num_sms(device.index))
-    joins = partial_o = partial_lse = None
-    lists = 1
-    if ctas:
-        tiles = _ceil_div(Sq, per_tile)
-        if page_table is not None and 1 < tiles <= ctas:  # new tokens over a long past: nearly the same keys
-            lists = tiles
-            ctas -= ctas % lists
-        rows = 2 * ctas * min(Sq, per_tile) * (Hq // Hkv if pack_gqa else 1)
-        workspace = q.new_empty(4 * ctas + rows * (D + 1), dtype=torch.float32)
-        joins = workspace.data_ptr()
-        partial_o = joins + 16 * ctas
-        partial_lse = partial_o + 4 * rows * D
-    paged = page_table is not None
-    args = _cabi.WindowFwdArgs(
-        q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr(), out_k.data_ptr(), _cabi.ptr(lse_k), _cabi.ptr(kv_lens),
-        _cabi.ptr(page_table), _cabi.ptr(tree_mask), partial_o, partial_lse, joins, _cabi.status_buffer(device).data_ptr(), q_st,
-        k_st, v_st, o_st, _dtype_code(q.dtype), B, Hq, Hkv, Sq, Sk, D, window, sinks, page_table.shape[1] if paged else 0,
-        page_size, k.shape[0] if paged else 0, 1 if pack_gqa else 0, ctas, lists, scale)
-    _cabi.launch(lib.bsa_window_fwd, "bsa_window_fwd", device, args)
-    if out_k is not out:
-        (out if layout == "bhsd" else out.transpose(1, 2)).copy_(out_k)
-    if lse is not None and lse_k is not lse:
-        lse.copy_(lse_k)
-
-
-def _out_buffers(q, out, lse, want_lse, B, H, S):
-    device = q.device
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == device
-        assert out.stride(-1) == 1
-    if lse is None:
-        lse = torch.empty((B, H, S), dtype=torch.float32, device=device) if want_lse else None
-    else:
-        assert lse.shape == (B, H, S) and lse.dtype == torch.float32 and lse.device == device
-    return out, lse
+    direct: bool            # the kernels can address the tensors as they are, up to the alignment of the addresses
+    empty: bool             # no key or no query: zeros, nothing to launch
+    out_shape: tuple
+    lse_shape: Optional[tuple]  # None: no LSE is returned
+    args: bytes             # WindowFwdArgs without addresses
+    workspace: int          # floats
+    partial_o: int          # byte offsets in it
+    partial_lse: int
+    q_dense: bool = False   # contiguous: empty_like, the cheaper call, gives the same
 
 
 def _check_qkv(q, k, v, layout):
+    """``q, k, v`` are ``_meta``s."""
     assert layout in ("bhsd", "bshd"), f"layout must be 'bhsd' or 'bshd', got {layout!r}"
-    assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "inputs must be 4-D"
-    assert q.is_cuda and k.is_cuda and v.is_cuda, "inputs must be on CUDA device"
-    assert q.device == k.device == v.device, "Q/K/V must be on the same CUDA device"
-    assert q.dtype == k.dtype == v.dtype, "inputs must have the same dtype"
-    assert q.dtype in (torch.float16, torch.bfloat16), "inputs must be float16 or bfloat16"
-    assert q.shape[-1] in (64, 96, 128), f"head dimension must be 64, 96 or 128, got {q.shape[-1]}"
+    assert len(q[0]) == 4 and len(k[0]) == 4 and len(v[0]) == 4, "inputs must be 4-D"
+    assert q[4] and k[4] and v[4], "inputs must be on CUDA device"
+    assert q[3] == k[3] == v[3], "Q/K/V must be on the same CUDA device"
+    assert q[2] == k[2] == v[2], "inputs must have the same dtype"
+    assert q[2] in (torch.float16, torch.bfloat16), "inputs must be float16 or bfloat16"
+    assert q[0][3] in (64, 96, 128), f"head dimension must be 64, 96 or 128, got {q[0][3]}"
 
 
 def _check_shapes(q, k, v, layout):
     h, n = (1, 2) if layout == "bhsd" else (2, 1)
-    qs, ks = q.shape, k.shape
-    B, Hq, Sq, D, Hkv, Sk = qs[0], qs[h], qs[n], qs[3], ks[h], ks[n]
-    assert v.shape == ks and ks[0] == B and ks[3] == D, "K and V must match Q's batch and head dimension, and each other"
+    B, Hq, Sq, D, Hkv, Sk = q[0], q[h], q[n], q[3], k[h], k[n]
+    B = q[0]
+    assert v == k and k[0] == B and k[3] == D, "K and V must match Q's batch and head dimension, and each other"
     assert Hkv >= 1 and Hq % Hkv == 0, "the number of query heads must be a multiple of the number of KV heads"
     assert Sq <= _MAX_LEN and Sk <= _MAX_LEN
     return B, Hq, Hkv, Sq, Sk, D
+
+
+def _make_plan(q, k, v, out, lse, lens, layout, shape, *, window, sinks, scale, pack_gqa, key_tiles, ragged, empty, want_lse,
+               table=None, tree=None) -> _Plan:
+    """The part that the two forward calls share; tensors are ``_meta``s, ``shape`` is (B, Hq, Hkv, Sq, Sk, D)."""
+    B, Hq, Hkv, Sq, Sk, D = shape
+    device = q[3]
+    if out is not None:
+        assert out[0] == q[0] and out[2] == q[2] and out[3] == device, "out must match q"
+        assert out[1][3] == 1, "out must have unit last stride"
+    if lse is not None:
+        assert lse[0] == (B, Hq, Sq) and lse[2] == torch.float32 and lse[3] == device, f"lse must be float32 ({B}, {Hq}, {Sq})"
+    lse_shape = (B, Hq, Sq) if want_lse else None
+    if empty or Sq == 0 or B == 0 or Hq == 0:
+        return _Plan(True, True, tuple(q[0]), lse_shape, b"", 0, 0, 0)
+    kv_layout = layout if table is None else "bhsd"
+    out_st = out[1] if out is not None else ((Hq * Sq * D, Sq * D, D, 1) if layout == "bhsd" else (Hq * Sq * D, Hq * D, D, 1))
+    direct = (_fits(q[1]) and _fits(k[1]) and _fits(v[1]) and _fits(out_st)
+              and all(t is None or _dense(t) for t in (lse, lens, table, tree)))
+    if not direct:
+        return _Plan(False, False, tuple(q[0]), lse_shape, b"", 0, 0, 0)
+    per_tile = 128 // (Hq // Hkv) if pack_gqa else 128  # query tokens of a tile
+    tiles = _ceil_div(Sq, per_tile)
+    items = B * tiles * (Hkv if pack_gqa else Hq)
+    ctas = _stream_ctas(items, key_tiles, ragged, _cabi.load().bsa_num_sms(device.index))
+    lists = 1
+    if table is not None and 1 < tiles <= ctas:  # new tokens over a long past: nearly the same keys
+        lists = tiles
+        ctas -= ctas % lists
+    rows = 2 * ctas * min(Sq, per_tile) * (Hq // Hkv if pack_gqa else 1)
+    args = _cabi.WindowFwdArgs(
+        None, None, None, None, None, None, None, None, None, None, None, None, _bhsd(q[1], layout), _bhsd(k[1], kv_layout),
+        _bhsd(v[1], kv_layout), _bhsd(out_st, layout), _dtype_code(q[2]), B, Hq, Hkv, Sq, Sk, D, window, sinks,
+        table[0][1] if table is not None else 0, k[0][2] if table is not None else 0, k[0][0] if table is not None else 0,
+        1 if pack_gqa else 0, ctas, lists, scale)
+    # workspace: the list of joins (four ints a CTA), the pieces' rows, their LSE
+    return _Plan(True, False, tuple(q[0]), lse_shape, bytes(args), (4 * ctas + rows * (D + 1)) if ctas else 0, 16 * ctas,
+                 16 * ctas + 4 * rows * D, q[1] == ((n := q[0])[1] * n[2] * n[3], n[2] * n[3], n[3], 1))
+
+
+def _run_plan(plan: _Plan, q, k, v, out, lse, lens, table, tree):
+    """Launches a checked call; returns (out, lse), or None if some address is not aligned (nothing was launched)."""
+    if out is None:
+        out = torch.empty_like(q) if plan.q_dense else q.new_empty(plan.out_shape)
+    if lse is None and plan.lse_shape is not None:
+        lse = q.new_empty(plan.lse_shape, dtype=torch.float32)
+    if plan.empty:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-math.inf)
+        return out, lse
+    a = _cabi.WindowFwdArgs.from_buffer_copy(plan.args)
+    a.q, a.k, a.v, a.out = at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if (at[0] | at[1] | at[2] | at[3]) % 16:
+        return None
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if lens is not None:
+        a.kv_lens = lens.data_ptr()
+    if table is not None:
+        a.page_table = table.data_ptr()
+    if tree is not None:
+        a.tree_mask = tree.data_ptr()
+    if plan.workspace:
+        workspace = q.new_empty(plan.workspace, dtype=torch.float32)
+        a.joins = w = workspace.data_ptr()
+        a.partial_o, a.partial_lse = w + plan.partial_o, w + plan.partial_lse
+    device = q.device
+    a.status = _cabi.status_buffer(device).data_ptr()
+    _cabi.launch(_cabi.load().bsa_window_fwd, "bsa_window_fwd", device, a)
+    return out, lse
+
+
+def _copied(call, q, k, v, out, lse, layout):
+    """Repeats a call on addressable copies of what the kernels cannot address; ``call(q, k, v)`` returns (out, lse)."""
+    got, got_lse = call(_aligned(q, layout), k, v)
+    if out is not None:
+        got = out.copy_(got)
+    if lse is not None:
+        got_lse = lse.copy_(got_lse)
+    return got, got_lse
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _window_plan(q, k, v, out, lse, lens, window, sinks, softmax_scale, layout, want_lse) -> _Plan:
+    window, sinks = _check_window(window, sinks)
+    _check_qkv(q, k, v, layout)
+    B, Hq, Hkv, Sq, Sk, D = shape = _check_shapes(q[0], k[0], v[0], layout)
+    if lens is not None:
+        _check_lens(lens, B, q[3], "kv_lens")
+    # one head's queries do not fill a 128-row tile: tiles of several heads then, so that the group reads its keys once
+    pack = Hq > Hkv and Sq < 128 and Hq // Hkv <= 128
+    span = min(Sq, 128) + min(window, Sk)
+    return _make_plan(q, k, v, out, lse, lens, layout, shape, window=window, sinks=sinks, scale=_check_scale(softmax_scale, D),
+                      pack_gqa=pack, key_tiles=min(_ceil_div(Sk, 128), _ceil_div(span, 128) + 2), ragged=False,
+                      empty=Sk == 0, want_lse=want_lse)
 
 
 def window_attn_fwd(
@@ -183,25 +251,16 @@ def window_attn_fwd(
 
     Inside a sequence, a NaN or infinity in a value that some query sees may reach other queries of the same 128 keys.
     """
-    window, sink_tokens = _check_window(window, sink_tokens)
-    _check_qkv(q, k, v, layout)
     want_lse = return_lse or lse is not None or q.requires_grad or k.requires_grad or v.requires_grad
-    shape = B, Hq, Hkv, Sq, Sk, D = _check_shapes(q, k, v, layout)
-    kv_lens = _check_lens(kv_lens, B, q.device, "kv_lens")
-    scale = _check_scale(softmax_scale, D)
-    out, lse_buf = _out_buffers(q, out, lse, want_lse, B, Hq, Sq)
-    if out.numel() == 0 or Sk == 0:
-        out.zero_()
-        if lse_buf is not None:
-            lse_buf.fill_(-math.inf)
-        return out, lse_buf
-    # one head's queries do not fill a 128-row tile: tiles of several heads then, so that the group reads its keys once
-    pack = Hq > Hkv and Sq < 128 and Hq // Hkv <= 128
-    span = min(Sq, 128) + min(window, Sk)
-    key_tiles = min(_ceil_div(Sk, 128), _ceil_div(span, 128) + 2)
-    _launch_window_fwd(q, k, v, out, lse_buf, layout, shape, kv_lens=kv_lens, window=window, sinks=sink_tokens,
-                       scale=scale, pack_gqa=pack, key_tiles=key_tiles, ragged=False)
-    return out, lse_buf
+    plan = _window_plan(_meta(q), _meta(k), _meta(v), _meta(out), _meta(lse), _meta(kv_lens), window, sink_tokens,
+                        None if softmax_scale is None else float(softmax_scale), layout, want_lse)
+    res = _run_plan(plan, q, k, v, out, lse, kv_lens, None, None) if plan.direct else None
+    if res is not None:
+        return res
+    lens = None if kv_lens is None else kv_lens.contiguous()
+    return _copied(lambda q, k, v: window_attn_fwd(q, _aligned(k, layout), _aligned(v, layout), window, sink_tokens, kv_lens=lens,
+                                                   softmax_scale=softmax_scale, return_lse=want_lse, layout=layout),
+                   q.detach(), k.detach(), v.detach(), out, lse, layout)
 
 
 def window_attn_bwd(
@@ -228,14 +287,16 @@ def window_attn_bwd(
     with the same arguments.
     """
     window, sink_tokens = _check_window(window, sink_tokens)
-    _check_qkv(q, k, v, layout)
+    _check_qkv(_meta(q), _meta(k), _meta(v), layout)
     assert out.dtype == dout.dtype == q.dtype and lse.dtype == torch.float32
     device = q.device
     assert out.device == dout.device == lse.device == device, "all tensors must be on the device of q"
     assert out.shape == q.shape and dout.shape == q.shape
-    B, Hq, Hkv, Sq, Sk, D = _check_shapes(q, k, v, layout)
+    B, Hq, Hkv, Sq, Sk, D = _check_shapes(q.shape, k.shape, v.shape, layout)
     assert lse.shape == (B, Hq, Sq)
-    kv_lens = _check_lens(kv_lens, B, device, "kv_lens")
+    if kv_lens is not None:
+        _check_lens(_meta(kv_lens), B, device, "kv_lens")
+        kv_lens = kv_lens.contiguous()
     scale = _check_scale(softmax_scale, D)
 
     def _grad(buf, like):
@@ -250,29 +311,22 @@ def window_attn_bwd(
             g.zero_()
         return grads
     lib = _cabi.load()
-    held, held_st = [], []
-    for g in grads:
-        st = g.stride()
-        st = (st[0], st[1], st[2]) if layout == "bhsd" else (st[0], st[2], st[1])
-        if not _can_hold(g, st):
-            g = torch.empty((B, g.shape[1], g.shape[2], D) if layout == "bhsd" else (B, g.shape[2], g.shape[1], D),
-                            dtype=g.dtype, device=device)
-            st = g.stride()[:3]
-        held.append(g)
-        held_st.append(st)
-    (do_k, do_st), (q_k, q_st), (k_k, k_st), (v_k, v_st), (o_k, o_st) = (_rows(t, layout) for t in (dout, q, k, v, out))
+    held = [g if _fits(g.stride()) and g.data_ptr() % 16 == 0 else torch.empty(g.shape, dtype=g.dtype, device=device)
+            for g in grads]
+    held = [_aligned(g, layout) for g in held]  # (a size-1 dimension of a fresh tensor may carry any stride)
+    inputs = [_aligned(t, layout) for t in (dout, q, k, v, out)]
+    strides = [_bhsd(t.stride(), layout) for t in inputs + held]
     lse_c = lse.contiguous()
     ws_bytes = max(16, lib.bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sink_tokens))
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
     a = _cabi.WindowBwdArgs(
-        do_k.data_ptr(), q_k.data_ptr(), k_k.data_ptr(), v_k.data_ptr(), o_k.data_ptr(), lse_c.data_ptr(),
-        held[0].data_ptr(), held[1].data_ptr(), held[2].data_ptr(), _cabi.ptr(kv_lens), workspace.data_ptr(),
-        _cabi.status_buffer(device).data_ptr(), ws_bytes, do_st, q_st, k_st, v_st, o_st, held_st[0], held_st[1], held_st[2],
-        _dtype_code(q.dtype), B, Hq, Hkv, Sq, Sk, D, window, sink_tokens, scale)
+        *(t.data_ptr() for t in inputs), lse_c.data_ptr(), *(t.data_ptr() for t in held), _cabi.ptr(kv_lens),
+        workspace.data_ptr(), _cabi.status_buffer(device).data_ptr(), ws_bytes, *strides, _dtype_code(q.dtype), B, Hq, Hkv,
+        Sq, Sk, D, window, sink_tokens, scale)
     _cabi.launch(lib.bsa_window_bwd, "bsa_window_bwd", device, a)
     for g, t in zip(grads, held):
         if t is not g:
-            (g if layout == "bhsd" else g.transpose(1, 2)).copy_(t)
+            g.copy_(t)
     return grads
 
 

@@ -75,9 +75,8 @@ struct Item {
   int slot;              // workspace slot of the piece, -1: the piece is the whole list
 };
 
+// Length, positions and key tiles of query tile (b, m): the same for all heads.
 __device__ __forceinline__ void describe(const WinFwdParams& p, Item& t) {
-  t.hkv = p.packed ? t.hidx : t.hidx / p.G;
-  t.g = p.packed ? 0 : t.hidx % p.G;
   t.len = p.kv_lens ? max(0, min(p.kv_lens[t.b], p.Sk)) : p.Sk;
   t.base = (p.page_table ? t.len : p.Sk) - p.Sq;
   t.seq0 = t.m * p.seq_per_tile;
@@ -91,16 +90,20 @@ __device__ __forceinline__ void describe(const WinFwdParams& p, Item& t) {
   }
   t.tiles = window_tiles(t.p_lo, t.p_hi, t.len, p.window, p.sinks);
 }
+__device__ __forceinline__ void describe_heads(const WinFwdParams& p, Item& t) {
+  t.hkv = p.packed ? t.hidx : t.hidx / p.G;
+  t.g = p.packed ? 0 : t.hidx % p.G;
+}
 
 // A query tile without key tiles still has its zeros to write: it counts as one.
 __device__ __forceinline__ int item_cost(const WinFwdParams& p, int b, int m) {
   Item t;
   t.b = b;
   t.m = m;
-  t.hidx = 0;
   describe(p, t);
   return max(t.tiles.n, 1);
 }
+
 // The list that a stream run is cut from: (sequence, head, query tile) in this order, all query tiles or only the CTA's
 // one (p.lists = NqT lists side by side, whose CTAs walk the same keys at the same time: one read from HBM serves them).
 __device__ __forceinline__ int list_first(const WinFwdParams& p) { return p.lists > 1 ? (int)blockIdx.x % p.lists : 0; }
@@ -183,6 +186,7 @@ __device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int
     t.hidx = s.hidx;
     t.m = s.m;
     describe(p, t);
+    describe_heads(p, t);
     const int cost = max(t.tiles.n, 1);
     const int end = min(cost, s.it + s.left);
     t.it_begin = s.it;
@@ -208,6 +212,7 @@ __device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int
   t.hidx = r % p.Hidx;
   t.b = r / p.Hidx;
   describe(p, t);
+  describe_heads(p, t);
   t.it_begin = 0;
   t.it_end = t.tiles.n;
   t.slot = -1;
