@@ -286,48 +286,77 @@ def window_attn_bwd(
     are bit-identical.  Tokens behind ``kv_lens`` get zero gradients.  ``out`` and ``lse`` are those of the forward call
     with the same arguments.
     """
-    window, sink_tokens = _check_window(window, sink_tokens)
-    _check_qkv(_meta(q), _meta(k), _meta(v), layout)
-    assert out.dtype == dout.dtype == q.dtype and lse.dtype == torch.float32
-    device = q.device
-    assert out.device == dout.device == lse.device == device, "all tensors must be on the device of q"
-    assert out.shape == q.shape and dout.shape == q.shape
-    B, Hq, Hkv, Sq, Sk, D = _check_shapes(q.shape, k.shape, v.shape, layout)
-    assert lse.shape == (B, Hq, Sq)
-    if kv_lens is not None:
-        _check_lens(_meta(kv_lens), B, device, "kv_lens")
-        kv_lens = kv_lens.contiguous()
-    scale = _check_scale(softmax_scale, D)
-
-    def _grad(buf, like):
-        if buf is None:
-            return torch.empty_like(like)
-        assert buf.shape == like.shape and buf.dtype == like.dtype and buf.device == device
-        return buf
-
-    grads = dq, dk, dv = _grad(dq, q), _grad(dk, k), _grad(dv, v)
-    if q.numel() == 0 or k.numel() == 0:
+    plan = _bwd_plan(_meta(dout), _meta(q), _meta(k), _meta(v), _meta(out), _meta(lse), _meta(kv_lens), _meta(dq), _meta(dk),
+                     _meta(dv), window, sink_tokens, None if softmax_scale is None else float(softmax_scale), layout)
+    if not plan.direct:
+        return _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout)
+    grads = (q.new_empty(plan.q_shape) if dq is None else dq, q.new_empty(plan.k_shape) if dk is None else dk,
+             q.new_empty(plan.k_shape) if dv is None else dv)
+    if plan.empty:
         for g in grads:
             g.zero_()
         return grads
-    lib = _cabi.load()
-    held = [g if _fits(g.stride()) and g.data_ptr() % 16 == 0 else torch.empty(g.shape, dtype=g.dtype, device=device)
-            for g in grads]
-    held = [_aligned(g, layout) for g in held]  # (a size-1 dimension of a fresh tensor may carry any stride)
-    inputs = [_aligned(t, layout) for t in (dout, q, k, v, out)]
-    strides = [_bhsd(t.stride(), layout) for t in inputs + held]
-    lse_c = lse.contiguous()
-    ws_bytes = max(16, lib.bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sink_tokens))
-    workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
-    a = _cabi.WindowBwdArgs(
-        *(t.data_ptr() for t in inputs), lse_c.data_ptr(), *(t.data_ptr() for t in held), _cabi.ptr(kv_lens),
-        workspace.data_ptr(), _cabi.status_buffer(device).data_ptr(), ws_bytes, *strides, _dtype_code(q.dtype), B, Hq, Hkv,
-        Sq, Sk, D, window, sink_tokens, scale)
-    _cabi.launch(lib.bsa_window_bwd, "bsa_window_bwd", device, a)
-    for g, t in zip(grads, held):
-        if t is not g:
-            g.copy_(t)
+    a = _cabi.WindowBwdArgs.from_buffer_copy(plan.args)
+    a.dout, a.q, a.k, a.v, a.out = at = dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.dq, a.dk, a.dv = to = grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr()
+    if (at[0] | at[1] | at[2] | at[3] | at[4] | to[0] | to[1] | to[2]) % 16:
+        return _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout)
+    a.lse = lse.data_ptr()
+    if kv_lens is not None:
+        a.kv_lens = kv_lens.data_ptr()
+    workspace = q.new_empty(plan.workspace, dtype=torch.uint8)
+    device = q.device
+    a.workspace, a.status = workspace.data_ptr(), _cabi.status_buffer(device).data_ptr()
+    _cabi.launch(_cabi.load().bsa_window_bwd, "bsa_window_bwd", device, a)
     return grads
+
+
+def _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout):
+    """Repeats a call on addressable copies of what the kernels cannot address."""
+    dout, q, k, v, out = (_aligned(t.detach(), layout) for t in (dout, q, k, v, out))
+    res = window_attn_bwd(dout, q, k, v, out, lse.contiguous(), window, sink_tokens,
+                          kv_lens=None if kv_lens is None else kv_lens.contiguous(), softmax_scale=softmax_scale, layout=layout)
+    return tuple(g if buf is None else buf.copy_(g) for g, buf in zip(res, (dq, dk, dv)))
+
+
+class _BwdPlan(NamedTuple):
+    """A checked backward call: everything but the addresses."""
+
+    direct: bool
+    empty: bool
+    q_shape: tuple
+    k_shape: tuple
+    args: bytes
+    workspace: int  # bytes
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _bwd_plan(dout, q, k, v, out, lse, lens, dq, dk, dv, window, sinks, softmax_scale, layout) -> _BwdPlan:
+    window, sinks = _check_window(window, sinks)
+    _check_qkv(q, k, v, layout)
+    device = q[3]
+    assert out[2] == dout[2] == q[2] and lse[2] == torch.float32, "out and dout must have q's dtype, lse float32"
+    assert out[3] == dout[3] == lse[3] == device, "all tensors must be on the device of q"
+    assert out[0] == q[0] and dout[0] == q[0], "out and dout must have q's shape"
+    B, Hq, Hkv, Sq, Sk, D = _check_shapes(q[0], k[0], v[0], layout)
+    assert lse[0] == (B, Hq, Sq), f"lse must have shape ({B}, {Hq}, {Sq})"
+    if lens is not None:
+        _check_lens(lens, B, device, "kv_lens")
+    scale = _check_scale(softmax_scale, D)
+    for buf, like in ((dq, q), (dk, k), (dv, v)):
+        assert buf is None or (buf[0] == like[0] and buf[2] == like[2] and buf[3] == device), "gradient buffers must match q, k, v"
+    q_shape, k_shape = tuple(q[0]), tuple(k[0])
+    if 0 in q_shape or 0 in k_shape:
+        return _BwdPlan(True, True, q_shape, k_shape, b"", 0)
+    contiguous = lambda n: (n[1] * n[2] * n[3], n[2] * n[3], n[3], 1)  # noqa: E731
+    grad_st = [like if buf is None else buf[1] for buf, like in ((dq, contiguous(q_shape)), (dk, contiguous(k_shape)), (dv, contiguous(k_shape)))]
+    strides = [t[1] for t in (dout, q, k, v, out)] + grad_st
+    if not (all(map(_fits, strides)) and _dense(lse) and (lens is None or _dense(lens))):
+        return _BwdPlan(False, False, q_shape, k_shape, b"", 0)
+    ws = max(16, int(_cabi.load().bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sinks)))
+    args = _cabi.WindowBwdArgs(*[None] * 12, ws, *(_bhsd(st, layout) for st in strides), _dtype_code(q[2]), B, Hq, Hkv, Sq, Sk, D,
+                               window, sinks, scale)
+    return _BwdPlan(True, False, q_shape, k_shape, bytes(args), ws)
 
 
 class WindowAttentionFunction(torch.autograd.Function):

@@ -2,13 +2,15 @@
 //   angle(b, s, p) = positions[b, s, axis(p)] * inv_freq[p].
 //
 // Bound by HBM: q and k are read and written once, three multiply-adds per element.  A block holds a few whole tokens:
-// its threads first compute the sines and cosines of the tokens' pairs, about one each, into shared memory; then a
-// thread owns one 16-byte chunk of a token (half-split pairing: the two chunks its pairs connect), takes its pairs'
-// values into registers and walks over every head_lanes-th head of q and k, four heads in flight at a time.
+// its threads first compute the sines and cosines of the tokens' pairs, about one each, into shared memory; a thread
+// owns one 16-byte chunk of a token (half-split pairing: the two chunks its pairs connect), takes its pairs' values
+// into registers and walks over every head_lanes-th head of q and k.  Four loads are in flight while the four before are
+// worked on, the first four under the sines.
 //
 // The angle of position 10^5 at frequency 1 is 10^5 radians; in 32 bits its fraction of a turn would be off by 10^-3.
-// So position * (inv_freq / 2 pi) is formed and reduced to [-1/2, 1/2] turns in 64 bits, and only the reduced turn is
-// rounded to 32 bits (sincospi of twice that: an error below 2^-24 turns).
+// So a frequency becomes a 64-bit fraction of a turn per position, whose product with the position wraps around whole
+// turns by itself (integer arithmetic modulo 2^64: off by less than 2^-32 turns for any 32-bit position), and only the
+// wrapped turn is rounded to 32 bits.
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"
@@ -35,7 +37,7 @@ struct Params {
   int Hq, heads, S, D, P;
   int per_token;           // units per token
   int heads_per_cta;
-  long long tokens;        // B * S
+  int tokens;              // B * S
   int tokens_per_block;    // vector form: whole tokens of a block, at most kThreads units
   int head_lanes;          // ... and the heads its threads work on side by side
   float sign;
@@ -85,53 +87,86 @@ struct Io<__half> {
   }
 };
 
-__device__ __forceinline__ void pair_sincos(const Params& p, const int32_t* pos, int pair, float& c, float& s) {
-  const int axis = (pair >= p.end0) + (pair >= p.end1) + (pair >= p.end2);
-  constexpr double kInvTwoPi = 0.15915494309189533576888;
-  const double turns = (double)pos[axis] * ((double)p.inv_freq[pair] * kInvTwoPi);
-  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-  s *= p.sign;
+// inv_freq in turns per position, modulo 1, as a 64-bit fraction.
+__device__ __forceinline__ unsigned long long turn_fraction(float inv_freq) {
+  constexpr double kInvTwoPi = 0.15915494309189533576888, kTwo64 = 18446744073709551616.0;
+  const double turns = (double)inv_freq * kInvTwoPi;
+  return (unsigned long long)((turns - floor(turns)) * kTwo64);  // (below 2^64: the largest double below 1 is 1 - 2^-53)
+}
+__device__ __forceinline__ int axis_of(const Params& p, int pair) {
+  return (pair >= p.end0) + (pair >= p.end1) + (pair >= p.end2);
+}
+__device__ __forceinline__ float2 position_sincos(const Params& p, int position, unsigned long long turns) {
+  const int wrapped = (int)((turns * (unsigned long long)(long long)position) >> 32);  // [-1/2, 1/2) turns, times 2^32
+  float s, c;
+  sincospif((float)wrapped * 0x1p-31f, &s, &c);
+  return make_float2(c, s * p.sign);
 }
 
-// Address of the row of (head slot h, batch, token): q heads first, then k heads.
-__device__ __forceinline__ void row_of(const Params& p, int h, long long b, int tok, const uint8_t*& src, uint8_t*& dst) {
-  if (h < p.Hq) {
-    src = p.q + b * p.q_b + h * p.q_h + tok * p.q_s;
-    dst = p.qo + b * p.qo_b + h * p.qo_h + tok * p.qo_s;
-  } else {
-    src = p.k + b * p.k_b + (h - p.Hq) * p.k_h + tok * p.k_s;
-    dst = p.ko + b * p.ko_b + (h - p.Hq) * p.ko_h + tok * p.ko_s;
-  }
-}
+// The rows of one token: q heads first, then k heads.
+struct Rows {
+  const uint8_t* q;
+  const uint8_t* k;
+  uint8_t* qo;
+  uint8_t* ko;
+  __device__ __forceinline__ Rows(const Params& p, int b, int tok)
+      : q(p.q + b * p.q_b + tok * p.q_s), k(p.k + b * p.k_b + tok * p.k_s - p.Hq * p.k_h),
+        qo(p.qo + b * p.qo_b + tok * p.qo_s), ko(p.ko + b * p.ko_b + tok * p.ko_s - p.Hq * p.ko_h) {}
+  __device__ __forceinline__ const uint8_t* from(const Params& p, int h) const { return h < p.Hq ? q + h * p.q_h : k + h * p.k_h; }
+  __device__ __forceinline__ uint8_t* to(const Params& p, int h) const { return h < p.Hq ? qo + h * p.qo_h : ko + h * p.ko_h; }
+};
 
 // Vector form: 16-byte chunks.  Interleaved: unit c = chunk c (its pairs lie inside it; pairs from P on are copied).
 // Half-split: units 0 .. P/V-1 are pairs of chunks (c, P/V + c), the rest single chunks that are copied.
 constexpr int kTable = 2048;  // P <= V * units per token, V <= 8, and a block's tokens have at most kThreads units
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 rotary_vec_kernel(const Params p) {
   constexpr int V = 16 / sizeof(T);
   constexpr int kPairs = INTERLEAVED ? V / 2 : V;
-  constexpr int kFly = 4;  // heads in flight
+  constexpr int kFly = INTERLEAVED ? 4 : 2;  // heads in flight: four 16-byte loads, twice
   __shared__ float2 table[kTable];
-  const long long token0 = (long long)blockIdx.x * p.tokens_per_block;
-  const int here = (int)min((long long)p.tokens_per_block, p.tokens - token0);
-  for (int i = threadIdx.x; i < here * p.P; i += kThreads) {
-    const int t = i / p.P, pair = i - t * p.P;
-    const long long token = token0 + t, b = token / p.S;
-    float c, s;
-    pair_sincos(p, p.positions + b * p.pos_b + (token - b * p.S) * p.pos_s, pair, c, s);
-    table[i] = make_float2(c, s);
-  }
-  __syncthreads();
+  __shared__ unsigned long long turns[kTable / 8];  // P <= D / 2 <= 256
+  const int token0 = blockIdx.x * p.tokens_per_block;
+  const int here = min(p.tokens_per_block, p.tokens - token0);
   const int units = p.tokens_per_block * p.per_token;
   const int lane = threadIdx.x / units, unit = threadIdx.x - lane * units;  // head lane, unit inside the block
   const int t = unit / p.per_token, c = unit - t * p.per_token;
-  if (lane >= p.head_lanes || t >= here) return;
-  const long long b = (token0 + t) / p.S;
-  const int tok = (int)(token0 + t - b * p.S);
+  const bool works = lane < p.head_lanes && t < here;
+  const int b = (token0 + t) / p.S, tok = token0 + t - b * p.S;
+  const Rows rows(p, b, tok);
   const int half_chunks = p.P / V;
   const bool turned = INTERLEAVED || c < half_chunks;  // half-split: the tail units only copy
+  const int chunk_a = turned ? c : half_chunks + c;
+  const int chunk_b = half_chunks + c;  // half-split only
+  const int h1 = min(p.heads, ((int)blockIdx.y + 1) * p.heads_per_cta), step = p.head_lanes;
+  struct Batch {
+    uint4 a[kFly], z[kFly];
+  };
+  auto load = [&](int h, Batch& x) {
+#pragma unroll
+    for (int i = 0; i < kFly; ++i) {
+      if (h + i * step < h1) {
+        const uint8_t* src = rows.from(p, h + i * step);
+        x.a[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_a);
+        if (!INTERLEAVED && turned) x.z[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_b);
+      }
+    }
+  };
+  int h = blockIdx.y * p.heads_per_cta + lane;
+  Batch now, then;
+  if (works) load(h, now);  // on their way while the sines are computed
+
+  for (int i = threadIdx.x; i < p.P; i += kThreads) turns[i] = turn_fraction(p.inv_freq[i]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < here * p.P; i += kThreads) {
+    const int at = i / p.P, pair = i - at * p.P;
+    const int bt = (token0 + at) / p.S;
+    const int position = p.positions[bt * p.pos_b + (token0 + at - bt * p.S) * p.pos_s + axis_of(p, pair)];
+    table[i] = position_sincos(p, position, turns[pair]);
+  }
+  __syncthreads();
+  if (!works) return;
   float cs[kPairs], sn[kPairs];
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
@@ -144,28 +179,15 @@ rotary_vec_kernel(const Params p) {
       sn[i] = v.y;
     }
   }
-  const int chunk_a = turned ? c : half_chunks + c;
-  const int chunk_b = half_chunks + c;  // half-split only
-  const int h1 = min(p.heads, ((int)blockIdx.y + 1) * p.heads_per_cta), step = p.head_lanes;
-  for (int h = blockIdx.y * p.heads_per_cta + lane; h < h1; h += kFly * step) {
-    uint4 a[kFly], z[kFly];
-    uint8_t* out[kFly];
-#pragma unroll
-    for (int i = 0; i < kFly; ++i) {
-      const uint8_t* src;
-      row_of(p, min(h + i * step, h1 - 1), b, tok, src, out[i]);
-      if (h + i * step < h1) {
-        a[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_a);
-        if (!INTERLEAVED && turned) z[i] = __ldcs(reinterpret_cast<const uint4*>(src) + chunk_b);
-      }
-    }
+  for (; h < h1; h += kFly * step) {
+    load(h + kFly * step, then);
 #pragma unroll
     for (int i = 0; i < kFly; ++i) {
       if (h + i * step >= h1) break;
-      uint4* dst = reinterpret_cast<uint4*>(out[i]);
+      uint4* dst = reinterpret_cast<uint4*>(rows.to(p, h + i * step));
       if (INTERLEAVED) {
         float x[V];
-        Io<T>::unpack(a[i], x);
+        Io<T>::unpack(now.a[i], x);
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {
           const float x0 = x[2 * e], x1 = x[2 * e + 1];
@@ -176,16 +198,16 @@ rotary_vec_kernel(const Params p) {
         if ((c + 1) * kPairs > p.P) {
           // the chunk reaches behind the turned channels: those leave with their bits unchanged
           const int turned_words = max(0, p.P - c * kPairs) * (int)(2 * sizeof(T)) / 4;
-          if (turned_words <= 0) r.x = a[i].x;
-          if (turned_words <= 1) r.y = a[i].y;
-          if (turned_words <= 2) r.z = a[i].z;
-          if (turned_words <= 3) r.w = a[i].w;
+          if (turned_words <= 0) r.x = now.a[i].x;
+          if (turned_words <= 1) r.y = now.a[i].y;
+          if (turned_words <= 2) r.z = now.a[i].z;
+          if (turned_words <= 3) r.w = now.a[i].w;
         }
         dst[chunk_a] = r;
       } else if (turned) {
         float x[V], y[V];
-        Io<T>::unpack(a[i], x);
-        Io<T>::unpack(z[i], y);
+        Io<T>::unpack(now.a[i], x);
+        Io<T>::unpack(now.z[i], y);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float x0 = x[e], x1 = y[e];
@@ -195,9 +217,10 @@ rotary_vec_kernel(const Params p) {
         dst[chunk_a] = Io<T>::pack(x);
         dst[chunk_b] = Io<T>::pack(y);
       } else {
-        dst[chunk_a] = a[i];
+        dst[chunk_a] = now.a[i];
       }
     }
+    now = then;
   }
 }
 
@@ -207,26 +230,23 @@ __global__ void __launch_bounds__(kThreads)
 rotary_elt_kernel(const Params p) {
   const long long unit = (long long)blockIdx.x * kThreads + threadIdx.x;
   if (unit >= p.units) return;
-  const long long token = unit / p.per_token;
-  const int c = (int)(unit - token * p.per_token);
-  const long long b = token / p.S;
-  const int tok = (int)(token - b * p.S);
+  const int token = (int)(unit / p.per_token), c = (int)(unit - (long long)token * p.per_token);
+  const int b = token / p.S, tok = token - b * p.S;
+  const Rows rows(p, b, tok);
   const bool turned = c < p.P;
-  float cs = 1.f, sn = 0.f;
-  if (turned) pair_sincos(p, p.positions + b * p.pos_b + tok * p.pos_s, c, cs, sn);
+  float2 cs = make_float2(1.f, 0.f);
+  if (turned)
+    cs = position_sincos(p, p.positions[b * p.pos_b + tok * p.pos_s + axis_of(p, c)], turn_fraction(p.inv_freq[c]));
   const int ia = turned ? (INTERLEAVED ? 2 * c : c) : p.P + c;
   const int ib = INTERLEAVED ? 2 * c + 1 : p.P + c;
   const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(p.heads, h0 + p.heads_per_cta);
   for (int h = h0; h < h1; ++h) {
-    const uint8_t* src;
-    uint8_t* out;
-    row_of(p, h, b, tok, src, out);
-    const T* x = reinterpret_cast<const T*>(src);
-    T* y = reinterpret_cast<T*>(out);
+    const T* x = reinterpret_cast<const T*>(rows.from(p, h));
+    T* y = reinterpret_cast<T*>(rows.to(p, h));
     if (turned) {
       const float x0 = Io<T>::load(x + ia), x1 = Io<T>::load(x + ib);
-      Io<T>::store(y + ia, x0 * cs - x1 * sn);
-      Io<T>::store(y + ib, x0 * sn + x1 * cs);
+      Io<T>::store(y + ia, x0 * cs.x - x1 * cs.y);
+      Io<T>::store(y + ib, x0 * cs.y + x1 * cs.x);
     } else {
       y[ia] = x[ia];
     }
@@ -236,28 +256,29 @@ rotary_elt_kernel(const Params p) {
 template <typename T>
 static int launch(Params& p, const bsa_rotary_args& a, bool vec, int num_sms, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  p.tokens = (long long)a.B * a.S;
+  if ((long long)a.B * a.S > 0x7fffffffLL - kThreads) return set_error(BSA_ERR_UNSUPPORTED, "bsa_rotary_nd: more than 2^31 tokens");
+  p.tokens = a.B * a.S;
   long long blocks, groups;
   if (vec) {
     p.per_token = a.interleaved ? a.D / V : p.P / V + (a.D - 2 * p.P) / V;
     // Many tokens to a block (head-major rows of neighbouring tokens are neighbours in memory), one head at a time; while
-    // that leaves SMs with less than four blocks, fewer tokens and more heads side by side.
+    // that leaves SMs with less than two blocks, fewer tokens and more heads side by side.
     p.head_lanes = 1;
     p.tokens_per_block = kThreads / p.per_token;
-    while (p.tokens_per_block > 1 && 2 * p.head_lanes <= p.heads && p.tokens < 4LL * num_sms * p.tokens_per_block) {
+    while (p.tokens_per_block > 1 && 2 * p.head_lanes <= p.heads && p.tokens < 2LL * num_sms * p.tokens_per_block) {
       p.head_lanes *= 2;
       p.tokens_per_block = kThreads / (p.per_token * p.head_lanes);
       if (p.tokens_per_block < 1) p.tokens_per_block = 1;
     }
     p.head_lanes = kThreads / (p.tokens_per_block * p.per_token);
     if (p.head_lanes > p.heads) p.head_lanes = p.heads;
-    blocks = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+    blocks = ((long long)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
     groups = (2LL * num_sms + blocks - 1) / blocks;  // blocks that share tokens, on different heads
     const long long rounds = (p.heads + p.head_lanes - 1) / p.head_lanes;
     if (groups > rounds) groups = rounds;
   } else {
     p.per_token = p.P + (a.D - 2 * p.P);
-    p.units = p.tokens * p.per_token;
+    p.units = (long long)p.tokens * p.per_token;
     blocks = (p.units + kThreads - 1) / kThreads;
     // one thread serves every head of its pair; heads are dealt to more threads while SMs are short of warps
     groups = (8LL * num_sms + blocks - 1) / blocks;

@@ -146,13 +146,17 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const long long b = bh / H;
   const uint8_t* o_base = o + (b * os_b + h * os_h + chunk * 8) * 2;
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
+  // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
+  const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, kv_lens[b] - base));
   uint4 ov[4], dv[4];
+  float lv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
+    lv[i] = (s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
     ov[i] = make_uint4(0, 0, 0, 0);
     dv[i] = make_uint4(0, 0, 0, 0);
-    if (s < Sq && chunk * 8 < D) {
+    if (s < rows && chunk * 8 < D) {
       ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * os_s * 2);
       dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
     }
@@ -171,14 +175,8 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
     if (chunk == 0) {
-      float l = INFINITY;
-      // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
-      const bool part = s < Sq && (kv_lens == nullptr || s + base < kv_lens[b]);
-      if (part) {
-        const float lv = lse[bh * Sq + s];
-        l = (lv == -INFINITY) ? INFINITY : lv * kLog2e;
-      }
-      delta[bh * SqPad + s] = part ? -acc : 0.f;
+      const float l = lv[i] == -INFINITY ? INFINITY : lv[i] * kLog2e;
+      delta[bh * SqPad + s] = -acc;
       lse_log2[bh * SqPad + s] = -l;
     }
   }
