@@ -84,13 +84,18 @@ def _aligned(t: torch.Tensor, layout: str) -> torch.Tensor:
 
 def _stream_ctas(items: int, key_tiles: int, ragged: bool, num_sms: int) -> int:
     """How the work of a call is dealt: 0 = whole query tiles in turn, otherwise the number of CTAs that share the list of
-    all key tiles evenly.  Sharing costs a second launch and fp32 rows of the cut query tiles, so it is for query tiles
-    that do not fill the two places of every SM, and for lists of unequal lengths that only the device knows while the
-    places get less than eight query tiles each (they do not even out)."""
+    all key tiles evenly.  Sharing costs a second launch, fp32 rows of the cut query tiles and the search for each CTA's
+    run, about the time of four key tiles; it saves the key tiles that the busiest of the places (two for each SM) has
+    above the average.  With lists of unequal lengths that only the device knows, places that get less than eight query
+    tiles each do not even out by themselves."""
     places = 2 * num_sms
-    if items >= (8 * places if ragged else places) or key_tiles <= 1 or items * (key_tiles + 1) >= 1 << 31:
+    if items < 1 or items * (key_tiles + 1) >= 1 << 31:
         return 0
-    return min(places, items * key_tiles)
+    if ragged:
+        share = items < 8 * places and key_tiles >= 8
+    else:
+        share = key_tiles * (places - items) >= 4 * places
+    return min(places, items * key_tiles) if share else 0
 
 
 class _Plan(NamedTuple):

@@ -160,11 +160,12 @@ def test_c_entry_points_refuse_bad_arguments():
 def test_rule_of_dealing_the_work():
     from block_sparse_attention.window_attn import _stream_ctas
     assert _stream_ctas(296, 100, False, 148) == 0      # query tiles for both places of every SM
-    assert _stream_ctas(295, 100, False, 148) == 296
-    assert _stream_ctas(295, 1, False, 148) == 0        # nothing to cut
+    assert _stream_ctas(148, 100, False, 148) == 296
+    assert _stream_ctas(148, 7, False, 148) == 0        # 3.5 key tiles to gain
     assert _stream_ctas(8, 9, False, 148) == 72         # no more CTAs than key tiles
     assert _stream_ctas(2367, 100, True, 148) == 296    # lengths that only the device knows
     assert _stream_ctas(2368, 100, True, 148) == 0
+    assert _stream_ctas(1, 7, True, 148) == 0
 
 
 def test_gradient_formula_against_differences():
