@@ -56,4 +56,43 @@ __device__ __forceinline__ TileList window_tiles(int p_lo, int p_hi, int len, in
   return t;
 }
 
+// Equal runs of a list: CTA c of the n that have work gets all / n entries, and one of the all % n that are left over.
+struct Runs {
+  int q, r;
+  __device__ __forceinline__ int begin(int c) const { return c * q + min(c, r); }
+  __device__ __forceinline__ int holder(int x) const { return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q; }
+};
+
+// Finds entry `lo` of a list of `items` items with cost(i) >= 1 entries each: its item, and `lo` becomes its place in
+// the item.  Called by whole warps.
+template <typename Cost>
+__device__ __forceinline__ int find_item(int items, int& lo, Cost cost) {
+  const int lane = threadIdx.x & 31;
+  for (int i0 = 0; i0 < items; i0 += 32) {
+    const int mine = i0 + lane < items ? cost(i0 + lane) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += below;
+    }
+    const uint32_t over = __ballot_sync(0xffffffffu, upto > lo);
+    if (over) {
+      const int holder = __ffs(over) - 1;
+      lo -= __shfl_sync(0xffffffffu, upto - mine, holder);
+      return i0 + holder;
+    }
+    lo -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return 0;
+}
+template <typename Cost>
+__device__ __forceinline__ int total_cost(int items, Cost cost) {
+  int all = 0;
+  for (int i = threadIdx.x & 31; i < items; i += 32) all += cost(i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  return all;
+}
+
 }  // namespace bsa

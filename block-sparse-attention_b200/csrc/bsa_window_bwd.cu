@@ -838,7 +838,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           if (!mbar_wait(BAR(kDpFull), dp_cnt & 1, wctx, 521)) return false;
           tc_fence_after();
-          const bool tail = kMasked && (p0 < 0 || p0 + 127 >= t.len);
+          // the query tile or the key tile reaches behind the end, where rows may hold anything
+          const bool tail = kMasked && (p0 < 0 || p0 + 127 >= t.len || t.nb * 128 + 127 >= t.len);
           if (kMasked) {
             if (tail) {
               // query rows that take no part: dV contracts over the dO rows and dK over the Q rows (both tiles have been
@@ -860,7 +861,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tmem_ld32(t_g, dp);
           tmem_ld32(t_g + 32, dp + 32);
           tmem_wait_ld();
-          if (tail) {  // (what dO holds there reaches dP^T: 0 * NaN is NaN)
+          if (tail) {  // (what dO and V hold there reaches dP^T: 0 * NaN is NaN)
 #pragma unroll
             for (int c = 0; c < 64; ++c) dp[c] = ((mw[c >> 5] >> (c & 31)) & 1u) ? dp[c] : 0u;
           }

@@ -117,25 +117,14 @@ struct Place {
   int q, r;  // of Runs
 };
 
-// CTA c of the n that have work gets all / n key tiles, and one of the all % n that are left over.
-struct Runs {
-  int q, r;
-  __device__ __forceinline__ int begin(int c) const { return c * q + min(c, r); }
-  __device__ __forceinline__ int holder(int x) const { return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q; }
-};
-
 // Called by whole warps.  (All sums fit 32 bits: the host deals whole query tiles otherwise.)
 __device__ __forceinline__ void first_place(const WinFwdParams& p, Place* at) {
   const int lane = threadIdx.x & 31;
   const int m0 = list_first(p), nm = list_size(p), pairs = p.B * nm;  // (sequence, query tile) pairs of a head
-  auto cost = [&](int i) { return i < pairs ? item_cost(p, i / nm, m0 + i % nm) : 0; };
+  auto cost = [&](int i) { return item_cost(p, i / nm, m0 + i % nm); };
   Place s;
   s.b = s.hidx = s.m = s.it = s.left = 0;
-  int per_head = 0;
-  for (int i = lane; i < pairs; i += 32) per_head += cost(i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, o);
-  const int all = per_head * p.Hidx;
+  const int per_head = total_cost(pairs, cost), all = per_head * p.Hidx;
   const int cta = (int)blockIdx.x / p.lists, n = min(all, p.ctas / p.lists);
   const Runs runs{all / n, all % n};
   s.q = runs.q;
@@ -145,24 +134,10 @@ __device__ __forceinline__ void first_place(const WinFwdParams& p, Place* at) {
     s.left = runs.begin(cta + 1) - lo;
     s.hidx = lo / per_head;
     lo -= s.hidx * per_head;
-    for (int i0 = 0; i0 < pairs; i0 += 32) {  // the pair that holds tile `lo` of the head
-      const int mine = cost(i0 + lane);
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int below = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += below;
-      }
-      const uint32_t over = __ballot_sync(0xffffffffu, upto > lo);
-      if (over) {
-        const int holder = __ffs(over) - 1;
-        s.b = (i0 + holder) / nm;
-        s.m = m0 + (i0 + holder) % nm;
-        s.it = lo - __shfl_sync(0xffffffffu, upto - mine, holder);
-        break;
-      }
-      lo -= __shfl_sync(0xffffffffu, upto, 31);
-    }
+    const int pair = find_item(pairs, lo, cost);
+    s.b = pair / nm;
+    s.m = m0 + pair % nm;
+    s.it = lo;
   }
   if (lane == 0) *at = s;
   __syncwarp();

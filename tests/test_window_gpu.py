@@ -45,6 +45,11 @@ CASES = [
     (1, 1, 1, 200, 100, 128, BF, 40, 2, None),          # queries before the first key
     (1, 2, 2, 1300, 1300, 128, BF, 1, 128, None),       # sinks only, and the row itself
     (1, 4, 1, 1100, 1100, 64, HF, 200, 2, None),
+    (1, 1, 1, 2000, 2000, 128, BF, 1000, 4, None),      # few long lists: cut into runs in every kernel
+    (2, 2, 1, 1500, 1500, 96, HF, 1 << 20, 0, [1500, 700]),
+    (1, 8, 1, 6, 38, 96, BF, 24, 1, None),              # one key tile, eight heads
+    (3, 2, 2, 1000, 1200, 64, BF, 900, 65, [1200, 0, 333]),
+    (2, 40, 40, 1200, 1200, 64, BF, 130, 70, None),     # many items: whole ones, the sinks' beyond them
 ]
 
 
