@@ -12,6 +12,8 @@
 //      would work on tile 0 while the others have finished).  They and tile 0's own item leave fp32 sums of the sink
 //      rows in the workspace,
 //   4. which the reduce kernel adds up in order.
+// With few key tiles the list of each is cut into parts instead (tile 0's with all that see its sinks), whose fp32 sums
+// a last pass adds up.
 // The structure of the two main kernels is the one that measured best for the block-sparse backward: warps 0-7 compute
 // (two groups of 128 threads, thread = tensor-memory lane, group g owns columns [64g, 64g + 64) of the score tiles),
 // warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
@@ -36,6 +38,7 @@ constexpr int kDkvLoadWarp = 10;
 constexpr int kTile = 128 * 128 * 2;
 constexpr int kSlab = 128 * 128;
 constexpr int kBarBytes = 256 + 16;  // 32 mbarriers, tensor-memory base, abort flag
+constexpr int kSmsForParts = 148;    // (a constant, so that the workspace's size does not depend on the device)
 
 struct Params {
   const int32_t* __restrict__ kv_lens;
@@ -51,6 +54,7 @@ struct Params {
   int window, sinks;
   int sink_items;  // further items of tile 0 per (batch, KV head); the workspace holds sink_items + 1 slots
   int sink_m0;     // first query tile beyond the reach of tile 0's windows
+  int parts;       // few key tiles: parts that each one's list is cut into (partial [B * Hkv * Nkv][parts][2][128][D]); else 0
   float scale_log2, softmax_scale;
 };
 
@@ -533,13 +537,37 @@ constexpr int kDkvSmem = 2 * kTile + kDkvStages * kTile + kStatSlots * 1024 + kB
 
 struct DkvItem {
   int b, hkv, nb;
-  int slot;    // workspace slot of the sink rows' sums; -1: every row is stored directly
+  int slot;    // workspace slot of the sink rows' sums (PARTS: of every row's); -1: every row is stored directly
   bool extra;  // an item of the sinks only
   int f0, m0, nm, T;  // pair i: f = f0 + i, query head f / nm of the group, query tile m0 + f % nm
   int len, base;
 };
+template <bool PARTS>
 __device__ __forceinline__ DkvItem dkv_item(const Params& p, int w) {
   DkvItem t;
+  if (PARTS) {
+    t.slot = w % p.parts;
+    w /= p.parts;
+    t.nb = w % p.Nkv;
+    t.hkv = (w / p.Nkv) % p.Hkv;
+    t.b = w / (p.Nkv * p.Hkv);
+    t.extra = false;
+    t.len = seq_len(p, t.b);
+    t.base = p.Sk - p.Sq;
+    t.f0 = t.m0 = t.T = 0;
+    t.nm = 1;
+    const int last = min(p.Sq, t.len - t.base) - 1;  // last query token that takes part
+    const int first = max(0, t.nb * 128 - t.base);
+    const int reach = (t.nb == 0 && p.sinks > 0) ? last : min(last, t.nb * 128 + 127 + p.window - 1 - t.base);
+    if (t.nb * 128 < t.len && first <= reach) {
+      t.m0 = first >> 7;
+      t.nm = (reach >> 7) - t.m0 + 1;
+      const int all = p.G * t.nm;
+      t.f0 = (int)((long long)all * t.slot / p.parts);
+      t.T = (int)((long long)all * (t.slot + 1) / p.parts) - t.f0;
+    }
+    return t;
+  }
   const int extras = p.B * p.Hkv * p.sink_items;
   int bh, chunk = 0;
   t.extra = w < extras;
@@ -582,7 +610,7 @@ __device__ __forceinline__ DkvItem dkv_item(const Params& p, int w) {
   return t;
 }
 
-template <bool F16>
+template <bool F16, bool PARTS>
 __global__ void __launch_bounds__(kDkvThreads, 1)
 window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                   const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
@@ -638,13 +666,13 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = s_tmem_base;
   const uint32_t tS = tmem, tG = tmem + 128u, tdV = tmem + 256u, tdK = tmem + 384u;
-  const int num_work = p.B * p.Hkv * (p.Nkv + p.sink_items);
+  const int num_work = PARTS ? p.B * p.Hkv * p.Nkv * p.parts : p.B * p.Hkv * (p.Nkv + p.sink_items);
 
   if (warp == kDkvLoadWarp) {
     uint32_t r_cnt = 0, kv_cnt = 0, tile_cnt = 0;
     bool ok = true;
     for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
-      const DkvItem t = dkv_item(p, w);
+      const DkvItem t = dkv_item<PARTS>(p, w);
       if (t.T == 0) continue;
       // K is read by S^T only and V by dP^T only: each is replaced as soon as the item before has issued its last one
       for (int which = 0; which < 2 && ok; ++which) {
@@ -698,7 +726,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int ksteps = p.D / 16;
     const uint32_t idesc_n = Idesc<F16>::kmn(p.D);
     for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
-      const int T = dkv_item(p, w).T;
+      const int T = dkv_item<PARTS>(p, w).T;
       if (T == 0) continue;
       ok = mbar_wait(BAR(who == 0 ? kKFull : kVFull), kv_cnt & 1, wctx, 510);
       if (!ok) break;
@@ -785,7 +813,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int cols = p.D - grp * 64;
     bool ok = true;
     for (int w = blockIdx.x; w < num_work && ok; w += gridDim.x) {
-      const DkvItem t = dkv_item(p, w);
+      const DkvItem t = dkv_item<PARTS>(p, w);
       const uint32_t base = r_cnt;
       r_cnt += 2 * t.T;
       const int kv = t.nb * 128 + row;
@@ -904,11 +932,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       if (!ok) break;
       // ---- epilogue
-      const bool to_slot = t.slot >= 0 && row < p.sinks;
+      const bool to_slot = PARTS || (t.slot >= 0 && row < p.sinks);
       const bool to_row = !t.extra && !to_slot && kv < p.Sk && cols > 0;
+      const int slot_rows = PARTS ? 128 : p.sinks;
       float* part = p.partial;
-      if (to_slot)
-        part += ((((long long)t.b * p.Hkv + t.hkv) * (p.sink_items + 1) + t.slot) * 2 * p.sinks + row) * p.D + grp * 64;
+      if (to_slot) {
+        const long long bh = (long long)t.b * p.Hkv + t.hkv;
+        const long long slot = PARTS ? (bh * p.Nkv + t.nb) * p.parts + t.slot : bh * (p.sink_items + 1) + t.slot;
+        part += (slot * 2 * slot_rows + row) * p.D + grp * 64;
+      }
       uint8_t* dk_row = p.dk + (t.b * p.dk_stride[0] + t.hkv * p.dk_stride[1] + (long long)kv * p.dk_stride[2] + grp * 64) * 2;
       uint8_t* dv_row = p.dv + (t.b * p.dv_stride[0] + t.hkv * p.dv_stride[1] + (long long)kv * p.dv_stride[2] + grp * 64) * 2;
       uint32_t acc[64];
@@ -925,7 +957,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int c = 0; c < 64; ++c) acc[c] = 0u;
       }
       if (to_row) store_half<F16>(dv_row, acc, 1.0f, cols);
-      if (to_slot) store_half_f32(part + (long long)p.sinks * p.D, acc, cols);
+      if (to_slot) store_half_f32(part + (long long)slot_rows * p.D, acc, cols);
       if (t.T > 0) {
         __syncwarp();
         tmem_ld32(tdK + lane_base + grp * 64, acc);
@@ -971,26 +1003,78 @@ window_bwd_reduce_kernel(const Params p) {
   *dst = (uint16_t)(pack16<F16>(sum, 0.f) & 0xffffu);
 }
 
-// Split of the sinks' query tiles: first tile beyond the reach of tile 0's windows, and the number of further items.
-static void sink_split(int Hq, int Hkv, int Sq, int Sk, int window, int sinks, int* m0, int* items) {
-  const int Nq = (Sq + 127) / 128, G = Hq / Hkv;
+// 4. dK and dV of key tiles whose lists were cut: the parts' sums in order.  One warp per row, four channels per lane.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+window_bwd_parts_kernel(const Params p) {
+  const int nb = blockIdx.x % p.Nkv, bh = blockIdx.x / p.Nkv;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), kv = nb * 128 + row, d = (threadIdx.x & 31) * 4;
+  if (kv >= p.Sk || d >= p.D) return;
+  const float* src = p.partial + (long long)blockIdx.x * p.parts * 2 * 128 * p.D + (long long)row * p.D + d;
+  float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+  for (int s = 0; s < p.parts; ++s) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const float4 v = *reinterpret_cast<const float4*>(src + (long long)(2 * s + which) * 128 * p.D);
+      sum[which].x += v.x;
+      sum[which].y += v.y;
+      sum[which].z += v.z;
+      sum[which].w += v.w;
+    }
+  }
+  const int hkv = bh % p.Hkv, b = bh / p.Hkv;
+  auto store = [&](uint8_t* base, const long long* st, float4 v, float scale) {
+    uint2 u;
+    u.x = pack16<F16>(v.x * scale, v.y * scale);
+    u.y = pack16<F16>(v.z * scale, v.w * scale);
+    *reinterpret_cast<uint2*>(base + (b * st[0] + hkv * st[1] + kv * st[2] + d) * 2) = u;
+  };
+  store(p.dk, p.dk_stride, sum[0], p.softmax_scale);
+  store(p.dv, p.dv_stride, sum[1], 1.f);
+}
+
+// How the dK/dV kernel's work is dealt.
+struct Deal {
+  int parts;                // few key tiles: parts of each one's list, else 0
+  int sink_m0, sink_items;  // otherwise: first query tile beyond the reach of tile 0's windows, further items of tile 0
+};
+static Deal deal(int B, int Hq, int Hkv, int Sq, int Sk, int window, int sinks) {
+  Deal r{};
+  const long long Nq = (Sq + 127) / 128, Nkv = (Sk + 127) / 128, G = Hq / Hkv;
   const long long reach = 127LL + window - 1 - ((long long)Sk - Sq);
-  *m0 = reach < 0 ? 0 : (int)((reach >> 7) + 1 < Nq ? (reach >> 7) + 1 : Nq);
-  *items = 0;
-  if (sinks <= 0 || *m0 >= Nq) return;
-  const long long pairs = (long long)G * (Nq - *m0);
-  long long per = (long long)G * ((long long)window / 128 + 2);  // pairs of an ordinary item
-  if (per < 16) per = 16;                                         // (below that the prologue and the slot's stores show)
-  long long n = (pairs + per - 1) / per;
-  *items = (int)(n > 128 ? 128 : n);
+  r.sink_m0 = (int)(reach < 0 ? 0 : ((reach >> 7) + 1 < Nq ? (reach >> 7) + 1 : Nq));
+  // Key tiles that leave half of the SMs or more without one are cut into as many parts as there are SMs for, where
+  // that takes at least two (query head, query tile) pairs off the longest list (one takes about 3 us, the pass over the
+  // parts 4).  Tile 0's list is as long as the sequence then if it holds sinks.
+  const long long span = ((long long)window + 127) / 128 + 1, pairs = G * (span < Nq ? span : Nq);
+  const long long longest = sinks > 0 ? G * Nq : pairs;
+  long long parts = kSmsForParts / (B * Hkv * Nkv);
+  if (parts > longest) parts = longest;
+  if (parts >= 2 && pairs - (longest + parts - 1) / parts >= 2) {
+    r.parts = (int)parts;
+    return r;
+  }
+  if (sinks <= 0 || r.sink_m0 >= Nq) return r;
+  const long long beyond = G * (Nq - r.sink_m0);
+  long long per = G * ((long long)window / 128 + 2);  // pairs of an ordinary item
+  if (per < 16) per = 16;                             // (below that the prologue and the slot's stores show)
+  const long long n = (beyond + per - 1) / per;
+  r.sink_items = (int)(n > 128 ? 128 : n);
+  return r;
+}
+static int64_t partial_floats(const Deal& d, int B, int Hkv, int Sk, int D, int sinks) {
+  if (d.parts > 0) return (int64_t)B * Hkv * ((Sk + 127) / 128) * d.parts * 2 * 128 * D;
+  return d.sink_items > 0 ? (int64_t)B * Hkv * (d.sink_items + 1) * 2 * sinks * D : 0;
 }
 
 template <bool F16>
 static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq, const CUtensorMap& tdo,
                   const CUtensorMap& tk, const CUtensorMap& tv, float* lse_log2, float* delta, int num_sms, cudaStream_t st) {
-  static SmemAttribute dq_attribute, dkv_attribute;
+  static SmemAttribute dq_attribute, dkv_attribute[2];
+  auto* dkv = p.parts > 0 ? window_dkv_kernel<F16, true> : window_dkv_kernel<F16, false>;
   cudaError_t e = dq_attribute.set(reinterpret_cast<const void*>(window_dq_kernel<F16>), kDqSmem);
-  if (e == cudaSuccess) e = dkv_attribute.set(reinterpret_cast<const void*>(window_dkv_kernel<F16>), kDkvSmem);
+  if (e == cudaSuccess) e = dkv_attribute[p.parts > 0].set(reinterpret_cast<const void*>(dkv), kDkvSmem);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "bsa_window_bwd: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
   window_bwd_pre_kernel<F16><<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
@@ -999,7 +1083,7 @@ static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq
       p.kv_lens, p.Sk - p.Sq);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward preprocess launch: %s", cudaGetErrorString(e));
-  const int work_q = p.B * p.Hq * p.Nq, work_kv = p.B * p.Hkv * (p.Nkv + p.sink_items);
+  const int work_q = p.B * p.Hq * p.Nq, work_kv = p.B * p.Hkv * (p.parts > 0 ? p.Nkv * p.parts : p.Nkv + p.sink_items);
   window_dq_kernel<F16><<<work_q < num_sms ? work_q : num_sms, kDqThreads, kDqSmem, st>>>(tq, tdo, tk, tv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window dQ launch: %s", cudaGetErrorString(e));
@@ -1017,8 +1101,13 @@ static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq
   dependent.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &dependent;
   config.numAttrs = work_q < 10 * num_sms ? 1 : 0;
-  e = cudaLaunchKernelEx(&config, window_dkv_kernel<F16>, tq, tdo, tk, tv, (const Params)p);
+  e = cudaLaunchKernelEx(&config, dkv, tq, tdo, tk, tv, (const Params)p);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window dK/dV launch: %s", cudaGetErrorString(e));
+  if (p.parts > 0) {
+    window_bwd_parts_kernel<F16><<<dim3((unsigned)(p.B * p.Hkv * p.Nkv), 16), 256, 0, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward parts launch: %s", cudaGetErrorString(e));
+  }
   if (p.sink_items > 0) {
     const long long n = (long long)p.B * p.Hkv * 2 * p.sinks * p.D;
     window_bwd_reduce_kernel<F16><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
@@ -1036,11 +1125,9 @@ using namespace bsa;
 extern "C" int64_t bsa_window_bwd_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Sk, int32_t D,
                                                   int32_t window, int32_t sinks) {
   if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || Sq < 1 || Sk < 1 || D < 1 || window < 1 || sinks < 0) return 0;
-  int m0, items;
-  winbwd::sink_split(Hq, Hkv, Sq, Sk, window < kWindowAll ? window : kWindowAll, sinks, &m0, &items);
+  const winbwd::Deal d = winbwd::deal(B, Hq, Hkv, Sq, Sk, window < kWindowAll ? window : kWindowAll, sinks);
   const int64_t rows = (int64_t)B * Hq * ((Sq + 127) / 128) * 128;
-  const int64_t part = items > 0 ? (int64_t)B * Hkv * (items + 1) * 2 * sinks * D : 0;
-  return (2 * rows + part) * (int64_t)sizeof(float);
+  return (2 * rows + winbwd::partial_floats(d, B, Hkv, Sk, D, sinks)) * (int64_t)sizeof(float);
 }
 
 extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
@@ -1097,7 +1184,10 @@ extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
   p.D = a->D;
   p.window = a->window < kWindowAll ? a->window : kWindowAll;
   p.sinks = a->sinks;
-  winbwd::sink_split(a->Hq, a->Hkv, a->Sq, a->Sk, p.window, a->sinks, &p.sink_m0, &p.sink_items);
+  const winbwd::Deal d = winbwd::deal(a->B, a->Hq, a->Hkv, a->Sq, a->Sk, p.window, a->sinks);
+  p.parts = d.parts;
+  p.sink_m0 = d.sink_m0;
+  p.sink_items = d.sink_items;
   p.softmax_scale = a->softmax_scale;
   p.scale_log2 = a->softmax_scale * kLog2e;
   const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
