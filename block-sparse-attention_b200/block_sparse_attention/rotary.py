@@ -184,6 +184,7 @@ class RotaryFunction(torch.autograd.Function):
         return rotary_nd(q, k, positions, inv_freq, axis_pairs, interleaved=interleaved, layout=layout)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         pairs, interleaved, layout = ctx.how

@@ -187,6 +187,7 @@ def _run_plan(plan: _Plan, q, k, v, out, lse, lens, table, tree):
     a.q, a.k, a.v, a.out = at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if (at[0] | at[1] | at[2] | at[3]) % 16:
         return None
+    assert at[3] != at[1] and at[3] != at[2], "out must not be k or v"
     if lse is not None:
         a.lse = lse.data_ptr()
     if lens is not None:
@@ -304,6 +305,7 @@ def window_attn_bwd(
     a = _cabi.WindowBwdArgs.from_buffer_copy(plan.args)
     a.dout, a.q, a.k, a.v, a.out = at = dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.dq, a.dk, a.dv = to = grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr()
+    assert not any(ptr in at for ptr in to), "a gradient buffer must not be one of the inputs"
     if (at[0] | at[1] | at[2] | at[3] | at[4] | to[0] | to[1] | to[2]) % 16:
         return _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout)
     a.lse = lse.data_ptr()
@@ -374,6 +376,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lens = ctx.saved_tensors
         window, sink_tokens, softmax_scale, layout = ctx.how

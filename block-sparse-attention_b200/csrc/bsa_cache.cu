@@ -49,7 +49,7 @@ cache_append_kernel(const Source s, const Pages pg, const int32_t* __restrict__ 
   const int t0 = (int)(r % groups) * kRows;
   r /= groups;
   const int h = (int)(r % H), b = (int)(r / H);
-  const int base = lens[b] - T;
+  const int base = max(lens[b], 0) - T;
   uint4 kv[kRows], vv[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
@@ -80,7 +80,7 @@ cache_keep_kernel(const Pages pg, const int32_t* __restrict__ lens, const int32_
   const int c = (int)(unit % chunks);
   const long long r = unit / chunks;
   const int h = (int)(r % H), b = (int)(r / H);
-  const int len = lens[b], base = len - T;
+  const int len = lens[b], base = max(len, 0) - T;
   const int32_t* mine = path + (long long)b * path_cap;
   int n = base < 0 ? 0 : max(0, min(path_lens[b], path_cap));
   int last = -1, kept = 0;

@@ -151,7 +151,7 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const uint8_t* o_base = o + (b * os_b + h * os_h + chunk * 8) * 2;
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
   // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
-  const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, kv_lens[b] - base));
+  const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
   uint4 ov[4], dv[4];
   float lv[4];
 #pragma unroll
@@ -1143,7 +1143,7 @@ extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
     return set_error(BSA_ERR_INVALID, "bsa_window_bwd: null pointer");
   if (a->window < 1 || a->sinks < 0 || a->sinks > kMaxSinks)
     return set_error(BSA_ERR_INVALID, "bsa_window_bwd: window must be >= 1 and sinks in [0, %d]", kMaxSinks);
-  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.0e38f)
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 2.0e38f)
     return set_error(BSA_ERR_INVALID, "bsa_window_bwd: softmax_scale must be positive and finite");
   const int64_t need = bsa_window_bwd_workspace_bytes(a->B, a->Hq, a->Hkv, a->Sq, a->Sk, a->D, a->window, a->sinks);
   if (a->workspace_bytes < need) return set_error(BSA_ERR_WORKSPACE, "bsa_window_bwd: workspace of %lld bytes needed", (long long)need);

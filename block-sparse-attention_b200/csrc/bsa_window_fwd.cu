@@ -675,7 +675,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ring_cnt += 2u * (uint32_t)max(n_it, 0);
 
       // ------------------------------------ tile epilogue ------------------------------------
-      const bool seen = r.live && l_sum > 0.f;
+      const bool seen = r.live && l_sum != 0.f;  // (NaN, where the inputs hold one, is passed on)
       const float inv = seen ? (1.f / l_sum) : 0.f;
       const float lse = seen ? (m_cur + lg2_approx(l_sum)) * kLn2 : -INFINITY;
       if (n_it > 0) {
@@ -759,7 +759,10 @@ window_join_kernel(const WinFwdParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (a dependent launch: the forward kernel has ended behind this)
   const int4 j = p.joins[blockIdx.x];
   const int pieces = j.w;
-  if (pieces == 0) return;
+  // (the list is written by the forward kernel, also when one of its waits expired; never trust it with an address)
+  if (pieces < 2 || pieces > p.ctas || (int)blockIdx.x + (pieces - 1) * p.lists >= p.ctas || j.x < 0 || j.x >= p.B ||
+      j.y < 0 || j.y >= p.Hidx || j.z < 0 || j.z >= p.NqT)
+    return;
   const int heads = p.packed ? p.G : 1, lane = threadIdx.x & 31;
   const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int seq = j.z * p.seq_per_tile + row / heads;
@@ -771,14 +774,14 @@ window_join_kernel(const WinFwdParams p) {
   for (int s = lane; s < pieces; s += 32) m = fmaxf(m, p.partial_lse[slot_row(s)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float top = m == -INFINITY ? 0.f : m;  // (the maximum passes over NaN, the sum does not)
   float sum = 0.f;
-  if (m != -INFINITY)
-    for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot_row(s)] - m);
+  for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot_row(s)] - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   if (lane == 0 && p.lse != nullptr)
-    p.lse[((long long)j.x * p.Hq + hq) * p.Sq + seq] = sum > 0.f ? m + __logf(sum) : -INFINITY;
+    p.lse[((long long)j.x * p.Hq + hq) * p.Sq + seq] = sum != 0.f ? top + __logf(sum) : -INFINITY;
   if (lane * 4 >= p.D) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < pieces; s0 += 8) {  // eight partial rows in flight
@@ -787,7 +790,7 @@ window_join_kernel(const WinFwdParams p) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const float l = s0 + u < pieces ? p.partial_lse[slot_row(s0 + u)] : -INFINITY;
-      w[u] = l == -INFINITY ? 0.f : __expf(l - m) * inv;
+      w[u] = l == -INFINITY ? 0.f : __expf(l - top) * inv;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (l != -INFINITY) v[u] = *reinterpret_cast<const float4*>(p.partial_o + slot_row(s0 + u) * p.D + lane * 4);
     }
@@ -864,7 +867,7 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   if (Sk < 1 || Sk > (1 << 29) || a->Sq > (1 << 29)) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: length out of [1, 2^29]");
   if (a->tree_mask && (a->Sq > kMaxTreeNodes || !paged))
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: a tree has at most %d drafts, over a paged cache", kMaxTreeNodes);
-  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.0e38f)  // the running maximum is taken before scaling
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 2.0e38f)  // the running maximum is taken before scaling
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: softmax_scale must be positive and finite");
   if (a->stream_ctas < 0 || a->stream_ctas > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_ctas out of [0, 65535]");
   if (a->stream_lists > 1 && a->stream_ctas % a->stream_lists != 0)

@@ -318,3 +318,46 @@ def test_graph_of_a_decoding_step():
         graph.replay()
         got = res.clone()
         assert torch.equal(got, step())
+
+
+def test_negative_lengths_are_empty_sequences():
+    from block_sparse_attention import cache_append, cache_keep, cached_attn_fwd
+    kc, vc, table, _, _ = make_cache(2, 2, 16, 64, [40, 40], BF, garbage=False)
+    kc, vc, table = kc.cuda(), vc.cuda(), table.cuda()
+    n = torch.tensor([-5, -2 ** 31], dtype=torch.int32, device="cuda")
+    x = torch.ones(2, 2, 3, 64, dtype=BF, device="cuda")
+    before = kc.clone()
+    cache_append(x, x, kc, vc, table, n)
+    path = torch.tensor([[1], [1]], dtype=torch.int32, device="cuda")
+    new = cache_keep(kc, vc, table, n, path, torch.ones(2, dtype=torch.int32, device="cuda"), 3)
+    assert torch.equal(kc, before) and torch.equal(new, n)
+    out, lse = cached_attn_fwd(x, kc, vc, table, n, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_strided_metadata_of_a_single_sequence():
+    """Row views whose strides are those of a larger table."""
+    from block_sparse_attention import cached_attn_fwd
+    kc, vc, table, ks, vs = make_cache(1, 2, 16, 64, [100], BF)
+    wide = torch.full((3, 20), -1, dtype=torch.int32)
+    wide[1, :7] = table[0]
+    lens = torch.tensor([1, 2, 100, 4], dtype=torch.int32)
+    q = torch.randn(1, 4, 1, 64, generator=torch.Generator().manual_seed(0)).bfloat16()
+    for t, n in ((wide.cuda()[1:2], lens.cuda()[2:3]), (wide.cuda()[1:2, :7], lens.cuda()[2::2][:1])):
+        out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), t, n, return_lse=True)
+        check(out, lse, q, ks, vs, [100], ALL, 0, 64 ** -0.5, BF)
+    cols = wide.cuda().t().contiguous().t()[1:2, :7]  # columns far apart
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), cols, lens.cuda()[2:3], return_lse=True)
+    check(out, lse, q, ks, vs, [100], ALL, 0, 64 ** -0.5, BF)
+
+
+def test_many_ragged_sequences():
+    """More sequences than a warp has lanes, lists of very different lengths cut into equal runs."""
+    from block_sparse_attention import cached_attn_fwd
+    g = torch.Generator().manual_seed(21)
+    lens = [int(x) for x in torch.randint(0, 2500, (70,), generator=g)]
+    lens[3] = 0
+    kc, vc, table, ks, vs = make_cache(70, 1, 64, 64, lens, BF)
+    q = torch.randn(70, 2, 1, 64, generator=g).bfloat16()
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), return_lse=True)
+    check(out, lse, q, ks, vs, lens, ALL, 0, 64 ** -0.5, BF)

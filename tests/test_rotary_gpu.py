@@ -121,3 +121,32 @@ def test_graph_and_stream():
     graph.replay()
     b = rotary_nd(q, k, pos, freq, (32, 32))
     assert torch.equal(res[0], b[0]) and torch.equal(res[1], b[1])
+
+
+def test_q_alone_has_a_gradient():
+    from block_sparse_attention import rotary_embedding, rotary_frequencies
+    freq = rotary_frequencies((32,)).cuda()
+    pos = torch.arange(7, dtype=torch.int32, device="cuda")[:, None]
+    x = torch.randn(1, 2, 7, 64, device="cuda", requires_grad=True)
+    y, none = rotary_embedding(x, None, pos, freq, (32,))
+    assert none is None
+    (y * y).sum().backward()
+    # a rotation keeps lengths: the gradient of the squared norm is 2 x (two rotations' 32-bit roundings)
+    torch.testing.assert_close(x.grad, 2 * x.detach(), rtol=0, atol=2.0 ** -18)
+
+
+def test_every_head_dimension_and_pair_count():
+    """Every form's edges: chunks that are turned in part, halves that do not fit chunks, tails."""
+    from block_sparse_attention import rotary_frequencies, rotary_nd
+    g = torch.Generator().manual_seed(3)
+    for dtype in (torch.bfloat16, torch.float32):
+        for D in (2, 4, 8, 16, 24, 62, 64, 200, 256):
+            for P in sorted({1, D // 2, max(1, D // 4), max(1, D // 2 - 1)}):
+                for interleaved in (True, False):
+                    x = torch.randn(1, 3, 5, D, generator=g).to(dtype)
+                    pos = torch.randint(0, 500, (1, 5, 1), generator=g, dtype=torch.int32)
+                    freq = rotary_frequencies((P,))
+                    got, _ = rotary_nd(x.cuda(), None, pos.cuda(), freq.cuda(), (P,), interleaved=interleaved)
+                    ref, size = rotate(x.double(), pos, freq, (P,), interleaved)
+                    assert_within(got, ref, tolerance(ref, size, dtype), f"D {D}, P {P}")
+                    assert torch.equal(got[..., 2 * P:].cpu(), x[..., 2 * P:])

@@ -215,3 +215,79 @@ def test_matches_dense_block_sparse_operator():
     _, _, tol, lse_tol, _, _ = attend(q.double().cpu(), k.double().cpu(), v.double().cpu(), torch.ones(1, 1, 512, dtype=torch.bool), 128 ** -0.5, BF)
     assert_within(a, b.double().cpu(), 2 * tol, "out")
     assert_within(la, lb.double().cpu(), 2 * lse_tol, "lse")
+
+
+def test_nan_is_passed_on_to_its_own_row():
+    from block_sparse_attention import window_attn_fwd
+    for S in (300, 6):  # whole query tiles, and lists cut into runs
+        Sk = 300 if S == 300 else 6000
+        q, k, v, _ = (t.cuda() for t in make(1, 2, 2, S, Sk, 128, BF, seed=12))
+        want, want_lse = window_attn_fwd(q, k, v, 1 << 20, 2, return_lse=True)
+        q[0, 1, 3] = float("nan")
+        out, lse = window_attn_fwd(q, k, v, 1 << 20, 2, return_lse=True)
+        assert out[0, 1, 3].isnan().all() and lse[0, 1, 3].isnan()
+        keep = torch.ones(1, 2, S, dtype=torch.bool, device="cuda")
+        keep[0, 1, 3] = False
+        assert torch.equal(out[keep], want[keep]) and torch.equal(lse[keep], want_lse[keep])
+
+
+def test_aliased_buffers_and_second_derivatives_are_refused():
+    from block_sparse_attention import window_attention, window_attn_bwd, window_attn_fwd
+    q, k, v, do = (t.cuda() for t in make(1, 2, 2, 64, 64, 64, BF))
+    out, lse = window_attn_fwd(q, k, v, 9, return_lse=True)
+    with pytest.raises(AssertionError):
+        window_attn_fwd(q, k, v, 9, out=k)
+    with pytest.raises(AssertionError):
+        window_attn_bwd(do, q, k, v, out, lse, 9, dq=do)
+    q.requires_grad_()
+    g, = torch.autograd.grad(window_attention(q, k, v, 9).float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
+def test_a_very_long_past():
+    """300 000 keys before one query: one list cut over the whole GPU."""
+    from block_sparse_attention import window_attn_fwd
+    q, k, v, _ = make(1, 2, 1, 1, 300000, 64, BF, seed=13)
+    ref, lse, tol, lse_tol, _, _ = attend(q.double(), k.double(), v.double(), torch.ones(1, 1, 300000, dtype=torch.bool), 0.125, BF)
+    out, got = window_attn_fwd(q.cuda(), k.cuda(), v.cuda(), 1 << 20, return_lse=True)
+    assert_within(out, ref, tol, "out")
+    assert_within(got, lse, lse_tol + 2.0 ** -20, "lse")  # (300 000 terms joined from 296 pieces: 2^-22 each of pieces and sum)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on the GPU: each has its own workspace."""
+    from block_sparse_attention import cached_attn_fwd, window_attn_bwd, window_attn_fwd
+    sets = [[t.cuda() for t in make(1, 8, 1, 200, 1500, 128, BF, seed=s)] for s in range(2)]
+    pools = [torch.randn(40, 1, 64, 128, device="cuda").bfloat16() for _ in range(2)]
+    table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+    n = torch.tensor([2500], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v, do):
+        out, lse = window_attn_fwd(q, k, v, 1000, 3, return_lse=True)
+        return (out, cached_attn_fwd(q, *pools, table, n)[0]) + window_attn_bwd(do, q, k, v, out, lse, 1000, 3)
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="one GPU")
+def test_another_device_than_the_current_one():
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    a = make(1, 2, 1, 300, 300, 64, BF)
+    res = []
+    for dev in ("cuda:0", "cuda:1"):
+        q, k, v, do = (t.to(dev) for t in a)
+        out, lse = window_attn_fwd(q, k, v, 50, 2, return_lse=True)
+        res.append([t.cpu() for t in (out,) + window_attn_bwd(do, q, k, v, out, lse, 50, 2)])
+    assert all(torch.equal(x, y) for x, y in zip(*res))
