@@ -148,6 +148,7 @@ class WindowFwdArgs(ctypes.Structure):
         ("pack_gqa", ctypes.c_int32),
         ("stream_ctas", ctypes.c_int32),
         ("stream_lists", ctypes.c_int32),
+        ("team", ctypes.c_int32),
         ("softmax_scale", ctypes.c_float),
     ]
 

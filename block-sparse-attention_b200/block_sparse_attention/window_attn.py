@@ -22,6 +22,7 @@ from .bsa_attn_interface import _ceil_div, _tma_ready
 __all__ = ["window_attn_fwd", "window_attn_bwd", "window_attention", "WindowAttentionFunction"]
 
 MAX_SINK_TOKENS = 128
+MAX_TEAM = 8
 _MAX_LEN = 1 << 29
 
 
@@ -82,20 +83,34 @@ def _aligned(t: torch.Tensor, layout: str) -> torch.Tensor:
     return bhsd if layout == "bhsd" else bhsd.transpose(1, 2)
 
 
-def _stream_ctas(items: int, key_tiles: int, ragged: bool, num_sms: int) -> int:
-    """How the work of a call is dealt: 0 = whole query tiles in turn, otherwise the number of CTAs that share the list of
-    all key tiles evenly.  Sharing costs a second launch, fp32 rows of the cut query tiles and the search for each CTA's
-    run, about the time of four key tiles; it saves the key tiles that the busiest of the places (two for each SM) has
-    above the average.  With lists of unequal lengths that only the device knows, places that get less than eight query
-    tiles each do not even out by themselves."""
+def _deal_work(items: int, key_tiles: int, rows: int, ragged: bool, num_sms: int) -> Tuple[int, int]:
+    """How the work of a call is dealt, as ``(ctas, team)``: ``(0, 1)`` whole query tiles in turn, ``(0, n)`` a cluster of n
+    CTAs for each query tile, ``(ctas, 1)`` that many CTAs share the list of all key tiles evenly.
+
+    The cheapest of the three in key tiles of the busiest place (two places for each SM; a key tile takes 1.5 us there).  A
+    team adds its start and the join through shared memory; sharing a list adds the search for each CTA's run, a second
+    launch, the fp32 rows of the cut query tiles that go through memory, and neighbours that share fewer loads.  The
+    coefficients fit times over 1 to 256 query tiles of 1 to 128 rows, lists of 2 to 256 key tiles, one token of
+    four heads per KV head: 8 query tiles of 8 key tiles take 17.2 us whole, 9.9 as teams, 11.7 shared, of 64 key tiles 101,
+    20.5 and 23.0; 2 query tiles of 128 full rows and 256 key tiles 401, 61.8 and 53.0; 128 of 16 key tiles 34.2, 42.8 and
+    53.0.
+
+    Lists of unequal lengths that only the device knows (``ragged``) are taken as half full on average: that is what
+    sharing makes of them, while whole query tiles, above eight for each place, even out by themselves."""
     places = 2 * num_sms
     if items < 1 or items * (key_tiles + 1) >= 1 << 31:
-        return 0
-    if ragged:
-        share = items < 8 * places and key_tiles >= 8
-    else:
-        share = key_tiles * (places - items) >= 4 * places
-    return min(places, items * key_tiles) if share else 0
+        return 0, 1
+    load = items / places
+    whole = key_tiles * (min(math.ceil(load), 0.5 * load + 0.7 * math.sqrt(load)) if ragged and load > 1 else math.ceil(load))
+    ctas = min(places, items * key_tiles)
+    stream = (0.625 if ragged else 1.25) * max(1.0, key_tiles * load) + 4 + 0.1 * ctas / items + 0.03 * (ctas + items) * rows / 128
+    if ragged and items >= 8 * places:
+        stream = math.inf
+    team = min(MAX_TEAM, key_tiles, places // items)
+    teams = _ceil_div(key_tiles, team) + 2 + 0.1 * rows / team + 0.01 * items if team >= 2 else math.inf
+    if teams < min(whole, stream):
+        return 0, team
+    return (ctas, 1) if stream < whole else (0, 1)
 
 
 class _Plan(NamedTuple):
@@ -156,17 +171,18 @@ def _make_plan(q, k, v, out, lse, lens, layout, shape, *, window, sinks, scale, 
     per_tile = 128 // (Hq // Hkv) if pack_gqa else 128  # query tokens of a tile
     tiles = _ceil_div(Sq, per_tile)
     items = B * tiles * (Hkv if pack_gqa else Hq)
-    ctas = _stream_ctas(items, key_tiles, ragged, _cabi.load().bsa_num_sms(device.index))
+    slot_rows = (Hq // Hkv if pack_gqa else 1) * min(Sq, per_tile)
+    ctas, team = _deal_work(items, key_tiles, slot_rows, ragged, _cabi.load().bsa_num_sms(device.index))
     lists = 1
     if table is not None and 1 < tiles <= ctas:  # new tokens over a long past: nearly the same keys
         lists = tiles
         ctas -= ctas % lists
-    rows = 2 * ctas * min(Sq, per_tile) * (Hq // Hkv if pack_gqa else 1)
+    rows = 2 * ctas * slot_rows
     args = _cabi.WindowFwdArgs(
         None, None, None, None, None, None, None, None, None, None, None, None, _bhsd(q[1], layout), _bhsd(k[1], kv_layout),
         _bhsd(v[1], kv_layout), _bhsd(out_st, layout), _dtype_code(q[2]), B, Hq, Hkv, Sq, Sk, D, window, sinks,
         table[0][1] if table is not None else 0, k[0][2] if table is not None else 0, k[0][0] if table is not None else 0,
-        1 if pack_gqa else 0, ctas, lists, scale)
+        1 if pack_gqa else 0, ctas, lists, team, scale)
     # workspace: the list of joins (four ints a CTA), the pieces' rows, their LSE
     return _Plan(True, False, tuple(q[0]), lse_shape, bytes(args), (4 * ctas + rows * (D + 1)) if ctas else 0, 16 * ctas,
                  16 * ctas + 4 * rows * D, q[1] == ((n := q[0])[1] * n[2] * n[3], n[2] * n[3], n[3], 1))

@@ -14,8 +14,10 @@
 // that share a KV head, so that a key tile is read once for the group.  Packing pays when one head cannot fill a
 // tile; the host packs below 128 query tokens.
 //
-// Two ways of dealing the work: whole query tiles in turn, or - when those are few or of unequal lengths - equal runs of
-// the list of all key tiles of all query tiles ("stream").  A run may begin and end inside a query tile: such pieces
+// Three ways of dealing the work: whole query tiles in turn; for few query tiles with short lists of key tiles (decoding
+// within a window), a cluster of up to eight CTAs for each ("team"), which join their results through one another's
+// shared memory; for few or unequal ones with longer lists, equal runs of the list of all key tiles of all query tiles
+// ("stream").  A run may begin and end inside a query tile: such pieces
 // leave fp32 rows and their LSE in one of the CTA's two slots of the workspace, and window_join_kernel joins them.  The
 // lengths are on the device only, so every warp finds its CTA's run itself from the lengths' prefix sums.
 //
@@ -47,11 +49,14 @@ struct WinFwdParams {
   int window, sinks;
   int max_pages, page_size, num_pages, seg, seg_log2;  // seg = rows of one key box: min(page_size, 128), 128 when contiguous
   int ctas, lists;  // stream
+  int team;         // CTAs of a cluster
   int num_work;     // query tiles
   float scale_log2;
 };
 
 namespace winfwd {
+enum Deal { kWhole, kStream, kTeam };
+constexpr int kMaxTeam = 8;  // (the portable cluster size)
 constexpr int kThreads = 256;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kMmaWarp = 4;
@@ -144,9 +149,9 @@ __device__ __forceinline__ void first_place(const WinFwdParams& p, Place* at) {
 }
 
 // The CTA's next piece.  `whole` counts the query tiles when whole ones are dealt.
-template <bool STREAM>
+template <int DEAL>
 __device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int& whole, Item& t) {
-  if (STREAM) {
+  if (DEAL == kStream) {
     Place s = *at;
     __syncwarp();
     if (s.left <= 0) return false;
@@ -184,9 +189,42 @@ __device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int
   t.it_begin = 0;
   t.it_end = t.tiles.n;
   t.slot = -1;
-  whole += gridDim.x;
+  if (DEAL == kTeam) {
+    t.slot = (int)blockIdx.x % p.team;
+    t.it_begin = (int)((long long)t.tiles.n * t.slot / p.team);
+    t.it_end = (int)((long long)t.tiles.n * (t.slot + 1) / p.team);
+  }
+  whole += gridDim.x;  // (past the end, for a team)
   return true;
 }
+
+// Cluster-wide barrier (all threads of all CTAs) and reads of another CTA's shared memory.
+__device__ __forceinline__ void team_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t team_address(uint32_t local, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float team_load(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float4 team_load4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
+// A team's piece in shared memory, over the tiles, which are done with by then: fp32 rows, four channels c of row r at
+// place (c + r) mod D / 4 (a thread writes a whole row: without the shift the writes of a warp would share a bank), and
+// behind them the rows' LSE.
+__device__ __forceinline__ uint32_t team_place(int row, int c, int D) {
+  return (uint32_t)(row * (D / 4) + (c + row) % (D / 4)) * 16u;
+}
+constexpr uint32_t kTeamLse = 128 * 128 * 4;
+static_assert(kTeamLse + 512 <= (1 + kStages) * kTileBytes, "a team's piece fits the tiles");
 
 // The sinks' tile takes MMAs of 32 or 64 columns where that holds them all (a fifth of a whole tile's time).
 __device__ __forceinline__ bool narrow_end(const WinFwdParams& p, const Item& t) {
@@ -245,11 +283,78 @@ __device__ __forceinline__ uint32_t row_word(const Row& r, int base, int sinks, 
   return w;
 }
 
-template <bool F16, bool STREAM>
+// Joins a team's pieces (window_join_kernel has the formula): the rows are dealt to the CTAs, a warp takes a row, a lane
+// four channels.  Called by the softmax warps - they have the registers - behind their last piece, while the other warps
+// only wait with them; also when a wait expired (the result is marked invalid then).
+template <bool F16>
+__device__ __forceinline__ void join_team(const WinFwdParams& p, uint32_t base) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  team_sync();
+  Item t;
+  int r = (int)blockIdx.x / p.team;
+  t.m = r % p.NqT;
+  r /= p.NqT;
+  t.hidx = r % p.Hidx;
+  t.b = r / p.Hidx;
+  describe(p, t);
+  describe_heads(p, t);
+  const int heads = p.packed ? p.G : 1, rows = heads * t.nseq, step = 4 * p.team;
+  constexpr int kRows = 2;  // of a warp at a time, all their loads in flight
+  for (int row0 = ((int)blockIdx.x % p.team) * 4 + warp; row0 < rows; row0 += kRows * step) {
+    float l[kRows][kMaxTeam];
+    float4 v[kRows][kMaxTeam];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int row = row0 + u * step;
+#pragma unroll
+      for (int s = 0; s < kMaxTeam; ++s) {
+        l[u][s] = -INFINITY;
+        v[u][s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < p.team && row < rows) {
+          l[u][s] = team_load(team_address(base + kTeamLse + row * 4, s));
+          if (lane * 4 < p.D) v[u][s] = team_load4(team_address(base + team_place(row, lane, p.D), s));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int row = row0 + u * step;
+      if (row >= rows) break;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < kMaxTeam; ++s) top = fmaxf(top, l[u][s]);
+      if (top == -INFINITY) top = 0.f;  // (a row that sees nothing, or NaN, which the maximum passes over)
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kMaxTeam; ++s) {  // (rows of a piece that sees nothing are zeros)
+        const float w = __expf(l[u][s] - top);
+        sum += w;
+        acc.x = fmaf(w, v[u][s].x, acc.x);
+        acc.y = fmaf(w, v[u][s].y, acc.y);
+        acc.z = fmaf(w, v[u][s].z, acc.z);
+        acc.w = fmaf(w, v[u][s].w, acc.w);
+      }
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      const int seq = t.seq0 + row / heads, hq = t.hkv * p.G + (p.packed ? row % heads : t.g);
+      if (lane == 0 && p.lse != nullptr)
+        p.lse[((long long)t.b * p.Hq + hq) * p.Sq + seq] = sum != 0.f ? top + __logf(sum) : -INFINITY;
+      if (lane * 4 < p.D) {
+        uint2 packed;
+        packed.x = F16 ? pack_f16x2(acc.x * inv, acc.y * inv) : pack_bf16x2(acc.x * inv, acc.y * inv);
+        packed.y = F16 ? pack_f16x2(acc.z * inv, acc.w * inv) : pack_bf16x2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(p.out + (long long)t.b * p.o_stride_b + (long long)hq * p.o_stride_h +
+                                  (long long)seq * p.o_stride_s + lane * 8) = packed;
+      }
+    }
+  }
+}
+
+template <bool F16, int DEAL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const WinFwdParams p) {
   constexpr int NS = kStages;
+  constexpr bool STREAM = DEAL == kStream;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* sQ = smem_raw;
   uint8_t* sKV = sQ + kTileBytes;
@@ -263,6 +368,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   volatile int& s_abort = *reinterpret_cast<volatile int*>(bars + 33);
   if ((smem_u32(smem_raw) & 1023u) != 0) {  // uniform over the CTA: nothing has been set up yet
     if (threadIdx.x == 0 && atomicCAS(p.status, 0, (int)kStatusBadIndex) == 0) p.status[2] = 996;
+    if (DEAL == kTeam) {  // (the others of the team wait twice)
+      team_sync();
+      team_sync();
+    }
     return;
   }
   const int warp = threadIdx.x >> 5;
@@ -292,7 +401,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tmem_relinquish();
   }
   if (STREAM && warp <= kLoadWarp) first_place(p, place);  // every warp for itself
-  int whole_next = blockIdx.x;
+  int whole_next = DEAL == kTeam ? (int)blockIdx.x / p.team : (int)blockIdx.x;
   if (warp == kLoadWarp && lane == 0) {
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
@@ -313,7 +422,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int segs = 128 / p.seg;  // key boxes of a tile
     int4 join = make_int4(0, 0, 0, 0);
     Item t;
-    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
+    while (ok && next_piece<DEAL>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       if (n_it <= 0) continue;
       if (STREAM && t.slot >= 0 && (t.slot & 1)) {  // the rest of this query tile begins the runs of the CTAs behind
@@ -377,6 +486,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
     }
     if (STREAM && lane == 0) p.joins[blockIdx.x] = join;
+    if (DEAL == kTeam) team_sync();
   } else if (warp == kMmaWarp) {
     // ========================================= MMA issue ========================================
     setmaxnreg_dec<kOtherRegs>();
@@ -391,7 +501,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint64_t v_desc0 = umma_desc_sw128(smem_u32(sKV), (uint32_t)kSlabBytes, 1024);  // MN-major view
     bool ok = true;
     Item t;
-    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
+    while (ok && next_piece<DEAL>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       if (n_it <= 0) continue;
       ok = mbar_wait(BAR(kQFull), q_cnt & 1, wctx, 200);
@@ -456,6 +566,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (ok) ok = issue_pv(std::true_type{}, n_main, true);
       }
     }
+    if (DEAL == kTeam) team_sync();
   } else if (warp < 4) {
     // ===================================== softmax + epilogue ===================================
     setmaxnreg_inc<kSoftmaxRegs>();
@@ -463,12 +574,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     uint32_t s_cnt = 0, of_cnt = 0, ring_cnt = 0;
     bool ok = true;
-    constexpr float kRescaleThreshold = 8.0f;
     const int heads = p.packed ? p.G : 1;  // heads of a tile's rows
     const int segs = 128 / p.seg;
 
     Item t;
-    while (ok && next_piece<STREAM>(p, place, whole_next, t)) {
+    while (ok && next_piece<DEAL>(p, place, whole_next, t)) {
       const int n_it = t.it_end - t.it_begin;
       float m_cur = -INFINITY;  // running max, log2 domain (scale applied)
       float l_sum = 0.f;        // running sum relative to m_cur
@@ -476,6 +586,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int hq = t.hkv * p.G + (p.packed ? row % heads : t.g);
       const bool row_valid = row < heads * t.nseq;
       const bool warp_active = (warp * 32) < heads * t.nseq;  // some row of this warp exists
+      // growth of the maximum (2^8) from which on O is rescaled.  Rows that do not exist have no say: behind the last head
+      // of a packed tile they hold what shared memory held before.
+      const float rescale_from = row_valid ? 8.f : INFINITY;
       const Row r = make_row(p, t, seq, row_valid && n_it > 0);
       // every row of the tile sees all keys of [free_lo, free_hi) that exist
       const int free_lo = min(t.p_hi, t.len - 1) - p.window + 1;
@@ -534,7 +647,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const float m_new = fmaxf(m_cur, top * p.scale_log2);
           if (i == 0) {
             m_cur = m_new;
-          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > kRescaleThreshold)) {
+          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > rescale_from)) {
             const float sc = (m_new == -INFINITY) ? 1.f : ex2_approx(m_cur - m_new);
             m_cur = m_new;
             l_sum *= sc;
@@ -690,7 +803,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const bool piece = STREAM && t.slot >= 0;  // uniform
       if (piece) {
         prow = (long long)t.slot * p.slot_rows + row;
-        dst_f = reinterpret_cast<float4*>(p.partial_o + prow * p.D);
+        // (four channels of all rows side by side: a thread has a row, so the writes of a warp are one run of memory)
+        dst_f = reinterpret_cast<float4*>(p.partial_o + (long long)t.slot * p.slot_rows * p.D) + row;
       } else {
         dst_h = reinterpret_cast<uint4*>(p.out + (long long)t.b * p.o_stride_b + (long long)hq * p.o_stride_h +
                                          (long long)seq * p.o_stride_s);
@@ -711,10 +825,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               for (int e = 0; e < 32; ++e) acc[e] = 0.f;
             }
             if (row_valid) {
-              if (piece) {
+              if (DEAL == kTeam) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  dst_f[c * 8 + e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+                  *reinterpret_cast<float4*>(smem_raw + team_place(row, c * 8 + e, p.D)) =
+                      make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+              } else if (piece) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  dst_f[(long long)(c * 8 + e) * p.slot_rows] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
               } else {
 #pragma unroll
                 for (int ch = 0; ch < 4; ++ch) {
@@ -734,12 +853,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       tc_fence_before();
       if (row_valid) {
-        if (piece) p.partial_lse[prow] = lse;
+        if (DEAL == kTeam) *reinterpret_cast<float*>(smem_raw + kTeamLse + row * 4) = lse;
+        else if (piece) p.partial_lse[prow] = lse;
         else if (p.lse != nullptr) p.lse[((long long)t.b * p.Hq + hq) * p.Sq + seq] = lse;
       }
     }
+    if (DEAL == kTeam) join_team<F16>(p, smem_u32(smem_raw));
   } else {
     setmaxnreg_dec<kOtherRegs>();
+    if (DEAL == kTeam) team_sync();
   }
 
   tc_fence_before();
@@ -748,14 +870,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
+  if (DEAL == kTeam) team_sync();  // nobody leaves while another may read its memory
 }
 
 // Joins the pieces of cut query tiles: lse = log sum_s exp(lse_s), out = sum_s exp(lse_s - lse) O_s.  Block (c, y) takes
-// eight rows of the query tile whose first piece ended CTA c's run, if there is one: one warp per row, four channels
-// per lane.  Pieces in which the row sees nothing carry -inf and are not read.
+// eight rows of the query tile whose first piece ended CTA c's run, if there is one: first a warp for each row's
+// statistics, then a thread for four channels of a row, eight rows side by side as the pieces hold them.  Pieces in which
+// the row sees nothing carry -inf and are not read.
 template <bool F16>
 __global__ void __launch_bounds__(256)
 window_join_kernel(const WinFwdParams p) {
+  __shared__ float s_top[8], s_inv[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (a dependent launch: the forward kernel has ended behind this)
   const int4 j = p.joins[blockIdx.x];
   const int pieces = j.w;
@@ -763,73 +888,96 @@ window_join_kernel(const WinFwdParams p) {
   if (pieces < 2 || pieces > p.ctas || (int)blockIdx.x + (pieces - 1) * p.lists >= p.ctas || j.x < 0 || j.x >= p.B ||
       j.y < 0 || j.y >= p.Hidx || j.z < 0 || j.z >= p.NqT)
     return;
-  const int heads = p.packed ? p.G : 1, lane = threadIdx.x & 31;
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int seq = j.z * p.seq_per_tile + row / heads;
-  if (row >= p.slot_rows || seq >= p.Sq) return;
-  const int hq = p.packed ? j.y * p.G + row % heads : j.y;
+  const int heads = p.packed ? p.G : 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = min(p.slot_rows, heads * (p.Sq - j.z * p.seq_per_tile));
   // the first piece is the last of its CTA's run, each of the others the first of its CTA's
-  auto slot_row = [&](int s) { return (long long)(2 * ((int)blockIdx.x + s * p.lists) + (s == 0 ? 1 : 0)) * p.slot_rows + row; };
-  float m = -INFINITY;
-  for (int s = lane; s < pieces; s += 32) m = fmaxf(m, p.partial_lse[slot_row(s)]);
+  auto slot = [&](int s) { return (long long)(2 * ((int)blockIdx.x + s * p.lists) + (s == 0 ? 1 : 0)); };
+  auto seq_of = [&](int row) { return j.z * p.seq_per_tile + row / heads; };
+  auto head_of = [&](int row) { return p.packed ? j.y * p.G + row % heads : j.y; };
+  {
+    const int row = blockIdx.y * 8 + warp;
+    if (row < rows) {
+      float m = -INFINITY, sum = 0.f;
+      for (int s = lane; s < pieces; s += 32) m = fmaxf(m, p.partial_lse[slot(s) * p.slot_rows + row]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float top = m == -INFINITY ? 0.f : m;  // (the maximum passes over NaN, the sum does not)
-  float sum = 0.f;
-  for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot_row(s)] - top);
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float top = m == -INFINITY ? 0.f : m;  // (the maximum passes over NaN, the sum does not)
+      for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot(s) * p.slot_rows + row] - top);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  if (lane == 0 && p.lse != nullptr)
-    p.lse[((long long)j.x * p.Hq + hq) * p.Sq + seq] = sum != 0.f ? top + __logf(sum) : -INFINITY;
-  if (lane * 4 >= p.D) return;
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) {
+        s_top[warp] = top;
+        s_inv[warp] = sum != 0.f ? 1.f / sum : 0.f;
+        if (p.lse != nullptr)
+          p.lse[((long long)j.x * p.Hq + head_of(row)) * p.Sq + seq_of(row)] = sum != 0.f ? top + __logf(sum) : -INFINITY;
+      }
+    }
+  }
+  __syncthreads();
+  const int u = threadIdx.x & 7, c = threadIdx.x >> 3, row = blockIdx.y * 8 + u;
+  if (row >= rows || c * 4 >= p.D) return;
+  const float top = s_top[u], inv = s_inv[u];
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < pieces; s0 += 8) {  // eight partial rows in flight
     float w[8];
     float4 v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float l = s0 + u < pieces ? p.partial_lse[slot_row(s0 + u)] : -INFINITY;
-      w[u] = l == -INFINITY ? 0.f : __expf(l - top) * inv;
-      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l != -INFINITY) v[u] = *reinterpret_cast<const float4*>(p.partial_o + slot_row(s0 + u) * p.D + lane * 4);
+    for (int e = 0; e < 8; ++e) {
+      const float l = s0 + e < pieces ? p.partial_lse[slot(s0 + e) * p.slot_rows + row] : -INFINITY;
+      w[e] = l == -INFINITY ? 0.f : __expf(l - top) * inv;
+      v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (l != -INFINITY)
+        v[e] = reinterpret_cast<const float4*>(p.partial_o)[(slot(s0 + e) * (p.D / 4) + c) * p.slot_rows + row];
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      acc.x = fmaf(w[u], v[u].x, acc.x);
-      acc.y = fmaf(w[u], v[u].y, acc.y);
-      acc.z = fmaf(w[u], v[u].z, acc.z);
-      acc.w = fmaf(w[u], v[u].w, acc.w);
+    for (int e = 0; e < 8; ++e) {
+      acc.x = fmaf(w[e], v[e].x, acc.x);
+      acc.y = fmaf(w[e], v[e].y, acc.y);
+      acc.z = fmaf(w[e], v[e].z, acc.z);
+      acc.w = fmaf(w[e], v[e].w, acc.w);
     }
   }
   uint2 packed;
   packed.x = F16 ? pack_f16x2(acc.x, acc.y) : pack_bf16x2(acc.x, acc.y);
   packed.y = F16 ? pack_f16x2(acc.z, acc.w) : pack_bf16x2(acc.z, acc.w);
-  *reinterpret_cast<uint2*>(p.out + (long long)j.x * p.o_stride_b + (long long)hq * p.o_stride_h +
-                            (long long)seq * p.o_stride_s + lane * 8) = packed;
+  *reinterpret_cast<uint2*>(p.out + (long long)j.x * p.o_stride_b + (long long)head_of(row) * p.o_stride_h +
+                            (long long)seq_of(row) * p.o_stride_s + c * 8) = packed;
 }
 
-template <bool F16, bool STREAM>
+template <bool F16, int DEAL>
 static int launch(const WinFwdParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                   int num_sms, cudaStream_t stream) {
-  auto kern = window_fwd_kernel<F16, STREAM>;
+  auto kern = window_fwd_kernel<F16, DEAL>;
   static SmemAttribute attribute;
   cudaError_t e = attribute.set(reinterpret_cast<const void*>(kern), kSmemBytes);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cudaFuncSetAttribute(smem): %s", cudaGetErrorString(e));
-  const int grid = STREAM ? p.ctas : (p.num_work < kCtasPerSm * num_sms ? p.num_work : kCtasPerSm * num_sms);
-  kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
-  e = cudaGetLastError();
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr = {};
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = kSmemBytes;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 0;
+  if (DEAL == kTeam) {
+    config.gridDim = dim3((unsigned)(p.num_work * p.team));
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.team;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.numAttrs = 1;
+  } else if (DEAL == kStream) {
+    config.gridDim = dim3((unsigned)p.ctas);
+  } else {
+    config.gridDim = dim3((unsigned)(p.num_work < kCtasPerSm * num_sms ? p.num_work : kCtasPerSm * num_sms));
+  }
+  e = cudaLaunchKernelEx(&config, kern, tq, tk, tv, p);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window forward launch: %s", cudaGetErrorString(e));
-  if (STREAM) {
-    // a dependent launch, set up while the forward kernel runs: 18.6 -> 17.3 us a call for one token of one sequence
-    cudaLaunchConfig_t config = {};
+  if (DEAL == kStream) {
+    // a dependent launch, set up while the forward kernel runs (1.3 us less a call for small ones)
     config.gridDim = dim3((unsigned)p.ctas, (unsigned)((p.slot_rows + 7) / 8));
     config.blockDim = dim3(256);
-    config.stream = stream;
-    cudaLaunchAttribute dependent = {};
-    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    dependent.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &dependent;
+    config.dynamicSmemBytes = 0;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     config.numAttrs = 1;
     e = cudaLaunchKernelEx(&config, window_join_kernel<F16>, p);
     if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window join launch: %s", cudaGetErrorString(e));
@@ -870,6 +1018,8 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   if (!(a->softmax_scale > 0.f) || a->softmax_scale > 2.0e38f)  // the running maximum is taken before scaling
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: softmax_scale must be positive and finite");
   if (a->stream_ctas < 0 || a->stream_ctas > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_ctas out of [0, 65535]");
+  if (a->team < 0 || a->team > winfwd::kMaxTeam || (a->team > 1 && a->stream_ctas > 0))
+    return set_error(BSA_ERR_INVALID, "bsa_window_fwd: team out of [0, %d], or together with stream_ctas", winfwd::kMaxTeam);
   if (a->stream_lists > 1 && a->stream_ctas % a->stream_lists != 0)
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_ctas must be a multiple of stream_lists");
   if (a->stream_ctas > 0 && (!a->partial_o || !a->partial_lse || !a->joins))
@@ -920,10 +1070,13 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   for (p.seg_log2 = 4; (1 << p.seg_log2) < p.seg;) ++p.seg_log2;
   p.ctas = a->stream_ctas;
   p.lists = a->stream_lists > 1 ? a->stream_lists : 1;
+  p.team = a->team > 1 ? a->team : 1;
   p.slot_rows = (packed ? G : 1) * (a->Sq < p.seq_per_tile ? a->Sq : p.seq_per_tile);
   const long long work = (long long)p.B * p.Hidx * p.NqT;
-  if (work > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 work items");
+  if (work > 0x7f000000LL)  // (a grid's width is added to an item's index)
+    return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 work items");
   p.num_work = (int)work;
+  if (p.team > 1 && work * p.team > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: more than 65535 CTAs in teams");
   if (p.ctas > 0 && p.lists > 1 && p.lists != p.NqT)
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_lists must be 1 or the number of query tiles per head (%d)", p.NqT);
   if (p.ctas > 0 && work * ((Sk + 127) / 128 + 1) > 0x7fffffffLL)
@@ -953,9 +1106,11 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
     if (rc) return rc;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  if (a->dtype == BSA_DTYPE_F16)
-    return p.ctas > 0 ? winfwd::launch<true, true>(p, tq, tk, tv, num_sms, st)
-                      : winfwd::launch<true, false>(p, tq, tk, tv, num_sms, st);
-  return p.ctas > 0 ? winfwd::launch<false, true>(p, tq, tk, tv, num_sms, st)
-                    : winfwd::launch<false, false>(p, tq, tk, tv, num_sms, st);
+  auto run = [&](auto f16) {
+    constexpr bool kF16 = decltype(f16)::value;
+    if (p.team > 1) return winfwd::launch<kF16, winfwd::kTeam>(p, tq, tk, tv, num_sms, st);
+    if (p.ctas > 0) return winfwd::launch<kF16, winfwd::kStream>(p, tq, tk, tv, num_sms, st);
+    return winfwd::launch<kF16, winfwd::kWhole>(p, tq, tk, tv, num_sms, st);
+  };
+  return a->dtype == BSA_DTYPE_F16 ? run(std::true_type{}) : run(std::false_type{});
 }

@@ -310,7 +310,8 @@ int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, in
  * so that they share their reads of the keys); partial_o [2 * stream_ctas, R,
  * D] and partial_lse [2 * stream_ctas, R] f32 (R = rows of a query tile: min(Sq, 128), packed G * min(Sq,
  * floor(128 / G))) hold the pieces of cut query tiles, joins [4 * stream_ctas] int32 their list; a second launch of the
- * same call joins them.
+ * same call joins them.  team = 2..8 (with stream_ctas = 0): a cluster of that many CTAs works on each query tile and
+ * joins its results itself, for few query tiles with short lists.
  * D = 64, 96 or 128; window >= 1 (2^29 and more: everything before the row); 0 <= sinks <= 128;
  * softmax_scale > 0; page_size 16, 32, 64 or a multiple of 128; lengths up to 2^29.
  */
@@ -341,6 +342,7 @@ typedef struct bsa_window_fwd_args {
   int32_t pack_gqa;
   int32_t stream_ctas;
   int32_t stream_lists;
+  int32_t team;
   float softmax_scale;
 } bsa_window_fwd_args;
 

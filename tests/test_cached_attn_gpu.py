@@ -361,3 +361,29 @@ def test_many_ragged_sequences():
     q = torch.randn(70, 2, 1, 64, generator=g).bfloat16()
     out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), return_lse=True)
     check(out, lse, q, ks, vs, lens, ALL, 0, 64 ** -0.5, BF)
+
+
+@pytest.fixture
+def deal(request, monkeypatch):
+    """Every call deals its work in the given way, whatever the rule says."""
+    from block_sparse_attention import cached_attn, window_attn
+
+    def clear():
+        cached_attn._cached_plan.cache_clear()
+        window_attn._window_plan.cache_clear()
+    monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
+    clear()
+    yield request.param
+    clear()
+
+
+DEALS = [(0, 1), (0, 2), (0, 5), (0, 8), (1, 1), (7, 1), (296, 1)]
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+def test_every_way_of_dealing_the_work(deal):
+    """More CTAs in a team than key tiles, runs that end anywhere, more CTAs than there is work."""
+    for case in CASES:
+        test_tokens(case, "bhsd")
+    for tree in TREES:
+        test_trees(tree, BF)

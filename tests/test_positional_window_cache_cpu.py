@@ -132,7 +132,7 @@ def test_c_entry_points_refuse_bad_arguments():
         return lib.bsa_window_fwd(a, None)
 
     for kw in (dict(dtype=1), dict(D=80), dict(B=0), dict(Hq=3), dict(q=None), dict(window=0), dict(sinks=129), dict(sinks=-1),
-               dict(stream_ctas=-1), dict(stream_ctas=2), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(Sk=0),
+               dict(stream_ctas=-1), dict(stream_ctas=2), dict(team=9), dict(team=-1), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")), dict(Sk=0),
                dict(Sk=(1 << 29) + 1), dict(out=(1 << 20) + 2), dict(o_stride=(ctypes.c_int64 * 3)(1024, 512, 60)),
                dict(tree_mask=1 << 20), dict(page_table=1 << 20), dict(page_table=1 << 20, page_size=24, max_pages=1, num_pages=1),
                dict(page_table=1 << 20, page_size=16, max_pages=1, num_pages=1),  # no lengths
@@ -158,14 +158,19 @@ def test_c_entry_points_refuse_bad_arguments():
 
 
 def test_rule_of_dealing_the_work():
-    from block_sparse_attention.window_attn import _stream_ctas
-    assert _stream_ctas(296, 100, False, 148) == 0      # query tiles for both places of every SM
-    assert _stream_ctas(148, 100, False, 148) == 296
-    assert _stream_ctas(148, 7, False, 148) == 0        # 3.5 key tiles to gain
-    assert _stream_ctas(8, 9, False, 148) == 72         # no more CTAs than key tiles
-    assert _stream_ctas(2367, 100, True, 148) == 296    # lengths that only the device knows
-    assert _stream_ctas(2368, 100, True, 148) == 0
-    assert _stream_ctas(1, 7, True, 148) == 0
+    from block_sparse_attention.window_attn import _deal_work
+    whole = (0, 1)
+    for items, key_tiles, rows, ragged, want in [
+            (296, 100, 128, False, whole),         # a query tile for both places of every SM
+            (304, 100, 128, False, (296, 1)),      # a second round for eight of them
+            (512, 33, 128, False, whole),          # 66 key tiles at the busiest place, 57 on average
+            (148, 100, 128, False, (0, 2)), (148, 7, 4, False, whole),
+            (8, 2, 4, False, whole), (8, 4, 4, False, (0, 4)), (8, 33, 4, False, (0, 8)), (8, 300, 4, False, (296, 1)),
+            (8, 64, 128, False, (0, 8)), (8, 256, 128, False, (296, 1)),
+            (1, 1, 1, True, whole), (1, 7, 128, True, (0, 7)),  # no larger team than there are key tiles
+            (2367, 100, 128, True, (296, 1)), (2368, 100, 128, True, whole),
+            (0, 5, 1, False, whole), (1 << 20, 1 << 12, 128, False, whole)]:
+        assert _deal_work(items, key_tiles, rows, ragged, 148) == want, (items, key_tiles, rows, ragged)
 
 
 def test_gradient_formula_against_differences():

@@ -291,3 +291,26 @@ def test_another_device_than_the_current_one():
         out, lse = window_attn_fwd(q, k, v, 50, 2, return_lse=True)
         res.append([t.cpu() for t in (out,) + window_attn_bwd(do, q, k, v, out, lse, 50, 2)])
     assert all(torch.equal(x, y) for x, y in zip(*res))
+
+
+@pytest.fixture
+def deal(request, monkeypatch):
+    """Every call deals its work in the given way, whatever the rule says."""
+    from block_sparse_attention import cached_attn, window_attn
+
+    def clear():
+        cached_attn._cached_plan.cache_clear()
+        window_attn._window_plan.cache_clear()
+    monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
+    clear()
+    yield request.param
+    clear()
+
+
+DEALS = [(0, 1), (0, 2), (0, 5), (0, 8), (1, 1), (7, 1), (296, 1)]
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+def test_every_way_of_dealing_the_work(deal):
+    for case in CASES:
+        test_forward(case, "bshd")
