@@ -48,6 +48,11 @@ def _check_pool_address(k_cache, v_cache) -> None:
     assert (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the pools must be 16-byte aligned"
 
 
+def _check_written_pools(k_cache, v_cache) -> None:
+    _check_pool_address(k_cache, v_cache)
+    assert k_cache.data_ptr() != v_cache.data_ptr(), "keys and values must not be written to one pool"
+
+
 @functools.lru_cache(maxsize=256, typed=True)
 def _cached_plan(q, k_cache, v_cache, table, lens, tree, out, lse, window, sinks, softmax_scale, layout, want_lse) -> _Plan:
     window, sinks = _check_window(_MAX_LEN if window is None else window, sinks)
@@ -195,7 +200,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     must not be reached through two sequences' tables for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
     """
     plan = _append_plan(_meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), layout)
-    _check_pool_address(k_cache, v_cache)
+    _check_written_pools(k_cache, v_cache)
     if plan.empty:
         return k_cache, v_cache
     at = k.data_ptr(), v.data_ptr()
@@ -218,7 +223,7 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     ``num_drafts`` tokens is left as it is.  A move from or to a page that is not in the pool is dropped.
     """
     plan = _keep_plan(_meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(path), _meta(path_lens), num_drafts)
-    _check_pool_address(k_cache, v_cache)
+    _check_written_pools(k_cache, v_cache)
     if plan.empty:
         return cache_lens.clone()
     if not plan.direct:

@@ -9,8 +9,8 @@
 //
 // The angle of position 10^5 at frequency 1 is 10^5 radians; in 32 bits its fraction of a turn would be off by 10^-3.
 // So a frequency becomes a 64-bit fraction of a turn per position, whose product with the position wraps around whole
-// turns by itself (integer arithmetic modulo 2^64: off by less than 2^-32 turns for any 32-bit position), and only the
-// wrapped turn is rounded to 32 bits.
+// turns by itself (integer arithmetic modulo 2^64; frequencies up to 1 are off by 2^-55 turns, their products with any
+// 32-bit position by 2^-24), and only the wrapped turn is rounded to 32 bits.
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"
@@ -91,16 +91,18 @@ struct Io<__half> {
 __device__ __forceinline__ unsigned long long turn_fraction(float inv_freq) {
   constexpr double kInvTwoPi = 0.15915494309189533576888, kTwo64 = 18446744073709551616.0;
   const double turns = (double)inv_freq * kInvTwoPi;
-  return (unsigned long long)((turns - floor(turns)) * kTwo64);  // (below 2^64: the largest double below 1 is 1 - 2^-53)
+  return (unsigned long long)((turns - floor(turns)) * kTwo64);  // (a tiny negative one rounds to a whole turn: the conversion saturates)
 }
+// 0, or NaN for a frequency that is infinite or NaN (the integers above would hide it).
+__device__ __forceinline__ float poison_of(float inv_freq) { return inv_freq - inv_freq; }
 __device__ __forceinline__ int axis_of(const Params& p, int pair) {
   return (pair >= p.end0) + (pair >= p.end1) + (pair >= p.end2);
 }
-__device__ __forceinline__ float2 position_sincos(const Params& p, int position, unsigned long long turns) {
+__device__ __forceinline__ float2 position_sincos(const Params& p, int position, unsigned long long turns, float poison) {
   const int wrapped = (int)((turns * (unsigned long long)(long long)position) >> 32);  // [-1/2, 1/2) turns, times 2^32
   float s, c;
   sincospif((float)wrapped * 0x1p-31f, &s, &c);
-  return make_float2(c, s * p.sign);
+  return make_float2(c + poison, s * p.sign + poison);
 }
 
 // The rows of one token: q heads first, then k heads.
@@ -127,6 +129,7 @@ rotary_vec_kernel(const Params p) {
   constexpr int kFly = INTERLEAVED ? 4 : 2;  // heads in flight: four 16-byte loads, twice
   __shared__ float2 table[kTable];
   __shared__ unsigned long long turns[kTable / 8];  // P <= D / 2 <= 256
+  __shared__ float poison[kTable / 8];
   const int token0 = blockIdx.x * p.tokens_per_block;
   const int here = min(p.tokens_per_block, p.tokens - token0);
   const int units = p.tokens_per_block * p.per_token;
@@ -157,13 +160,17 @@ rotary_vec_kernel(const Params p) {
   Batch now, then;
   if (works) load(h, now);  // on their way while the sines are computed
 
-  for (int i = threadIdx.x; i < p.P; i += kThreads) turns[i] = turn_fraction(p.inv_freq[i]);
+  for (int i = threadIdx.x; i < p.P; i += kThreads) {
+    const float f = p.inv_freq[i];
+    turns[i] = turn_fraction(f);
+    poison[i] = poison_of(f);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < here * p.P; i += kThreads) {
     const int at = i / p.P, pair = i - at * p.P;
     const int bt = (token0 + at) / p.S;
     const int position = p.positions[bt * p.pos_b + (token0 + at - bt * p.S) * p.pos_s + axis_of(p, pair)];
-    table[i] = position_sincos(p, position, turns[pair]);
+    table[i] = position_sincos(p, position, turns[pair], poison[pair]);
   }
   __syncthreads();
   if (!works) return;
@@ -235,8 +242,10 @@ rotary_elt_kernel(const Params p) {
   const Rows rows(p, b, tok);
   const bool turned = c < p.P;
   float2 cs = make_float2(1.f, 0.f);
-  if (turned)
-    cs = position_sincos(p, p.positions[b * p.pos_b + tok * p.pos_s + axis_of(p, c)], turn_fraction(p.inv_freq[c]));
+  if (turned) {
+    const float f = p.inv_freq[c];
+    cs = position_sincos(p, p.positions[b * p.pos_b + tok * p.pos_s + axis_of(p, c)], turn_fraction(f), poison_of(f));
+  }
   const int ia = turned ? (INTERLEAVED ? 2 * c : c) : p.P + c;
   const int ib = INTERLEAVED ? 2 * c + 1 : p.P + c;
   const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(p.heads, h0 + p.heads_per_cta);

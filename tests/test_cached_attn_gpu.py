@@ -200,6 +200,18 @@ def test_append(page, T, D, layout):
     assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v)
 
 
+def test_one_pool_for_keys_and_values_is_not_written():
+    from block_sparse_attention import cache_append, cache_keep
+    pool = torch.zeros(4, 2, 16, 64, dtype=BF, device="cuda")
+    table, lens = torch.tensor([[0]], dtype=torch.int32).cuda(), torch.tensor([3], dtype=torch.int32).cuda()
+    rows = torch.ones(1, 2, 3, 64, dtype=BF, device="cuda")
+    with pytest.raises(AssertionError):
+        cache_append(rows, rows, pool, pool, table, lens)
+    with pytest.raises(AssertionError):
+        cache_keep(pool, pool, table, lens, table, lens, 3)
+    assert not pool.any()
+
+
 def test_append_from_strided_and_broadcast_rows():
     from block_sparse_attention import cache_append
     kc, vc, table, _, _ = make_cache(2, 2, 16, 64, [20, 20], BF, garbage=False)

@@ -168,7 +168,7 @@ def test_rule_of_dealing_the_work():
             (8, 2, 4, False, whole), (8, 4, 4, False, (0, 4)), (8, 33, 4, False, (0, 8)), (8, 300, 4, False, (296, 1)),
             (8, 64, 128, False, (0, 8)), (8, 256, 128, False, (296, 1)),
             (1, 1, 1, True, whole), (1, 7, 128, True, (0, 7)),  # no larger team than there are key tiles
-            (2367, 100, 128, True, (296, 1)), (2368, 100, 128, True, whole),
+            (1024, 32, 4, True, (296, 1)), (2048, 16, 4, True, whole), (1024, 9, 128, True, whole),
             (0, 5, 1, False, whole), (1 << 20, 1 << 12, 128, False, whole)]:
         assert _deal_work(items, key_tiles, rows, ragged, 148) == want, (items, key_tiles, rows, ragged)
 

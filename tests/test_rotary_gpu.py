@@ -150,3 +150,18 @@ def test_every_head_dimension_and_pair_count():
                     ref, size = rotate(x.double(), pos, freq, (P,), interleaved)
                     assert_within(got, ref, tolerance(ref, size, dtype), f"D {D}, P {P}")
                     assert torch.equal(got[..., 2 * P:].cpu(), x[..., 2 * P:])
+
+
+@pytest.mark.parametrize("D", [64, 20])  # 16-byte chunks, and rows that they do not fit
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_bad_frequencies_show_in_their_own_pairs(D, interleaved):
+    from block_sparse_attention import rotary_nd
+    P = D // 2
+    x = torch.randn(1, 2, 3, D, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).cuda()
+    freq = torch.rand(P, generator=torch.Generator().manual_seed(1))
+    freq[1], freq[4] = float("nan"), float("-inf")
+    got, _ = rotary_nd(x, None, torch.arange(1, 4, dtype=torch.int32)[:, None].cuda(), freq.cuda(), (P,), interleaved=interleaved)
+    bad = torch.zeros(D, dtype=torch.bool)
+    for p in (1, 4):
+        bad[[2 * p, 2 * p + 1] if interleaved else [p, P + p]] = True
+    assert torch.equal(got.isnan().cpu(), bad.expand(1, 2, 3, D))

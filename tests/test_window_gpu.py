@@ -239,6 +239,9 @@ def test_aliased_buffers_and_second_derivatives_are_refused():
         window_attn_fwd(q, k, v, 9, out=k)
     with pytest.raises(AssertionError):
         window_attn_bwd(do, q, k, v, out, lse, 9, dq=do)
+    both = torch.empty_like(k)
+    with pytest.raises(AssertionError):
+        window_attn_bwd(do, q, k, v, out, lse, 9, dk=both, dv=both)
     q.requires_grad_()
     g, = torch.autograd.grad(window_attention(q, k, v, 9).float().square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
