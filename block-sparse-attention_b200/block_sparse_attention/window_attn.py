@@ -92,8 +92,8 @@ def _deal_work(items: int, key_tiles: int, rows: int, ragged: bool, num_sms: int
     launch, the fp32 rows of the cut query tiles that go through memory, and neighbours that share fewer loads.  The
     coefficients fit times over 1 to 256 query tiles of 1 to 128 rows, lists of 2 to 256 key tiles, one token of
     four heads per KV head: 8 query tiles of 8 key tiles take 17.2 us whole, 9.9 as teams, 11.7 shared, of 64 key tiles 101,
-    20.5 and 23.0; 2 query tiles of 128 full rows and 256 key tiles 401, 61.8 and 53.0; 128 of 16 key tiles 34.2, 42.8 and
-    53.0.
+    20.5 and 23.0; 16 query tiles of 128 full rows and 128 key tiles 204, 44.7 and 37.2; 128 of 16 key tiles 34.2, 42.4
+    and 46.7.
 
     Lists of unequal lengths that only the device knows (``ragged``) are taken as half full on average: that is what
     sharing makes of them, while several whole query tiles for each place even out by themselves (sequences of equally
@@ -104,7 +104,7 @@ def _deal_work(items: int, key_tiles: int, rows: int, ragged: bool, num_sms: int
     load = items / places
     whole = key_tiles * (min(math.ceil(load), 0.5 * load + 0.42 * math.sqrt(load)) if ragged and load > 1 else math.ceil(load))
     ctas = min(places, items * key_tiles)
-    stream = (0.625 if ragged else 1.25) * max(1.0, key_tiles * load) + 4 + 0.1 * ctas / items + 0.03 * (ctas + items) * rows / 128
+    stream = (0.625 if ragged else 1.25) * max(1.0, key_tiles * load) + 4 + 0.07 * ctas / items + 0.02 * (ctas + items) * rows / 128
     team = min(MAX_TEAM, key_tiles, places // items)
     teams = _ceil_div(key_tiles, team) + 2 + 0.1 * rows / team + 0.01 * items if team >= 2 else math.inf
     if teams < min(whole, stream):

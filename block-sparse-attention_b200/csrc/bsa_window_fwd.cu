@@ -874,13 +874,18 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 }
 
 // Joins the pieces of cut query tiles: lse = log sum_s exp(lse_s), out = sum_s exp(lse_s - lse) O_s.  Block (c, y) takes
-// eight rows of the query tile whose first piece ended CTA c's run, if there is one: first a warp for each row's
-// statistics, then a thread for four channels of a row, eight rows side by side as the pieces hold them.  Pieces in which
-// the row sees nothing carry -inf and are not read.
-template <bool F16>
+// kJoinRows * R rows of the query tile whose first piece ended CTA c's run, if there is one: first each row's statistics,
+// then a thread for four channels of R rows, eight rows side by side as the pieces hold them.  Pieces in which the row
+// sees nothing carry -inf and are not read.
+// Bound by the latency of its chain of loads, so eight are in flight: of eight pieces of one row where tiles have few rows
+// or many pieces, of two pieces of four rows otherwise (128 query tiles of 128 rows, two or three pieces each: 12 us, with
+// one row a thread 24).
+constexpr int kJoinRows = 8;
+template <bool F16, int R>
 __global__ void __launch_bounds__(256)
 window_join_kernel(const WinFwdParams p) {
-  __shared__ float s_top[8], s_inv[8];
+  constexpr int kFly = 8 / R;  // pieces of a row in flight
+  __shared__ float s_top[kJoinRows * R], s_inv[kJoinRows * R];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (a dependent launch: the forward kernel has ended behind this)
   const int4 j = p.joins[blockIdx.x];
   const int pieces = j.w;
@@ -889,59 +894,97 @@ window_join_kernel(const WinFwdParams p) {
       j.y < 0 || j.y >= p.Hidx || j.z < 0 || j.z >= p.NqT)
     return;
   const int heads = p.packed ? p.G : 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = min(p.slot_rows, heads * (p.Sq - j.z * p.seq_per_tile));
+  const int rows = min(p.slot_rows, heads * (p.Sq - j.z * p.seq_per_tile)), row0 = (int)blockIdx.y * kJoinRows * R;
   // the first piece is the last of its CTA's run, each of the others the first of its CTA's
   auto slot = [&](int s) { return (long long)(2 * ((int)blockIdx.x + s * p.lists) + (s == 0 ? 1 : 0)); };
+  auto piece_lse = [&](int s, int row) { return p.partial_lse[slot(s) * p.slot_rows + row]; };
   auto seq_of = [&](int row) { return j.z * p.seq_per_tile + row / heads; };
   auto head_of = [&](int row) { return p.packed ? j.y * p.G + row % heads : j.y; };
-  {
-    const int row = blockIdx.y * 8 + warp;
+  auto statistics = [&](int at, float top, float sum) {
+    const int row = row0 + at;
+    s_top[at] = top;
+    s_inv[at] = sum != 0.f ? 1.f / sum : 0.f;
+    if (p.lse != nullptr)
+      p.lse[((long long)j.x * p.Hq + head_of(row)) * p.Sq + seq_of(row)] = sum != 0.f ? top + __logf(sum) : -INFINITY;
+  };
+  if (R == 1) {  // a warp for a row
+    const int row = row0 + warp;
     if (row < rows) {
       float m = -INFINITY, sum = 0.f;
-      for (int s = lane; s < pieces; s += 32) m = fmaxf(m, p.partial_lse[slot(s) * p.slot_rows + row]);
+      for (int s = lane; s < pieces; s += 32) m = fmaxf(m, piece_lse(s, row));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float top = m == -INFINITY ? 0.f : m;  // (the maximum passes over NaN, the sum does not)
-      for (int s = lane; s < pieces; s += 32) sum += __expf(p.partial_lse[slot(s) * p.slot_rows + row] - top);
+      for (int s = lane; s < pieces; s += 32) sum += __expf(piece_lse(s, row) - top);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) {
-        s_top[warp] = top;
-        s_inv[warp] = sum != 0.f ? 1.f / sum : 0.f;
-        if (p.lse != nullptr)
-          p.lse[((long long)j.x * p.Hq + head_of(row)) * p.Sq + seq_of(row)] = sum != 0.f ? top + __logf(sum) : -INFINITY;
+      if (lane == 0) statistics(warp, top, sum);
+    }
+  } else if (warp == 0) {  // a lane for a row
+    const int row = row0 + lane;
+    if (row < rows) {
+      float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < pieces; ++s) m = fmaxf(m, piece_lse(s, row));
+      const float top = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+      for (int s = 0; s < pieces; ++s) sum += __expf(piece_lse(s, row) - top);
+      statistics(lane, top, sum);
+    }
+  }
+  static_assert(R == 1 || kJoinRows * R == 32, "a lane for a row");
+  const int u = threadIdx.x & 7, c = threadIdx.x >> 3;
+  float w[R][kFly];
+  float4 v[R][kFly], acc[R];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int row = row0 + u + i * kJoinRows;
+#pragma unroll
+      for (int e = 0; e < kFly; ++e) {
+        w[i][e] = -INFINITY;
+        v[i][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s0 + e < pieces && row < rows && c * 4 < p.D) {
+          w[i][e] = piece_lse(s0 + e, row);
+          v[i][e] = reinterpret_cast<const float4*>(p.partial_o)[(slot(s0 + e) * (p.D / 4) + c) * p.slot_rows + row];
+        }
       }
     }
-  }
+  };
+  load(0);  // (under the statistics)
   __syncthreads();
-  const int u = threadIdx.x & 7, c = threadIdx.x >> 3, row = blockIdx.y * 8 + u;
-  if (row >= rows || c * 4 >= p.D) return;
-  const float top = s_top[u], inv = s_inv[u];
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < pieces; s0 += 8) {  // eight partial rows in flight
-    float w[8];
-    float4 v[8];
+  if (c * 4 >= p.D) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float l = s0 + e < pieces ? p.partial_lse[slot(s0 + e) * p.slot_rows + row] : -INFINITY;
-      w[e] = l == -INFINITY ? 0.f : __expf(l - top) * inv;
-      v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l != -INFINITY)
-        v[e] = reinterpret_cast<const float4*>(p.partial_o)[(slot(s0 + e) * (p.D / 4) + c) * p.slot_rows + row];
-    }
+  for (int i = 0; i < R; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0;;) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      acc.x = fmaf(w[e], v[e].x, acc.x);
-      acc.y = fmaf(w[e], v[e].y, acc.y);
-      acc.z = fmaf(w[e], v[e].z, acc.z);
-      acc.w = fmaf(w[e], v[e].w, acc.w);
+    for (int i = 0; i < R; ++i) {
+      const float top = s_top[u + i * kJoinRows], inv = s_inv[u + i * kJoinRows];
+#pragma unroll
+      for (int e = 0; e < kFly; ++e) {
+        if (w[i][e] != -INFINITY) {
+          const float f = __expf(w[i][e] - top) * inv;
+          acc[i].x = fmaf(f, v[i][e].x, acc[i].x);
+          acc[i].y = fmaf(f, v[i][e].y, acc[i].y);
+          acc[i].z = fmaf(f, v[i][e].z, acc[i].z);
+          acc[i].w = fmaf(f, v[i][e].w, acc[i].w);
+        }
+      }
     }
+    s0 += kFly;
+    if (s0 >= pieces) break;
+    load(s0);
   }
-  uint2 packed;
-  packed.x = F16 ? pack_f16x2(acc.x, acc.y) : pack_bf16x2(acc.x, acc.y);
-  packed.y = F16 ? pack_f16x2(acc.z, acc.w) : pack_bf16x2(acc.z, acc.w);
-  *reinterpret_cast<uint2*>(p.out + (long long)j.x * p.o_stride_b + (long long)head_of(row) * p.o_stride_h +
-                            (long long)seq_of(row) * p.o_stride_s + c * 8) = packed;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = row0 + u + i * kJoinRows;
+    if (row >= rows) break;
+    uint2 packed;
+    packed.x = F16 ? pack_f16x2(acc[i].x, acc[i].y) : pack_bf16x2(acc[i].x, acc[i].y);
+    packed.y = F16 ? pack_f16x2(acc[i].z, acc[i].w) : pack_bf16x2(acc[i].z, acc[i].w);
+    *reinterpret_cast<uint2*>(p.out + (long long)j.x * p.o_stride_b + (long long)head_of(row) * p.o_stride_h +
+                              (long long)seq_of(row) * p.o_stride_s + c * 8) = packed;
+  }
 }
 
 template <bool F16, int DEAL>
@@ -973,13 +1016,17 @@ static int launch(const WinFwdParams& p, const CUtensorMap& tq, const CUtensorMa
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window forward launch: %s", cudaGetErrorString(e));
   if (DEAL == kStream) {
     // a dependent launch, set up while the forward kernel runs (1.3 us less a call for small ones)
-    config.gridDim = dim3((unsigned)p.ctas, (unsigned)((p.slot_rows + 7) / 8));
+    // (32 query tiles of 128 rows, nine pieces each: equal; 16 with 18 pieces: 28.8 us for the call against 35.1)
+    const bool one_row = p.slot_rows <= kJoinRows || p.ctas > 12LL * p.num_work;
+    const int block_rows = one_row ? kJoinRows : 4 * kJoinRows;
+    config.gridDim = dim3((unsigned)p.ctas, (unsigned)((p.slot_rows + block_rows - 1) / block_rows));
     config.blockDim = dim3(256);
     config.dynamicSmemBytes = 0;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     config.numAttrs = 1;
-    e = cudaLaunchKernelEx(&config, window_join_kernel<F16>, p);
+    e = one_row ? cudaLaunchKernelEx(&config, window_join_kernel<F16, 1>, p)
+                : cudaLaunchKernelEx(&config, window_join_kernel<F16, 4>, p);
     if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window join launch: %s", cudaGetErrorString(e));
   }
   return BSA_OK;
