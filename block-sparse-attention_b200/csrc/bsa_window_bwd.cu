@@ -17,9 +17,16 @@
 // The structure of the two main kernels is the one that measured best for the block-sparse backward: warps 0-7 compute
 // (two groups of 128 threads, thread = tensor-memory lane, group g owns columns [64g, 64g + 64) of the score tiles),
 // warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
-// P and dS are rounded to 16 bits for the tensor cores (all sums are fp32).  What padding holds - NaN included - reaches
+// P and dS are rounded to 16 bits for the tensor cores (all sums are fp32), and delta is that of the 16-bit `out` that the
+// forward call returned: relative to the gradients' own rounding the three give errors of 1.4 to 1.5 times in all for long
+// windows, 1.8 for windows of two keys, where delta nearly cancels dP.  What padding holds - NaN included - reaches
 // no sum: P is replaced by 0 on masked pairs, dP too where a tile reaches behind the end, the statistics of such rows are
-// those of a row that sees nothing, and the rows are zeroed in shared memory where an MMA contracts over them.  With fp16, small gradients need the loss scaling that fp16 training uses anyway.
+// those of a row that sees nothing, and the rows are zeroed in shared memory where an MMA contracts over them.  With fp16,
+// small gradients need the loss scaling that fp16 training uses anyway.
+//
+// Bound by the instructions of the compute warps between two MMAs of a chain, like the block-sparse backward.  Measured: 16
+// heads of 16384 tokens, window 1024, 4 sinks, bf16: 25 + 254 + 356 + 4 us; dQ executes 790, dK/dV 750 TFLOP/s of the
+// visible pairs (6 D and 8 D operations each).
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"
