@@ -62,6 +62,7 @@ struct Params {
   int sink_items;  // further items of tile 0 per (batch, KV head); the workspace holds sink_items + 1 slots
   int sink_m0;     // first query tile beyond the reach of tile 0's windows
   int parts;       // few key tiles: parts that each one's list is cut into (partial [B * Hkv * Nkv][parts][2][128][D]); else 0
+  int dq_group, dkv_group;  // of deal_item
   float scale_log2, softmax_scale;
 };
 
@@ -209,9 +210,10 @@ struct DqItem {
 };
 __device__ __forceinline__ DqItem dq_item(const Params& p, int w) {
   DqItem t;
-  t.m = w % p.Nq;
-  t.h = (w / p.Nq) % p.Hq;
-  t.b = w / (p.Nq * p.Hq);
+  const Dealt d = deal_item(w, p.B * p.Hq, p.Nq, p.dq_group);
+  t.m = p.Nq - 1 - d.rank;  // (the last ones have the longest lists)
+  t.h = d.column % p.Hq;
+  t.b = d.column / p.Hq;
   t.len = seq_len(p, t.b);
   t.base = p.Sk - p.Sq;
   t.p_lo = t.base + t.m * 128;
@@ -584,9 +586,9 @@ __device__ __forceinline__ DkvItem dkv_item(const Params& p, int w) {
     t.nb = 0;
     t.slot = 1 + chunk;
   } else {
-    w -= extras;
-    t.nb = w % p.Nkv;
-    bh = w / p.Nkv;
+    const Dealt d = deal_item(w - extras, p.B * p.Hkv, p.Nkv, p.dkv_group);
+    t.nb = d.rank;  // (the first ones have the longest lists)
+    bh = d.column;
     t.slot = (t.nb == 0 && p.sink_items > 0) ? 0 : -1;
   }
   t.hkv = bh % p.Hkv;
@@ -1190,6 +1192,8 @@ extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
   p.Nkv = (a->Sk + 127) / 128;
   p.D = a->D;
   p.window = a->window < kWindowAll ? a->window : kWindowAll;
+  p.dq_group = head_group((long long)a->B * a->Hq, a->Sk < p.window ? a->Sk : p.window, a->D, a->Hq / a->Hkv);
+  p.dkv_group = head_group((long long)a->B * a->Hkv, (long long)(a->Hq / a->Hkv) * (a->Sq < p.window ? a->Sq : p.window), a->D, 1);
   p.sinks = a->sinks;
   const winbwd::Deal d = winbwd::deal(a->B, a->Hq, a->Hkv, a->Sq, a->Sk, p.window, a->sinks);
   p.parts = d.parts;

@@ -22,7 +22,7 @@
 // its CTA's run itself from the lengths' prefix sums.  (The host's rule has the times of the three.)
 //
 // Bound, where many rows share a key, by the chain QK - softmax - PV of a tile, two of which overlap on an SM; where few
-// do, by the reads of the keys.  Measured: 32 heads (8 of keys) of 32768 tokens, window 2048, 1126 us, 947 TFLOP/s of the
+// do, by the reads of the keys.  Measured: 32 heads (8 of keys) of 32768 tokens, window 2048, 1055 us, 1010 TFLOP/s of the
 // visible pairs; one token of each of 64 sequences, 4096 visible keys, 175 us, 6.1 TB/s; one token of one sequence, 1024
 // visible keys, 11 us; trees of 48 drafts over 8 sequences of up to 16384 tokens, 102 us and the join's 12.
 //
@@ -58,6 +58,7 @@ struct WinFwdParams {
   int max_pages, page_size, num_pages, seg, seg_log2;  // seg = rows of one key box: min(page_size, 128), 128 when contiguous
   int ctas, lists;  // stream
   int team;         // CTAs of a cluster
+  int group;        // of deal_item
   int num_work;     // query tiles
   float scale_log2;
 };
@@ -187,11 +188,10 @@ __device__ __forceinline__ bool next_piece(const WinFwdParams& p, Place* at, int
     return true;
   }
   if (whole >= p.num_work) return false;
-  int r = whole;
-  t.m = r % p.NqT;
-  r /= p.NqT;
-  t.hidx = r % p.Hidx;
-  t.b = r / p.Hidx;
+  const Dealt d = deal_item(whole, p.B * p.Hidx, p.NqT, p.group);
+  t.m = p.NqT - 1 - d.rank;  // (the last ones have the longest lists)
+  t.hidx = d.column % p.Hidx;
+  t.b = d.column / p.Hidx;
   describe(p, t);
   describe_heads(p, t);
   t.it_begin = 0;
@@ -299,11 +299,10 @@ __device__ __forceinline__ void join_team(const WinFwdParams& p, uint32_t base) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   team_sync();
   Item t;
-  int r = (int)blockIdx.x / p.team;
-  t.m = r % p.NqT;
-  r /= p.NqT;
-  t.hidx = r % p.Hidx;
-  t.b = r / p.Hidx;
+  const Dealt d = deal_item((int)blockIdx.x / p.team, p.B * p.Hidx, p.NqT, p.group);
+  t.m = p.NqT - 1 - d.rank;
+  t.hidx = d.column % p.Hidx;
+  t.b = d.column / p.Hidx;
   describe(p, t);
   describe_heads(p, t);
   const int heads = p.packed ? p.G : 1, rows = heads * t.nseq, step = 4 * p.team;
@@ -397,8 +396,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(BAR(kKvEmpty + i), 1);
     }
     mbar_init(BAR(kSFull), 1);
-    mbar_init(BAR(kPHalf), kSoftmaxThreads);
-    mbar_init(BAR(kPFull), kSoftmaxThreads);
+    mbar_init(BAR(kPHalf), kSoftmaxThreads / 32);  // (one arrival a warp: those of its lanes are taken in turn)
+    mbar_init(BAR(kPFull), kSoftmaxThreads / 32);
     mbar_init(BAR(kOFinal), 1);
     mbar_fence_init();
     fence_proxy_async_smem();
@@ -501,7 +500,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     constexpr uint32_t kFmt = F16 ? 0u : 1u;
     const uint32_t idesc_qk = umma_idesc(kFmt, kFmt, 0, 0, 128, 128);
     const uint32_t idesc_pv = umma_idesc(kFmt, kFmt, 0, 1, 128, (uint32_t)p.D);
-    const int qk_steps = p.D / 16;
     const uint32_t led = lane == 0;
     uint32_t ring_pos = 0, q_cnt = 0, p_cnt = 0;
     const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ), 0, 1024);
@@ -526,11 +524,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const uint64_t kd = k_desc0 + (uint64_t)stage * (kTileBytes >> 4);
         // (the columns of whole tiles are a constant: with a computed number every tile's MMAs were issued more slowly)
         const uint32_t idesc = decltype(is_narrow)::value ? umma_idesc(kFmt, kFmt, 0, 0, 128, 32u * groups) : idesc_qk;
+        auto steps = [&](int k0, int k1) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t off = (uint64_t)((k >> 2) * (kSlabBytes >> 4) + (k & 3) * 2);
-          umma_f16_ss_led(tS, q_desc + off, kd + off, idesc, k > 0, (k < qk_steps) ? led : 0u);
-        }
+          for (int k = k0; k < k1; ++k) {
+            const uint64_t off = (uint64_t)((k >> 2) * (kSlabBytes >> 4) + (k & 3) * 2);
+            umma_f16_ss_led(tS, q_desc + off, kd + off, idesc, k > 0, led);
+          }
+        };
+        steps(0, 4);
+        if (p.D > 64) steps(4, 6);  // (an MMA that is predicated off takes as long to issue as one that runs)
+        if (p.D > 96) steps(6, 8);
         umma_commit_led(BAR(kSFull), led);
         umma_commit_led(BAR(kKvEmpty + stage), led);
         if (last) umma_commit_led(BAR(kQEmpty), led);
@@ -583,15 +586,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     uint32_t s_cnt = 0, of_cnt = 0, ring_cnt = 0;
     bool ok = true;
     const int heads = p.packed ? p.G : 1;  // heads of a tile's rows
+    const int row_seq = p.packed ? row / heads : row, row_head = p.packed ? row % heads : 0;
     const int segs = 128 / p.seg;
 
     Item t;
-    while (ok && next_piece<DEAL>(p, place, whole_next, t)) {
+    bool more = next_piece<DEAL>(p, place, whole_next, t);
+    while (ok && more) {
       const int n_it = t.it_end - t.it_begin;
       float m_cur = -INFINITY;  // running max, log2 domain (scale applied)
       float l_sum = 0.f;        // running sum relative to m_cur
-      const int seq = t.seq0 + row / heads;
-      const int hq = t.hkv * p.G + (p.packed ? row % heads : t.g);
+      const int seq = t.seq0 + row_seq;
+      const int hq = t.hkv * p.G + t.g + row_head;
       const bool row_valid = row < heads * t.nseq;
       const bool warp_active = (warp * 32) < heads * t.nseq;  // some row of this warp exists
       // growth of the maximum (2^8) from which on O is rescaled.  Rows that do not exist have no say: behind the last head
@@ -643,8 +648,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (!warp_active) {  // no row of this warp exists: only the barrier protocol
           tc_fence_before();
-          mbar_arrive(BAR(kPHalf));
-          mbar_arrive(BAR(kPFull));
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(BAR(kPHalf));
+            mbar_arrive(BAR(kPFull));
+          }
           continue;
         }
         const uint32_t t_row = tS + lane_base;
@@ -742,7 +750,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (c4 == 2) {  // the first half of P is released on its own barrier, its stores long landed
               tmem_wait_st();
               tc_fence_before();
-              mbar_arrive(BAR(kPHalf));
+              __syncwarp();
+              if (lane == 0) mbar_arrive(BAR(kPHalf));
             }
             tmem_st16(t_row + c4 * 16, pk);
           }
@@ -780,7 +789,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(BAR(kPHalf));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(kPHalf));
         };
         if (whole) tile(std::false_type{});
         else if (narrow && i == n_it - 1) narrow_tile();
@@ -790,10 +800,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         unpack2(s1, y2, y3);
         l_sum += (y0 + y1) + (y2 + y3);
         tc_fence_before();
-        mbar_arrive(BAR(kPFull));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(kPFull));
       }
       if (!ok) break;
       ring_cnt += 2u * (uint32_t)max(n_it, 0);
+
+      Item next;
+      more = next_piece<DEAL>(p, place, whole_next, next);  // (while the last PV runs)
 
       // ------------------------------------ tile epilogue ------------------------------------
       const bool seen = r.live && l_sum != 0.f;  // (NaN, where the inputs hold one, is passed on)
@@ -818,6 +832,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                                          (long long)seq * p.o_stride_s);
       }
       if (warp_active) {
+        // Four lanes hold the same 64 bytes of four rows; they exchange them so that a store covers 64 bytes of eight rows
+        // instead of 16 of 32, each of which takes a cycle of its own.
+        const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_valid) >> (lane & ~3);
+        uint4* dst[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          dst[s] = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst_h), s, 4)) + (lane & 3);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < p.D) {
@@ -832,28 +853,40 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
               for (int e = 0; e < 32; ++e) acc[e] = 0.f;
             }
-            if (row_valid) {
-              if (DEAL == kTeam) {
+            if (DEAL == kTeam) {
+              if (row_valid) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   *reinterpret_cast<float4*>(smem_raw + team_place(row, c * 8 + e, p.D)) =
                       make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
-              } else if (piece) {
+              }
+            } else if (piece) {
+              if (row_valid) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   dst_f[(long long)(c * 8 + e) * p.slot_rows] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
-              } else {
+              }
+            } else {
+              uint32_t u[4][4];
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                  uint32_t u[4];
+              for (int e = 0; e < 16; ++e)
+                u[e >> 2][e & 3] = F16 ? pack_f16x2(acc[2 * e], acc[2 * e + 1]) : pack_bf16x2(acc[2 * e], acc[2 * e + 1]);
+#pragma unroll
+              for (int bit = 1; bit < 4; bit <<= 1) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                  if (s & bit) continue;
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
-                    const float a = acc[ch * 8 + 2 * e], b = acc[ch * 8 + 2 * e + 1];
-                    u[e] = F16 ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & bit) ? u[s][e] : u[s | bit][e], bit);
+                    if (lane & bit) u[s][e] = got;
+                    else u[s | bit][e] = got;
                   }
-                  dst_h[c * 4 + ch] = make_uint4(u[0], u[1], u[2], u[3]);
                 }
               }
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                if ((rows_ok >> s) & 1u) dst[s][c * 4] = make_uint4(u[s][0], u[s][1], u[s][2], u[s][3]);
             }
           }
           __syncwarp();
@@ -865,6 +898,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         else if (piece) p.partial_lse[prow] = lse;
         else if (p.lse != nullptr) p.lse[((long long)t.b * p.Hq + hq) * p.Sq + seq] = lse;
       }
+      t = next;
     }
     if (DEAL == kTeam) join_team<F16>(p, smem_u32(smem_raw));
   } else {
@@ -1131,6 +1165,7 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   if (work > 0x7f000000LL)  // (a grid's width is added to an item's index)
     return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 work items");
   p.num_work = (int)work;
+  p.group = head_group((long long)p.B * p.Hidx, Sk < p.window ? Sk : p.window, p.D, packed ? 1 : G);
   if (p.team > 1 && work * p.team > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: more than 65535 CTAs in teams");
   if (p.ctas > 0 && p.lists > 1 && p.lists != p.NqT)
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_lists must be 1 or the number of query tiles per head (%d)", p.NqT);
