@@ -83,6 +83,35 @@ inline int head_group(long long columns, long long span, int D, int share) {
   return (int)(g < columns ? g : columns);
 }
 
+// Stores 64 bytes of each thread's row, u[chunk][word], at `dst` = (lane's chunk in the rows of its group of four lanes):
+// four lanes exchange their chunks, so that a store covers 64 bytes of eight rows instead of 16 of 32, each of which takes
+// a cycle of its own.  `rows_ok` = bits of the group's rows that exist.  Called by whole warps.
+__device__ __forceinline__ void store_exchanged(uint4* const* dst, int at, uint32_t (*u)[4], uint32_t rows_ok) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int bit = 1; bit < 4; bit <<= 1) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (s & bit) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & bit) ? u[s][e] : u[s | bit][e], bit);
+        if (lane & bit) u[s][e] = got;
+        else u[s | bit][e] = got;
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    if ((rows_ok >> s) & 1u) dst[s][at] = make_uint4(u[s][0], u[s][1], u[s][2], u[s][3]);
+}
+// The addresses for it: those of the group's rows, at the lane's chunk.
+__device__ __forceinline__ void exchange_rows(void* row, uint4** dst) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    dst[s] = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), s, 4)) + (threadIdx.x & 3);
+}
+
 // Equal runs of a list: CTA c of the n that have work gets all / n entries, and one of the all % n that are left over.
 struct Runs {
   int q, r;

@@ -92,15 +92,19 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint
 
 // Up to 64 fp32 accumulator columns of a row -> 16 bits, scaled -> global.
 template <bool F16>
-__device__ __forceinline__ void store_half(uint8_t* dst, const uint32_t* acc, float scale, int cols) {
+__device__ __forceinline__ void store_half(uint8_t* row, bool valid, const uint32_t* acc, float scale, int cols) {
+  const uint32_t all_ok = __ballot_sync(0xffffffffu, valid);
+  if (all_ok == 0) return;
+  uint4* dst[4];
+  exchange_rows(row, dst);
 #pragma unroll
-  for (int ch = 0; ch < 8; ++ch) {
-    if (ch * 8 < cols) {
-      uint32_t u[4];
+  for (int h = 0; h < 2; ++h) {
+    if (h * 32 < cols) {
+      uint32_t u[4][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        u[e] = pack16<F16>(__uint_as_float(acc[ch * 8 + 2 * e]) * scale, __uint_as_float(acc[ch * 8 + 2 * e + 1]) * scale);
-      reinterpret_cast<uint4*>(dst)[ch] = make_uint4(u[0], u[1], u[2], u[3]);
+      for (int e = 0; e < 16; ++e)
+        u[e >> 2][e & 3] = pack16<F16>(__uint_as_float(acc[h * 32 + 2 * e]) * scale, __uint_as_float(acc[h * 32 + 2 * e + 1]) * scale);
+      store_exchanged(dst, h * 4, u, all_ok >> (threadIdx.x & 28));
     }
   }
 }
@@ -123,11 +127,16 @@ constexpr uint64_t kTileStep = kTile >> 4;
 // D = A(smem, K-major) * B(smem, K-major)^T, contracting over the head dimension in `ksteps` = D / 16 steps.
 template <bool F16>
 __device__ __forceinline__ void mma_ss_kk(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t led, int ksteps) {
+  auto steps = [&](int k0, int k1) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint64_t off = (uint64_t)((k >> 2) * (kSlab >> 4) + (k & 3) * 2);
-    umma_f16_ss_led(d, a_desc + off, b_desc + off, Idesc<F16>::kKK, k > 0 ? 1u : 0u, (k < ksteps) ? led : 0u);
-  }
+    for (int k = k0; k < k1; ++k) {
+      const uint64_t off = (uint64_t)((k >> 2) * (kSlab >> 4) + (k & 3) * 2);
+      umma_f16_ss_led(d, a_desc + off, b_desc + off, Idesc<F16>::kKK, k > 0 ? 1u : 0u, led);
+    }
+  };
+  steps(0, 4);
+  if (ksteps > 4) steps(4, 6);  // (an MMA that is predicated off takes as long to issue as one that runs)
+  if (ksteps > 6) steps(6, 8);
 }
 // D (+)= A(tmem, 16 bits, two 32-column halves) * B(smem, MN-major), contracting over 128 tokens.
 __device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint64_t b_desc, bool acc, uint32_t led, uint32_t idesc) {
@@ -259,14 +268,14 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     mbar_init(BAR(kDoFull), 1);
     mbar_init(BAR(kDoEmpty), 1);
     mbar_init(BAR(kSFull), 1);
-    mbar_init(BAR(kSFree), 256);
+    mbar_init(BAR(kSFree), 8);  // (one arrival a warp: those of its lanes are taken in turn)
     for (int i = 0; i < 2; ++i) {
       mbar_init(BAR(kDpFull + i), 1);
-      mbar_init(BAR(kDsFull + i), 256);
+      mbar_init(BAR(kDsFull + i), 8);
       mbar_init(BAR(kDsUsed + i), 1);
     }
     mbar_init(BAR(kDqFinal), 1);
-    mbar_init(BAR(kDqFree), 256);
+    mbar_init(BAR(kDqFree), 8);
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -453,7 +462,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
               tmem_wait_ld();
             }
             tc_fence_before();
-            mbar_arrive(BAR(kSFree));  // S_j is in registers: the next S may be computed
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(kSFree));  // S_j is in registers: the next S may be computed
             const bool tail = kMasked && j0 + 128 > t.len;
             if (tail) {  // K rows behind the end may hold anything, and dQ contracts over them (S_j has read the tile)
               if (j0 + row >= t.len) {
@@ -505,7 +515,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           ++dp_cnt;
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(BAR(kDsFull + buf));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(kDsFull + buf));
         }
         if (!ok) break;
         r_cnt += 2 * n;
@@ -517,13 +528,14 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_ld32(tdQ + lane_base + grp * 64 + 32, acc + 32);
         tmem_wait_ld();
         tc_fence_before();
-        mbar_arrive(BAR(kDqFree));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(kDqFree));
       }
       if (n == 0 || !live) {  // takes no part
 #pragma unroll
         for (int c = 0; c < 64; ++c) acc[c] = 0u;
       }
-      if (seq < p.Sq) store_half<F16>(dq_row, acc, p.softmax_scale, cols);
+      store_half<F16>(dq_row, seq < p.Sq, acc, p.softmax_scale, cols);
     }
   }
   tc_fence_before();
@@ -657,12 +669,12 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     mbar_init(BAR(kSFull), 1);
     mbar_init(BAR(kDpFull), 1);
-    mbar_init(BAR(kSFree), 256);
-    mbar_init(BAR(kPFull), 256);
-    mbar_init(BAR(kDsFull), 256);
+    mbar_init(BAR(kSFree), 8);
+    mbar_init(BAR(kPFull), 8);
+    mbar_init(BAR(kDsFull), 8);
     mbar_init(BAR(kGFree), 1);
     mbar_init(BAR(kFinal), 2);
-    mbar_init(BAR(kFree), 256);
+    mbar_init(BAR(kFree), 8);
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -856,7 +868,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             tmem_wait_ld();
           }
           tc_fence_before();
-          mbar_arrive(BAR(kSFree));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(kSFree));
 #pragma unroll
           for (int c4 = 0; c4 < 16; ++c4) {
             const float4 l = st_l[c4];  // negated
@@ -914,7 +927,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(BAR(kPFull));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(kPFull));
           uint32_t pk[32];
 #pragma unroll
           for (int c4 = 0; c4 < 16; ++c4) {
@@ -937,7 +951,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!ok) break;
         ++dp_cnt;
         tc_fence_before();
-        mbar_arrive(BAR(kDsFull));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(kDsFull));
       }
       if (!ok) break;
       // ---- epilogue
@@ -965,7 +980,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
         for (int c = 0; c < 64; ++c) acc[c] = 0u;
       }
-      if (to_row) store_half<F16>(dv_row, acc, 1.0f, cols);
+      store_half<F16>(dv_row, to_row, acc, 1.0f, cols);
       if (to_slot) store_half_f32(part + (long long)slot_rows * p.D, acc, cols);
       if (t.T > 0) {
         __syncwarp();
@@ -973,9 +988,10 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tmem_ld32(tdK + lane_base + grp * 64 + 32, acc + 32);
         tmem_wait_ld();
         tc_fence_before();
-        mbar_arrive(BAR(kFree));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR(kFree));
       }
-      if (to_row) store_half<F16>(dk_row, acc, p.softmax_scale, cols);
+      store_half<F16>(dk_row, to_row, acc, p.softmax_scale, cols);
       if (to_slot) store_half_f32(part, acc, cols);
       __syncwarp();
     }

@@ -832,13 +832,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                                          (long long)seq * p.o_stride_s);
       }
       if (warp_active) {
-        // Four lanes hold the same 64 bytes of four rows; they exchange them so that a store covers 64 bytes of eight rows
-        // instead of 16 of 32, each of which takes a cycle of its own.
         const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_valid) >> (lane & ~3);
         uint4* dst[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          dst[s] = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst_h), s, 4)) + (lane & 3);
+        exchange_rows(dst_h, dst);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           if (c * 32 < p.D) {
@@ -871,22 +867,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 u[e >> 2][e & 3] = F16 ? pack_f16x2(acc[2 * e], acc[2 * e + 1]) : pack_bf16x2(acc[2 * e], acc[2 * e + 1]);
-#pragma unroll
-              for (int bit = 1; bit < 4; bit <<= 1) {
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                  if (s & bit) continue;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const uint32_t got = __shfl_xor_sync(0xffffffffu, (lane & bit) ? u[s][e] : u[s | bit][e], bit);
-                    if (lane & bit) u[s][e] = got;
-                    else u[s | bit][e] = got;
-                  }
-                }
-              }
-#pragma unroll
-              for (int s = 0; s < 4; ++s)
-                if ((rows_ok >> s) & 1u) dst[s][c * 4] = make_uint4(u[s][0], u[s][1], u[s][2], u[s][3]);
+              store_exchanged(dst, c * 4, u, rows_ok);
             }
           }
           __syncwarp();
