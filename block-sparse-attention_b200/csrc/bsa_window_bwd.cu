@@ -25,7 +25,7 @@
 // small gradients need the loss scaling that fp16 training uses anyway.
 //
 // Bound by the instructions of the compute warps between two MMAs of a chain, like the block-sparse backward.  Measured: 16
-// heads of 16384 tokens, window 1024, 4 sinks, bf16: 25 + 254 + 356 + 4 us; dQ executes 790, dK/dV 750 TFLOP/s of the
+// heads of 16384 tokens, window 1024, 4 sinks, bf16: 24 + 225 + 355 + 4 us; dQ executes 890, dK/dV 750 TFLOP/s of the
 // visible pairs (6 D and 8 D operations each).
 #include "bsa_b200.h"
 #include "bsa_common.cuh"

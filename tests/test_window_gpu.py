@@ -317,3 +317,16 @@ DEALS = [(0, 1), (0, 2), (0, 5), (0, 8), (1, 1), (7, 1), (296, 1)]
 def test_every_way_of_dealing_the_work(deal):
     for case in CASES:
         test_forward(case, "bshd")
+
+
+GROUPED = [
+    (1, 14, 14, 256, 9000, 128, BF, 1 << 20, 2, None),   # ten heads' keys fill the group of the forward and dQ kernels
+    (15, 11, 1, 600, 600, 128, BF, 1 << 20, 0, None),    # fourteen heads' queries that of the dK/dV kernel
+]
+
+
+@pytest.mark.parametrize("deal", [(0, 1)], indirect=True, ids=str)
+@pytest.mark.parametrize("case", GROUPED, ids=["keys", "queries"])
+def test_more_heads_than_are_dealt_at_a_time(deal, case):
+    test_forward(case, "bhsd")
+    test_backward(case)
