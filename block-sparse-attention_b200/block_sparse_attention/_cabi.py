@@ -192,6 +192,15 @@ class WindowBwdArgs(ctypes.Structure):
     ]
 
 
+class CacheArgs(ctypes.Structure):
+    """Mirror of ``struct bsa_cache_args``."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_cache", "v_cache", "page_table", "lens", "path", "path_lens",
+                                                "new_lens")]
+                + [(n, _c_i64x3) for n in ("k_stride", "v_stride", "kc_stride", "vc_stride")]
+                + [(n, ctypes.c_int32) for n in ("B", "H", "T", "D", "max_pages", "page_size", "num_pages", "path_cap")])
+
+
 class RotaryArgs(ctypes.Structure):
     """Mirror of ``struct bsa_rotary_args``."""
 
@@ -224,7 +233,6 @@ class RotaryArgs(ctypes.Structure):
 # name -> (restype, argtypes); every symbol include/bsa_b200.h declares
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
-_pi64 = ctypes.POINTER(ctypes.c_int64)
 SIGNATURES = {
     "bsa_abi_version": (ctypes.c_int, []),
     "bsa_last_error": (ctypes.c_char_p, []),
@@ -250,8 +258,8 @@ SIGNATURES = {
     "bsa_window_bwd": (ctypes.c_int, [ctypes.POINTER(WindowBwdArgs), _vp]),
     "bsa_window_bwd_workspace_bytes": (ctypes.c_int64, [_i32] * 8),
     "bsa_tree_mask": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp]),
-    "bsa_cache_append": (ctypes.c_int, [_vp] * 4 + [_pi64] * 4 + [_vp] * 2 + [_i32] * 7 + [_vp]),
-    "bsa_cache_keep": (ctypes.c_int, [_vp] * 2 + [_pi64] * 2 + [_vp] * 5 + [_i32] * 8 + [_vp]),
+    "bsa_cache_append": (ctypes.c_int, [ctypes.POINTER(CacheArgs), _vp]),
+    "bsa_cache_keep": (ctypes.c_int, [ctypes.POINTER(CacheArgs), _vp]),
     "bsa_rotary_nd": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), _vp]),
 }
 

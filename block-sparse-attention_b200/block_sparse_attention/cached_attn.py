@@ -21,8 +21,6 @@ from .bsa_attn_interface import _ceil_div
 from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_lens, _check_qkv, _check_scale, _check_window, _copied, _dense, _fits,
                           _make_plan, _meta, _run_plan)
 
-_c_i64x3 = _cabi._c_i64x3
-
 __all__ = ["cached_attn_fwd", "tree_mask_from_parents", "cache_append", "cache_keep"]
 
 MAX_TREE_TOKENS = 64
@@ -147,8 +145,7 @@ class _WritePlan(NamedTuple):
 
     direct: bool
     empty: bool
-    strides: tuple = ()
-    sizes: tuple = ()
+    args: bytes = b""  # CacheArgs without addresses
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -166,8 +163,9 @@ def _append_plan(k, v, k_cache, v_cache, table, lens, layout) -> _WritePlan:
     rows_ok = all(t[1][3] == 1 and (t[1][0] | t[1][1] | t[1][2]) % 8 == 0 for t in (k, v))
     if not (rows_ok and _dense(table) and _dense(lens)):
         return _WritePlan(False, False)
-    return _WritePlan(True, False, (_c_i64x3(*_bhsd(k[1], layout)), _c_i64x3(*_bhsd(v[1], layout)), _c_i64x3(*k_cache[1][:3]),
-                                    _c_i64x3(*v_cache[1][:3])), (B, H, T, D, table[0][1], page_size, num_pages))
+    return _WritePlan(True, False, bytes(_cabi.CacheArgs(
+        *[None] * 9, _bhsd(k[1], layout), _bhsd(v[1], layout), k_cache[1][:3], v_cache[1][:3], B, H, T, D, table[0][1], page_size,
+        num_pages, 0)))
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -186,8 +184,9 @@ def _keep_plan(k_cache, v_cache, table, lens, path, path_lens, num_drafts) -> _W
         return _WritePlan(True, True)
     if path[0][1] == 0 or table[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
         return _WritePlan(False, False)
-    return _WritePlan(True, False, (_c_i64x3(*k_cache[1][:3]), _c_i64x3(*v_cache[1][:3])),
-                      (B, H, num_drafts, path[0][1], D, table[0][1], page_size, num_pages))
+    return _WritePlan(True, False, bytes(_cabi.CacheArgs(
+        *[None] * 9, (0, 0, 0), (0, 0, 0), k_cache[1][:3], v_cache[1][:3], B, H, num_drafts, D, table[0][1], page_size, num_pages,
+        path[0][1])))
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -207,8 +206,11 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     if not plan.direct or (at[0] | at[1]) % 16 != 0:
         k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         return cache_append(k, v, k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), layout=layout)
-    _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, *at, k_cache.data_ptr(), v_cache.data_ptr(),
-                 *plan.strides, page_table.data_ptr(), cache_lens.data_ptr(), *plan.sizes)
+    a = _cabi.CacheArgs.from_buffer_copy(plan.args)
+    a.k, a.v = at
+    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    a.page_table, a.lens = page_table.data_ptr(), cache_lens.data_ptr()
+    _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, a)
     return k_cache, v_cache
 
 
@@ -234,7 +236,9 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
         return cache_keep(k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), path.contiguous(),
                           path_lens.contiguous(), num_drafts)
     new_lens = torch.empty_like(cache_lens)
-    _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", k_cache.device, k_cache.data_ptr(), v_cache.data_ptr(),
-                 *plan.strides, page_table.data_ptr(), cache_lens.data_ptr(), path.data_ptr(), path_lens.data_ptr(),
-                 new_lens.data_ptr(), *plan.sizes)
+    a = _cabi.CacheArgs.from_buffer_copy(plan.args)
+    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    a.page_table, a.lens = page_table.data_ptr(), cache_lens.data_ptr()
+    a.path, a.path_lens, a.new_lens = path.data_ptr(), path_lens.data_ptr(), new_lens.data_ptr()
+    _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", k_cache.device, a)
     return new_lens

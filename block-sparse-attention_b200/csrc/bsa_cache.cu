@@ -142,32 +142,33 @@ tree_mask_kernel(const int32_t* __restrict__ parents, long long* __restrict__ ma
   mask[row + t] = (long long)m;
 }
 
-static int check_pages(const char* what, const void* kc, const void* vc, const int64_t* ks, const int64_t* vs,
-                       const int32_t* table, const int32_t* lens, int B, int H, int T, int D, int max_pages,
-                       int page_size, int num_pages) {
-  if (!kc || !vc || !ks || !vs || !table || !lens) return set_error(BSA_ERR_INVALID, "%s: null pointer", what);
-  if (B < 1 || H < 1 || T < 1 || max_pages < 1 || page_size < 1 || num_pages < 1)
+static int check_pages(const char* what, const bsa_cache_args* a) {
+  if (!a) return set_error(BSA_ERR_INVALID, "%s: null args", what);
+  if (!a->k_cache || !a->v_cache || !a->page_table || !a->lens) return set_error(BSA_ERR_INVALID, "%s: null pointer", what);
+  if (a->B < 1 || a->H < 1 || a->T < 1 || a->max_pages < 1 || a->page_size < 1 || a->num_pages < 1)
     return set_error(BSA_ERR_INVALID, "%s: non-positive extent", what);
-  if (D < 8 || D % 8 != 0) return set_error(BSA_ERR_INVALID, "%s: D must be a multiple of 8", what);
-  if ((long long)max_pages * page_size > (1 << 29)) return set_error(BSA_ERR_UNSUPPORTED, "%s: more than 2^29 tokens per sequence", what);
-  if (((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & 15u) != 0)
+  if (a->D < 8 || a->D % 8 != 0) return set_error(BSA_ERR_INVALID, "%s: D must be a multiple of 8", what);
+  if ((long long)a->max_pages * a->page_size > (1 << 29))
+    return set_error(BSA_ERR_UNSUPPORTED, "%s: more than 2^29 tokens per sequence", what);
+  if (a->k_cache == a->v_cache) return set_error(BSA_ERR_INVALID, "%s: keys and values share a pool", what);
+  if (((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15u) != 0)
     return set_error(BSA_ERR_INVALID, "%s: the caches must be 16-byte aligned", what);
   for (int i = 0; i < 3; ++i)
-    if ((ks[i] | vs[i]) % 8 != 0) return set_error(BSA_ERR_INVALID, "%s: cache strides must be multiples of 8 elements", what);
+    if ((a->kc_stride[i] | a->vc_stride[i]) % 8 != 0)
+      return set_error(BSA_ERR_INVALID, "%s: cache strides must be multiples of 8 elements", what);
   return BSA_OK;
 }
 
-static Pages make_pages(void* kc, void* vc, const int64_t* ks, const int64_t* vs, const int32_t* table, int max_pages,
-                        int page_size, int num_pages) {
+static Pages make_pages(const bsa_cache_args* a) {
   Pages pg{};
-  pg.k = static_cast<uint8_t*>(kc);
-  pg.v = static_cast<uint8_t*>(vc);
-  pg.k_page = ks[0] * 2; pg.k_head = ks[1] * 2; pg.k_row = ks[2] * 2;
-  pg.v_page = vs[0] * 2; pg.v_head = vs[1] * 2; pg.v_row = vs[2] * 2;
-  pg.table = table;
-  pg.max_pages = max_pages;
-  pg.page_size = page_size;
-  pg.num_pages = num_pages;
+  pg.k = static_cast<uint8_t*>(a->k_cache);
+  pg.v = static_cast<uint8_t*>(a->v_cache);
+  pg.k_page = a->kc_stride[0] * 2; pg.k_head = a->kc_stride[1] * 2; pg.k_row = a->kc_stride[2] * 2;
+  pg.v_page = a->vc_stride[0] * 2; pg.v_head = a->vc_stride[1] * 2; pg.v_row = a->vc_stride[2] * 2;
+  pg.table = a->page_table;
+  pg.max_pages = a->max_pages;
+  pg.page_size = a->page_size;
+  pg.num_pages = a->num_pages;
   return pg;
 }
 
@@ -186,53 +187,42 @@ extern "C" int bsa_tree_mask(const int32_t* parents, int32_t B, int32_t T, int64
   return BSA_OK;
 }
 
-extern "C" int bsa_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int64_t k_stride[3],
-                                const int64_t v_stride[3], const int64_t kc_stride[3], const int64_t vc_stride[3],
-                                const int32_t* page_table, const int32_t* lens, int32_t B, int32_t H, int32_t T,
-                                int32_t D, int32_t max_pages, int32_t page_size, int32_t num_pages, void* cuda_stream) {
-  int rc = cache::check_pages("bsa_cache_append", k_cache, v_cache, kc_stride, vc_stride, page_table, lens, B, H, T, D,
-                              max_pages, page_size, num_pages);
+extern "C" int bsa_cache_append(const bsa_cache_args* a, void* cuda_stream) {
+  int rc = cache::check_pages("bsa_cache_append", a);
   if (rc) return rc;
-  if (!k || !v || !k_stride || !v_stride) return set_error(BSA_ERR_INVALID, "bsa_cache_append: null pointer");
-  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) != 0)
+  if (!a->k || !a->v) return set_error(BSA_ERR_INVALID, "bsa_cache_append: null pointer");
+  if (((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15u) != 0)
     return set_error(BSA_ERR_INVALID, "bsa_cache_append: k and v must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
-    if ((k_stride[i] | v_stride[i]) % 8 != 0)
+    if ((a->k_stride[i] | a->v_stride[i]) % 8 != 0)
       return set_error(BSA_ERR_INVALID, "bsa_cache_append: strides must be multiples of 8 elements");
   cache::Source s{};
-  s.k = static_cast<const uint8_t*>(k);
-  s.v = static_cast<const uint8_t*>(v);
-  s.k_b = k_stride[0] * 2; s.k_h = k_stride[1] * 2; s.k_t = k_stride[2] * 2;
-  s.v_b = v_stride[0] * 2; s.v_h = v_stride[1] * 2; s.v_t = v_stride[2] * 2;
-  const int chunks = D / 8;
-  const long long units = (long long)B * H * ((T + cache::kRows - 1) / cache::kRows) * chunks;
+  s.k = static_cast<const uint8_t*>(a->k);
+  s.v = static_cast<const uint8_t*>(a->v);
+  s.k_b = a->k_stride[0] * 2; s.k_h = a->k_stride[1] * 2; s.k_t = a->k_stride[2] * 2;
+  s.v_b = a->v_stride[0] * 2; s.v_h = a->v_stride[1] * 2; s.v_t = a->v_stride[2] * 2;
+  const int chunks = a->D / 8;
+  const long long units = (long long)a->B * a->H * ((a->T + cache::kRows - 1) / cache::kRows) * chunks;
   const long long blocks = (units + 255) / 256;
   if (blocks > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_cache_append: too many tokens");
   cache::cache_append_kernel<<<(unsigned)blocks, 256, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
-      s, cache::make_pages(k_cache, v_cache, kc_stride, vc_stride, page_table, max_pages, page_size, num_pages), lens,
-      B, H, T, chunks, units);
+      s, cache::make_pages(a), a->lens, a->B, a->H, a->T, chunks, units);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cache append launch: %s", cudaGetErrorString(e));
   return BSA_OK;
 }
 
-extern "C" int bsa_cache_keep(void* k_cache, void* v_cache, const int64_t kc_stride[3], const int64_t vc_stride[3],
-                              const int32_t* page_table, const int32_t* lens, const int32_t* path,
-                              const int32_t* path_lens, int32_t* new_lens, int32_t B, int32_t H, int32_t T,
-                              int32_t path_cap, int32_t D, int32_t max_pages, int32_t page_size, int32_t num_pages,
-                              void* cuda_stream) {
-  int rc = cache::check_pages("bsa_cache_keep", k_cache, v_cache, kc_stride, vc_stride, page_table, lens, B, H, T, D,
-                              max_pages, page_size, num_pages);
+extern "C" int bsa_cache_keep(const bsa_cache_args* a, void* cuda_stream) {
+  int rc = cache::check_pages("bsa_cache_keep", a);
   if (rc) return rc;
-  if (!path || !path_lens || !new_lens) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: null pointer");
-  if (path_cap < 1) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: non-positive extent");
-  const int chunks = D / 8;
-  const long long units = (long long)B * H * chunks;
+  if (!a->path || !a->path_lens || !a->new_lens) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: null pointer");
+  if (a->path_cap < 1) return set_error(BSA_ERR_INVALID, "bsa_cache_keep: non-positive extent");
+  const int chunks = a->D / 8;
+  const long long units = (long long)a->B * a->H * chunks;
   const long long blocks = (units + 127) / 128;
   if (blocks > 0x7fffffffLL) return set_error(BSA_ERR_UNSUPPORTED, "bsa_cache_keep: too many heads");
   cache::cache_keep_kernel<<<(unsigned)blocks, 128, 0, reinterpret_cast<cudaStream_t>(cuda_stream)>>>(
-      cache::make_pages(k_cache, v_cache, kc_stride, vc_stride, page_table, max_pages, page_size, num_pages), lens, path,
-      path_lens, new_lens, B, H, T, path_cap, chunks, units);
+      cache::make_pages(a), a->lens, a->path, a->path_lens, a->new_lens, a->B, a->H, a->T, a->path_cap, chunks, units);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "cache keep launch: %s", cudaGetErrorString(e));
   return BSA_OK;

@@ -404,14 +404,31 @@ int bsa_tree_mask(const int32_t* parents, int32_t B, int32_t T, int64_t* mask, v
  *                     [0, T).  A sequence with lens[b] < T keeps its length and is not touched.
  * A page must not be written through two sequences' tables in one call.
  */
-int bsa_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int64_t k_stride[3],
-                     const int64_t v_stride[3], const int64_t kc_stride[3], const int64_t vc_stride[3],
-                     const int32_t* page_table, const int32_t* lens, int32_t B, int32_t H, int32_t T, int32_t D,
-                     int32_t max_pages, int32_t page_size, int32_t num_pages, void* cuda_stream);
-int bsa_cache_keep(void* k_cache, void* v_cache, const int64_t kc_stride[3], const int64_t vc_stride[3],
-                   const int32_t* page_table, const int32_t* lens, const int32_t* path, const int32_t* path_lens,
-                   int32_t* new_lens, int32_t B, int32_t H, int32_t T, int32_t path_cap, int32_t D, int32_t max_pages,
-                   int32_t page_size, int32_t num_pages, void* cuda_stream);
+typedef struct bsa_cache_args {
+  const void* k;            /* append */
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* page_table; /* [B, max_pages] */
+  const int32_t* lens;       /* [B] */
+  const int32_t* path;       /* keep: [B, path_cap] */
+  const int32_t* path_lens;  /* [B] */
+  int32_t* new_lens;         /* [B] */
+  int64_t k_stride[3];       /* batch, head, token */
+  int64_t v_stride[3];
+  int64_t kc_stride[3];      /* page, head, row */
+  int64_t vc_stride[3];
+  int32_t B;
+  int32_t H;
+  int32_t T;
+  int32_t D;
+  int32_t max_pages;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t path_cap;
+} bsa_cache_args;
+int bsa_cache_append(const bsa_cache_args* args, void* cuda_stream);
+int bsa_cache_keep(const bsa_cache_args* args, void* cuda_stream);
 
 /*
  * Rotary positions with several axes.  Pair p of a head (p < P = axis_pairs[0] + ... + axis_pairs[A-1]) turns by

@@ -152,9 +152,22 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.bsa_rotary_nd(r, None) < 0
     st = (ctypes.c_int64 * 3)(1024, 512, 64)
     assert lib.bsa_tree_mask(1 << 20, 1, 65, 1 << 20, None) < 0
-    assert lib.bsa_cache_append(1 << 20, 1 << 20, (1 << 20) + 2, 1 << 20, st, st, st, st, 1 << 20, 1 << 20, 1, 1, 1, 64, 1, 16, 1, None) < 0
-    assert lib.bsa_cache_append(1 << 20, 1 << 20, 1 << 20, 1 << 20, st, st, st, st, 1 << 20, 1 << 20, 1, 1, 1, 63, 1, 16, 1, None) < 0
-    assert lib.bsa_cache_keep(1 << 20, 1 << 20, st, st, 1 << 20, 1 << 20, None, 1 << 20, 1 << 20, 1, 1, 1, 1, 64, 1, 16, 1, None) < 0
+
+    def cache(entry, **kw):
+        a = _cabi.CacheArgs(*[1 << 20] * 9, st, st, st, st, 1, 1, 1, 64, 1, 16, 1, 1)
+        a.v_cache = 1 << 21
+        for n, v in kw.items():
+            setattr(a, n, v)
+        return entry(a, None)
+
+    for kw in (dict(k_cache=(1 << 20) + 2), dict(k_cache=None), dict(lens=None), dict(page_table=None), dict(v_cache=1 << 20), dict(D=63),
+               dict(D=0), dict(B=0), dict(T=0), dict(num_pages=0), dict(page_size=1 << 15, max_pages=1 << 15),
+               dict(kc_stride=(ctypes.c_int64 * 3)(1024, 512, 60))):
+        assert cache(lib.bsa_cache_append, **kw) < 0 and cache(lib.bsa_cache_keep, **kw) < 0, kw
+    for kw in (dict(k=None), dict(v=(1 << 20) + 8), dict(k_stride=(ctypes.c_int64 * 3)(1024, 512, 60))):
+        assert cache(lib.bsa_cache_append, **kw) < 0, kw
+    for kw in (dict(path=None), dict(path_lens=None), dict(new_lens=None), dict(path_cap=0)):
+        assert cache(lib.bsa_cache_keep, **kw) < 0, kw
 
 
 def test_rule_of_dealing_the_work():
