@@ -402,5 +402,8 @@ class WindowAttentionFunction(torch.autograd.Function):
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sink_tokens: int = 0,
                      kv_lens: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
                      layout: str = "bhsd") -> torch.Tensor:
-    """Differentiable sliding-window attention with sinks (see ``window_attn_fwd`` for the arguments)."""
+    """Differentiable sliding-window attention with sinks (see ``window_attn_fwd`` for the arguments).
+
+    Once differentiable.  To capture a training step in a CUDA graph, warm it up on a side stream and drop every eager
+    graph of the same leaves first, as PyTorch asks for any captured backward pass."""
     return WindowAttentionFunction.apply(q, k, v, window, sink_tokens, kv_lens, softmax_scale, layout)

@@ -307,8 +307,8 @@ int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, in
  * stream_ctas = 0: whole query tiles are dealt to the CTAs in turn.  stream_ctas > 0: the list of all key tiles of all
  * query tiles is cut into that many equal runs, for few query tiles or unequal lengths (stream_lists = the number of
  * query tiles per head: one list for each of them instead, stream_ctas / stream_lists runs each, worked on side by side
- * so that they share their reads of the keys); partial_o [2 * stream_ctas, R,
- * D] and partial_lse [2 * stream_ctas, R] f32 (R = rows of a query tile: min(Sq, 128), packed G * min(Sq,
+ * so that they share their reads of the keys); partial_o [2 * stream_ctas, D / 4,
+ * R, 4] and partial_lse [2 * stream_ctas, R] f32 (R = rows of a query tile: min(Sq, 128), packed G * min(Sq,
  * floor(128 / G))) hold the pieces of cut query tiles, joins [4 * stream_ctas] int32 their list; a second launch of the
  * same call joins them.  team = 2..8 (with stream_ctas = 0): a cluster of that many CTAs works on each query tile and
  * joins its results itself, for few query tiles with short lists.

@@ -330,3 +330,41 @@ GROUPED = [
 def test_more_heads_than_are_dealt_at_a_time(deal, case):
     test_forward(case, "bhsd")
     test_backward(case)
+
+
+def test_captured_training_step():
+    """Rotation and attention with their gradients in one captured step, replayed on new inputs, against direct calls."""
+    from block_sparse_attention import (rotary_embedding, rotary_frequencies, rotary_nd, window_attention, window_attn_bwd,
+                                        window_attn_fwd)
+    pairs = (8, 12, 12)
+    sets = [[t.cuda() for t in make(2, 6, 2, 333, 333, 64, BF, seed=s)] for s in range(2)]
+    q, k, v = (t.clone().requires_grad_() for t in sets[0][:3])
+    do = sets[0][3].clone()
+    pos = torch.randint(0, 500, (333, 3), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    freq = rotary_frequencies(pairs, device="cuda")
+
+    def step():
+        a, b = rotary_embedding(q, k, pos, freq, pairs)
+        window_attention(a, b, v, 90, 3).backward(do)
+
+    side = torch.cuda.Stream()  # (warmed up there, and the eager graphs dropped, as captures of a backward pass need it)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+            q.grad = k.grad = v.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for new in sets[::-1]:
+        with torch.no_grad():
+            for held, t in zip((q, k, v, do), new):
+                held.copy_(t)
+        graph.replay()
+        a, b = rotary_nd(new[0], new[1], pos, freq, pairs)
+        out, lse = window_attn_fwd(a, b, new[2], 90, 3, return_lse=True)
+        da, db, dv = window_attn_bwd(new[3], a, b, new[2], out, lse, 90, 3)
+        dq, dk = rotary_nd(da, db, pos, freq, pairs, inverse=True)
+        for got, want in zip((q.grad, k.grad, v.grad), (dq, dk, dv)):
+            assert torch.equal(got, want)
