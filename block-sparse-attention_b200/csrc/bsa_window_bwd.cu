@@ -18,8 +18,8 @@
 // (two groups of 128 threads, thread = tensor-memory lane, group g owns columns [64g, 64g + 64) of the score tiles),
 // warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
 // P and dS are rounded to 16 bits for the tensor cores (all sums are fp32), and delta is that of the 16-bit `out` that the
-// forward call returned: relative to the gradients' own rounding the three give errors of 1.4 to 1.5 times in all for long
-// windows, 1.8 for windows of two keys, where delta nearly cancels dP.  What padding holds - NaN included - reaches
+// forward call returned: relative to the gradients' own rounding the three give errors of 1.4 to 1.6 times in all (rows of a
+// few keys, where delta nearly cancels dP, get a delta of their own).  What padding holds - NaN included - reaches
 // no sum: P is replaced by 0 on masked pairs, dP too where a tile reaches behind the end, the statistics of such rows are
 // those of a row that sees nothing, and the rows are zeroed in shared memory where an MMA contracts over them.  With fp16,
 // small gradients need the loss scaling that fp16 training uses anyway.
@@ -150,13 +150,39 @@ __device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a
 // ------------------------------------------------------------------------------------------------
 // 1. preprocess: HBM-bound, reads O and dO once.  A warp handles eight consecutive padded rows: sixteen lanes per row
 //    with 16 bytes each, all loads of a thread in flight before the first use.
+//    Rows that see at most kFewKeys keys (FEW) take delta = sum_j P_ij dO_i v_j instead, from q, k, v and the LSE: the
+//    rounding of O to 16 bits is not small against dP - delta there.  Error of dQ and dK, in half steps of the type, from
+//    the rounded O: 0.94 for windows of two keys, 0.81, 0.74, 0.70 for three to five, 0.68 for eight; this way 0.61.  For
+//    16 heads of 16384 tokens and two keys the pass takes 89 us instead of 26 (the whole backward 290 instead of 230).
 // ------------------------------------------------------------------------------------------------
+constexpr int kFewKeys = 5;
+struct FewKeys {
+  const uint8_t* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  long long q_stride[3], k_stride[3], v_stride[3];  // elements
+  int G, window, sinks;
+  float scale_log2;
+};
 template <bool F16>
+__device__ __forceinline__ float dot16(uint4 x, uint4 y) {
+  const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+  float acc = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 u = unpack16<F16>(a[e]), w = unpack16<F16>(b[e]);
+    acc = fmaf(u.x, w.x, acc);
+    acc = fmaf(u.y, w.y, acc);
+  }
+  return acc;
+}
+
+template <bool F16, bool FEW>
 __global__ void __launch_bounds__(256)
 window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ d_o, const float* __restrict__ lse,
                       float* __restrict__ lse_log2, float* __restrict__ delta, long long os_b, long long os_h,
                       long long os_s, long long ds_b, long long ds_h, long long ds_s, int H, int Sq, int SqPad,
-                      long long rows_pad, int D, const int32_t* __restrict__ kv_lens, int base) {
+                      long long rows_pad, int D, const int32_t* __restrict__ kv_lens, int base, const FewKeys few) {
   const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8;
   if (row0 >= rows_pad) return;
   const int lane = threadIdx.x & 31;
@@ -165,7 +191,9 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const int s0 = (int)(row0 - bh * SqPad);
   const int h = (int)(bh % H);
   const long long b = bh / H;
-  const uint8_t* o_base = o + (b * os_b + h * os_h + chunk * 8) * 2;
+  const long long hkv = FEW ? h / few.G : 0;
+  const uint8_t* o_base = FEW ? few.q + (b * few.q_stride[0] + h * few.q_stride[1] + chunk * 8) * 2 : o + (b * os_b + h * os_h + chunk * 8) * 2;
+  const long long o_row = FEW ? few.q_stride[2] : os_s;  // (FEW: q in the place of O)
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
   // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
   const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
@@ -174,25 +202,60 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    lv[i] = (s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
+    lv[i] = (!FEW && s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
     ov[i] = make_uint4(0, 0, 0, 0);
     dv[i] = make_uint4(0, 0, 0, 0);
     if (s < rows && chunk * 8 < D) {
-      ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * os_s * 2);
+      ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * o_row * 2);
       dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
     }
+  }
+  if (FEW) {
+    // The dot products of four rows are summed over the sixteen lanes together, each exchange halving the values a lane
+    // carries: q k and dO v of row `own` end at the lanes whose chunk has its bits 3 and 2.
+    const int own = chunk >> 2, s_own = s0 + 2 * own + sub, p_own = base + s_own;
+    const float l_own = s_own < rows ? lse[bh * Sq + s_own] * kLog2e : -INFINITY;
+    const uint8_t* k_base = few.k + (b * few.k_stride[0] + hkv * few.k_stride[1] + chunk * 8) * 2;
+    const uint8_t* v_base = few.v + (b * few.v_stride[0] + hkv * few.v_stride[1] + chunk * 8) * 2;
+    auto key = [&](int pos, int t) { return t < few.window ? pos - t : t - few.window; };
+    auto sees = [&](int pos, int t, int j) { return j >= 0 && (t < few.window || j <= pos - few.window); };
+    float acc = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < few.window + few.sinks; ++t) {
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = s0 + 2 * i + sub, j = key(base + row, t);
+        d[2 * i] = d[2 * i + 1] = 0.f;
+        if (row < rows && sees(base + row, t, j) && chunk * 8 < D) {
+          d[2 * i] = dot16<F16>(ov[i], *reinterpret_cast<const uint4*>(k_base + j * few.k_stride[2] * 2));
+          d[2 * i + 1] = dot16<F16>(dv[i], *reinterpret_cast<const uint4*>(v_base + j * few.v_stride[2] * 2));
+        }
+      }
+#pragma unroll
+      for (int n = 4; n > 0; n >>= 1) {  // n values are left; lanes whose bit 2n is set keep the upper ones
+        const bool upper = (chunk & (2 * n)) != 0;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          const float got = __shfl_xor_sync(0xffffffffu, upper ? d[e] : d[e + n], 2 * n);
+          d[e] = (upper ? d[e + n] : d[e]) + got;
+        }
+      }
+      d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+      const float other = __shfl_xor_sync(0xffffffffu, d[0], 2);
+      const float qk = (chunk & 2) ? other : d[0], dov = (chunk & 2) ? d[0] : other;
+      if (l_own != -INFINITY && sees(p_own, t, key(p_own, t))) acc = fmaf(ex2_approx(fmaf(qk, few.scale_log2, -l_own)), dov, acc);
+    }
+    if ((chunk & 3) == 0) {
+      delta[bh * SqPad + s_own] = -acc;
+      lse_log2[bh * SqPad + s_own] = l_own == -INFINITY ? -INFINITY : -l_own;
+    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    const uint32_t ow[4] = {ov[i].x, ov[i].y, ov[i].z, ov[i].w}, dw[4] = {dv[i].x, dv[i].y, dv[i].z, dv[i].w};
-    float acc = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a = unpack16<F16>(ow[e]), c = unpack16<F16>(dw[e]);
-      acc = fmaf(a.x, c.x, acc);
-      acc = fmaf(a.y, c.y, acc);
-    }
+    float acc = dot16<F16>(ov[i], dv[i]);
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
     if (chunk == 0) {
@@ -1102,10 +1165,21 @@ static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq
   if (e == cudaSuccess) e = dkv_attribute[p.parts > 0].set(reinterpret_cast<const void*>(dkv), kDkvSmem);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "bsa_window_bwd: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
-  window_bwd_pre_kernel<F16><<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
+  FewKeys few{static_cast<const uint8_t*>(a.q), static_cast<const uint8_t*>(a.k), static_cast<const uint8_t*>(a.v)};
+  for (int i = 0; i < 3; ++i) {
+    few.q_stride[i] = a.q_stride[i];
+    few.k_stride[i] = a.k_stride[i];
+    few.v_stride[i] = a.v_stride[i];
+  }
+  few.G = p.G;
+  few.window = p.window;
+  few.sinks = p.sinks;
+  few.scale_log2 = p.scale_log2;
+  auto pre = p.window <= kFewKeys - p.sinks ? window_bwd_pre_kernel<F16, true> : window_bwd_pre_kernel<F16, false>;
+  pre<<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
       static_cast<const uint8_t*>(a.out), static_cast<const uint8_t*>(a.dout), a.lse, lse_log2, delta, a.o_stride[0],
       a.o_stride[1], a.o_stride[2], a.do_stride[0], a.do_stride[1], a.do_stride[2], p.Hq, p.Sq, p.Nq * 128, rows_pad, p.D,
-      p.kv_lens, p.Sk - p.Sq);
+      p.kv_lens, p.Sk - p.Sq, few);
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward preprocess launch: %s", cudaGetErrorString(e));
   const int work_q = p.B * p.Hq * p.Nq, work_kv = p.B * p.Hkv * (p.parts > 0 ? p.Nkv * p.parts : p.Nkv + p.sink_items);
