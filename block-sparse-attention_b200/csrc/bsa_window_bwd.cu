@@ -150,12 +150,13 @@ __device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a
 // ------------------------------------------------------------------------------------------------
 // 1. preprocess: HBM-bound, reads O and dO once.  A warp handles eight consecutive padded rows: sixteen lanes per row
 //    with 16 bytes each, all loads of a thread in flight before the first use.
-//    Rows that see at most kFewKeys keys (FEW) take delta = sum_j P_ij dO_i v_j instead, from q, k, v and the LSE: the
-//    rounding of O to 16 bits is not small against dP - delta there.  Error of dQ and dK, in half steps of the type, from
-//    the rounded O: 0.94 for windows of two keys, 0.81, 0.74, 0.70 for three to five, 0.68 for eight; this way 0.61.  For
-//    16 heads of 16384 tokens and two keys the pass takes 89 us instead of 26 (the whole backward 290 instead of 230).
+//    FEW, for tiny windows and short sequences: rows that see kFewKeys keys or a few more take delta = sum_j P_ij dO_i v_j
+//    instead, from q, k, v and the LSE: the rounding of O to 16 bits is not small against dP - delta there.  Error of dQ
+//    and dK, in half steps of the type, from the rounded O: 0.94 for windows of two keys, 0.81, 0.74, 0.70 for three to
+//    five, 0.68 for eight; this way 0.61.  For 16 heads of 16384 tokens and two keys the pass takes 95 us instead of 26
+//    (the whole backward 300 instead of 230).
 // ------------------------------------------------------------------------------------------------
-constexpr int kFewKeys = 5;
+constexpr int kFewKeys = 5, kShort = 64;
 struct FewKeys {
   const uint8_t* q;
   const uint8_t* k;
@@ -191,9 +192,11 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const int s0 = (int)(row0 - bh * SqPad);
   const int h = (int)(bh % H);
   const long long b = bh / H;
+  const int last = base + s0 + 8;  // behind the position of the last of the rows
+  const bool is_few = FEW && (few.window + few.sinks <= kFewKeys || last - 8 < kFewKeys);  // (uniform over the warp)
   const long long hkv = FEW ? h / few.G : 0;
-  const uint8_t* o_base = FEW ? few.q + (b * few.q_stride[0] + h * few.q_stride[1] + chunk * 8) * 2 : o + (b * os_b + h * os_h + chunk * 8) * 2;
-  const long long o_row = FEW ? few.q_stride[2] : os_s;  // (FEW: q in the place of O)
+  const uint8_t* o_base = is_few ? few.q + (b * few.q_stride[0] + h * few.q_stride[1] + chunk * 8) * 2 : o + (b * os_b + h * os_h + chunk * 8) * 2;
+  const long long o_row = is_few ? few.q_stride[2] : os_s;  // (few keys: q in the place of O)
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
   // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
   const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
@@ -202,7 +205,7 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    lv[i] = (!FEW && s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
+    lv[i] = (!is_few && s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
     ov[i] = make_uint4(0, 0, 0, 0);
     dv[i] = make_uint4(0, 0, 0, 0);
     if (s < rows && chunk * 8 < D) {
@@ -210,18 +213,19 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
       dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
     }
   }
-  if (FEW) {
+  if (is_few) {
     // The dot products of four rows are summed over the sixteen lanes together, each exchange halving the values a lane
     // carries: q k and dO v of row `own` end at the lanes whose chunk has its bits 3 and 2.
     const int own = chunk >> 2, s_own = s0 + 2 * own + sub, p_own = base + s_own;
     const float l_own = s_own < rows ? lse[bh * Sq + s_own] * kLog2e : -INFINITY;
     const uint8_t* k_base = few.k + (b * few.k_stride[0] + hkv * few.k_stride[1] + chunk * 8) * 2;
     const uint8_t* v_base = few.v + (b * few.v_stride[0] + hkv * few.v_stride[1] + chunk * 8) * 2;
-    auto key = [&](int pos, int t) { return t < few.window ? pos - t : t - few.window; };
-    auto sees = [&](int pos, int t, int j) { return j >= 0 && (t < few.window || j <= pos - few.window); };
+    const int win = min(few.window, max(last, 0)), all = win + min(few.sinks, max(last - few.window, 0));  // at most 12 keys
+    auto key = [&](int pos, int t) { return t < win ? pos - t : t - win; };
+    auto sees = [&](int pos, int t, int j) { return j >= 0 && (t < win || j <= pos - few.window); };
     float acc = 0.f;
 #pragma unroll 1
-    for (int t = 0; t < few.window + few.sinks; ++t) {
+    for (int t = 0; t < all; ++t) {
       float d[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1175,7 +1179,9 @@ static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq
   few.window = p.window;
   few.sinks = p.sinks;
   few.scale_log2 = p.scale_log2;
-  auto pre = p.window <= kFewKeys - p.sinks ? window_bwd_pre_kernel<F16, true> : window_bwd_pre_kernel<F16, false>;
+  // a tiny window, or a short sequence from its start on (of a longer one the first rows are a small part)
+  const bool few_keys = p.window <= kFewKeys - p.sinks || (p.Sq <= kShort && p.Sk - p.Sq < kFewKeys);
+  auto pre = few_keys ? window_bwd_pre_kernel<F16, true> : window_bwd_pre_kernel<F16, false>;
   pre<<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
       static_cast<const uint8_t*>(a.out), static_cast<const uint8_t*>(a.dout), a.lse, lse_log2, delta, a.o_stride[0],
       a.o_stride[1], a.o_stride[2], a.do_stride[0], a.do_stride[1], a.do_stride[2], p.Hq, p.Sq, p.Nq * 128, rows_pad, p.D,

@@ -385,3 +385,15 @@ def test_few_visible_keys_keep_their_gradients(window, sinks, dtype):
     out, lse = window_attn_fwd(q, k, v, window, sinks, kv_lens=n, return_lse=True)
     for name, g, ref in zip(("dq", "dk", "dv"), window_attn_bwd(do, q, k, v, out, lse, window, sinks, kv_lens=n), refs):
         assert_close_norm(g, ref, 0.82 * half_step(dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("Sq,Sk", [(4, 4), (13, 13), (20, 9)])
+def test_short_sequences_keep_their_gradients(Sq, Sk, dtype):
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    q, k, v, do = make(40, 6, 2, Sq, Sk, 64, dtype, seed=6)
+    refs, _ = gradients(q.double(), k.double(), v.double(), do.double(), masks(40, Sq, Sk, 100, 3, None), 64 ** -0.5, dtype)
+    q, k, v, do = (t.cuda() for t in (q, k, v, do))
+    out, lse = window_attn_fwd(q, k, v, 100, 3, return_lse=True)
+    for name, g, ref in zip(("dq", "dk", "dv"), window_attn_bwd(do, q, k, v, out, lse, 100, 3), refs):
+        assert_close_norm(g, ref, 0.82 * half_step(dtype), name)
