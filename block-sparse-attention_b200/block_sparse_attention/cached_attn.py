@@ -100,7 +100,8 @@ def cached_attn_fwd(
 
     ``tree_mask`` (int64 ``[B, T]``, ``T <= 64``; see ``tree_mask_from_parents``) makes the new tokens drafts of a tree: bit
     ``u`` of entry ``t`` says that draft ``t`` sees draft ``u``.  A draft's position is that of its text,
-    ``cache_lens[b] - T + (number of its bits) - 1``; window and sinks go by these positions.  An entry 0 is an unused slot.
+    ``cache_lens[b] - T + (number of its bits) - 1``; window and sinks go by these positions (all bits count, also those of
+    drafts that would lie before a sequence shorter than the tree).  An entry 0 is an unused slot.
 
     Rows that see nothing give ``out = 0`` and ``lse = -inf``: unused slots, tokens at negative positions
     (``cache_lens[b] < T``), sequences without pages.  Tokens whose page is not in the pool are not visible.  What the

@@ -5,7 +5,8 @@
 // sequence's length minus the number of new tokens over a cache).  Key j is visible to a row at position p iff
 //     0 <= p < len,   j <= p,   (j > p - window  or  j < sinks).
 // Rows of a tree of drafts hold a 64-bit mask: bit u = draft u (the key at base + u) is visible; the row's position
-// is base + popcount - 1 (its depth), and it sees the keys before base by the rule above.
+// is base + popcount - 1 (its depth), and it sees the keys before base by the rule above.  In a sequence shorter than the
+// tree base is negative: drafts with base + u < 0 have no key but count for the positions.
 //
 // The kernels work on 128-token key tiles.  The tiles a query tile needs are those its rows' windows touch, walked
 // from the diagonal downwards (so the running maximum is set by visible scores from the first tile on), and then

@@ -255,19 +255,19 @@ __device__ __forceinline__ Row make_row(const WinFwdParams& p, const Item& t, in
   if (!valid) return r;
   if (p.tree_mask) {
     const unsigned long long* masks = p.tree_mask + (long long)t.b * p.Sq;
-    // drafts that exist: u < Sq, at a position that exists
-    unsigned long long all = p.Sq >= 64 ? ~0ull : ((1ull << p.Sq) - 1ull);
-    if (t.base < 0) all = (-t.base >= 64) ? 0ull : (all & (~0ull << (-t.base)));
-    const unsigned long long mine = masks[seq];
-    const int depth = __popcll(mine & all) - 1;
-    r.tree = mine & all;
-    if (depth >= p.window) {  // (only a window shorter than the branch leaves ancestors behind)
-      for (int u = 0; u < p.Sq; ++u) {
-        const int du = __popcll(masks[u] & all) - 1;
-        if (((r.tree >> u) & 1ull) && depth - du >= p.window && t.base + du >= p.sinks) r.tree &= ~(1ull << u);
+    // positions go by all bits of a mask; keys exist from the sequence's start on (a short sequence holds the last drafts)
+    const unsigned long long all = p.Sq >= 64 ? ~0ull : ((1ull << p.Sq) - 1ull);
+    const unsigned long long there = t.base >= 0 ? all : (-t.base >= 64 ? 0ull : (all & (~0ull << (-t.base))));
+    const unsigned long long mine = masks[seq] & all;
+    const int depth = __popcll(mine) - 1;
+    if (mine != 0 && t.base + depth >= 0) {
+      r.tree = mine & there;
+      if (depth >= p.window) {  // (only a window shorter than the branch leaves ancestors behind)
+        for (int u = 0; u < p.Sq; ++u) {
+          const int du = __popcll(masks[u] & all) - 1;
+          if (((r.tree >> u) & 1ull) && depth - du >= p.window && t.base + du >= p.sinks) r.tree &= ~(1ull << u);
+        }
       }
-    }
-    if (mine & all) {
       r.lo = t.base + depth - p.window + 1;
       r.hi = max(t.base, 0);
       r.live = true;

@@ -301,7 +301,8 @@ int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, in
  *   len - Sq, i.e. the Sq query tokens are the newest tokens of the sequence and their keys are in the cache
  *   already.  Tokens whose table entry is outside [0, num_pages) are not visible.
  * tree_mask [B, Sq] (paged, Sq <= 64): bit u of word t = draft u (the key at base + u) is visible to draft t.  The
- *   draft's position is then base + popcount - 1, that of a key u likewise; word 0 marks an unused slot (out = 0).
+ *   draft's position is then base + popcount - 1, that of a key u likewise; word 0 marks an unused slot (out = 0).  With
+ *   len < Sq, drafts whose key would lie before the sequence have none, but count for positions as any other.
  *
  * pack_gqa != 0: the rows of a tile are floor(128 / G) tokens x the G heads of a KV head.
  * stream_ctas = 0: whole query tiles are dealt to the CTAs in turn.  stream_ctas > 0: the list of all key tiles of all

@@ -1,0 +1,82 @@
+"""GPU parity of cached attention at its edges: trees over sequences shorter than the tree."""
+import pytest
+import torch
+
+from plain_ops import ancestors, assert_within, attend, cached_visible
+from test_cached_attn_gpu import ALL, BF, HF, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+def tree_visible(T, length, window, sinks, parents):
+    """[T, length] bool: a draft's position is base + (drafts on its branch) - 1, also where the branch begins before the
+    sequence; drafts whose key would lie before the sequence have none, rows at negative positions see nothing."""
+    base = length - T
+    chains = ancestors(parents)
+    at = [None if c is None else base + len(c) - 1 for c in chains]
+    seen = torch.zeros(T, max(length, 0), dtype=torch.bool)
+    for t, c in enumerate(chains):
+        if c is None or at[t] < 0:
+            continue
+        keys = [(j, j) for j in range(max(base, 0))] + [(base + u, at[u]) for u in c if base + u >= 0]
+        for j, rank in keys:
+            seen[t, j] = rank > at[t] - window or rank < sinks
+    return seen
+
+
+def random_tree(T, g):
+    return [int(torch.randint(-1, t, (1,), generator=g)) if t else -1 for t in range(T)]
+
+
+def check(out, lse, q, ks, vs, masks, dtype):
+    for b, mask in enumerate(masks):
+        ref, rl, tol, lt, _, _ = attend(q[b:b + 1].double(), ks[b][None].double(), vs[b][None].double(), mask[None],
+                                        q.shape[-1] ** -0.5, dtype)
+        assert_within(out[b:b + 1], ref, tol, f"out of sequence {b}")
+        assert_within(lse[b:b + 1], rl, lt, f"lse of sequence {b}")
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+# T, window, sinks, page, Hq, Hkv, D, dtype, lens
+SHORT_TREES = [
+    (17, 2, 0, 16, 2, 2, 128, BF, [5, 16, 1, 17]),
+    (17, 3, 1, 16, 4, 2, 64, HF, [5, 16, 0, 30]),
+    (40, 6, 2, 32, 8, 1, 96, BF, [39, 11, 3, 41]),  # several packed query tiles
+    (64, None, 0, 64, 2, 1, 64, BF, [63, 20, 1, 64]),
+    (64, 4, 3, 128, 6, 2, 96, HF, [63, 20, 2, 700]),
+    (33, 1, 0, 384, 2, 2, 64, BF, [32, 500, 7, 33]),
+]
+
+
+@pytest.mark.parametrize("case", SHORT_TREES, ids=[str(i) for i in range(len(SHORT_TREES))])
+@pytest.mark.parametrize("shape", ["chain", "random", "star"])
+def test_trees_over_sequences_shorter_than_the_tree(case, shape):
+    from block_sparse_attention import cached_attn_fwd, tree_mask_from_parents
+    T, window, sinks, page, Hq, Hkv, D, dtype, lens = case
+    g = torch.Generator().manual_seed(T)
+    B = len(lens)
+    make = {"chain": lambda: [t - 1 for t in range(T)], "random": lambda: random_tree(T, g), "star": lambda: [-1] + [0] * (T - 1)}
+    parents = [make[shape]() for _ in range(B)]
+    kc, vc, table, ks, vs = make_cache(B, Hkv, page, D, lens, dtype, seed=T)
+    q = torch.randn(B, Hq, T, D, generator=g).to(dtype)
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens), tree_mask=tree_mask_from_parents(i32(parents)),
+                               window=window, sink_tokens=sinks, return_lse=True)
+    check(out, lse, q, ks, vs, [tree_visible(T, n, window or ALL, sinks, p) for n, p in zip(lens, parents)], dtype)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2, 0), (5, 2), (1, 1)])
+def test_a_chain_is_a_chunk_of_tokens_also_where_it_begins_before_the_sequence(window, sinks):
+    from block_sparse_attention import cached_attn_fwd, tree_mask_from_parents
+    lens, T = [5, 29, 1, 0, 30], 30
+    kc, vc, table, ks, vs = make_cache(5, 2, 16, 128, lens, BF)
+    q = torch.randn(5, 4, T, 128, generator=torch.Generator().manual_seed(2)).bfloat16()
+    args = (q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens))
+    chain = tree_mask_from_parents((torch.arange(T, dtype=torch.int32) - 1).expand(5, T).cuda())
+    a = cached_attn_fwd(*args, window=window, sink_tokens=sinks, return_lse=True)
+    b = cached_attn_fwd(*args, window=window, sink_tokens=sinks, tree_mask=chain, return_lse=True)
+    for got in (a, b):
+        check(*got, q, ks, vs, [cached_visible(T, n, window or ALL, sinks) for n in lens], BF)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
