@@ -29,8 +29,9 @@
 // Roundings: scores, maximum, sums and O are fp32.  P is rounded to the inputs' type for the tensor cores; the sum is that of
 // the unrounded P, so a rounding does not shift the others.
 //
-// Keys behind the sequence's end may hold anything (padding, the unused end of a page): their scores are replaced,
-// not added to, and their V rows are set to zero in shared memory before PV reads them (0 * NaN is NaN).
+// Keys that no query of the call sees may hold anything (padding, the unused end of a page, an unused draft, what every window
+// has left behind): their scores are replaced, not added to, and their V rows are set to zero in shared memory before PV
+// reads them (0 * NaN is NaN).
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"
@@ -246,6 +247,36 @@ struct Row {
   bool live;  // sees anything at all
 };
 
+__device__ __forceinline__ unsigned long long all_drafts(const WinFwdParams& p) {
+  return p.Sq >= 64 ? ~0ull : ((1ull << p.Sq) - 1ull);
+}
+// The drafts whose keys a row with the (non-empty) mask `mine` sees.  Positions go by all bits of a mask; keys exist from the
+// sequence's start on (a short sequence holds the last drafts).
+__device__ __forceinline__ unsigned long long seen_drafts(const WinFwdParams& p, int base, const unsigned long long* masks,
+                                                          unsigned long long mine) {
+  unsigned long long seen = mine;
+  if (base < 0) seen = -base >= 64 ? 0ull : (mine & (~0ull << (-base)));
+  const int depth = __popcll(mine) - 1;
+  if (depth >= p.window) {  // (only a window shorter than the branch leaves ancestors behind)
+    for (int u = 0; u < p.Sq; ++u) {
+      const int du = __popcll(masks[u] & all_drafts(p)) - 1;
+      if (((seen >> u) & 1ull) && depth - du >= p.window && base + du >= p.sinks) seen &= ~(1ull << u);
+    }
+  }
+  return seen;
+}
+// The drafts that no draft of the sequence sees: unused slots.  Called by whole warps.
+__device__ __forceinline__ unsigned long long unseen_drafts(const WinFwdParams& p, const Item& t) {
+  const unsigned long long* masks = p.tree_mask + (long long)t.b * p.Sq;
+  unsigned long long seen = 0;
+  for (int u = threadIdx.x & 31; u < p.Sq; u += 32) {
+    const unsigned long long mine = masks[u] & all_drafts(p);
+    if (mine != 0 && t.base + __popcll(mine) - 1 >= 0) seen |= seen_drafts(p, t.base, masks, mine);
+  }
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)seen), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(seen >> 32));
+  return all_drafts(p) & ~((unsigned long long)hi << 32 | lo);
+}
+
 __device__ __forceinline__ Row make_row(const WinFwdParams& p, const Item& t, int seq, bool valid) {
   Row r;
   r.tree = 0;
@@ -255,19 +286,10 @@ __device__ __forceinline__ Row make_row(const WinFwdParams& p, const Item& t, in
   if (!valid) return r;
   if (p.tree_mask) {
     const unsigned long long* masks = p.tree_mask + (long long)t.b * p.Sq;
-    // positions go by all bits of a mask; keys exist from the sequence's start on (a short sequence holds the last drafts)
-    const unsigned long long all = p.Sq >= 64 ? ~0ull : ((1ull << p.Sq) - 1ull);
-    const unsigned long long there = t.base >= 0 ? all : (-t.base >= 64 ? 0ull : (all & (~0ull << (-t.base))));
-    const unsigned long long mine = masks[seq] & all;
+    const unsigned long long mine = masks[seq] & all_drafts(p);
     const int depth = __popcll(mine) - 1;
     if (mine != 0 && t.base + depth >= 0) {
-      r.tree = mine & there;
-      if (depth >= p.window) {  // (only a window shorter than the branch leaves ancestors behind)
-        for (int u = 0; u < p.Sq; ++u) {
-          const int du = __popcll(masks[u] & all) - 1;
-          if (((r.tree >> u) & 1ull) && depth - du >= p.window && t.base + du >= p.sinks) r.tree &= ~(1ull << u);
-        }
-      }
+      r.tree = seen_drafts(p, t.base, masks, mine);
       r.lo = t.base + depth - p.window + 1;
       r.hi = max(t.base, 0);
       r.live = true;
@@ -607,6 +629,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int free_lo = min(t.p_hi, t.len - 1) - p.window + 1;
       const int free_hi = p.tree_mask ? t.base : t.p_lo + 1;
       const bool narrow = narrow_end(p, t);
+      // no query of the call sees keys [sinks, unseen_hi): they lie before every window
+      const int unseen_hi = max(t.base, 0) - p.window + 1;
 
       for (int i = 0; i < n_it && ok; ++i) {
         const int it = t.it_begin + i;
@@ -625,23 +649,25 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           pages_ok = __ballot_sync(0xffffffffu, good);
         }
         const bool whole = j0 >= free_lo && j0 + 128 <= free_hi && pages_ok == 0xffffffffu;  // uniform over the warp
+        const unsigned long long unused = p.tree_mask && j0 + 128 > t.base ? unseen_drafts(p, t) : 0ull;
         ok = mbar_wait(BAR(kSFull), s_cnt & 1, wctx, 300);
         if (!ok) break;
         ++s_cnt;
         tc_fence_after();
-        if (j0 + 128 > t.len) {
-          // V rows behind the end may hold anything: zero them.  PV(i) of this tile waits for our P, so the stage
-          // cannot have been refilled when its arrival is observed here.
+        if (j0 + 128 > t.len || (j0 < unseen_hi && j0 + 128 > p.sinks) || unused != 0) {
+          // V rows behind the end, and others that no query of the call sees, may hold anything: zero them.  PV(i) of this
+          // tile waits for our P, so the stage cannot have been refilled when its arrival is observed here.
           const uint32_t pos = ring_cnt + 2u * (uint32_t)i + 1u;
           const uint32_t stage = pos % NS;
           ok = mbar_wait(BAR(kKvFull + stage), (pos / NS) & 1, wctx, 301);
           if (!ok) break;
-          if (j0 + row >= t.len) {
+          const int j = j0 + row, u = j - t.base;
+          if (j >= t.len || (j >= p.sinks && j < unseen_hi) || (u >= 0 && u < 64 && ((unused >> u) & 1ull))) {
             uint4* v0 = reinterpret_cast<uint4*>(sKV + stage * kTileBytes + row * 128);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              v0[c] = make_uint4(0, 0, 0, 0);
-              v0[c + kSlabBytes / 16] = make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < 8; ++c) {  // (each row begins at another chunk: other banks than its neighbours')
+              v0[(c + row) & 7] = make_uint4(0, 0, 0, 0);
+              v0[((c + row) & 7) + kSlabBytes / 16] = make_uint4(0, 0, 0, 0);
             }
           }
           fence_proxy_async_smem();

@@ -1,4 +1,4 @@
-"""GPU parity of cached attention at its edges: trees over sequences shorter than the tree."""
+"""GPU parity of cached attention at its edges: trees over sequences shorter than the tree, what unseen keys hold."""
 import pytest
 import torch
 
@@ -80,3 +80,78 @@ def test_a_chain_is_a_chunk_of_tokens_also_where_it_begins_before_the_sequence(w
     for got in (a, b):
         check(*got, q, ks, vs, [cached_visible(T, n, window or ALL, sinks) for n in lens], BF)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.fixture
+def deal(request, monkeypatch):
+    """Every call deals its work in the given way, whatever the rule says; None: the rule's."""
+    from block_sparse_attention import cached_attn, window_attn
+    if request.param is not None:
+        monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
+    cached_attn._cached_plan.cache_clear()
+    yield request.param
+    cached_attn._cached_plan.cache_clear()
+
+
+DEALS = [None, (0, 1), (0, 3), (0, 8), (7, 1), (296, 1)]
+
+
+def poison_unseen(pools, table, masks, holds):
+    """Fills the rows of every key in its sequence that no row of its mask sees."""
+    page = pools[0].shape[2]
+    some = False
+    for b, mask in enumerate(masks):
+        for j in (~mask.any(0)).nonzero()[:, 0].tolist() if mask.shape[1] else []:
+            for pool in pools:
+                pool[table[b, j // page], :, j % page] = holds
+            some = True
+    assert some
+
+
+# T, window, sinks, page, Hq, Hkv, D, dtype, lens; the trees hold unused slots
+UNSEEN = [
+    (1, 100, 4, 16, 8, 2, 128, BF, [700, 64, 300]),
+    (40, 70, 0, 64, 4, 4, 64, HF, [500, 41]),
+    (9, 130, 100, 256, 2, 1, 96, BF, [1000, 300]),
+]
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+@pytest.mark.parametrize("case", UNSEEN, ids=[str(i) for i in range(len(UNSEEN))])
+def test_cached_tokens_before_every_window_may_hold_anything(case, deal):
+    from block_sparse_attention import cached_attn_fwd
+    T, window, sinks, page, Hq, Hkv, D, dtype, lens = case
+    kc, vc, table, ks, vs = make_cache(len(lens), Hkv, page, D, lens, dtype, seed=T)
+    masks = [cached_visible(T, n, window, sinks) for n in lens]
+    poison_unseen((kc, vc), table, masks, float("nan"))
+    q = torch.randn(len(lens), Hq, T, D, generator=torch.Generator().manual_seed(T)).to(dtype)
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens), window=window, sink_tokens=sinks, return_lse=True)
+    check(out, lse, q, ks, vs, masks, dtype)
+
+
+UNUSED = [
+    (20, None, 0, 16, 4, 2, 128, BF, [300, 20, 12, 140]),
+    (64, 30, 2, 64, 2, 2, 64, HF, [64, 500, 191, 40]),
+    (48, None, 0, 128, 8, 2, 96, BF, [48, 300, 127, 170]),   # two query tiles; drafts on both sides of a key tile's end
+    (64, 1, 0, 32, 16, 2, 128, BF, [66, 64, 129, 700]),
+]
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+@pytest.mark.parametrize("case", UNUSED, ids=[str(i) for i in range(len(UNUSED))])
+def test_unused_drafts_may_hold_anything(case, deal):
+    from block_sparse_attention import cached_attn_fwd, tree_mask_from_parents
+    T, window, sinks, page, Hq, Hkv, D, dtype, lens = case
+    g = torch.Generator().manual_seed(T)
+    parents = [random_tree(T, g) for _ in lens]
+    for p in parents:
+        for t in (3, 7, T - 1):
+            p[t] = -2
+    parents[1] = [-2] * T  # no draft at all
+    kc, vc, table, ks, vs = make_cache(len(lens), Hkv, page, D, lens, dtype, seed=T)
+    masks = [tree_visible(T, n, window or ALL, sinks, p) for n, p in zip(lens, parents)]
+    poison_unseen((kc, vc), table, masks, float("nan"))
+    q = torch.randn(len(lens), Hq, T, D, generator=g).to(dtype)
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens), tree_mask=tree_mask_from_parents(i32(parents)),
+                               window=window, sink_tokens=sinks, return_lse=True)
+    check(out, lse, q, ks, vs, masks, dtype)

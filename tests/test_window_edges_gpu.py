@@ -1,0 +1,58 @@
+"""GPU parity of sliding-window attention at its edges: what keys hold that no query sees."""
+import pytest
+import torch
+
+from plain_ops import assert_within, attend
+from test_window_gpu import BF, HF, make, masks
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    return None if x is None else torch.tensor(x, dtype=torch.int32).cuda()
+
+
+@pytest.fixture
+def deal(request, monkeypatch):
+    """Every call deals its work in the given way, whatever the rule says; None: the rule's."""
+    from block_sparse_attention import window_attn
+    if request.param is not None:
+        monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
+    window_attn._window_plan.cache_clear()
+    yield request.param
+    window_attn._window_plan.cache_clear()
+
+
+DEALS = [None, (0, 1), (0, 3), (0, 8), (7, 1), (296, 1)]
+
+# B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens
+CHUNKS = [
+    (1, 2, 2, 100, 500, 128, BF, 50, 3, None),       # keys between the sinks and the first window
+    (2, 6, 2, 130, 700, 64, HF, 200, 0, [700, 640]),
+    (1, 2, 1, 300, 1000, 96, BF, 300, 70, None),     # more sinks than the narrow tile's columns
+    (1, 4, 1, 1, 400, 128, HF, 128, 128, None),      # one query, sinks up to the tile's end
+    (2, 2, 2, 40, 129, 64, BF, 1, 0, [129, 100]),
+    (1, 40, 40, 200, 900, 64, BF, 260, 33, None),
+]
+
+
+def poison_unseen(k, v, mask, holds):
+    """k, v [B, H, S, D] with `holds` in the keys that no row of mask [B, Sq, S] sees."""
+    unseen = ~mask.any(1)[:, None, :, None]
+    assert unseen.any()
+    return k.masked_fill(unseen, holds), v.masked_fill(unseen, holds)
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+@pytest.mark.parametrize("case", CHUNKS, ids=[str(i) for i in range(len(CHUNKS))])
+def test_keys_before_every_window_may_hold_anything(case, deal):
+    from block_sparse_attention import window_attn_fwd
+    B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens = case
+    q, k, v, _ = make(B, Hq, Hkv, Sq, Sk, D, dtype, seed=3)
+    mask = masks(B, Sq, Sk, window, sinks, lens)
+    ref, lse, tol, lse_tol, _, _ = attend(q.double(), k.double(), v.double(), mask, D ** -0.5, dtype)
+    for holds in (float("nan"), float("inf")):
+        kp, vp = poison_unseen(k, v, mask, holds)
+        out, got = window_attn_fwd(q.cuda(), kp.cuda(), vp.cuda(), window, sinks, kv_lens=i32(lens), return_lse=True)
+        assert_within(out, ref, tol, "out")
+        assert_within(got, lse, lse_tol, "lse")
