@@ -19,9 +19,10 @@
 // warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
 // P and dS are rounded to 16 bits for the tensor cores (all sums are fp32), and delta is that of the 16-bit `out` that the
 // forward call returned: relative to the gradients' own rounding the three give errors of 1.4 to 1.6 times in all (rows of a
-// few keys, where delta nearly cancels dP, get a delta of their own).  What padding holds - NaN included - reaches
-// no sum: P is replaced by 0 on masked pairs, dP too where a tile reaches behind the end, the statistics of such rows are
-// those of a row that sees nothing, and the rows are zeroed in shared memory where an MMA contracts over them.  With fp16,
+// few keys, where delta nearly cancels dP, get a delta of their own).  What rows that take no part hold -
+// padding, keys before every window, NaN included - reaches no sum: P is replaced by 0 on masked pairs, dP too where a tile
+// holds such rows, the statistics of such queries are those of a row that sees nothing, and the rows are zeroed in shared
+// memory where an MMA contracts over them.  With fp16,
 // small gradients need the loss scaling that fp16 training uses anyway.
 //
 // Bound by the instructions of the compute warps between two MMAs of a chain, like the block-sparse backward.  Measured: 16
@@ -63,7 +64,10 @@ struct Params {
   int sink_m0;     // first query tile beyond the reach of tile 0's windows
   int parts;       // few key tiles: parts that each one's list is cut into (partial [B * Hkv * Nkv][parts][2][128][D]); else 0
   int dq_group, dkv_group;  // of deal_item
+  int unseen_hi;   // keys [sinks, unseen_hi) lie before every window: no query of the call sees them
   float scale_log2, softmax_scale;
+  __device__ __forceinline__ bool holds_unseen(int j0) const { return j0 < unseen_hi && j0 + 128 > sinks; }  // of a key tile
+  __device__ __forceinline__ bool unseen(int j) const { return j >= sinks && j < unseen_hi; }
 };
 
 template <bool F16>
@@ -531,9 +535,9 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(BAR(kSFree));  // S_j is in registers: the next S may be computed
-            const bool tail = kMasked && j0 + 128 > t.len;
-            if (tail) {  // K rows behind the end may hold anything, and dQ contracts over them (S_j has read the tile)
-              if (j0 + row >= t.len) {
+            const bool tail = kMasked && (j0 + 128 > t.len || p.holds_unseen(j0));
+            if (tail) {  // K rows that no query sees may hold anything, and dQ contracts over them (S_j has read the tile)
+              if (j0 + row >= t.len || p.unseen(j0 + row)) {
                 uint4* k0 = reinterpret_cast<uint4*>(sRing + ((r_cnt + 2u * j) % NS) * kTile + grp * kSlab + row * 128);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) k0[c] = make_uint4(0, 0, 0, 0);
@@ -562,7 +566,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             tmem_ld32(t_g, dp);
             tmem_ld32(t_g + 32, dp + 32);
             tmem_wait_ld();
-            if (tail) {  // (V rows behind the end: 0 * NaN is NaN)
+            if (tail) {  // (such V rows: 0 * NaN is NaN)
 #pragma unroll
               for (int c = 0; c < 64; ++c) dp[c] = ((mw[c >> 5] >> (c & 31)) & 1u) ? dp[c] : 0u;
             }
@@ -957,8 +961,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           if (!mbar_wait(BAR(kDpFull), dp_cnt & 1, wctx, 521)) return false;
           tc_fence_after();
-          // the query tile or the key tile reaches behind the end, where rows may hold anything
-          const bool tail = kMasked && (p0 < 0 || p0 + 127 >= t.len || t.nb * 128 + 127 >= t.len);
+          // rows that take no part may hold anything: the query tile or the key tile reaches behind the end, or holds keys that
+          // no query sees
+          const bool tail = kMasked && (p0 < 0 || p0 + 127 >= t.len || t.nb * 128 + 127 >= t.len || p.holds_unseen(t.nb * 128));
           if (kMasked) {
             if (tail) {
               // query rows that take no part: dV contracts over the dO rows and dK over the Q rows (both tiles have been
@@ -1291,6 +1296,7 @@ extern "C" int bsa_window_bwd(const bsa_window_bwd_args* a, void* cuda_stream) {
   p.dq_group = head_group((long long)a->B * a->Hq, a->Sk < p.window ? a->Sk : p.window, a->D, a->Hq / a->Hkv);
   p.dkv_group = head_group((long long)a->B * a->Hkv, (long long)(a->Hq / a->Hkv) * (a->Sq < p.window ? a->Sq : p.window), a->D, 1);
   p.sinks = a->sinks;
+  p.unseen_hi = (a->Sk > a->Sq ? a->Sk - a->Sq : 0) - p.window + 1;
   const winbwd::Deal d = winbwd::deal(a->B, a->Hq, a->Hkv, a->Sq, a->Sk, p.window, a->sinks);
   p.parts = d.parts;
   p.sink_m0 = d.sink_m0;

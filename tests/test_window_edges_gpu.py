@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from plain_ops import assert_within, attend
+from plain_ops import assert_within, attend, gradients
 from test_window_gpu import BF, HF, make, masks
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,19 @@ def test_keys_before_every_window_may_hold_anything(case, deal):
         out, got = window_attn_fwd(q.cuda(), kp.cuda(), vp.cuda(), window, sinks, kv_lens=i32(lens), return_lse=True)
         assert_within(out, ref, tol, "out")
         assert_within(got, lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("case", CHUNKS, ids=[str(i) for i in range(len(CHUNKS))])
+def test_gradients_with_anything_in_keys_before_every_window(case):
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens = case
+    q, k, v, do = make(B, Hq, Hkv, Sq, Sk, D, dtype, seed=4)
+    mask = masks(B, Sq, Sk, window, sinks, lens)
+    refs, tols = gradients(q.double(), k.double(), v.double(), do.double(), mask, D ** -0.5, dtype)
+    n = i32(lens)
+    for holds in (float("nan"), float("inf")):
+        kp, vp = (t.cuda() for t in poison_unseen(k, v, mask, holds))
+        out, lse = window_attn_fwd(q.cuda(), kp, vp, window, sinks, kv_lens=n, return_lse=True)
+        grads = window_attn_bwd(do.cuda(), q.cuda(), kp, vp, out, lse, window, sinks, kv_lens=n)
+        for name, g, ref, tol in zip(("dq", "dk", "dv"), grads, refs, tols):
+            assert_within(g, ref, tol, name)
