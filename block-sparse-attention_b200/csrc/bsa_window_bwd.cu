@@ -202,17 +202,18 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const uint8_t* o_base = is_few ? few.q + (b * few.q_stride[0] + h * few.q_stride[1] + chunk * 8) * 2 : o + (b * os_b + h * os_h + chunk * 8) * 2;
   const long long o_row = is_few ? few.q_stride[2] : os_s;  // (few keys: q in the place of O)
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
-  // (rows behind the end may hold anything: their statistics are those of a row that sees nothing)
-  const int rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
+  // (rows before the first key or behind the end may hold anything: their statistics are those of a row that sees nothing)
+  const int first = max(0, -base), rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
   uint4 ov[4], dv[4];
   float lv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    lv[i] = (!is_few && s < rows && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
+    const bool live = s >= first && s < rows;
+    lv[i] = (!is_few && live && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
     ov[i] = make_uint4(0, 0, 0, 0);
     dv[i] = make_uint4(0, 0, 0, 0);
-    if (s < rows && chunk * 8 < D) {
+    if (live && chunk * 8 < D) {
       ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * o_row * 2);
       dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
     }
@@ -221,7 +222,7 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
     // The dot products of four rows are summed over the sixteen lanes together, each exchange halving the values a lane
     // carries: q k and dO v of row `own` end at the lanes whose chunk has its bits 3 and 2.
     const int own = chunk >> 2, s_own = s0 + 2 * own + sub, p_own = base + s_own;
-    const float l_own = s_own < rows ? lse[bh * Sq + s_own] * kLog2e : -INFINITY;
+    const float l_own = s_own >= first && s_own < rows ? lse[bh * Sq + s_own] * kLog2e : -INFINITY;
     const uint8_t* k_base = few.k + (b * few.k_stride[0] + hkv * few.k_stride[1] + chunk * 8) * 2;
     const uint8_t* v_base = few.v + (b * few.v_stride[0] + hkv * few.v_stride[1] + chunk * 8) * 2;
     const int win = min(few.window, max(last, 0)), all = win + min(few.sinks, max(last - few.window, 0));  // at most 12 keys

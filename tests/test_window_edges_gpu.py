@@ -72,3 +72,31 @@ def test_gradients_with_anything_in_keys_before_every_window(case):
         grads = window_attn_bwd(do.cuda(), q.cuda(), kp, vp, out, lse, window, sinks, kv_lens=n)
         for name, g, ref, tol in zip(("dq", "dk", "dv"), grads, refs, tols):
             assert_within(g, ref, tol, name)
+
+
+# more queries than keys: the first ones sit before the first key
+LATE = [
+    (1, 2, 2, 200, 100, 64, BF, 40, 2),
+    (2, 6, 2, 400, 150, 128, HF, 1 << 20, 0),
+    (1, 40, 40, 700, 260, 96, BF, 100, 5),   # many key tiles: not cut into parts
+    (3, 2, 1, 30, 7, 64, HF, 3, 0),          # a few visible keys
+]
+
+
+@pytest.mark.parametrize("case", LATE, ids=[str(i) for i in range(len(LATE))])
+def test_queries_before_the_first_key_may_hold_anything(case):
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks = case
+    q, k, v, do = make(B, Hq, Hkv, Sq, Sk, D, dtype, seed=5)
+    mask = masks(B, Sq, Sk, window, sinks, None)
+    refs, tols = gradients(q.double(), k.double(), v.double(), do.double(), mask, D ** -0.5, dtype)
+    ref, rl, tol, lt, _, _ = attend(q.double(), k.double(), v.double(), mask, D ** -0.5, dtype)
+    for holds in (float("nan"), float("inf")):
+        for t in (q, do):
+            t[:, :, :Sq - Sk] = holds
+        out, lse = window_attn_fwd(q.cuda(), k.cuda(), v.cuda(), window, sinks, return_lse=True)
+        assert_within(out, ref, tol, "out")
+        assert_within(lse, rl, lt, "lse")
+        grads = window_attn_bwd(do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, window, sinks)
+        for name, g, want, t in zip(("dq", "dk", "dv"), grads, refs, tols):
+            assert_within(g, want, t, name)
