@@ -203,7 +203,7 @@ window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__
   const long long o_row = is_few ? few.q_stride[2] : os_s;  // (few keys: q in the place of O)
   const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
   // (rows before the first key or behind the end may hold anything: their statistics are those of a row that sees nothing)
-  const int first = max(0, -base), rows = kv_lens == nullptr ? Sq : max(0, min(Sq, max(kv_lens[b], 0) - base));
+  const int first = max(0, -base), rows = kv_lens == nullptr ? Sq : max(0, max(0, min(kv_lens[b], base + Sq)) - base);
   uint4 ov[4], dv[4];
   float lv[4];
 #pragma unroll

@@ -100,3 +100,18 @@ def test_queries_before_the_first_key_may_hold_anything(case):
         grads = window_attn_bwd(do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, window, sinks)
         for name, g, want, t in zip(("dq", "dk", "dv"), grads, refs, tols):
             assert_within(g, want, t, name)
+
+
+@pytest.mark.parametrize("Sq,Sk", [(200, 100), (150, 150), (40, 300), (60, 9)])
+def test_a_length_without_a_limit_is_the_whole_sequence(Sq, Sk):
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    q, k, v, do = (t.cuda() for t in make(2, 4, 2, Sq, Sk, 64, BF, seed=6))
+
+    def step(n):
+        out, lse = window_attn_fwd(q, k, v, 40, 2, kv_lens=n, return_lse=True)
+        return (out, lse) + window_attn_bwd(do, q, k, v, out, lse, 40, 2, kv_lens=n)
+
+    want = step(None)
+    assert all(t.any() for t in want)
+    for n in (2 ** 31 - 1, 2 ** 31 - 40, Sk + 1, Sk):
+        assert all(torch.equal(a, b) for a, b in zip(step(i32([n, n])), want)), n
