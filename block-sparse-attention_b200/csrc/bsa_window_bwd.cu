@@ -154,21 +154,36 @@ __device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a
 // ------------------------------------------------------------------------------------------------
 // 1. preprocess: HBM-bound, reads O and dO once.  A warp handles eight consecutive padded rows: sixteen lanes per row
 //    with 16 bytes each, all loads of a thread in flight before the first use.
-//    FEW, for tiny windows and short sequences: rows that see kFewKeys keys or a few more take delta = sum_j P_ij dO_i v_j
-//    instead, from q, k, v and the LSE: the rounding of O to 16 bits is not small against dP - delta there.  Error of dQ
-//    and dK, in half steps of the type, from the rounded O: 0.94 for windows of two keys, 0.81, 0.74, 0.70 for three to
-//    five, 0.68 for eight; this way 0.61.  For 16 heads of 16384 tokens and two keys the pass takes 95 us instead of 26
-//    (the whole backward 300 instead of 230).
+//    Rows that see at most kFewKeys keys take delta = sum_j P_ij dO_i v_j instead, from q, k, v and the LSE: the rounding of
+//    O to 16 bits is not small against dP - delta there.  Error of dQ and dK in half steps of the type, from the rounded O: 0.94
+//    for rows of two keys, 0.81, 0.74, 0.70 for three to five, 0.68 for eight; this way 0.61.  Those are the first rows of any
+//    sequence (blocks of their own, in front of the others: dQ of the rows at positions 0 to 4 0.81 -> 0.61, the whole
+//    backward of 8 heads of 300 tokens 15.7 -> 16.0 us, of 16 heads of 16384 equal), and every row of a window that holds no more,
+//    which has a kernel of its own (16 heads of 16384 tokens, window 2: backward 296 us, from the rounded O 227).
 // ------------------------------------------------------------------------------------------------
-constexpr int kFewKeys = 5, kShort = 64;
-struct FewKeys {
-  const uint8_t* q;
-  const uint8_t* k;
-  const uint8_t* v;
-  long long q_stride[3], k_stride[3], v_stride[3];  // elements
-  int G, window, sinks;
+constexpr int kFewKeys = 5;
+struct PreParams {
+  const uint8_t *o, *d_o, *q, *k, *v;
+  const float* __restrict__ lse;
+  float* __restrict__ lse_log2;
+  float* __restrict__ delta;
+  const int32_t* __restrict__ kv_lens;
+  long long o_stride[3], do_stride[3], q_stride[3], k_stride[3], v_stride[3];  // elements
+  long long rows_pad;
+  int H, G, Sq, SqPad, D, base, window, sinks;
+  int first_blocks;  // blocks of the first rows: B * H, or none
   float scale_log2;
+
+  // Rows [first, behind) of a sequence take part; the others may hold anything: their statistics are those of a row that sees
+  // nothing.
+  __device__ __forceinline__ int first() const { return max(0, -base); }
+  __device__ __forceinline__ int behind(long long b) const {
+    return kv_lens == nullptr ? Sq : max(0, max(0, min(kv_lens[b], base + Sq)) - base);
+  }
 };
+__device__ __forceinline__ uint4 load16(const uint8_t* p, const long long* stride, long long b, long long h, long long s, int chunk) {
+  return *reinterpret_cast<const uint4*>(p + (b * stride[0] + h * stride[1] + s * stride[2] + chunk * 8) * 2);
+}
 template <bool F16>
 __device__ __forceinline__ float dot16(uint4 x, uint4 y) {
   const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
@@ -181,97 +196,151 @@ __device__ __forceinline__ float dot16(uint4 x, uint4 y) {
   }
   return acc;
 }
+__device__ __forceinline__ float sum16(float x) {  // over sixteen lanes
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
 
-template <bool F16, bool FEW>
+// The first rows of a head, at positions below kFewKeys of a wider window: row p sees keys 0..p.  A block takes a head, a
+// half-warp one of the 15 pairs of row and key (one round of loads), then a thread each row.
+template <bool F16>
+__device__ __forceinline__ void first_rows(const PreParams& p) {
+  __shared__ float s_qk[16], s_dov[16];
+  const long long bh = blockIdx.x, b = bh / p.H;
+  const int h = (int)(bh % p.H), pair = threadIdx.x >> 4, chunk = threadIdx.x & 15;
+  int pos = 0;
+  while ((pos + 1) * (pos + 2) / 2 <= pair) ++pos;
+  const int j = pair - pos * (pos + 1) / 2, behind = p.behind(b);
+  float qk = 0.f, dov = 0.f;
+  if (pos < kFewKeys && pos >= p.base && pos - p.base < behind && chunk * 8 < p.D) {
+    qk = dot16<F16>(load16(p.q, p.q_stride, b, h, pos - p.base, chunk), load16(p.k, p.k_stride, b, h / p.G, j, chunk));
+    dov = dot16<F16>(load16(p.d_o, p.do_stride, b, h, pos - p.base, chunk), load16(p.v, p.v_stride, b, h / p.G, j, chunk));
+  }
+  qk = sum16(qk);
+  dov = sum16(dov);
+  if (chunk == 0) {
+    s_qk[pair] = qk;
+    s_dov[pair] = dov;
+  }
+  __syncthreads();
+  pos = threadIdx.x;
+  const int s = pos - p.base;
+  if (pos >= kFewKeys || s < 0 || s >= p.SqPad) return;
+  float acc = 0.f, l = -INFINITY;
+  if (s < behind) {
+    l = p.lse[bh * p.Sq + s] * kLog2e;
+    for (int key = 0; key <= pos; ++key) {
+      const int e = pos * (pos + 1) / 2 + key;
+      if (l != -INFINITY) acc = fmaf(ex2_approx(fmaf(s_qk[e], p.scale_log2, -l)), s_dov[e], acc);
+    }
+  }
+  p.delta[bh * p.SqPad + s] = -acc;
+  p.lse_log2[bh * p.SqPad + s] = l == -INFINITY ? -INFINITY : -l;
+}
+
+template <bool F16>
 __global__ void __launch_bounds__(256)
-window_bwd_pre_kernel(const uint8_t* __restrict__ o, const uint8_t* __restrict__ d_o, const float* __restrict__ lse,
-                      float* __restrict__ lse_log2, float* __restrict__ delta, long long os_b, long long os_h,
-                      long long os_s, long long ds_b, long long ds_h, long long ds_s, int H, int Sq, int SqPad,
-                      long long rows_pad, int D, const int32_t* __restrict__ kv_lens, int base, const FewKeys few) {
-  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8;
-  if (row0 >= rows_pad) return;
+window_bwd_pre_kernel(const PreParams p) {
+  if ((int)blockIdx.x < p.first_blocks) {
+    first_rows<F16>(p);
+    return;
+  }
+  const long long row0 = ((long long)(blockIdx.x - p.first_blocks) * 8 + (threadIdx.x >> 5)) * 8;
+  if (row0 >= p.rows_pad) return;
   const int lane = threadIdx.x & 31;
   const int sub = lane >> 4, chunk = lane & 15;
-  const long long bh = row0 / SqPad;  // the eight rows lie in one (batch, head) plane: SqPad is a multiple of 128
-  const int s0 = (int)(row0 - bh * SqPad);
-  const int h = (int)(bh % H);
-  const long long b = bh / H;
-  const int last = base + s0 + 8;  // behind the position of the last of the rows
-  const bool is_few = FEW && (few.window + few.sinks <= kFewKeys || last - 8 < kFewKeys);  // (uniform over the warp)
-  const long long hkv = FEW ? h / few.G : 0;
-  const uint8_t* o_base = is_few ? few.q + (b * few.q_stride[0] + h * few.q_stride[1] + chunk * 8) * 2 : o + (b * os_b + h * os_h + chunk * 8) * 2;
-  const long long o_row = is_few ? few.q_stride[2] : os_s;  // (few keys: q in the place of O)
-  const uint8_t* d_base = d_o + (b * ds_b + h * ds_h + chunk * 8) * 2;
-  // (rows before the first key or behind the end may hold anything: their statistics are those of a row that sees nothing)
-  const int first = max(0, -base), rows = kv_lens == nullptr ? Sq : max(0, max(0, min(kv_lens[b], base + Sq)) - base);
+  const long long bh = row0 / p.SqPad;  // the eight rows lie in one (batch, head) plane: SqPad is a multiple of 128
+  const int s0 = (int)(row0 - bh * p.SqPad);
+  const int h = (int)(bh % p.H);
+  const long long b = bh / p.H;
+  const int first = p.first(), behind = p.behind(b), done = p.first_blocks > 0 ? kFewKeys - p.base : 0;
   uint4 ov[4], dv[4];
   float lv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    const bool live = s >= first && s < rows;
-    lv[i] = (!is_few && live && chunk == 0) ? lse[bh * Sq + s] : -INFINITY;
+    const bool live = s >= first && s < behind;
+    lv[i] = (live && chunk == 0) ? p.lse[bh * p.Sq + s] : -INFINITY;
     ov[i] = make_uint4(0, 0, 0, 0);
     dv[i] = make_uint4(0, 0, 0, 0);
-    if (live && chunk * 8 < D) {
-      ov[i] = *reinterpret_cast<const uint4*>(o_base + (long long)s * o_row * 2);
-      dv[i] = *reinterpret_cast<const uint4*>(d_base + (long long)s * ds_s * 2);
+    if (live && chunk * 8 < p.D) {
+      ov[i] = load16(p.o, p.o_stride, b, h, s, chunk);
+      dv[i] = load16(p.d_o, p.do_stride, b, h, s, chunk);
     }
-  }
-  if (is_few) {
-    // The dot products of four rows are summed over the sixteen lanes together, each exchange halving the values a lane
-    // carries: q k and dO v of row `own` end at the lanes whose chunk has its bits 3 and 2.
-    const int own = chunk >> 2, s_own = s0 + 2 * own + sub, p_own = base + s_own;
-    const float l_own = s_own >= first && s_own < rows ? lse[bh * Sq + s_own] * kLog2e : -INFINITY;
-    const uint8_t* k_base = few.k + (b * few.k_stride[0] + hkv * few.k_stride[1] + chunk * 8) * 2;
-    const uint8_t* v_base = few.v + (b * few.v_stride[0] + hkv * few.v_stride[1] + chunk * 8) * 2;
-    const int win = min(few.window, max(last, 0)), all = win + min(few.sinks, max(last - few.window, 0));  // at most 12 keys
-    auto key = [&](int pos, int t) { return t < win ? pos - t : t - win; };
-    auto sees = [&](int pos, int t, int j) { return j >= 0 && (t < win || j <= pos - few.window); };
-    float acc = 0.f;
-#pragma unroll 1
-    for (int t = 0; t < all; ++t) {
-      float d[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = s0 + 2 * i + sub, j = key(base + row, t);
-        d[2 * i] = d[2 * i + 1] = 0.f;
-        if (row < rows && sees(base + row, t, j) && chunk * 8 < D) {
-          d[2 * i] = dot16<F16>(ov[i], *reinterpret_cast<const uint4*>(k_base + j * few.k_stride[2] * 2));
-          d[2 * i + 1] = dot16<F16>(dv[i], *reinterpret_cast<const uint4*>(v_base + j * few.v_stride[2] * 2));
-        }
-      }
-#pragma unroll
-      for (int n = 4; n > 0; n >>= 1) {  // n values are left; lanes whose bit 2n is set keep the upper ones
-        const bool upper = (chunk & (2 * n)) != 0;
-#pragma unroll
-        for (int e = 0; e < n; ++e) {
-          const float got = __shfl_xor_sync(0xffffffffu, upper ? d[e] : d[e + n], 2 * n);
-          d[e] = (upper ? d[e + n] : d[e]) + got;
-        }
-      }
-      d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
-      const float other = __shfl_xor_sync(0xffffffffu, d[0], 2);
-      const float qk = (chunk & 2) ? other : d[0], dov = (chunk & 2) ? d[0] : other;
-      if (l_own != -INFINITY && sees(p_own, t, key(p_own, t))) acc = fmaf(ex2_approx(fmaf(qk, few.scale_log2, -l_own)), dov, acc);
-    }
-    if ((chunk & 3) == 0) {
-      delta[bh * SqPad + s_own] = -acc;
-      lse_log2[bh * SqPad + s_own] = l_own == -INFINITY ? -INFINITY : -l_own;
-    }
-    return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = s0 + 2 * i + sub;
-    float acc = dot16<F16>(ov[i], dv[i]);
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    if (chunk == 0) {
+    const float acc = sum16(dot16<F16>(ov[i], dv[i]));
+    if (chunk == 0 && (s >= done || s < first)) {
       const float l = lv[i] == -INFINITY ? INFINITY : lv[i] * kLog2e;
-      delta[bh * SqPad + s] = -acc;
-      lse_log2[bh * SqPad + s] = -l;
+      p.delta[bh * p.SqPad + s] = -acc;
+      p.lse_log2[bh * p.SqPad + s] = -l;
     }
+  }
+}
+
+// Every row, for windows that hold at most kFewKeys keys together with the sinks.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+window_bwd_pre_few_kernel(const PreParams p) {
+  const long long row0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8;
+  if (row0 >= p.rows_pad) return;
+  const int lane = threadIdx.x & 31;
+  const int sub = lane >> 4, chunk = lane & 15;
+  const long long bh = row0 / p.SqPad;
+  const int s0 = (int)(row0 - bh * p.SqPad);
+  const int h = (int)(bh % p.H);
+  const long long b = bh / p.H;
+  const int first = p.first(), behind = p.behind(b);
+  uint4 qv[4], dv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = s0 + 2 * i + sub;
+    qv[i] = make_uint4(0, 0, 0, 0);
+    dv[i] = make_uint4(0, 0, 0, 0);
+    if (s >= first && s < behind && chunk * 8 < p.D) {
+      qv[i] = load16(p.q, p.q_stride, b, h, s, chunk);
+      dv[i] = load16(p.d_o, p.do_stride, b, h, s, chunk);
+    }
+  }
+  // The dot products of four rows are summed over the sixteen lanes together, each exchange halving the values a lane
+  // carries: q k and dO v of row `own` end at the lanes whose chunk has its bits 3 and 2.
+  const int own = chunk >> 2, s_own = s0 + 2 * own + sub, p_own = p.base + s_own;
+  const float l_own = s_own >= first && s_own < behind ? p.lse[bh * p.Sq + s_own] * kLog2e : -INFINITY;
+  auto key = [&](int pos, int t) { return t < p.window ? pos - t : t - p.window; };
+  auto sees = [&](int pos, int t, int j) { return j >= 0 && (t < p.window || j <= pos - p.window); };
+  float acc = 0.f;
+#pragma unroll 1
+  for (int t = 0; t < p.window + p.sinks; ++t) {
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = s0 + 2 * i + sub, j = key(p.base + row, t);
+      d[2 * i] = d[2 * i + 1] = 0.f;
+      if (row < behind && sees(p.base + row, t, j) && chunk * 8 < p.D) {
+        d[2 * i] = dot16<F16>(qv[i], load16(p.k, p.k_stride, b, h / p.G, j, chunk));
+        d[2 * i + 1] = dot16<F16>(dv[i], load16(p.v, p.v_stride, b, h / p.G, j, chunk));
+      }
+    }
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1) {  // n values are left; lanes whose bit 2n is set keep the upper ones
+      const bool upper = (chunk & (2 * n)) != 0;
+#pragma unroll
+      for (int e = 0; e < n; ++e) {
+        const float got = __shfl_xor_sync(0xffffffffu, upper ? d[e] : d[e + n], 2 * n);
+        d[e] = (upper ? d[e + n] : d[e]) + got;
+      }
+    }
+    d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+    const float other = __shfl_xor_sync(0xffffffffu, d[0], 2);
+    const float qk = (chunk & 2) ? other : d[0], dov = (chunk & 2) ? d[0] : other;
+    if (l_own != -INFINITY && sees(p_own, t, key(p_own, t))) acc = fmaf(ex2_approx(fmaf(qk, p.scale_log2, -l_own)), dov, acc);
+  }
+  if ((chunk & 3) == 0) {
+    p.delta[bh * p.SqPad + s_own] = -acc;
+    p.lse_log2[bh * p.SqPad + s_own] = l_own == -INFINITY ? -INFINITY : -l_own;
   }
 }
 
@@ -1175,23 +1244,40 @@ static int launch(const bsa_window_bwd_args& a, Params& p, const CUtensorMap& tq
   if (e == cudaSuccess) e = dkv_attribute[p.parts > 0].set(reinterpret_cast<const void*>(dkv), kDkvSmem);
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "bsa_window_bwd: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const long long rows_pad = (long long)p.B * p.Hq * p.Nq * 128;
-  FewKeys few{static_cast<const uint8_t*>(a.q), static_cast<const uint8_t*>(a.k), static_cast<const uint8_t*>(a.v)};
+  PreParams pre{};
+  pre.o = static_cast<const uint8_t*>(a.out);
+  pre.d_o = static_cast<const uint8_t*>(a.dout);
+  pre.q = static_cast<const uint8_t*>(a.q);
+  pre.k = static_cast<const uint8_t*>(a.k);
+  pre.v = static_cast<const uint8_t*>(a.v);
+  pre.lse = a.lse;
+  pre.lse_log2 = lse_log2;
+  pre.delta = delta;
+  pre.kv_lens = p.kv_lens;
   for (int i = 0; i < 3; ++i) {
-    few.q_stride[i] = a.q_stride[i];
-    few.k_stride[i] = a.k_stride[i];
-    few.v_stride[i] = a.v_stride[i];
+    pre.o_stride[i] = a.o_stride[i];
+    pre.do_stride[i] = a.do_stride[i];
+    pre.q_stride[i] = a.q_stride[i];
+    pre.k_stride[i] = a.k_stride[i];
+    pre.v_stride[i] = a.v_stride[i];
   }
-  few.G = p.G;
-  few.window = p.window;
-  few.sinks = p.sinks;
-  few.scale_log2 = p.scale_log2;
-  // a tiny window, or a short sequence from its start on (of a longer one the first rows are a small part)
-  const bool few_keys = p.window <= kFewKeys - p.sinks || (p.Sq <= kShort && p.Sk - p.Sq < kFewKeys);
-  auto pre = few_keys ? window_bwd_pre_kernel<F16, true> : window_bwd_pre_kernel<F16, false>;
-  pre<<<(unsigned)((rows_pad + 63) / 64), 256, 0, st>>>(
-      static_cast<const uint8_t*>(a.out), static_cast<const uint8_t*>(a.dout), a.lse, lse_log2, delta, a.o_stride[0],
-      a.o_stride[1], a.o_stride[2], a.do_stride[0], a.do_stride[1], a.do_stride[2], p.Hq, p.Sq, p.Nq * 128, rows_pad, p.D,
-      p.kv_lens, p.Sk - p.Sq, few);
+  pre.rows_pad = rows_pad;
+  pre.H = p.Hq;
+  pre.G = p.G;
+  pre.Sq = p.Sq;
+  pre.SqPad = p.Nq * 128;
+  pre.D = p.D;
+  pre.base = p.Sk - p.Sq;
+  pre.window = p.window;
+  pre.sinks = p.sinks;
+  pre.scale_log2 = p.scale_log2;
+  const unsigned blocks = (unsigned)((rows_pad + 63) / 64);
+  if (p.window <= kFewKeys - p.sinks) {
+    window_bwd_pre_few_kernel<F16><<<blocks, 256, 0, st>>>(pre);
+  } else {
+    pre.first_blocks = pre.base < kFewKeys ? p.B * p.Hq : 0;
+    window_bwd_pre_kernel<F16><<<blocks + pre.first_blocks, 256, 0, st>>>(pre);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(BSA_ERR_CUDA, "window backward preprocess launch: %s", cudaGetErrorString(e));
   const int work_q = p.B * p.Hq * p.Nq, work_kv = p.B * p.Hkv * (p.parts > 0 ? p.Nkv * p.parts : p.Nkv + p.sink_items);
