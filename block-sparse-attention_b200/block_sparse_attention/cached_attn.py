@@ -7,7 +7,8 @@ the context visible.
 The cache is a pair of pools ``[num_pages, Hkv, page_size, D]``.  ``page_table`` (int32 ``[B, max_pages]``) names the
 pages of each sequence in order; entries outside the pool (-1, say) are pages the sequence does not have.
 ``cache_lens`` (int32 ``[B]``) counts a sequence's tokens *with* the ``T`` new ones, whose keys and values
-``cache_append`` has put at positions ``cache_lens[b] - T .. cache_lens[b] - 1``.
+``cache_append`` has put at positions ``cache_lens[b] - T .. cache_lens[b] - 1``.  A length beyond the table
+(``max_pages * page_size``) counts as the table's in every call, a negative one as 0.
 """
 from __future__ import annotations
 

@@ -18,6 +18,8 @@ struct Pages {
   const int32_t* __restrict__ table;
   int max_pages, page_size, num_pages;
 
+  // A length beyond the table counts as the tokens that the table holds, as in the attention over the cache.
+  __device__ __forceinline__ int cut(int len) const { return max(0, min(len, max_pages * page_size)); }
   // Byte offsets of (sequence, head, position) in K and V; false when the position has no page in the pool.
   __device__ __forceinline__ bool at(int b, int h, int pos, long long& ko, long long& vo) const {
     if (pos < 0) return false;
@@ -51,7 +53,7 @@ cache_append_kernel(const Source s, const Pages pg, const int32_t* __restrict__ 
   const int t0 = (int)(r % groups) * kRows;
   r /= groups;
   const int h = (int)(r % H), b = (int)(r / H);
-  const int base = max(lens[b], 0) - T;
+  const int base = pg.cut(lens[b]) - T;
   uint4 kv[kRows], vv[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
@@ -82,7 +84,7 @@ cache_keep_kernel(const Pages pg, const int32_t* __restrict__ lens, const int32_
   const int c = (int)(unit % chunks);
   const long long r = unit / chunks;
   const int h = (int)(r % H), b = (int)(r / H);
-  const int len = lens[b], base = max(len, 0) - T;
+  const int len = lens[b], base = pg.cut(len) - T;
   const int32_t* mine = path + (long long)b * path_cap;
   int n = base < 0 ? 0 : max(0, min(path_lens[b], path_cap));
   int last = -1, kept = 0;

@@ -155,3 +155,25 @@ def test_unused_drafts_may_hold_anything(case, deal):
     out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens), tree_mask=tree_mask_from_parents(i32(parents)),
                                window=window, sink_tokens=sinks, return_lse=True)
     check(out, lse, q, ks, vs, masks, dtype)
+
+
+@pytest.mark.parametrize("beyond", [1, 5, 40, 2 ** 31 - 1 - 96])
+def test_a_length_beyond_the_table_is_the_table_in_every_call(beyond):
+    """Write, attend, keep: what the calls do for the table's own length."""
+    from block_sparse_attention import cache_append, cache_keep, cached_attn_fwd
+    T, full = 5, 96
+    g = torch.Generator().manual_seed(8)
+    kc, vc, table, _, _ = make_cache(2, 2, 32, 64, [full, full], BF, garbage=False)
+    q, k, v = (torch.randn(2, h, T, 64, generator=g).bfloat16().cuda() for h in (4, 2, 2))
+    path = i32([[0, 2, 4], [1, 3, 4]])
+
+    def step(n):
+        pools = kc.clone().cuda(), vc.clone().cuda()
+        cache_append(k, v, *pools, table.cuda(), i32(n))
+        out, lse = cached_attn_fwd(q, *pools, table.cuda(), i32(n), window=40, return_lse=True)
+        new = cache_keep(*pools, table.cuda(), i32(n), path, i32([3, 2]), T)
+        return (out, lse, new) + pools
+
+    want = step([full, full])
+    assert torch.equal(want[2], i32([full - 2, full - 3])) and not torch.equal(want[3].cpu(), kc)
+    assert all(torch.equal(a, b) for a, b in zip(step([full + beyond, full]), want))
