@@ -1176,7 +1176,10 @@ extern "C" int bsa_window_fwd(const bsa_window_fwd_args* a, void* cuda_stream) {
   if (p.team > 1 && work * p.team > 65535) return set_error(BSA_ERR_INVALID, "bsa_window_fwd: more than 65535 CTAs in teams");
   if (p.ctas > 0 && p.lists > 1 && p.lists != p.NqT)
     return set_error(BSA_ERR_INVALID, "bsa_window_fwd: stream_lists must be 1 or the number of query tiles per head (%d)", p.NqT);
-  if (p.ctas > 0 && work * ((Sk + 127) / 128 + 1) > 0x7fffffffLL)
+  // key tiles of a query tile: those that its rows' windows touch, and the sinks'
+  const long long rows = a->Sq < p.seq_per_tile ? a->Sq : p.seq_per_tile, touched = (rows + p.window + 127) / 128 + 1;
+  const long long most = (Sk + 127) / 128 < touched ? (Sk + 127) / 128 : touched;
+  if (p.ctas > 0 && work * (most + 1) > 0x7fffffffLL)
     return set_error(BSA_ERR_UNSUPPORTED, "bsa_window_fwd: more than 2^31 key tiles in a stream run");
   p.scale_log2 = a->softmax_scale * kLog2e;
 

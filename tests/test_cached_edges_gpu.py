@@ -177,3 +177,20 @@ def test_a_length_beyond_the_table_is_the_table_in_every_call(beyond):
     want = step([full, full])
     assert torch.equal(want[2], i32([full - 2, full - 3])) and not torch.equal(want[3].cpu(), kc)
     assert all(torch.equal(a, b) for a, b in zip(step([full + beyond, full]), want))
+
+
+def test_a_window_over_the_longest_table():
+    """2^29 places a sequence, of which a window sees a few: the list of key tiles is that of the windows."""
+    from block_sparse_attention import cached_attn_fwd
+    from block_sparse_attention.window_attn import _deal_work
+    B, page, n = 607, 1 << 20, 5000
+    assert _deal_work(B, 18, 1, False, 148)[0] > 0  # shared evenly, as the call below
+    g = torch.Generator().manual_seed(9)
+    k, v = (torch.randn(1, 1, n, 64, generator=g).bfloat16() for _ in range(2))
+    pools = [torch.zeros(1, 1, page, 64, dtype=BF, device="cuda") for _ in range(2)]
+    for pool, x in zip(pools, (k, v)):
+        pool[:, :, :n] = x.cuda()
+    table = torch.zeros(B, 512, dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 1, 1, 64, generator=g).bfloat16()
+    out, lse = cached_attn_fwd(q.cuda().expand(B, 1, 1, 64).contiguous(), *pools, table, i32([n] * B), window=2000, return_lse=True)
+    check(out[::150], lse[::150], q.expand(5, 1, 1, 64), [k[0]] * 5, [v[0]] * 5, [cached_visible(1, n, 2000, 0)] * 5, BF)
