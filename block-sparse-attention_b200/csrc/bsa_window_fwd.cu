@@ -621,9 +621,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int hq = t.hkv * p.G + t.g + row_head;
       const bool row_valid = row < heads * t.nseq;
       const bool warp_active = (warp * 32) < heads * t.nseq;  // some row of this warp exists
-      // growth of the maximum (2^8) from which on O is rescaled.  Rows that do not exist have no say: behind the last head
-      // of a packed tile they hold what shared memory held before.
-      const float rescale_from = row_valid ? 8.f : INFINITY;
       const Row r = make_row(p, t, seq, row_valid && n_it > 0);
       // every row of the tile sees all keys of [free_lo, free_hi) that exist
       const int free_lo = min(t.p_hi, t.len - 1) - p.window + 1;
@@ -684,12 +681,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const uint32_t t_row = tS + lane_base;
         uint64_t s0 = pack2(0.f, 0.f), s1 = s0;
         // The running maximum takes in a tile's largest score; O and the sum are rescaled only when it grew by more than
-        // the threshold in some row of the warp.  Returns the addend of the exponents.
+        // 2^8 in some row of the warp.  Rows that see nothing have no say: they may hold anything, and the others' roundings
+        // must not depend on it.  Returns the addend of the exponents.
         auto grow = [&](float top) -> float {
           const float m_new = fmaxf(m_cur, top * p.scale_log2);
           if (i == 0) {
             m_cur = m_new;
-          } else if (__any_sync(0xffffffffu, (m_new - m_cur) > rescale_from)) {
+          } else if (__any_sync(0xffffffffu, r.live && (m_new - m_cur) > 8.f)) {
             const float sc = (m_new == -INFINITY) ? 1.f : ex2_approx(m_cur - m_new);
             m_cur = m_new;
             l_sum *= sc;

@@ -194,3 +194,25 @@ def test_a_window_over_the_longest_table():
     q = torch.randn(1, 1, 1, 64, generator=g).bfloat16()
     out, lse = cached_attn_fwd(q.cuda().expand(B, 1, 1, 64).contiguous(), *pools, table, i32([n] * B), window=2000, return_lse=True)
     check(out[::150], lse[::150], q.expand(5, 1, 1, 64), [k[0]] * 5, [v[0]] * 5, [cached_visible(1, n, 2000, 0)] * 5, BF)
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+def test_results_do_not_depend_on_unused_queries(deal):
+    """To the bit: queries of unused slots and of tokens before the sequence."""
+    from block_sparse_attention import cached_attn_fwd, tree_mask_from_parents
+    lens, T = [900, 20, 300], 40
+    kc, vc, table, _, _ = make_cache(3, 2, 64, 128, lens, BF)
+    g = torch.Generator().manual_seed(10)
+    q = torch.randn(3, 4, T, 128, generator=g).bfloat16()
+    parents = [[-1 if t % 7 == 0 else -2 if t % 7 == 3 else t - 1 for t in range(T)] for _ in lens]
+    mask = tree_mask_from_parents(i32(parents))
+    unused = (mask == 0).cpu()[:, None, :, None]
+    before = (torch.arange(T) + torch.tensor(lens)[:, None] < T)[:, None, :, None]
+    assert unused.any() and before.any()
+    pools = kc.cuda(), vc.cuda(), table.cuda(), i32(lens)
+    for dead, tree in ((unused | before, mask), (before, None)):
+        got = []
+        for holds in (1.0, 30.0, -1000.0, float("nan")):
+            got.append(cached_attn_fwd(torch.where(dead, q * holds, q).cuda(), *pools, tree_mask=tree, return_lse=True))
+        for other in got[1:]:
+            assert torch.equal(got[0][0], other[0]) and torch.equal(got[0][1], other[1])

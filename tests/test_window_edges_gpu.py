@@ -139,3 +139,21 @@ def test_first_rows_keep_their_gradients(Sq, Sk, window, sinks, lens, dtype):
     out, lse = window_attn_fwd(q, k, v, window, sinks, kv_lens=i32(n), return_lse=True)
     dq, _, _ = window_attn_bwd(do, q, k, v, out, lse, window, sinks, kv_lens=i32(n))
     assert_close_norm(dq[:, :, rows], ref, 0.82 * half_step(dtype), "dq")
+
+
+@pytest.mark.parametrize("deal", DEALS, indirect=True, ids=str)
+def test_results_do_not_depend_on_what_padding_holds(deal):
+    """To the bit: forward and backward, padded query rows beside live ones of the same warp."""
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    q, k, v, do = (t.cuda() for t in make(3, 4, 2, 400, 400, 128, BF, seed=8))
+    lens = [200, 307, 5]
+    n, got = i32(lens), []
+    for holds in (0.0, 30.0, -1000.0, float("nan")):
+        q2, k2, v2, do2 = q.clone(), k.clone(), v.clone(), do.clone()
+        for b, m in enumerate(lens):
+            for t in (q2, k2, v2, do2):
+                t[b, :, m:] = t[b, :, m:] * holds
+        out, lse = window_attn_fwd(q2, k2, v2, 4096, 0, kv_lens=n, return_lse=True)
+        got.append((out, lse) + window_attn_bwd(do2, q2, k2, v2, out, lse, 4096, 0, kv_lens=n))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
