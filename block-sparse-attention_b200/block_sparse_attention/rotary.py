@@ -141,7 +141,7 @@ def _rotary_plan(q, k, positions, inv_freq, pairs, interleaved, inverse, q_out, 
     if B == 0 or S == 0 or (Hq == 0 and Hk == 0):
         return _RotaryPlan(True, True, q_shape, k_shape, b"")
     assert Hq >= 1, "q has no heads"
-    if q[1][3] != 1 or (k is not None and k[1][3] != 1) or (A > 1 and positions[1][-1] != 1) or (P > 1 and inv_freq[1] != (1,)):
+    if q[1][3] != 1 or (Hk > 0 and k[1][3] != 1) or (A > 1 and positions[1][-1] != 1) or (P > 1 and inv_freq[1] != (1,)):
         return _RotaryPlan(False, False, q_shape, k_shape, b"")
 
     def strides(t, out=None):
