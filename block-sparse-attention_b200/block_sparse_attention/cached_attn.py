@@ -19,7 +19,8 @@ import torch
 
 from . import _cabi
 from .bsa_attn_interface import _ceil_div
-from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_lens, _check_qkv, _check_scale, _check_window, _copied, _dense, _fits,
+from .overlap import meet, span_bytes, spread
+from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_buffers, _check_lens, _check_qkv, _check_scale, _check_window, _copied, _dense, _fits,
                           _make_plan, _meta, _run_plan)
 
 __all__ = ["cached_attn_fwd", "tree_mask_from_parents", "cache_append", "cache_keep"]
@@ -47,9 +48,17 @@ def _check_pool_address(k_cache, v_cache) -> None:
     assert (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the pools must be 16-byte aligned"
 
 
-def _check_written_pools(k_cache, v_cache) -> None:
+def _check_written_pools(k_cache, v_cache, span: int, k=None, v=None, k_span: int = 0, v_span: int = 0) -> None:
+    """Pools that are written share no memory with each other nor with the rows that are written to them; the spans (bytes) settle
+    all but interleaved views."""
     _check_pool_address(k_cache, v_cache)
-    assert k_cache.data_ptr() != v_cache.data_ptr(), "keys and values must not be written to one pool"
+    at_k, at_v = k_cache.data_ptr(), v_cache.data_ptr()
+    assert not -span < at_k - at_v < span or not meet(k_cache, v_cache), "keys and values must not be written to one pool"
+    for rows, n in ((k, k_span), (v, v_span)):
+        if n > 0:
+            at = rows.data_ptr()
+            if -n < at - at_k < span or -n < at - at_v < span:
+                assert not meet(rows, k_cache) and not meet(rows, v_cache), "k and v must not share memory with the pools"
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -113,6 +122,8 @@ def cached_attn_fwd(
                         _meta(out), _meta(lse), window, sink_tokens, None if softmax_scale is None else float(softmax_scale),
                         layout, want_lse)
     _check_pool_address(k_cache, v_cache)
+    if out is not None or lse is not None:
+        _check_buffers(plan, out, lse, q, k_cache, v_cache, cache_lens, page_table, tree_mask)
     res = _run_plan(plan, q, k_cache, v_cache, out, lse, cache_lens, page_table, tree_mask) if plan.direct else None
     if res is not None:
         return res
@@ -147,7 +158,14 @@ class _WritePlan(NamedTuple):
 
     direct: bool
     empty: bool
+    spans: Tuple[int, ...]  # bytes: a pool, k, v
     args: bytes = b""  # CacheArgs without addresses
+
+
+def _pool_span(k_cache, v_cache) -> int:
+    for t in (k_cache, v_cache):
+        assert spread(*t[:2]), "a pool that is written must not overlap itself"
+    return max(span_bytes(*k_cache[:2], 2), span_bytes(*v_cache[:2], 2))
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -160,12 +178,13 @@ def _append_plan(k, v, k_cache, v_cache, table, lens, layout) -> _WritePlan:
     _check_cache(k_cache, v_cache, table, lens, B, k[3])
     num_pages, pool_heads, page_size, pool_dim = k_cache[0]
     assert pool_heads == H and pool_dim == D and D % 8 == 0, "the pools must match k's heads and head dimension"
+    spans = _pool_span(k_cache, v_cache), span_bytes(*k[:2], 2), span_bytes(*v[:2], 2)
     if B == 0 or T == 0 or table[0][1] == 0:
-        return _WritePlan(True, True)
+        return _WritePlan(True, True, spans)
     rows_ok = all(t[1][3] == 1 and (t[1][0] | t[1][1] | t[1][2]) % 8 == 0 for t in (k, v))
     if not (rows_ok and _dense(table) and _dense(lens)):
-        return _WritePlan(False, False)
-    return _WritePlan(True, False, bytes(_cabi.CacheArgs(
+        return _WritePlan(False, False, spans)
+    return _WritePlan(True, False, spans, bytes(_cabi.CacheArgs(
         *[None] * 9, _bhsd(k[1], layout), _bhsd(v[1], layout), k_cache[1][:3], v_cache[1][:3], B, H, T, D, table[0][1], page_size,
         num_pages, 0)))
 
@@ -182,11 +201,12 @@ def _keep_plan(k_cache, v_cache, table, lens, path, path_lens, num_drafts) -> _W
         f"path must be int32 of shape ({B}, n) on the device of the pools")
     assert path_lens is not None, "path_lens must be given"
     _check_lens(path_lens, B, device, "path_lens")
+    spans = (_pool_span(k_cache, v_cache),)
     if B == 0:
-        return _WritePlan(True, True)
+        return _WritePlan(True, True, spans)
     if path[0][1] == 0 or table[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
-        return _WritePlan(False, False)
-    return _WritePlan(True, False, bytes(_cabi.CacheArgs(
+        return _WritePlan(False, False, spans)
+    return _WritePlan(True, False, spans, bytes(_cabi.CacheArgs(
         *[None] * 9, (0, 0, 0), (0, 0, 0), k_cache[1][:3], v_cache[1][:3], B, H, num_drafts, D, table[0][1], page_size, num_pages,
         path[0][1])))
 
@@ -201,7 +221,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     must not be reached through two sequences' tables for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
     """
     plan = _append_plan(_meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), layout)
-    _check_written_pools(k_cache, v_cache)
+    _check_written_pools(k_cache, v_cache, plan.spans[0], k, v, *plan.spans[1:])
     if plan.empty:
         return k_cache, v_cache
     at = k.data_ptr(), v.data_ptr()
@@ -227,7 +247,7 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     ``num_drafts`` tokens is left as it is.  A move from or to a page that is not in the pool is dropped.
     """
     plan = _keep_plan(_meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(path), _meta(path_lens), num_drafts)
-    _check_written_pools(k_cache, v_cache)
+    _check_written_pools(k_cache, v_cache, plan.spans[0])
     if plan.empty:
         return cache_lens.clone()
     if not plan.direct:

@@ -11,6 +11,7 @@ from typing import NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _cabi
+from .overlap import check_apart, pairs_apart, spread
 from .window_attn import _meta
 
 __all__ = ["rotary_frequencies", "rotary_nd", "rotary_embedding", "RotaryFunction"]
@@ -26,20 +27,6 @@ def rotary_frequencies(axis_pairs: Sequence[int], theta: float = 10000.0, *, sha
     counts = [sum(axis_pairs)] if shared_ladder else list(axis_pairs)
     parts = [float(theta) ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in counts]
     return torch.cat(parts).to(device=device, dtype=torch.float32)
-
-
-def _span(t: torch.Tensor) -> Tuple[int, int]:
-    end = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (end + 1) * t.element_size()
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
-
-
-def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
 
 def rotary_nd(
@@ -63,25 +50,24 @@ def rotary_nd(
     ``interleaved=False``; it belongs to the axis whose share of ``axis_pairs`` (1 to 4 axes, in order) holds ``p`` and turns
     by ``positions[b, s, axis] * inv_freq[p]`` (``inverse=True``: by the opposite angle).  ``positions`` is int32
     ``[S, axes]`` or ``[B, S, axes]``, ``inv_freq`` fp32 ``[P]`` (``rotary_frequencies``).  Angles are reduced in 64 bits, so
-    positions of any size keep their accuracy.  ``q_out`` / ``k_out`` may be q and k themselves (in place); other overlaps
-    are refused.
+    positions of any size keep their accuracy.  ``q_out`` / ``k_out`` may be q and k themselves (in place); outputs that share
+    other memory are refused.
     """
     pairs = tuple(map(int, axis_pairs))
     plan = _rotary_plan(_meta(q), _meta(k), _meta(positions), _meta(inv_freq), pairs, bool(interleaved), bool(inverse),
                         _meta(q_out), _meta(k_out), layout)
+    if q_out is not None or k_out is not None:
+        check_apart(plan.apart, [0 if t is None else t.data_ptr() for t in (q_out, k_out, q, k, positions, inv_freq)])
     if not plan.direct:
         return rotary_nd(q if q.stride(3) == 1 else q.contiguous(), k if k is None or k.stride(3) == 1 else k.contiguous(),
                          positions.contiguous(), inv_freq.contiguous(), pairs, interleaved=interleaved, inverse=inverse,
                          q_out=q_out, k_out=k_out, layout=layout)
-    fresh = q_out is None and (k is None or k_out is None)
     if q_out is None:
         q_out = torch.empty_like(q) if plan.q_dense else q.new_empty(plan.q_shape)
     if k is None:
         k_out = None
     elif k_out is None:
         k_out = torch.empty_like(k) if plan.k_dense else q.new_empty(plan.k_shape)
-    if not fresh:  # fresh outputs overlap nothing
-        _check_overlap(q, q_out, k, k_out)
     if plan.empty:
         return q_out, k_out
     a = _cabi.RotaryArgs.from_buffer_copy(plan.args)
@@ -106,6 +92,7 @@ class _RotaryPlan(NamedTuple):
     q_shape: tuple
     k_shape: Optional[tuple]
     args: bytes
+    apart: tuple  # of overlap.check_apart: q_out, k_out, q, k, positions, inv_freq
     q_dense: bool = False  # contiguous: empty_like, the cheaper call, gives the same
     k_dense: bool = False
 
@@ -135,14 +122,15 @@ def _rotary_plan(q, k, positions, inv_freq, pairs, interleaved, inverse, q_out, 
     for name, x, out in (("q_out", q, q_out), ("k_out", k, k_out)):
         if out is not None:
             assert x is not None and out[0] == x[0] and out[2] == x[2] and out[3] == device, f"{name} must match its input"
-            assert out[1][3] == 1 and all(n == 1 or st > 0 for n, st in zip(out[0], out[1])), (
-                f"{name} must have unit last stride and no broadcast dimension")
+            assert out[1][3] == 1 and spread(*out[:2]), f"{name} must have unit last stride and not overlap itself"
     q_shape, k_shape = tuple(q[0]), None if k is None else tuple(k[0])
+    apart = pairs_apart((("q_out", q_out), ("k_out", k_out)), (("q", q), ("k", k), ("positions", positions), ("inv_freq", inv_freq)),
+                        (("q_out", "q"), ("k_out", "k")))
     if B == 0 or S == 0 or (Hq == 0 and Hk == 0):
-        return _RotaryPlan(True, True, q_shape, k_shape, b"")
+        return _RotaryPlan(True, True, q_shape, k_shape, b"", apart)
     assert Hq >= 1, "q has no heads"
     if q[1][3] != 1 or (Hk > 0 and k[1][3] != 1) or (A > 1 and positions[1][-1] != 1) or (P > 1 and inv_freq[1] != (1,)):
-        return _RotaryPlan(False, False, q_shape, k_shape, b"")
+        return _RotaryPlan(False, False, q_shape, k_shape, b"", apart)
 
     def strides(t, out=None):
         if t is None:
@@ -158,21 +146,7 @@ def _rotary_plan(q, k, positions, inv_freq, pairs, interleaved, inverse, q_out, 
     args = _cabi.RotaryArgs(None, None, None, None, None, None, strides(q, q), strides(k, k), strides(q, q_out), strides(k, k_out),
                             (pos_st[0] if len(at) == 3 else 0, pos_st[-2]), pairs, A, code, B, Hq, Hk, S, D, int(interleaved),
                             int(inverse))
-    return _RotaryPlan(True, False, q_shape, k_shape, bytes(args), _contiguous(q), k is not None and _contiguous(k))
-
-
-def _check_overlap(q, qo, k, ko) -> None:
-    if any(t is not None and t.numel() == 0 for t in (q, k)):
-        return
-    for out, own, other, other_out in ((qo, q, k, ko), (ko, k, q, qo)):
-        if out is None:
-            continue
-        assert _same_view(out, own) or not _overlap(out, own), "an output may be its input or apart from it, not overlap it"
-        if other is not None:
-            # views of one fused projection may interleave; then both have to be rotated in place
-            apart = not _overlap(out, other) and not _overlap(out, other_out)
-            assert apart or (_same_view(out, own) and _same_view(other_out, other) and out.data_ptr() != other.data_ptr()), (
-                "q and k and their outputs must not overlap, unless both are rotated in place")
+    return _RotaryPlan(True, False, q_shape, k_shape, bytes(args), apart, _contiguous(q), k is not None and _contiguous(k))
 
 
 class RotaryFunction(torch.autograd.Function):

@@ -18,6 +18,7 @@ import torch
 
 from . import _cabi
 from .bsa_attn_interface import _ceil_div, _tma_ready
+from .overlap import check_apart, pairs_apart, spread
 
 __all__ = ["window_attn_fwd", "window_attn_bwd", "window_attention", "WindowAttentionFunction"]
 
@@ -124,6 +125,7 @@ class _Plan(NamedTuple):
     workspace: int          # floats
     partial_o: int          # byte offsets in it
     partial_lse: int
+    apart: tuple            # of overlap.check_apart: out, lse, q, k, v, lens, table, tree
     q_dense: bool = False   # contiguous: empty_like, the cheaper call, gives the same
 
 
@@ -154,18 +156,21 @@ def _make_plan(q, k, v, out, lse, lens, layout, shape, *, window, sinks, scale, 
     device = q[3]
     if out is not None:
         assert out[0] == q[0] and out[2] == q[2] and out[3] == device, "out must match q"
-        assert out[1][3] == 1, "out must have unit last stride"
+        assert out[1][3] == 1 and spread(*out[:2]), "out must have unit last stride and not overlap itself"
     if lse is not None:
         assert lse[0] == (B, Hq, Sq) and lse[2] == torch.float32 and lse[3] == device, f"lse must be float32 ({B}, {Hq}, {Sq})"
+        assert spread(*lse[:2]), "lse must not overlap itself"
     lse_shape = (B, Hq, Sq) if want_lse else None
+    apart = pairs_apart((("out", out), ("lse", lse)), (("q", q), ("k", k), ("v", v), ("lengths", lens), ("page_table", table),
+                                                       ("tree_mask", tree)), (("out", "q"),))  # (a query tile is read first)
     if empty or Sq == 0 or B == 0 or Hq == 0:
-        return _Plan(True, True, tuple(q[0]), lse_shape, b"", 0, 0, 0)
+        return _Plan(True, True, tuple(q[0]), lse_shape, b"", 0, 0, 0, apart)
     kv_layout = layout if table is None else "bhsd"
     out_st = out[1] if out is not None else ((Hq * Sq * D, Sq * D, D, 1) if layout == "bhsd" else (Hq * Sq * D, Hq * D, D, 1))
     direct = (_fits(q[1]) and _fits(k[1]) and _fits(v[1]) and _fits(out_st)
               and all(t is None or _dense(t) for t in (lse, lens, table, tree)))
     if not direct:
-        return _Plan(False, False, tuple(q[0]), lse_shape, b"", 0, 0, 0)
+        return _Plan(False, False, tuple(q[0]), lse_shape, b"", 0, 0, 0, apart)
     per_tile = 128 // (Hq // Hkv) if pack_gqa else 128  # query tokens of a tile
     tiles = _ceil_div(Sq, per_tile)
     items = B * tiles * (Hkv if pack_gqa else Hq)
@@ -183,7 +188,7 @@ def _make_plan(q, k, v, out, lse, lens, layout, shape, *, window, sinks, scale, 
         1 if pack_gqa else 0, ctas, lists, team, scale)
     # workspace: the list of joins (four ints a CTA), the pieces' rows, their LSE
     return _Plan(True, False, tuple(q[0]), lse_shape, bytes(args), (4 * ctas + rows * (D + 1)) if ctas else 0, 16 * ctas,
-                 16 * ctas + 4 * rows * D, q[1] == ((n := q[0])[1] * n[2] * n[3], n[2] * n[3], n[3], 1))
+                 16 * ctas + 4 * rows * D, apart, q[1] == ((n := q[0])[1] * n[2] * n[3], n[2] * n[3], n[3], 1))
 
 
 def _run_plan(plan: _Plan, q, k, v, out, lse, lens, table, tree):
@@ -201,7 +206,6 @@ def _run_plan(plan: _Plan, q, k, v, out, lse, lens, table, tree):
     a.q, a.k, a.v, a.out = at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if (at[0] | at[1] | at[2] | at[3]) % 16:
         return None
-    assert at[3] != at[1] and at[3] != at[2], "out must not be k or v"
     if lse is not None:
         a.lse = lse.data_ptr()
     if lens is not None:
@@ -218,6 +222,11 @@ def _run_plan(plan: _Plan, q, k, v, out, lse, lens, table, tree):
     a.status = _cabi.status_buffer(device).data_ptr()
     _cabi.launch(_cabi.load().bsa_window_fwd, "bsa_window_fwd", device, a)
     return out, lse
+
+
+def _check_buffers(plan: _Plan, *tensors) -> None:
+    """What the caller's buffers may share memory with; ``tensors`` in the order of ``plan.apart``."""
+    check_apart(plan.apart, [0 if t is None else t.data_ptr() for t in tensors])
 
 
 def _copied(call, q, k, v, out, lse, layout):
@@ -274,6 +283,8 @@ def window_attn_fwd(
     want_lse = return_lse or lse is not None or q.requires_grad or k.requires_grad or v.requires_grad
     plan = _window_plan(_meta(q), _meta(k), _meta(v), _meta(out), _meta(lse), _meta(kv_lens), window, sink_tokens,
                         None if softmax_scale is None else float(softmax_scale), layout, want_lse)
+    if out is not None or lse is not None:
+        _check_buffers(plan, out, lse, q, k, v, kv_lens, None, None)
     res = _run_plan(plan, q, k, v, out, lse, kv_lens, None, None) if plan.direct else None
     if res is not None:
         return res
@@ -308,6 +319,8 @@ def window_attn_bwd(
     """
     plan = _bwd_plan(_meta(dout), _meta(q), _meta(k), _meta(v), _meta(out), _meta(lse), _meta(kv_lens), _meta(dq), _meta(dk),
                      _meta(dv), window, sink_tokens, None if softmax_scale is None else float(softmax_scale), layout)
+    if dq is not None or dk is not None or dv is not None:
+        check_apart(plan.apart, [0 if t is None else t.data_ptr() for t in (dq, dk, dv, dout, q, k, v, out, lse, kv_lens)])
     if not plan.direct:
         return _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout)
     grads = (q.new_empty(plan.q_shape) if dq is None else dq, q.new_empty(plan.k_shape) if dk is None else dk,
@@ -319,7 +332,6 @@ def window_attn_bwd(
     a = _cabi.WindowBwdArgs.from_buffer_copy(plan.args)
     a.dout, a.q, a.k, a.v, a.out = at = dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.dq, a.dk, a.dv = to = grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr()
-    assert not any(ptr in at for ptr in to) and len(set(to)) == 3, "a gradient buffer must not be one of the inputs or another one"
     if (at[0] | at[1] | at[2] | at[3] | at[4] | to[0] | to[1] | to[2]) % 16:
         return _bwd_copied(dout, q, k, v, out, lse, window, sink_tokens, kv_lens, softmax_scale, dq, dk, dv, layout)
     a.lse = lse.data_ptr()
@@ -349,6 +361,7 @@ class _BwdPlan(NamedTuple):
     k_shape: tuple
     args: bytes
     workspace: int  # bytes
+    apart: tuple  # of overlap.check_apart: dq, dk, dv, dout, q, k, v, out, lse, kv_lens
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -365,19 +378,22 @@ def _bwd_plan(dout, q, k, v, out, lse, lens, dq, dk, dv, window, sinks, softmax_
         _check_lens(lens, B, device, "kv_lens")
     scale = _check_scale(softmax_scale, D)
     for buf, like in ((dq, q), (dk, k), (dv, v)):
-        assert buf is None or (buf[0] == like[0] and buf[2] == like[2] and buf[3] == device), "gradient buffers must match q, k, v"
+        assert buf is None or (buf[0] == like[0] and buf[2] == like[2] and buf[3] == device and spread(*buf[:2])), (
+            "gradient buffers must match q, k, v and not overlap themselves")
     q_shape, k_shape = tuple(q[0]), tuple(k[0])
+    apart = pairs_apart((("dq", dq), ("dk", dk), ("dv", dv)), (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out),
+                                                               ("lse", lse), ("kv_lens", lens)))
     if 0 in q_shape or 0 in k_shape:
-        return _BwdPlan(True, True, q_shape, k_shape, b"", 0)
+        return _BwdPlan(True, True, q_shape, k_shape, b"", 0, apart)
     contiguous = lambda n: (n[1] * n[2] * n[3], n[2] * n[3], n[3], 1)  # noqa: E731
     grad_st = [like if buf is None else buf[1] for buf, like in ((dq, contiguous(q_shape)), (dk, contiguous(k_shape)), (dv, contiguous(k_shape)))]
     strides = [t[1] for t in (dout, q, k, v, out)] + grad_st
     if not (all(map(_fits, strides)) and _dense(lse) and (lens is None or _dense(lens))):
-        return _BwdPlan(False, False, q_shape, k_shape, b"", 0)
+        return _BwdPlan(False, False, q_shape, k_shape, b"", 0, apart)
     ws = max(16, int(_cabi.load().bsa_window_bwd_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sinks)))
     args = _cabi.WindowBwdArgs(*[None] * 12, ws, *(_bhsd(st, layout) for st in strides), _dtype_code(q[2]), B, Hq, Hkv, Sq, Sk, D,
                                window, sinks, scale)
-    return _BwdPlan(True, False, q_shape, k_shape, bytes(args), ws)
+    return _BwdPlan(True, False, q_shape, k_shape, bytes(args), ws, apart)
 
 
 class WindowAttentionFunction(torch.autograd.Function):

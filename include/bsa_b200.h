@@ -294,6 +294,7 @@ int64_t bsa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t Sq, int32_t Sk, in
  * Keys sit at positions 0..len-1 of their sequence, query row i at position p = base + i.  Key j is visible iff
  *   0 <= p < len,  j <= p,  and (j > p - window  or  j < sinks).
  * Rows that see nothing give out = 0, lse = -inf.  Layouts as in bsa_fwd (strides in elements, innermost contiguous).
+ * Outputs share no memory with inputs or with each other, here and in the entry points below (out may be q).
  *
  * Contiguous keys (page_table == NULL): k, v [B, Hkv, Sk, D]; len = kv_lens[b] (NULL: Sk); base = Sk - Sq.
  * Paged keys: k, v [num_pages, Hkv, page_size, D]; the token at position j of sequence b lies in page

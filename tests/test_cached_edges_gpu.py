@@ -216,3 +216,18 @@ def test_results_do_not_depend_on_unused_queries(deal):
             got.append(cached_attn_fwd(torch.where(dead, q * holds, q).cuda(), *pools, tree_mask=tree, return_lse=True))
         for other in got[1:]:
             assert torch.equal(got[0][0], other[0]) and torch.equal(got[0][1], other[1])
+
+
+def test_pools_that_interleave_are_written():
+    from block_sparse_attention import cache_append, cache_keep
+    kc, vc, table, _, _ = make_cache(2, 2, 16, 64, [50, 40], BF, garbage=False)
+    both = torch.stack((kc, vc), 1).cuda()
+    rows = torch.stack([torch.randn(2, 2, 9, 64, generator=torch.Generator().manual_seed(s)).bfloat16() for s in (1, 2)], 2).cuda()
+    k, v = rows[:, :, 0], rows[:, :, 1]
+    kc, vc, table, n = kc.cuda(), vc.cuda(), table.cuda(), i32([50, 40])
+    path, counts = i32([[1, 4, 8], [0, 2, 3]]), i32([3, 2])
+    for pools in ((kc, vc), (both[:, 0], both[:, 1])):
+        cache_append(k, v, *pools, table, n)
+        new = cache_keep(*pools, table, n, path, counts, 9)
+        assert new.tolist() == [44, 33]
+    assert torch.equal(both[:, 0], kc) and torch.equal(both[:, 1], vc)

@@ -14,3 +14,17 @@ def test_a_k_without_heads():
         assert k.shape == (2, 0, 5, 64)
         got, none = rotary_nd(q, k, pos, freq, (32,))
         assert torch.equal(got, want) and none.shape == k.shape
+
+
+def test_slices_of_a_fused_projection_one_of_them_in_place():
+    from block_sparse_attention import rotary_frequencies, rotary_nd
+    fused = torch.randn(2, 30, 6, 64, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    pos, freq = torch.arange(30, dtype=torch.int32, device="cuda")[:, None], rotary_frequencies((32,)).cuda()
+    q, k = fused[:, :, :3], fused[:, :, 3:5]
+    want = rotary_nd(q, k, pos, freq, (32,), layout="bshd")
+    before = fused.clone()
+    a, b = rotary_nd(q, k, pos, freq, (32,), layout="bshd", q_out=q)
+    assert a is q and torch.equal(q, want[0]) and torch.equal(b, want[1]) and torch.equal(fused[:, :, 3:], before[:, :, 3:])
+    fused.copy_(before)
+    rotary_nd(q, None, pos, freq, (32,), layout="bshd", q_out=fused[:, :, 3:])
+    assert torch.equal(fused[:, :, 3:], want[0]) and torch.equal(q, before[:, :, :3])

@@ -157,3 +157,24 @@ def test_results_do_not_depend_on_what_padding_holds(deal):
         got.append((out, lse) + window_attn_bwd(do2, q2, k2, v2, out, lse, 4096, 0, kv_lens=n))
     for other in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+def test_buffers_that_interleave_without_meeting():
+    """Slices of fused tensors as outputs, `out` in the place of q."""
+    from block_sparse_attention import window_attn_bwd, window_attn_fwd
+    B, S, H, Hkv, D = 2, 300, 4, 2, 64
+    q, k, v, do = (t.transpose(1, 2).contiguous().cuda() for t in make(B, H, Hkv, S, S, D, BF, seed=9))
+    how = dict(layout="bshd")
+    want, lse = window_attn_fwd(q, k, v, 70, 2, return_lse=True, **how)
+    fused = torch.cat((q, k, v), 2)
+    parts = fused.split((H, Hkv, Hkv), 2)
+    grads = window_attn_bwd(do, q, k, v, want, lse, 70, 2, **how)
+    into = torch.full_like(fused, 7.0)
+    slices = into.split((H, Hkv, Hkv), 2)
+    window_attn_bwd(do, *parts, want, lse, 70, 2, dq=slices[0], dk=slices[1], dv=slices[2], **how)
+    assert torch.equal(into, torch.cat(grads, 2))
+    for sizes in ((300, 300), (300, 20)):  # whole query tiles; packed heads and shared lists
+        q2 = fused[:, :sizes[1], :H]
+        ref, _ = window_attn_fwd(q2.clone(), parts[1], parts[2], 70, 2, **how)
+        out, _ = window_attn_fwd(q2, parts[1], parts[2], 70, 2, out=q2, **how)
+        assert out is q2 and torch.equal(q2, ref) and torch.equal(parts[1], k) and torch.equal(parts[2], v)
