@@ -231,3 +231,31 @@ def test_pools_that_interleave_are_written():
         new = cache_keep(*pools, table, n, path, counts, 9)
         assert new.tolist() == [44, 33]
     assert torch.equal(both[:, 0], kc) and torch.equal(both[:, 1], vc)
+
+
+@pytest.mark.parametrize("deal", DEALS[1:], indirect=True, ids=str)
+def test_every_way_of_dealing_short_trees(deal):
+    for case in SHORT_TREES:
+        test_trees_over_sequences_shorter_than_the_tree(case, "random")
+
+
+# Hq, Hkv, T, page, D, dtype, lens, window, sinks
+CHUNKS = [
+    (4, 2, 600, 384, 64, HF, [1500, 640], None, 0),       # pages of three key tiles
+    (8, 1, 300, 64, 96, BF, [2000, 300, 299], 500, 4),
+    (2, 2, 1024, 16, 128, BF, [1024], 129, 1),
+    (32, 8, 512, 128, 128, BF, [4096], None, 0),
+]
+
+
+@pytest.mark.parametrize("case", CHUNKS, ids=[str(i) for i in range(len(CHUNKS))])
+def test_chunks_of_a_prompt(case):
+    from block_sparse_attention import cached_attn_fwd
+    Hq, Hkv, T, page, D, dtype, lens, window, sinks = case
+    kc, vc, table, ks, vs = make_cache(len(lens), Hkv, page, D, lens, dtype, seed=T)
+    q = torch.randn(len(lens), Hq, T, D, generator=torch.Generator().manual_seed(T)).to(dtype)
+    out, lse = cached_attn_fwd(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), i32(lens), window=window, sink_tokens=sinks, return_lse=True)
+    p = [torch.arange(n - T, n)[:, None] for n in lens]
+    masks = [(torch.arange(n) <= x) & ((torch.arange(n) > x - (window or ALL)) | (torch.arange(n) < sinks)) & (x >= 0)
+             for n, x in zip(lens, p)]
+    check(out, lse, q, ks, vs, masks, dtype)

@@ -133,3 +133,26 @@ def test_outputs_that_share_memory_are_refused(monkeypatch):
         with pytest.raises(AssertionError):
             call()
             raise RuntimeError(f"call {at} was not refused")
+
+
+def test_every_operator_struct_matches_the_header():
+    """Names, types and array lengths of the header's fields, in order."""
+    import ctypes
+    import os
+    import re
+    from block_sparse_attention import _cabi
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "bsa_b200.h")).read()
+    plain = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "float": ctypes.c_float}
+    for struct, cls in (("bsa_window_fwd_args", _cabi.WindowFwdArgs), ("bsa_window_bwd_args", _cabi.WindowBwdArgs),
+                        ("bsa_rotary_args", _cabi.RotaryArgs), ("bsa_cache_args", _cabi.CacheArgs)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (struct, struct), text, flags=re.S).group(1)
+        fields = []
+        for decl in filter(None, (d.strip() for d in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"))):
+            kind, names = re.match(r"(?:const\s+)?(\w+)\s*(.*)", decl, flags=re.S).groups()
+            for name in names.split(","):
+                star, name, count = re.match(r"\s*(\*?)\s*(\w+)(?:\[(\d+)\])?\s*$", name).groups()
+                one = ctypes.c_void_p if star else plain[kind]
+                fields.append((name, one * int(count) if count else one))
+        assert [f[0] for f in fields] == [f[0] for f in cls._fields_], struct
+        for (name, want), (_, got) in zip(fields, cls._fields_):
+            assert (got is want) or (issubclass(got, ctypes.Array) and got._type_ is want._type_ and got._length_ == want._length_), (struct, name)
