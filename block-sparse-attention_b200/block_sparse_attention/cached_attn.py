@@ -20,8 +20,8 @@ import torch
 from . import _cabi
 from .bsa_attn_interface import _ceil_div
 from .overlap import meet, span_bytes, spread
-from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_buffers, _check_lens, _check_qkv, _check_scale, _check_window, _copied, _dense, _fits,
-                          _make_plan, _meta, _run_plan)
+from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_buffers, _check_lens, _check_qkv, _check_scale, _check_window, _copied,
+                          _dense, _fits, _make_plan, _meta, _run_plan)
 
 __all__ = ["cached_attn_fwd", "tree_mask_from_parents", "cache_append", "cache_keep"]
 
@@ -115,7 +115,8 @@ def cached_attn_fwd(
 
     Rows that see nothing give ``out = 0`` and ``lse = -inf``: unused slots, tokens at negative positions
     (``cache_lens[b] < T``), sequences without pages.  Tokens whose page is not in the pool are not visible.  What the
-    pages hold behind ``cache_lens[b]`` is never used.  The call is inference only: it has no gradient.
+    pages hold behind ``cache_lens[b]``, for unused slots and before every window reaches no result.  ``out`` may be q.  The
+    call is inference only: it has no gradient.
     """
     want_lse = return_lse or lse is not None
     plan = _cached_plan(_meta(q), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(tree_mask),
@@ -218,7 +219,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     sequence at positions ``cache_lens[b] - T .. cache_lens[b] - 1``, in place; returns the pools.
 
     Tokens at negative positions and tokens whose page is not in the pool are dropped; nothing else is touched.  A page
-    must not be reached through two sequences' tables for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
+    must not be reached through two entries of the table for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
     """
     plan = _append_plan(_meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), layout)
     _check_written_pools(k_cache, v_cache, plan.spans[0], k, v, *plan.spans[1:])

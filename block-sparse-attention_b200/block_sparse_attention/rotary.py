@@ -51,7 +51,7 @@ def rotary_nd(
     by ``positions[b, s, axis] * inv_freq[p]`` (``inverse=True``: by the opposite angle).  ``positions`` is int32
     ``[S, axes]`` or ``[B, S, axes]``, ``inv_freq`` fp32 ``[P]`` (``rotary_frequencies``).  Angles are reduced in 64 bits, so
     positions of any size keep their accuracy.  ``q_out`` / ``k_out`` may be q and k themselves (in place); outputs that share
-    other memory are refused.
+    other memory are refused.  The call records no gradient: ``rotary_embedding`` does.
     """
     pairs = tuple(map(int, axis_pairs))
     plan = _rotary_plan(_meta(q), _meta(k), _meta(positions), _meta(inv_freq), pairs, bool(interleaved), bool(inverse),
@@ -173,5 +173,6 @@ class RotaryFunction(torch.autograd.Function):
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
                      axis_pairs: Sequence[int], interleaved: bool = True, layout: str = "bhsd"
                      ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Differentiable ``rotary_nd`` (with respect to q and k)."""
+    """Differentiable ``rotary_nd`` (with respect to q and k).  Once differentiable; captured in a CUDA graph as
+    ``window_attention`` is."""
     return RotaryFunction.apply(q, k, positions, inv_freq, axis_pairs, interleaved, layout)

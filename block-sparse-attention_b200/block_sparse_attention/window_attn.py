@@ -88,8 +88,9 @@ def _deal_work(items: int, key_tiles: int, rows: int, ragged: bool, num_sms: int
     """How the work of a call is dealt, as ``(ctas, team)``: ``(0, 1)`` whole query tiles in turn, ``(0, n)`` a cluster of n
     CTAs for each query tile, ``(ctas, 1)`` that many CTAs share the list of all key tiles evenly.
 
-    The cheapest of the three in key tiles of the busiest place (two places for each SM; a key tile takes 1.5 us there).  A
-    team adds its start and the join through shared memory; sharing a list adds the search for each CTA's run, a second
+    The cheapest of the three in key tiles of the busiest place (two places for each SM; a key tile takes 1.5 us there, two at
+    once 1.9).  The costs choose between the three and are no forecast of a call; they are from before whole query tiles were dealt
+    to heads in turn, which made those 5 to 27 % faster.  A team adds its start and the join through shared memory; sharing a list adds the search for each CTA's run, a second
     launch, the fp32 rows of the cut query tiles that go through memory, and neighbours that share fewer loads.  The
     coefficients fit times over 1 to 256 query tiles of 1 to 128 rows, lists of 2 to 256 key tiles, one token of
     four heads per KV head: 8 query tiles of 8 key tiles take 17.2 us whole, 9.9 as teams, 11.7 shared, of 64 key tiles 101,
@@ -278,7 +279,8 @@ def window_attn_fwd(
     Rows that see nothing give ``out = 0`` and ``lse = -inf``.  LSE (natural log, scale included, fp32 ``[B, Hq, Sq]``)
     is returned iff ``return_lse``, a gradient is required or an ``lse`` buffer was passed.
 
-    Inside a sequence, a NaN or infinity in a value that some query sees may reach other queries of the same 128 keys.
+    Inside a sequence, a NaN or infinity in a value that some query sees may reach other queries of the same 128 keys;
+    keys that no query sees may hold anything.  The call records no gradient: ``window_attention`` does.
     """
     want_lse = return_lse or lse is not None or q.requires_grad or k.requires_grad or v.requires_grad
     plan = _window_plan(_meta(q), _meta(k), _meta(v), _meta(out), _meta(lse), _meta(kv_lens), window, sink_tokens,
@@ -313,7 +315,7 @@ def window_attn_bwd(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Backward of ``window_attn_fwd``: returns ``(dq, dk, dv)`` in the shapes of q, k, v.
 
-    The gradients of a KV head sum over the query heads that share it, in fp32 and in a fixed order, so repeated calls
+    Gradient buffers share no memory with the inputs or with each other.  The gradients of a KV head sum over the query heads that share it, in fp32 and in a fixed order, so repeated calls
     are bit-identical.  Tokens behind ``kv_lens`` get zero gradients.  ``out`` and ``lse`` are those of the forward call
     with the same arguments.
     """

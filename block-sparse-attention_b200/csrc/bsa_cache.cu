@@ -2,8 +2,9 @@
 //
 // The token at position j of sequence b lies in page page_table[b][j / page_size] at row j % page_size.  All of it is
 // bound by HBM (append) or by latency (keep, masks): 16 bytes per thread and access, K and V together.  Measured at 8 heads
-// of 128 channels: append of 2048 tokens to each of 8 sequences 23.0 us, 5.8 TB/s, of 32 tokens to 64 sequences 3.7 us; keep
-// 8 of these 32 drafts 5.8 us (one load waits for the path's entry, which waits for the length).
+// of 128 channels (changing inputs, in a captured graph): append of 2048 tokens to each of 8 sequences 23.7 us, 5.7 TB/s; append of 32
+// drafts to 64 sequences and keep of 8 of them 9.2 us together (in keep one load waits for the path's entry, which waits for the
+// length).
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"

@@ -5,8 +5,10 @@
 // its threads first compute the sines and cosines of the tokens' pairs, about one each, into shared memory; a thread
 // owns one 16-byte chunk of a token (half-split pairing: the two chunks its pairs connect), takes its pairs' values
 // into registers and walks over every head_lanes-th head of q and k.  Four loads are in flight while the four before are
-// worked on, the first four under the sines.  Measured: 76800 tokens of 24 + 24 heads of 128 channels, bf16, 303 us, 6.2 TB/s
-// (95 % of a plain copy's rate); 3 x 4097 tokens of 16 + 4 heads of 96, fp16, 18.5 us; 64 tokens of 32 + 8 heads, 3.1 us.
+// worked on, the first four under the sines.  Measured (changing
+// inputs, in a captured graph): 76800 tokens of 24 + 24 heads of 128 channels, bf16, 309 us, 6.1 TB/s (93 % of a plain copy's
+// rate); 16384 tokens of 16 + 16 heads, fp32, 91 us, 5.9 TB/s; 3 x 4097 tokens of 16 + 4 heads of 96, fp16, 18.1 us; 64 tokens of
+// 32 + 8 heads, 2.9 us.
 //
 // The angle of position 10^5 at frequency 1 is 10^5 radians; in 32 bits its fraction of a turn would be off by 10^-3.
 // So a frequency becomes a 64-bit fraction of a turn per position, whose product with the position wraps around whole

@@ -26,8 +26,8 @@
 // small gradients need the loss scaling that fp16 training uses anyway.
 //
 // Bound by the instructions of the compute warps between two MMAs of a chain, like the block-sparse backward.  Measured: 16
-// heads of 16384 tokens, window 1024, 4 sinks, bf16: 24 + 225 + 355 + 4 us; dQ executes 890, dK/dV 750 TFLOP/s of the
-// visible pairs (6 D and 8 D operations each).
+// heads of 16384 tokens, window 1024, 4 sinks, bf16: 685 us for the four launches, 680 TFLOP/s of the operations that they execute
+// on the visible pairs (14 D each, where the formula has 10 D).
 #include "bsa_b200.h"
 #include "bsa_common.cuh"
 #include "bsa_host.h"
@@ -159,7 +159,7 @@ __device__ __forceinline__ void mma_ts_kmn(uint32_t d, uint32_t a_lo, uint32_t a
 //    for rows of two keys, 0.81, 0.74, 0.70 for three to five, 0.68 for eight; this way 0.61.  Those are the first rows of any
 //    sequence (blocks of their own, in front of the others: dQ of the rows at positions 0 to 4 0.81 -> 0.61, the whole
 //    backward of 8 heads of 300 tokens 15.7 -> 16.0 us, of 16 heads of 16384 equal), and every row of a window that holds no more,
-//    which has a kernel of its own (16 heads of 16384 tokens, window 2: backward 296 us, from the rounded O 227).
+//    which has a kernel of its own (16 heads of 16384 tokens, window 2: the whole backward 227 -> 296 us).
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewKeys = 5;
 struct PreParams {
@@ -592,7 +592,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           tc_fence_after();
           const uint32_t buf = dp_cnt & 1;
           const uint32_t t_s = tS + lane_base + grp * 64, t_g = tdP + buf * 128u + lane_base + grp * 64;
-          // one body for whole tiles, one for masked ones: tests inside one body slowed every tile
+          // one body for whole tiles, one for masked ones (the dK/dV kernel's has the times)
           auto tile = [&](auto masked) -> bool {
             constexpr bool kMasked = decltype(masked)::value;
             float pr[64];
@@ -997,8 +997,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!ok) break;
         tc_fence_after();
         const uint32_t t_s = tS + lane_base + grp * 64, t_g = tG + lane_base + grp * 64;
-        // One body for whole tiles and one for masked ones: tests inside one body slowed every tile (403 us against 303
-        // without any mask at 16 heads, 16384 tokens, window 1024).
+        // One body for whole tiles and one for masked ones: with the masked body for every tile, here and in the dQ kernel, 16
+        // heads of 16384 tokens, window 1024, take 740 us for the backward instead of 685.
         auto tile = [&](auto masked) -> bool {
           constexpr bool kMasked = decltype(masked)::value;
           float pr[64];

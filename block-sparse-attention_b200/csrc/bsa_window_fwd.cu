@@ -22,9 +22,10 @@
 // its CTA's run itself from the lengths' prefix sums.  (The host's rule has the times of the three.)
 //
 // Bound, where many rows share a key, by the chain QK - softmax - PV of a tile, two of which overlap on an SM; where few
-// do, by the reads of the keys.  Measured: 32 heads (8 of keys) of 32768 tokens, window 2048, 1055 us, 1010 TFLOP/s of the
-// visible pairs; one token of each of 64 sequences, 4096 visible keys, 175 us, 6.1 TB/s; one token of one sequence, 1024
-// visible keys, 11 us; trees of 48 drafts over 8 sequences of up to 16384 tokens, 102 us and the join's 12.
+// do, by the reads of the keys.  Measured: 32 heads (8 of keys) of 32768 tokens, window 2048, 1219 us, 875 TFLOP/s of the
+// visible pairs; one token of each of 64 sequences, 4096 visible keys, 196 us, 5.5 TB/s; one token of one sequence, 1024
+// visible keys, 13 us; trees of 48 drafts over 8 sequences of up to 16384 tokens, 137 us; 2048 new tokens over 65536 cached,
+// window 4096, 32 (8) heads, 159 us in pages of 64, 153 contiguous.
 //
 // Roundings: scores, maximum, sums and O are fp32.  P is rounded to the inputs' type for the tensor cores; the sum is that of
 // the unrounded P, so a rounding does not shift the others.
@@ -718,9 +719,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             pk[e] = F16 ? pack_f16x2(x0, x1) : pack_bf16x2(x0, x1);
           }
         };
-        // One body for whole tiles and one for masked tiles, both straight-line: tests inside one body slowed every
-        // tile, and loops over the 32-column groups that a warp sees doubled the time of a tile on the diagonal (4000
-        // clocks against 2000 for the warp that sees all groups; the others wait for it).
+        // One body for whole tiles and one for masked tiles, both straight-line: with the masked body for every tile 16 heads
+        // of 16384 tokens, window 1024, take 220 us instead of 200, and loops over the 32-column groups that a warp sees
+        // doubled the time of a tile on the diagonal (4000 clocks against 2000 for the warp that sees all groups; the
+        // others wait for it).
         auto tile = [&](auto masked) {
           constexpr bool kMasked = decltype(masked)::value;
           float sv[128];

@@ -405,7 +405,7 @@ int bsa_tree_mask(const int32_t* parents, int32_t B, int32_t T, int64_t* mask, v
  *                     lens[b] - T + the number kept.  A path ends at its first entry that is not ascending or not in
  *                     [0, T).  A sequence with lens[b] < T keeps its length and is not touched.
  * A length beyond max_pages * page_size counts as that, as in bsa_window_fwd (the last T places of the table then).
- * A page must not be written through two sequences' tables in one call.
+ * A page must not be written through two entries of the table in one call.
  */
 typedef struct bsa_cache_args {
   const void* k;            /* append */
