@@ -19,7 +19,7 @@ import torch
 
 from . import _cabi
 from .bsa_attn_interface import _ceil_div
-from .overlap import meet, span_bytes, spread
+from .overlap import check_apart, pairs_apart, spread
 from .window_attn import (_MAX_LEN, _Plan, _bhsd, _check_buffers, _check_lens, _check_qkv, _check_scale, _check_window, _copied,
                           _dense, _fits, _make_plan, _meta, _run_plan)
 
@@ -44,21 +44,8 @@ def _check_cache(k_cache, v_cache, page_table, cache_lens, B: int, device) -> No
     _check_lens(cache_lens, B, device, "cache_lens")
 
 
-def _check_pool_address(k_cache, v_cache) -> None:
-    assert (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the pools must be 16-byte aligned"
-
-
-def _check_written_pools(k_cache, v_cache, span: int, k=None, v=None, k_span: int = 0, v_span: int = 0) -> None:
-    """Pools that are written share no memory with each other nor with the rows that are written to them; the spans (bytes) settle
-    all but interleaved views."""
-    _check_pool_address(k_cache, v_cache)
-    at_k, at_v = k_cache.data_ptr(), v_cache.data_ptr()
-    assert not -span < at_k - at_v < span or not meet(k_cache, v_cache), "keys and values must not be written to one pool"
-    for rows, n in ((k, k_span), (v, v_span)):
-        if n > 0:
-            at = rows.data_ptr()
-            if -n < at - at_k < span or -n < at - at_v < span:
-                assert not meet(rows, k_cache) and not meet(rows, v_cache), "k and v must not share memory with the pools"
+def _check_pool_address(*pools: int) -> None:
+    assert (pools[0] | pools[1]) % 16 == 0, "the pools must be 16-byte aligned"
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -122,7 +109,7 @@ def cached_attn_fwd(
     plan = _cached_plan(_meta(q), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(tree_mask),
                         _meta(out), _meta(lse), window, sink_tokens, None if softmax_scale is None else float(softmax_scale),
                         layout, want_lse)
-    _check_pool_address(k_cache, v_cache)
+    _check_pool_address(k_cache.data_ptr(), v_cache.data_ptr())
     if out is not None or lse is not None:
         _check_buffers(plan, out, lse, q, k_cache, v_cache, cache_lens, page_table, tree_mask)
     res = _run_plan(plan, q, k_cache, v_cache, out, lse, cache_lens, page_table, tree_mask) if plan.direct else None
@@ -159,14 +146,15 @@ class _WritePlan(NamedTuple):
 
     direct: bool
     empty: bool
-    spans: Tuple[int, ...]  # bytes: a pool, k, v
+    apart: tuple  # of overlap.check_apart: k_cache, v_cache, k, v
     args: bytes = b""  # CacheArgs without addresses
 
 
-def _pool_span(k_cache, v_cache) -> int:
+def _written_pools(k_cache, v_cache, k=None, v=None) -> tuple:
+    """Pools that are written share no memory with each other nor with the rows that are written to them."""
     for t in (k_cache, v_cache):
         assert spread(*t[:2]), "a pool that is written must not overlap itself"
-    return max(span_bytes(*k_cache[:2], 2), span_bytes(*v_cache[:2], 2))
+    return pairs_apart((("k_cache", k_cache), ("v_cache", v_cache)), (("k", k), ("v", v)))
 
 
 @functools.lru_cache(maxsize=256, typed=True)
@@ -179,13 +167,13 @@ def _append_plan(k, v, k_cache, v_cache, table, lens, layout) -> _WritePlan:
     _check_cache(k_cache, v_cache, table, lens, B, k[3])
     num_pages, pool_heads, page_size, pool_dim = k_cache[0]
     assert pool_heads == H and pool_dim == D and D % 8 == 0, "the pools must match k's heads and head dimension"
-    spans = _pool_span(k_cache, v_cache), span_bytes(*k[:2], 2), span_bytes(*v[:2], 2)
+    apart = _written_pools(k_cache, v_cache, k, v)
     if B == 0 or T == 0 or table[0][1] == 0:
-        return _WritePlan(True, True, spans)
+        return _WritePlan(True, True, apart)
     rows_ok = all(t[1][3] == 1 and (t[1][0] | t[1][1] | t[1][2]) % 8 == 0 for t in (k, v))
     if not (rows_ok and _dense(table) and _dense(lens)):
-        return _WritePlan(False, False, spans)
-    return _WritePlan(True, False, spans, bytes(_cabi.CacheArgs(
+        return _WritePlan(False, False, apart)
+    return _WritePlan(True, False, apart, bytes(_cabi.CacheArgs(
         *[None] * 9, _bhsd(k[1], layout), _bhsd(v[1], layout), k_cache[1][:3], v_cache[1][:3], B, H, T, D, table[0][1], page_size,
         num_pages, 0)))
 
@@ -202,12 +190,12 @@ def _keep_plan(k_cache, v_cache, table, lens, path, path_lens, num_drafts) -> _W
         f"path must be int32 of shape ({B}, n) on the device of the pools")
     assert path_lens is not None, "path_lens must be given"
     _check_lens(path_lens, B, device, "path_lens")
-    spans = (_pool_span(k_cache, v_cache),)
+    apart = _written_pools(k_cache, v_cache)
     if B == 0:
-        return _WritePlan(True, True, spans)
+        return _WritePlan(True, True, apart)
     if path[0][1] == 0 or table[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
-        return _WritePlan(False, False, spans)
-    return _WritePlan(True, False, spans, bytes(_cabi.CacheArgs(
+        return _WritePlan(False, False, apart)
+    return _WritePlan(True, False, apart, bytes(_cabi.CacheArgs(
         *[None] * 9, (0, 0, 0), (0, 0, 0), k_cache[1][:3], v_cache[1][:3], B, H, num_drafts, D, table[0][1], page_size, num_pages,
         path[0][1])))
 
@@ -219,19 +207,21 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     sequence at positions ``cache_lens[b] - T .. cache_lens[b] - 1``, in place; returns the pools.
 
     Tokens at negative positions and tokens whose page is not in the pool are dropped; nothing else is touched.  A page
-    must not be reached through two entries of the table for writing.  BF16 or FP16, ``D`` a multiple of 8, any page size.
+    must not be reached through two entries of the table for writing, and k and v share no memory with the pools.  BF16 or
+    FP16, ``D`` a multiple of 8, any page size.
     """
     plan = _append_plan(_meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), layout)
-    _check_written_pools(k_cache, v_cache, plan.spans[0], k, v, *plan.spans[1:])
+    pools, at = (k_cache.data_ptr(), v_cache.data_ptr()), (k.data_ptr(), v.data_ptr())
+    _check_pool_address(*pools)
+    check_apart(plan.apart, pools + at)
     if plan.empty:
         return k_cache, v_cache
-    at = k.data_ptr(), v.data_ptr()
     if not plan.direct or (at[0] | at[1]) % 16 != 0:
         k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         return cache_append(k, v, k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), layout=layout)
     a = _cabi.CacheArgs.from_buffer_copy(plan.args)
     a.k, a.v = at
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    a.k_cache, a.v_cache = pools
     a.page_table, a.lens = page_table.data_ptr(), cache_lens.data_ptr()
     _cabi.launch(_cabi.load().bsa_cache_append, "bsa_cache_append", k.device, a)
     return k_cache, v_cache
@@ -248,7 +238,9 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     ``num_drafts`` tokens is left as it is.  A move from or to a page that is not in the pool is dropped.
     """
     plan = _keep_plan(_meta(k_cache), _meta(v_cache), _meta(page_table), _meta(cache_lens), _meta(path), _meta(path_lens), num_drafts)
-    _check_written_pools(k_cache, v_cache, plan.spans[0])
+    pools = k_cache.data_ptr(), v_cache.data_ptr()
+    _check_pool_address(*pools)
+    check_apart(plan.apart, pools)
     if plan.empty:
         return cache_lens.clone()
     if not plan.direct:
@@ -260,7 +252,7 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
                           path_lens.contiguous(), num_drafts)
     new_lens = torch.empty_like(cache_lens)
     a = _cabi.CacheArgs.from_buffer_copy(plan.args)
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    a.k_cache, a.v_cache = pools
     a.page_table, a.lens = page_table.data_ptr(), cache_lens.data_ptr()
     a.path, a.path_lens, a.new_lens = path.data_ptr(), path_lens.data_ptr(), new_lens.data_ptr()
     _cabi.launch(_cabi.load().bsa_cache_keep, "bsa_cache_keep", k_cache.device, a)

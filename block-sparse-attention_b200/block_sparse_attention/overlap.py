@@ -8,9 +8,7 @@ from __future__ import annotations
 import functools
 from typing import NamedTuple, Optional, Sequence, Tuple
 
-import torch
-
-__all__ = ["span_bytes", "spread", "same_places", "meet", "pairs_apart", "check_apart"]
+__all__ = ["span_bytes", "spread", "same_places", "pairs_apart", "check_apart"]
 
 _MOST_STEPS = 20000  # of the exact comparison; views that need more (strides that do not nest) count as meeting
 
@@ -79,14 +77,6 @@ def _meet(a, b, distance: int) -> bool:
         return any(solve(k + 1, lo - s * m, hi - s * m) for m in range(first, last + 1))
 
     return solve(0, distance - a_run, distance + b_run)
-
-
-def meet(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two views share a byte."""
-    views = [(tuple(t.shape), t.stride(), t.element_size()) for t in (a, b)]
-    a_span, b_span = (span_bytes(*view) for view in views)
-    distance = b.data_ptr() - a.data_ptr()
-    return -b_span < distance < a_span and b_span > 0 < a_span and _meet(*views, distance)
 
 
 class _Pair(NamedTuple):
