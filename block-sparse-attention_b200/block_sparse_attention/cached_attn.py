@@ -191,9 +191,9 @@ def _keep_plan(k_cache, v_cache, table, lens, path, path_lens, num_drafts) -> _W
     assert path_lens is not None, "path_lens must be given"
     _check_lens(path_lens, B, device, "path_lens")
     apart = _written_pools(k_cache, v_cache)
-    if B == 0:
+    if B == 0 or table[0][1] == 0:  # (a table without places holds no draft)
         return _WritePlan(True, True, apart)
-    if path[0][1] == 0 or table[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
+    if path[0][1] == 0 or not all(_dense(t) for t in (table, lens, path, path_lens)):
         return _WritePlan(False, False, apart)
     return _WritePlan(True, False, apart, bytes(_cabi.CacheArgs(
         *[None] * 9, (0, 0, 0), (0, 0, 0), k_cache[1][:3], v_cache[1][:3], B, H, num_drafts, D, table[0][1], page_size, num_pages,
@@ -246,8 +246,6 @@ def cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.T
     if not plan.direct:
         if path.shape[1] == 0:
             path = path.new_full((path.shape[0], 1), -1)
-        if page_table.shape[1] == 0:
-            page_table = page_table.new_full((page_table.shape[0], 1), -1)
         return cache_keep(k_cache, v_cache, page_table.contiguous(), cache_lens.contiguous(), path.contiguous(),
                           path_lens.contiguous(), num_drafts)
     new_lens = torch.empty_like(cache_lens)

@@ -259,3 +259,14 @@ def test_chunks_of_a_prompt(case):
     masks = [(torch.arange(n) <= x) & ((torch.arange(n) > x - (window or ALL)) | (torch.arange(n) < sinks)) & (x >= 0)
              for n, x in zip(lens, p)]
     check(out, lse, q, ks, vs, masks, dtype)
+
+
+def test_a_table_without_pages_holds_no_token():
+    from block_sparse_attention import cache_append, cache_keep, cached_attn_fwd
+    pools = [torch.ones(3, 2, 16, 64, dtype=BF, device="cuda") for _ in range(2)]
+    x, table, n = torch.ones(2, 2, 4, 64, dtype=BF, device="cuda"), torch.empty(2, 0, dtype=torch.int32, device="cuda"), i32([9, 0])
+    cache_append(2 * x, 2 * x, *pools, table, n)
+    new = cache_keep(*pools, table, n, i32([[1, 2], [0, 1]]), i32([2, 2]), 4)
+    out, lse = cached_attn_fwd(x, *pools, table, n, return_lse=True)
+    assert torch.equal(new, n) and new.data_ptr() != n.data_ptr()  # fewer tokens than drafts: left as they are
+    assert all((p == 1).all() for p in pools) and (out == 0).all() and lse.isneginf().all()
