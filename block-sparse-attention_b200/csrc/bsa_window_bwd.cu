@@ -19,11 +19,11 @@
 // warps 8-10 (dQ) or 8-9 (dK/dV) issue the MMAs of one dependency chain each, the last warp loads by TMA.
 // P and dS are rounded to 16 bits for the tensor cores (all sums are fp32), and delta is that of the 16-bit `out` that the
 // forward call returned: relative to the gradients' own rounding the three give errors of 1.4 to 1.6 times in all (rows of a
-// few keys, where delta nearly cancels dP, get a delta of their own).  What rows that take no part hold -
-// padding, keys before every window, NaN included - reaches no sum: P is replaced by 0 on masked pairs, dP too where a tile
-// holds such rows, the statistics of such queries are those of a row that sees nothing, and the rows are zeroed in shared
-// memory where an MMA contracts over them.  With fp16,
-// small gradients need the loss scaling that fp16 training uses anyway.
+// few keys, where delta nearly cancels dP, get a delta of their own).  With fp16, small gradients need the loss scaling that
+// fp16 training uses anyway.
+// What rows that take no part hold - padding, keys before every window, NaN included - reaches no sum: P is replaced by 0 on
+// masked pairs, dP too where a tile holds such rows, the statistics of such queries are those of a row that sees nothing, and
+// the rows are zeroed in shared memory where an MMA contracts over them.
 //
 // Bound by the instructions of the compute warps between two MMAs of a chain, like the block-sparse backward.  Measured: 16
 // heads of 16384 tokens, window 1024, 4 sinks, bf16: 685 us for the four launches, 680 TFLOP/s of the operations that they execute

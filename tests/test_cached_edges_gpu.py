@@ -1,7 +1,8 @@
-"""GPU parity of cached attention at its edges: trees over sequences shorter than the tree, what unseen keys hold."""
+"""GPU parity of cached attention at its edges: short trees, what unseen keys and unused queries hold, lengths and tables, pools."""
 import pytest
 import torch
 
+from dealing import DEALS, deal  # noqa: F401
 from plain_ops import ancestors, assert_within, attend, cached_visible
 from test_cached_attn_gpu import ALL, BF, HF, make_cache
 
@@ -80,20 +81,6 @@ def test_a_chain_is_a_chunk_of_tokens_also_where_it_begins_before_the_sequence(w
     for got in (a, b):
         check(*got, q, ks, vs, [cached_visible(T, n, window or ALL, sinks) for n in lens], BF)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
-
-
-@pytest.fixture
-def deal(request, monkeypatch):
-    """Every call deals its work in the given way, whatever the rule says; None: the rule's."""
-    from block_sparse_attention import cached_attn, window_attn
-    if request.param is not None:
-        monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
-    cached_attn._cached_plan.cache_clear()
-    yield request.param
-    cached_attn._cached_plan.cache_clear()
-
-
-DEALS = [None, (0, 1), (0, 3), (0, 8), (7, 1), (296, 1)]
 
 
 def poison_unseen(pools, table, masks, holds):

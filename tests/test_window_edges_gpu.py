@@ -1,7 +1,8 @@
-"""GPU parity of sliding-window attention at its edges: what keys hold that no query sees."""
+"""GPU parity of sliding-window attention at its edges: what rows hold that take no part, first rows, unbounded lengths, buffers."""
 import pytest
 import torch
 
+from dealing import DEALS, deal  # noqa: F401
 from plain_ops import assert_close_norm, assert_within, attend, gradients, half_step
 from test_window_gpu import BF, HF, make, masks
 
@@ -11,19 +12,6 @@ pytestmark = pytest.mark.gpu
 def i32(x):
     return None if x is None else torch.tensor(x, dtype=torch.int32).cuda()
 
-
-@pytest.fixture
-def deal(request, monkeypatch):
-    """Every call deals its work in the given way, whatever the rule says; None: the rule's."""
-    from block_sparse_attention import window_attn
-    if request.param is not None:
-        monkeypatch.setattr(window_attn, "_deal_work", lambda *sizes: request.param)
-    window_attn._window_plan.cache_clear()
-    yield request.param
-    window_attn._window_plan.cache_clear()
-
-
-DEALS = [None, (0, 1), (0, 3), (0, 8), (7, 1), (296, 1)]
 
 # B, Hq, Hkv, Sq, Sk, D, dtype, window, sinks, lens
 CHUNKS = [
